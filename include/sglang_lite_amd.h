@@ -490,6 +490,83 @@ int sgl_split_swa_compress_indices(const void* topk, int idx_int64, int64_t BS, 
                                    int64_t window, int32_t* swa, int32_t* swa_lens,
                                    int32_t* comp, int32_t* comp_lens, sgl_stream_t stream);
 
+/* --------------------------- rotary positions and the 8-bit paged cache */
+
+/* The operators of this section have no counterpart in the reference's V4
+ * path; they serve models whose attention keeps keys and values per head. */
+
+/* Table of rotations: table[p][i] = length * (cos, sin)(p * freq[i]) in fp32,
+ * angles in 64 bits; freq fp64 [rot_dim / 2] in device memory, table fp32
+ * [n_positions, rot_dim / 2, 2], 8-byte aligned (16 for the fast paths). */
+int sgl_rotary_table(const double* freq, double length, int64_t n_positions, int rot_dim, float* table,
+                     sgl_stream_t stream);
+
+/* Rotary positions of x [T, H, D] (sgl_dtype; strides in elements, the last
+ * dimension dense): elements [offset, offset + rot_dim) of each head are pairs
+ * (a, b) turned to (a c - b s, b c + a s) with (c, s) = table[positions[t]][i],
+ * or s negated with `inverse` (the transpose: also the gradient).  Pair i is
+ * elements i and i + rot_dim / 2, or 2 i and 2 i + 1 with `interleaved`.  The
+ * other elements are copied.  fp32 arithmetic, rounded once.  A position below
+ * zero (a padding row) leaves its row as it is, one of n_positions or more
+ * gives NaN.  out may be x itself with the same strides; otherwise they must
+ * not overlap.  16-byte aligned pointers and strides, rot_dim % 16 == 0,
+ * offset % 8 == 0 and D % 8 == 0 take 16-byte accesses, everything else single
+ * elements. */
+int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_token_stride,
+               int64_t x_head_stride, const float* table, int64_t n_positions, int rot_dim, int offset,
+               const void* positions, int positions_int64, int interleaved, int inverse, void* out,
+               int64_t out_token_stride, int64_t out_head_stride, sgl_stream_t stream);
+
+/* The 8-bit paged cache: e4m3 codes [n_pages, Hkv, page_size, D] of keys and of
+ * values, and fp32 scales [n_pages, Hkv, page_size / block], one for every
+ * `block` tokens of a page and head; a stored value is code * scale.  D a
+ * multiple of 16 up to 256; page_size a power of two from 16 to 1024, block
+ * one from 16 to 128 and at most page_size.  block_table int32 [B, row_pages]:
+ * the pages of each sequence in order, token p in entry p / page_size.
+ * Sequence b's rows of the token-major inputs are [cu_tokens[b],
+ * cu_tokens[b + 1]) (int32 [B + 1], device), or row b with cu_tokens NULL.
+ *
+ * Appends k and v [T, Hkv, D] (sgl_dtype, 16-byte aligned strides): row i of
+ * sequence b becomes token start[b] + i.  With a table the keys are rotated
+ * first (arguments as for sgl_rotary, 16-byte aligned; positions int32 [T], NULL
+ * for the token's own place).  A block's scale is the smallest power of two,
+ * 2^-100 at least, that brings the largest finite magnitude among its new values
+ * down to 448, and not below the scale it had where it holds earlier tokens of
+ * the sequence (block start <= p < start[b]); those are rounded again where it
+ * grew.  code = e4m3(x / scale), round to nearest even; NaN and infinities
+ * become the NaN code.  Rows behind cu_tokens[B], tokens that the table does not
+ * reach, entries outside [0, n_pages) and sequences with a negative start are
+ * skipped.  Every page that is written to must belong to one sequence of the call. */
+int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv,
+                   int D, const int32_t* cu_tokens, const int32_t* start, const int32_t* block_table,
+                   int64_t row_pages, int page_size, int block, int64_t n_pages, const float* table,
+                   int64_t n_positions, int rot_dim, int offset, const int32_t* positions, int interleaved,
+                   void* k_codes, void* v_codes, float* k_scale, float* v_scale, sgl_stream_t stream);
+
+/* Attention of q [T, Hkv * G, D] (bf16 or f16, 16-byte aligned strides; query
+ * head h reads kv head h / G) over the cache: lens[b] keys of sequence b, its n
+ * queries being the last n of them (query i at position lens[b] - n + i).
+ * Causal: a query sees the keys up to its own position, with window > 0 the last
+ * `window` of them; otherwise all lens[b].
+ *   o = sum_j e^(s_j) v_j / (sum_j e^(s_j) + e^(sink[h])),  s_j = softmax_scale q . k_j
+ * (sink fp32 [Hkv * G] or NULL: no such term).  fp32 sums; a row that sees no key
+ * gives zeros.  Keys behind lens[b], and those on entries outside [0, n_pages),
+ * are not seen, whatever their codes and scales hold; a lens[b] past the block
+ * table is cut to it.  out [T, Hkv * G, D] dense, in q's type; rows behind
+ * cu_tokens[B] are left as they are.  The workspace has
+ * sgl_kv8_attn_workspace_size bytes, 16-byte aligned; calls that overlap need
+ * their own. */
+int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T,
+                 int64_t B, int Hkv, int G, int D, const int32_t* cu_tokens, const int32_t* lens,
+                 const int32_t* block_table, int64_t row_pages, int page_size, int block, int64_t n_pages,
+                 const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                 float softmax_scale, int causal, int64_t window, const float* sink, void* out,
+                 void* workspace, size_t workspace_bytes, sgl_stream_t stream);
+
+/* Workspace bytes of sgl_kv8_attn on the current device. */
+size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D);
+
 /* ------------------------------------------------- host-side self checks */
 
 /* The device numeric code compiled for the host, so the CPU test suite can

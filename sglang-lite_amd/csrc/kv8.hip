@@ -1,0 +1,291 @@
+// New keys and values into the 8-bit paged cache, the keys rotated on the way.
+//
+// Tokens [start, start + n) of a sequence fall into blocks of `block` tokens of
+// a page; a block and head has one power-of-two scale for its keys and one for
+// its values.  Of the new values x of a block, s = kv8_scale(max |x|) over the
+// finite ones, and not below the scale that the block had if it holds earlier
+// tokens of the sequence; code = e4m3(x / s), NaN for a NaN or an infinity.
+// Earlier tokens are written again, e4m3(code s_old / s), only where the scale
+// grew: a power of two, so nothing but codes near the smallest are rounded.
+//
+// Bound by HBM (6 bytes for an element of k and of v: 2 x 2 read, 2 x 1
+// written); for single tokens by the chain table entry -> old scale -> codes.
+// One workgroup takes one block, head and side (keys or values), so that the
+// scale is one reduction in registers and LDS and no block has two writers.
+#include "sgl_kv8.h"
+
+namespace sgl {
+namespace {
+
+struct AppendArgs {
+  const void *k, *v;
+  int64_t kt, kh, vt, vh;  // elements between tokens, heads
+  uint8_t *kc, *vc;
+  float *ks, *vs;
+  const int32_t* pages;  // [B, row_pages]
+  const int32_t* start;  // [B]
+  const int32_t* cu;     // [B + 1] or null: one token each
+  const float* table;    // or null: no rotation
+  const int32_t* positions;
+  int64_t n_positions;
+  int64_t n_pages;
+  int T, B, Hkv, D, row_pages, page_shift, block_shift;
+  int rot, offset;
+  bool interleaved;
+};
+
+// A unit of work: the new tokens of one block of one sequence.
+struct Unit {
+  int row0, n;  // their rows
+  int at;       // position of the first
+  int page;
+};
+
+// Unit u of the batch, sequences in order; n = 0 behind the last, and where a
+// table does not reach or names no page of the cache.
+__device__ __forceinline__ Unit find_unit(const AppendArgs& a, int u) {
+  const Unit none = {0, 0, 0, 0};
+  const int bs = a.block_shift;
+  int b = u, before = u;
+  if (a.cu) {
+    const int lane = threadIdx.x & 63;
+    before = 0;
+    for (int b0 = 0;; b0 += 64) {
+      if (b0 >= a.B) return none;
+      int c = 0;
+      if (b0 + lane < a.B) {
+        const SeqRows r = seq_rows(a.cu, b0 + lane, a.T);
+        const int st = a.start[b0 + lane];
+        if (r.n > 0 && st >= 0) c = (int)((((int64_t)st + r.n - 1) >> bs) - (st >> bs)) + 1;
+      }
+      const int incl = wave_incl_scan(c);
+      const int total = __builtin_amdgcn_readlane(incl, 63);
+      if (u < before + total) {
+        const int l = __builtin_ctzll(__ballot(before + incl > u));
+        b = b0 + l;
+        before += __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(c, l);
+        break;
+      }
+      before += total;
+    }
+  }
+  if (b >= a.B) return none;
+  const SeqRows r = seq_rows(a.cu, b, a.T);
+  const int64_t st = a.start[b];
+  if (r.n <= 0 || st < 0) return none;
+  const int64_t j = (st >> bs) + (u - before);  // block of the sequence
+  const int64_t lo = (j << bs) > st ? (j << bs) : st;
+  const int64_t hi = ((j + 1) << bs) < st + r.n ? ((j + 1) << bs) : st + r.n;
+  if (hi > ((int64_t)a.row_pages << a.page_shift)) return none;
+  const int page = a.pages[(int64_t)b * a.row_pages + (lo >> a.page_shift)];
+  if (page < 0 || page >= a.n_pages) return none;
+  return {r.first + (int)(lo - st), (int)(hi - lo), (int)lo, page};
+}
+
+// NT threads, IT units of 16 elements a thread
+template <int DT, int NT, int IT>
+__global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
+  const int head = (int)blockIdx.y >> 1;
+  const bool keys = (blockIdx.y & 1) == 0;
+  const Unit w = find_unit(a, (int)blockIdx.x);
+  if (w.n == 0) return;
+  const void* src = keys ? a.k : a.v;
+  const int64_t st = keys ? a.kt : a.vt, sh = keys ? a.kh : a.vh;
+  const int rot = keys ? a.rot : 0;
+  const int per = a.D >> 4, rot_units = rot >> 4;
+  const int count = w.n * per;
+
+  float x[IT][16];
+  int e0[IT], e1[IT], tok[IT];
+  float amax = 0.0f;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int i = it * NT + (int)threadIdx.x;
+    tok[it] = -1;
+    if (i < count) {
+      const int t = i / per, u = i - t * per;
+      int p0, p1;  // two chunks of 8 elements: those of 8 pairs, or two of the others
+      if (u < rot_units) {
+        p0 = a.offset + (a.interleaved ? 16 : 8) * u;
+        p1 = p0 + (a.interleaved ? 8 : rot >> 1);
+      } else {
+        const int c = 16 * (u - rot_units), off = rot ? a.offset : 0;
+        p0 = c < off ? c : c + rot;
+        p1 = c + 8 < off ? c + 8 : c + 8 + rot;
+      }
+      const int64_t at = (int64_t)(w.row0 + t) * st + (int64_t)head * sh;
+      load8<DT>(src, at + p0, x[it]);
+      load8<DT>(src, at + p1, x[it] + 8);
+      tok[it] = t;
+      e0[it] = p0;
+      e1[it] = p1;
+      if (u < rot_units) {
+        float cs[8], sn[8];
+        const int64_t pos = a.positions ? a.positions[w.row0 + t] : w.at + t;
+        load_turn<8>(a.table, a.n_positions, a.rot >> 1, pos, 8 * u, false, cs, sn);
+        if (a.interleaved) {
+          float p[8], q[8];
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            p[v] = x[it][2 * v];
+            q[v] = x[it][2 * v + 1];
+          }
+          rotate_pairs<8>(p, q, cs, sn);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            x[it][2 * v] = p[v];
+            x[it][2 * v + 1] = q[v];
+          }
+        } else {
+          rotate_pairs<8>(x[it], x[it] + 8, cs, sn);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float m = __builtin_fabsf(x[it][v]);
+        amax = m < __builtin_huge_valf() ? __builtin_fmaxf(amax, m) : amax;  // finite values alone
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) amax = __builtin_fmaxf(amax, __shfl_xor(amax, d, 64));
+
+  // the block's place
+  const int spot = w.at & ((1 << a.page_shift) - 1);
+  const int begin = spot & ~((1 << a.block_shift) - 1);
+  const int64_t line = (int64_t)w.page * a.Hkv + head;
+  uint8_t* codes = (keys ? a.kc : a.vc) + (line << a.page_shift) * a.D;
+  float* scale = (keys ? a.ks : a.vs) + (line << (a.page_shift - a.block_shift)) + (spot >> a.block_shift);
+  const float was = spot > begin ? *scale : 0.0f;
+  if constexpr (NT > 64) {
+    __shared__ float part[NT / 64];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = amax;
+    __syncthreads();  // (the old scale is read by then)
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) amax = __builtin_fmaxf(amax, part[i]);
+  }
+  float s = kv8_scale(amax);
+  if (was >= s) {
+    s = was;
+  } else if (was > 0.0f) {
+    const float inv = 1.0f / s;  // exact
+    const int bytes = (spot - begin) * a.D;
+    for (int i = 16 * (int)threadIdx.x; i < bytes; i += 16 * NT) {
+      uint4* at = reinterpret_cast<uint4*>(codes + (int64_t)begin * a.D + i);
+      const uint4 c = *at;
+      uint32_t q[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        unpack4_e4m3(q[j], f);
+        const uint32_t keep = ((((q[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xFFu;  // NaN codes
+        const uint32_t r = pk4_e4m3(f[0] * was * inv, f[1] * was * inv, f[2] * was * inv, f[3] * was * inv);
+        q[j] = (q[j] & keep) | (r & ~keep);
+      }
+      *at = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+  }
+  const float inv = 1.0f / s;  // exact for the powers of two that this kernel writes
+  if (threadIdx.x == 0) *scale = s;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    if (tok[it] >= 0) {
+      uint8_t* row = codes + (int64_t)(spot + tok[it]) * a.D;
+      float* f = x[it];
+#pragma unroll
+      for (int v = 0; v < 16; ++v) f[v] *= inv;  // at most 448; an infinity becomes the NaN code
+      *reinterpret_cast<uint2*>(row + e0[it]) =
+          make_uint2(pk4_e4m3_exact(f[0], f[1], f[2], f[3]), pk4_e4m3_exact(f[4], f[5], f[6], f[7]));
+      *reinterpret_cast<uint2*>(row + e1[it]) =
+          make_uint2(pk4_e4m3_exact(f[8], f[9], f[10], f[11]), pk4_e4m3_exact(f[12], f[13], f[14], f[15]));
+    }
+  }
+}
+
+template <int DT>
+void launch_append(const AppendArgs& a, int64_t units, int64_t per_unit, hipStream_t st) {
+  const dim3 grid((unsigned)units, (unsigned)(2 * a.Hkv));
+  if (per_unit <= 64)
+    append_kernel<DT, 64, 1><<<grid, 64, 0, st>>>(a);
+  else if (per_unit <= 256)
+    append_kernel<DT, 256, 1><<<grid, 256, 0, st>>>(a);
+  else if (per_unit <= 512)
+    append_kernel<DT, 256, 2><<<grid, 256, 0, st>>>(a);
+  else if (per_unit <= 1024)
+    append_kernel<DT, 256, 4><<<grid, 256, 0, st>>>(a);
+  else
+    append_kernel<DT, 256, 8><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace sgl
+
+extern "C" {
+
+int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv, int D,
+                   const int32_t* cu_tokens, const int32_t* start, const int32_t* block_table, int64_t row_pages,
+                   int page_size, int block, int64_t n_pages, const float* table, int64_t n_positions, int rot_dim,
+                   int offset, const int32_t* positions, int interleaved, void* k_codes, void* v_codes,
+                   float* k_scale, float* v_scale, sgl_stream_t stream) {
+  SGL_REQUIRE(dtype == SGL_BF16 || dtype == SGL_F16 || dtype == SGL_F32, "kv8_append: dtype %d", dtype);
+  const int rc = sgl::kv8_check_cache("kv8_append", Hkv, D, page_size, block, n_pages, row_pages);
+  if (rc != SGL_OK) return rc;
+  SGL_REQUIRE(T >= 0 && T <= (1 << 30) && B >= 0 && B <= (1 << 24), "kv8_append: T=%lld B=%lld out of range",
+              (long long)T, (long long)B);
+  SGL_REQUIRE(cu_tokens || T == B, "kv8_append: without cu_tokens every sequence has one token (T=%lld, B=%lld)",
+              (long long)T, (long long)B);
+  if (table) {
+    SGL_REQUIRE(rot_dim >= 16 && rot_dim % 16 == 0 && offset >= 0 && offset % 8 == 0 && offset + rot_dim <= D,
+                "kv8_append: rot_dim=%d must be a multiple of 16 and fit at offset %d (a multiple of 8) into D=%d",
+                rot_dim, offset, D);
+    SGL_REQUIRE(n_positions >= 1 && sgl::aligned(table, 16), "kv8_append: bad rotary table");
+  }
+  if (T == 0 || B == 0) return SGL_OK;
+  SGL_REQUIRE(k && v && start && block_table && k_codes && v_codes && k_scale && v_scale,
+              "kv8_append: null pointer");
+  const int size = dtype == SGL_F32 ? 4 : 2;
+  SGL_REQUIRE(sgl::aligned(k, 16) && sgl::aligned(v, 16) && k_token_stride * size % 16 == 0 &&
+                  k_head_stride * size % 16 == 0 && v_token_stride * size % 16 == 0 && v_head_stride * size % 16 == 0,
+              "kv8_append: k and v and their strides must be 16-byte aligned");
+  SGL_REQUIRE(sgl::aligned(k_codes, 16) && sgl::aligned(v_codes, 16), "kv8_append: misaligned cache");
+  sgl::AppendArgs a;
+  a.k = k;
+  a.v = v;
+  a.kt = k_token_stride;
+  a.kh = k_head_stride;
+  a.vt = v_token_stride;
+  a.vh = v_head_stride;
+  a.kc = (uint8_t*)k_codes;
+  a.vc = (uint8_t*)v_codes;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.pages = block_table;
+  a.start = start;
+  a.cu = cu_tokens;
+  a.table = table;
+  a.positions = positions;
+  a.n_positions = n_positions;
+  a.n_pages = n_pages;
+  a.T = (int)T;
+  a.B = (int)B;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.row_pages = (int)row_pages;
+  a.page_shift = __builtin_ctz((unsigned)page_size);
+  a.block_shift = __builtin_ctz((unsigned)block);
+  a.rot = table ? rot_dim : 0;
+  a.offset = table ? offset : 0;
+  a.interleaved = interleaved != 0;
+  const int64_t units = cu_tokens ? sgl::kv8_append_units(T, B, block) : B;
+  const int64_t per_unit = (cu_tokens ? (int64_t)block : 1) * (D / 16);
+  if (dtype == SGL_BF16)
+    sgl::launch_append<SGL_BF16>(a, units, per_unit, (hipStream_t)stream);
+  else if (dtype == SGL_F16)
+    sgl::launch_append<SGL_F16>(a, units, per_unit, (hipStream_t)stream);
+  else
+    sgl::launch_append<SGL_F32>(a, units, per_unit, (hipStream_t)stream);
+  return sgl::check_launch("kv8_append");
+}
+
+}  // extern "C"

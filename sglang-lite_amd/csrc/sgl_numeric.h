@@ -165,6 +165,14 @@ SGL_HD float clampf_(float x, float lo, float hi) {
   return x < lo ? lo : (x > hi ? hi : x);
 }
 
+// Scale of a block of the 8-bit paged cache: the smallest power of two, 2^-100 at least, with amax <= 448 s (448 = 1.75 2^8); amax finite.
+SGL_HD float kv8_scale(float amax) {
+  const uint32_t u = f32_bits(amax);
+  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  e = e < -100 ? -100 : e;
+  return pow2_f32(e);
+}
+
 // Activation-quant scale modes (see the mode table in sglang_lite_amd.h).
 enum ScaleMode : int {
   SCALE_TORCH_FP32 = 0,     // sf = max(amax,1e-4)/448 ; q = e4m3(x * (1/sf))

@@ -239,4 +239,34 @@ SGL_RULE int permute_rounds(int E, bool table) {
   return (table && E <= 512 ? 2 : 3) + (E <= (table ? 16 : 32) ? 1 : 0);
 }
 
+// ---- rotary positions: threads that share the heads of a token's unit, each
+// with four heads in flight at a time.  One head a thread while that leaves CUs
+// without a full round of wavefronts.
+SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cus) {
+  return T * units * ((H + 3) / 4) < cus * 1024 ? (int)H : (int)((H + 3) / 4);
+}
+
+// ---- append to the 8-bit cache: the most blocks that T tokens of B sequences
+// touch.  n tokens touch at most (n - 2) / block + 2, and no more than n.
+SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {
+  const int64_t most = T / block + 2 * B;
+  return most < T ? most : T;
+}
+
+// ---- attention over the 8-bit cache: rows of a tile, and the workgroups that
+// share the line of key tiles.
+struct Kv8AttnPlan {
+  int64_t row_tile, wgs;
+};
+// the most items (row tile, kv head) that T queries of B sequences make
+SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t row_tile) {
+  const int64_t tiles = T * G / row_tile + B, most = T * ((G + row_tile - 1) / row_tile + 1);
+  return Hkv * (tiles < most ? tiles : most);
+}
+SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t cus) {
+  (void)Hkv;
+  const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
+  return {D <= 128 && rows > 16 ? 32 : 16, 2 * cus};
+}
+
 }  // namespace sgl

@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 from typing import Optional
 
@@ -109,6 +109,23 @@ SIGNATURES = {
     "sgl_kv_to_paged": (c_int, [P, I64, c_int, P, P]),
     "sgl_kv_gather_dequant": (c_int, [P, c_int, c_int, c_int, I64, P, I64, I64, P, P]),
     "sgl_split_swa_compress_indices": (c_int, [P, c_int, I64, I64, I64, P, P, P, P, P]),
+    "sgl_rotary_table": (c_int, [P, c_double, I64, c_int, P, P]),
+    "sgl_rotary": (
+        c_int,
+        [P, c_int, I64, c_int, c_int, I64, I64, P, I64, c_int, c_int, P, c_int, c_int, c_int, P, I64,
+         I64, P],
+    ),
+    "sgl_kv8_append": (
+        c_int,
+        [P, I64, I64, P, I64, I64, c_int, I64, I64, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P,
+         I64, c_int, c_int, P, c_int, P, P, P, P, P],
+    ),
+    "sgl_kv8_attn": (
+        c_int,
+        [P, I64, I64, c_int, I64, I64, c_int, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P, P, P,
+         P, c_float, c_int, I64, P, P, P, c_size_t, P],
+    ),
+    "sgl_kv8_attn_workspace_size": (c_size_t, [I64, I64, c_int, c_int, c_int]),
     "sgl_host_f32_to_e4m3": (c_int, [P, P, I64]),
     "sgl_host_e4m3_to_f32": (c_int, [P, P, I64]),
     "sgl_host_group_scale": (c_int, [c_int, P, P, I64]),
@@ -237,3 +254,37 @@ def require_device(*tensors, what: str) -> None:
                 f"{what}: sglang_lite_amd runs only on a ROCm (gfx950) device tensor; "
                 f"got a {t.device} tensor (there is no CPU path)"
             )
+
+
+def require_same_device(*tensors, what: str) -> None:
+    """One call's tensors lie on one GPU."""
+    at = None
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if at is None:
+                at = d
+            elif d != at:
+                raise ValueError(f"{what}: tensors on devices {at} and {d}")
+
+
+class _Here:
+    """The context of :func:`on_device` where nothing has to change."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(t):
+    """A context in which ``t``'s device is the current one: a launch goes to the
+    current device, whatever device its stream and pointers belong to."""
+    import torch
+
+    d = t.get_device()
+    return _HERE if torch._C._cuda_getDevice() == d else torch.cuda.device(d)

@@ -1,0 +1,143 @@
+"""Rotary positions on gfx950.
+
+* ``rotary_table(n_positions, rot_dim, ...)`` -- the rotations of every
+  position, made once: fp32 ``[n_positions, rot_dim / 2, 2]`` (cos, sin), from
+  angles in 64 bits; plain, or scaled for long contexts.
+* ``rotary(x, table, positions, ...)`` -- ``x`` ``[T, H, D]`` with the pairs of
+  ``rot_dim`` elements of each head turned by their row's position; ``inverse``
+  turns them back, which is also the gradient with respect to ``x``.
+
+``paged_kv.append_kv`` takes the same table and turns the keys on their way
+into the cache.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.bfloat16: _lib.SGL_BF16, torch.float16: _lib.SGL_F16, torch.float32: _lib.SGL_F32}
+
+
+def frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
+    """Radians per position of each pair (fp64 on the CPU), and the factor that
+    the rotated elements are multiplied by.
+
+    ``scaling``: None, or a dict with ``type``
+      ``"linear"``  ``factor``: every frequency divided by it;
+      ``"ntk"``     ``factor``: the base grows so that the slowest pair turns
+                    ``factor`` times slower and the fastest as before;
+      ``"yarn"``    ``factor``, ``original`` (positions the model was trained
+                    on), ``beta_fast`` (32), ``beta_slow`` (1): pairs that turn
+                    more than ``beta_fast`` times over ``original`` positions
+                    keep their frequency, those below ``beta_slow`` turns have
+                    it divided, a linear ramp over the pairs between; ``length``
+                    (1 + 0.1 ln factor) multiplies the elements."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even and at least 2, got {rot_dim}")
+    if not base > 1.0:
+        raise ValueError(f"base must be greater than 1, got {base}")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    if scaling is None:
+        return base ** (-i / rot_dim), 1.0
+    kind, factor = scaling.get("type"), float(scaling.get("factor", 0.0))
+    if kind not in ("linear", "ntk", "yarn"):
+        raise ValueError(f"scaling type must be linear, ntk or yarn, got {kind!r}")
+    if not factor >= 1.0:
+        raise ValueError(f"scaling factor must be at least 1, got {factor}")
+    if kind == "linear":
+        return base ** (-i / rot_dim) / factor, 1.0
+    if kind == "ntk":
+        if rot_dim == 2:
+            return base ** (-i / rot_dim), 1.0
+        return (base * factor ** (rot_dim / (rot_dim - 2))) ** (-i / rot_dim), 1.0
+    original = float(scaling["original"])
+    freq = base ** (-i / rot_dim)
+
+    def pair(turns: float) -> float:  # the pair that makes so many turns over `original` positions
+        return rot_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    lo = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
+    hi = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+    ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+    length = scaling.get("length")
+    return freq / factor * ramp + freq * (1 - ramp), \
+        0.1 * math.log(factor) + 1.0 if length is None else float(length)
+
+
+def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, *,
+                 scaling: Optional[dict] = None, device="cuda") -> torch.Tensor:
+    """fp32 ``[n_positions, rot_dim / 2, 2]``: (cos, sin) of each position and pair."""
+    if n_positions < 1:
+        raise ValueError(f"rotary_table: n_positions must be at least 1, got {n_positions}")
+    freq, length = frequencies(rot_dim, base, scaling)
+    if torch.device(device).type == "cpu":
+        raise RuntimeError("rotary_table: sglang_lite_amd runs only on a ROCm (gfx950) device "
+                           "(there is no CPU path)")
+    freq = freq.to(device)
+    table = torch.empty(n_positions, rot_dim // 2, 2, dtype=torch.float32, device=freq.device)
+    with _lib.on_device(freq):
+        _lib.call("sgl_rotary_table", freq.data_ptr(), length, n_positions, rot_dim, table.data_ptr(),
+                  _lib.stream_of(freq))
+    return table
+
+
+def check_table(table: torch.Tensor, offset: int, dim: int, what: str) -> int:
+    """rot_dim of a table that fits into heads of ``dim`` elements at ``offset``."""
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or \
+            not table.is_contiguous():
+        raise ValueError(f"{what}: table must be a contiguous float32 [positions, pairs, 2], got "
+                         f"{table.dtype} {tuple(table.shape)}")
+    rot = 2 * table.shape[1]
+    if offset < 0 or offset + rot > dim:
+        raise ValueError(f"{what}: {rot} rotated elements at offset {offset} do not fit into {dim}")
+    return rot
+
+
+def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
+           interleaved: bool = False, offset: int = 0, inverse: bool = False,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x`` ``[T, H, D]`` (bf16, f16 or f32; any strides with a dense last
+    dimension) with elements ``[offset, offset + rot_dim)`` of every head turned
+    by ``positions`` (int32 or int64 ``[T]``): pair ``i`` is elements ``i`` and
+    ``i + rot_dim / 2`` of them, or ``2 i`` and ``2 i + 1`` with ``interleaved``.
+    A negative position (a padding row) leaves its row as it is, one behind the
+    table gives NaN.  ``out`` may be ``x`` itself."""
+    if x.dim() != 3:
+        raise ValueError(f"rotary: expected x [T, H, D], got {tuple(x.shape)}")
+    T, H, D = x.shape
+    dt = DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"rotary: x must be bfloat16, float16 or float32, got {x.dtype}")
+    rot = check_table(table, offset, D, "rotary")
+    if positions.dim() != 1 or positions.shape[0] != T:
+        raise ValueError(f"rotary: expected positions [{T}], got {tuple(positions.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"rotary: positions must be int32 or int64, got {positions.dtype}")
+    _lib.require_device(x, table, positions, out, what="rotary")
+    _lib.require_same_device(x, table, positions, out, what="rotary")
+    if x.stride(2) != 1 and D > 1:
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or (out.stride(2) != 1 and D > 1):
+            raise ValueError(f"rotary: out must be {x.dtype} {tuple(x.shape)} with a dense last "
+                             f"dimension, got {out.dtype} {tuple(out.shape)}")
+        if (T > 1 and abs(out.stride(0)) < D) or (H > 1 and abs(out.stride(1)) < D):
+            raise ValueError("rotary: rows of out overlap")
+    if positions.stride(0) != 1:
+        positions = positions.contiguous()
+    with _lib.on_device(x):
+        _lib.call("sgl_rotary", x.data_ptr(), dt, T, H, D, x.stride(0), x.stride(1), table.data_ptr(),
+                  table.shape[0], rot, offset, positions.data_ptr(), positions.dtype == torch.int64,
+                  interleaved, inverse, out.data_ptr(), out.stride(0), out.stride(1),
+                  _lib.stream_of(x))
+    return out
+
+
+__all__ = ["frequencies", "rotary", "rotary_table"]
