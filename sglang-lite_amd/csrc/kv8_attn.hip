@@ -17,9 +17,10 @@
 //     C = D / 16 bytes from C m on, transposes them in registers (v_perm), and
 //     holds the A operands of C tiles of 16 dims (row m of tile j: dim C m + j).
 // A conversion e4m3 -> bf16 (exact) is one instruction for two codes.  The
-// scales are one number for 16 tokens: s_k multiplies the score, s_v the
-// probability, both fp32, before P is rounded to bf16 (relative 2^-9, the only
-// rounding between the codes and the output's own).
+// scales are one number for 16 tokens: s_k multiplies the score, log2 s_v is added
+// to it, so that P carries s_v.  P is rounded to q's type (half a step: 2^-9
+// relative in bf16, 2^-12 in f16), the only rounding between the codes and the
+// output's own.
 #include "sgl_kv8_attn.h"
 
 namespace sgl {
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
     };
 
     // acc += V^T . P^T for the codes v of the step
-    auto accumulate = [&](const uint32_t (*v)[W], const v8bf* p) {
+    auto accumulate = [&](const uint32_t (*v)[W], const typename Op<QT>::V* p) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         uint32_t x0[4], x1[4];
@@ -214,9 +215,9 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
         transpose4(v[4][w], v[5][w], v[6][w], v[7][w], x1);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const v8bf f = cvt8<SGL_BF16>(x0[k], x1[k]);
+          const typename Op<QT>::V f = cvt8<QT>(x0[k], x1[k]);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) acc[c][4 * w + k] = Op<SGL_BF16>::mfma(f, p[c], acc[c][4 * w + k]);
+          for (int c = 0; c < NC; ++c) acc[c][4 * w + k] = Op<QT>::mfma(f, p[c], acc[c][4 * w + k]);
         }
       }
     };
@@ -252,12 +253,22 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
           }
         }
       }
-      v8bf p[NC];
+      // P^T = 2^(s + log2 s_v - m): the value's scale is part of the exponent, so that
+      // P fits f16 as well, and the sum of the probabilities takes it back
+      float kc[2], ev[2], iv[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool there = r.ok[u] && tok + 16 * u < s.len;  // (else its scales may never have been written)
+        kc[u] = there ? r.ks[u] * a.c1 : 0.0f;
+        ev[u] = there ? __builtin_fmaxf(__builtin_amdgcn_logf(r.vs[u]), -100.0f) : 0.0f;
+        iv[u] = __builtin_amdgcn_exp2f(-ev[u]);
+      }
+      typename Op<QT>::V p[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = sc[c][i >> 2][i & 3] * (r.ks[i >> 2] * a.c1);
+        for (int i = 0; i < 8; ++i) f[i] = __builtin_fmaf(sc[c][i >> 2][i & 3], kc[i >> 2], ev[i >> 2]);
         if (!plain) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = (seen[c] >> i) & 1u ? f[i] : NEG_INF;
@@ -265,13 +276,13 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
         float mx = f[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = __builtin_fmaxf(mx, f[i]);
-        // The reference moves only when a score exceeds it by more than 8 (log2
-        // units): any reference gives the same softmax, the probabilities stay
-        // at most 256, and the accumulators are rarely rescaled.
-        if (__ballot(!(mx <= m_run[c] + 8.0f) && mx != NEG_INF)) {
+        // The reference moves only when a weight's exponent exceeds it by more than 6
+        // (log2 units): any reference gives the same softmax, the weights stay at
+        // most 64, and the accumulators are rarely rescaled.
+        if (__ballot(!(mx <= m_run[c] + 6.0f) && mx != NEG_INF)) {
           mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
           mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float next = mx <= m_run[c] + 8.0f ? m_run[c] : __builtin_fmaxf(m_run[c], mx);
+          const float next = mx <= m_run[c] + 6.0f ? m_run[c] : __builtin_fmaxf(m_run[c], mx);
           const float alpha = next == m_run[c] ? 1.0f : __builtin_amdgcn_exp2f(m_run[c] - next);
           m_run[c] = next;
           l_run[c] *= alpha;
@@ -286,14 +297,12 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           f[i] = __builtin_amdgcn_exp2f(f[i] - ref);
-          l += f[i];
-          f[i] *= r.vs[i >> 2];
-          if (!plain) f[i] = (seen[c] >> i) & 1u ? f[i] : 0.0f;  // (a scale that was never written)
+          l = __builtin_fmaf(f[i], iv[i >> 2], l);
         }
         l_run[c] += l;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pk2_bf16(f[2 * i], f[2 * i + 1]);
-        p[c] = __builtin_bit_cast(v8bf, u4v{w[0], w[1], w[2], w[3]});
+        for (int i = 0; i < 4; ++i) w[i] = pack2<QT>(f[2 * i], f[2 * i + 1]);
+        p[c] = __builtin_bit_cast(typename Op<QT>::V, u4v{w[0], w[1], w[2], w[3]});
       }
       if (!plain) {
         // What no row sees must not reach the product: keys behind the last
@@ -417,7 +426,9 @@ void launch_few(const Kv8AttnArgs& a, hipStream_t st) {
 
 template <int QT>
 void launch_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
-  if (a.D <= 64)
+  if (p.row_tile == 128)
+    launch_kv8_prefill(a, p, QT, st);
+  else if (a.D <= 64)
     p.row_tile == 16 ? launch_few<64, 1, QT>(a, st) : launch_few<64, 2, QT>(a, st);
   else if (a.D <= 128)
     p.row_tile == 16 ? launch_few<128, 1, QT>(a, st) : launch_few<128, 2, QT>(a, st);
@@ -461,7 +472,7 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
               "kv8_attn: misaligned cache or output");
   const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, sgl::device_cu_count());
   const size_t need = (size_t)(2 * p.wgs * p.row_tile * (D + 2)) * sizeof(float);
-  if (!workspace || workspace_bytes < need) {
+  if (need && (!workspace || workspace_bytes < need)) {
     sgl::set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
     return SGL_ERR_WORKSPACE;
   }

@@ -171,4 +171,7 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
   }
 }
 
+// kv8_prefill.hip: row tiles of 128.  plan.wgs == 0: a workgroup takes a whole item.
+void launch_kv8_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& plan, int dtype, hipStream_t stream);
+
 }  // namespace sgl

@@ -256,7 +256,8 @@ SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {
 // ---- attention over the 8-bit cache: rows of a tile, and the workgroups that
 // share the line of key tiles.
 struct Kv8AttnPlan {
-  int64_t row_tile, wgs;
+  int64_t row_tile;  // 16 or 32: kv8_attn.hip; 128: kv8_prefill.hip
+  int64_t wgs;       // 0: a workgroup takes a whole item
 };
 // the most items (row tile, kv head) that T queries of B sequences make
 SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t row_tile) {
@@ -264,8 +265,8 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
   return Hkv * (tiles < most ? tiles : most);
 }
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t cus) {
-  (void)Hkv;
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
+  if (rows > 32) return {128, kv8_attn_items(T, B, Hkv, G, 128) >= 2 * cus ? 0 : 2 * cus};
   return {D <= 128 && rows > 16 ? 32 : 16, 2 * cus};
 }
 

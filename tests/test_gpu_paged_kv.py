@@ -415,6 +415,19 @@ def test_chunk_attention_matches_float64(gpu, new, lens, Hq, Hkv, D, page, block
     _check_attn(c, q, lens, cu, causal=causal, window=window, sink=s)
 
 
+@pytest.mark.parametrize("new,lens,window,D,dtype", [
+    ([513], [700], 0, 64, torch.bfloat16),
+    ([1, 500, 20], [90, 500, 333], 100, 128, torch.float16),
+])
+def test_chunks_of_many_row_tiles(gpu, new, lens, window, D, dtype):
+    """Enough row tiles to fill the device without sharing any."""
+    c = _filled(gpu, lens, 8, D, 32, 32, seed=D)
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], 128, D, dtype, 8)
+    s = (np.random.default_rng(2).standard_normal(128) * 2).astype(np.float32)
+    _check_attn(c, q, lens, cu, window=window, sink=s)
+
+
 def test_attention_leaves_rows_behind_the_last_sequence(gpu):
     c = _filled(gpu, [40, 70], 2, 64, 16, 16, seed=2)
     q = _queries(gpu, 20, 4, 64, torch.bfloat16, 3)
