@@ -26,6 +26,7 @@
 namespace sgl {
 namespace {
 
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
@@ -79,13 +80,11 @@ template <int DP>
 struct Codes {
   uint4 k[2][DP / 64];
   uint32_t v[8][DP / 64];  // tokens as above, C = DP / 16 bytes each
-  float ks[2], vs[2];
-  bool ok[2];  // the granule lies on a page of the cache
 };
 
 // DP: head dim rounded up to 64, 128 or 256; NC: 16-row column tiles
 template <int DP, int NC, int QT>
-__global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
   constexpr int RT = 16 * NC, KI = DP / 64, C = DP / 16, W = C / 4;
   __shared__ __align__(16) float sAcc[kWaves][16][DP + 4];
   __shared__ float sM[kWaves][16], sL[kWaves][16];
@@ -93,29 +92,14 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
   const int m = lane & 15, g = lane >> 4;
   const float NEG_INF = -__builtin_huge_valf();
 
-  const int64_t total = kv8_total<RT, kTile>(a);
-  const int64_t per = (total + a.wgs - 1) / a.wgs;
-  int64_t x = (int64_t)blockIdx.x * per;
-  const int64_t end = x + per < total ? x + per : total;
-  if (x >= end) return;
-  Kv8Place at = kv8_find<RT, kTile, false>(a, x);
-  int b = at.b;
-  int64_t base = at.before;
-  const bool in_v = C * m < a.D;
-
-  while (x < end) {
-    const Kv8Seq s = kv8_seq<RT, kTile>(a, b);
-    const int64_t mine = (int64_t)s.tiles * s.row_tiles * a.Hkv;
-    if (x >= base + mine) {
-      base += mine;
-      ++b;
-      continue;
-    }
-    const int off = (int)(x - base);
-    const int item = off / s.tiles, t0 = off - item * s.tiles;
-    const int64_t left = end - x;
-    const int t1 = s.tiles - t0 < left ? s.tiles : t0 + (int)left;
-    const int rt = item / a.Hkv, head = item - rt * a.Hkv;
+  int head, part;
+  kv8_wg_at(a, (int)blockIdx.x, &head, &part);
+  Kv8Walk<RT, kTile> walk;
+  if (!walk.start(a, part)) return;
+  Kv8Segment seg;
+  while (walk.next(a, seg)) {
+    const Kv8Seq& s = seg.s;
+    const int b = seg.b, rt = seg.rt, t0 = seg.t0, t1 = seg.t1;
     const int rows = s.n * a.G - rt * RT;  // valid rows of the tile (may be more than RT)
 
     // the rows: their queries and what they see
@@ -162,52 +146,72 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
 
     const int32_t* table = a.pages + (int64_t)b * a.row_pages;
     const int pmask = (1 << a.page_shift) - 1;
-    const int first = (s.tile0 + t0) * kTile + 32 * wave, stop = (s.tile0 + t1) * kTile;
-    const int last_tok = s.len > 0 ? s.len - 1 : 0;
+    const int first = (s.tile0 + t0) * kTile + 32 * wave;
+    int stop = (s.tile0 + t1) * kTile;
+    stop = stop < s.len ? stop : s.len;
+    const int steps = first < stop ? (stop - first + kTile - 1) / kTile : 0;  // step i: tokens first + i kTile on
 
-    auto load = [&](int tok, Codes<DP>& r) {
+    // Pages and scales of 32 steps at a time: lane l has granule l & 1 of step l >> 1.
+    // Loaded a batch ahead, so that no step waits for its table entry.
+    struct Batch {
+      int page;  // 0 where there is none
+      float ks, vs;
+      bool ok;
+    };
+    auto load_pages = [&](int batch) __attribute__((always_inline)) {
+      Batch o;
+      const int t = first + (32 * batch + (lane >> 1)) * kTile + 16 * (lane & 1);
+      const int page = table[(t < s.len ? t : s.len - 1) >> a.page_shift];
+      o.ok = t < s.len && page >= 0 && page < a.n_pages;
+      o.page = o.ok ? page : 0;
+      return o;
+    };
+    auto load_scales = [&](int batch, Batch& o) __attribute__((always_inline)) {
+      const int t = first + (32 * batch + (lane >> 1)) * kTile + 16 * (lane & 1);
+      const int64_t piece = (((int64_t)o.page * a.Hkv + head) << (a.page_shift - a.block_shift)) +
+                            ((t & pmask) >> a.block_shift);
+      o.ks = a.ks[piece];
+      o.vs = a.vs[piece];
+    };
+
+    // lane offsets; dims behind D repeat others of the same token, whose scores
+    // meet zeros of q and whose outputs are not stored
+    int kd[KI], vd;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) kd[i] = m * a.D + (64 * i + 16 * g < a.D ? 64 * i + 16 * g : 0);
+    vd = 4 * g * a.D + (C * m < a.D ? C * m : 0);
+    auto load = [&](int i, int pages, Codes<DP>& r) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        int p = tok + 16 * u;
-        p = p < s.len ? p : last_tok & ~15;  // behind the last key: any granule that is there
-        const int page = table[p >> a.page_shift];
-        r.ok[u] = page >= 0 && page < a.n_pages && s.len > 0;
-        const int64_t line = (int64_t)(r.ok[u] ? page : 0) * a.Hkv + head;
-        const int spot = p & pmask;
-        const int64_t piece = (line << (a.page_shift - a.block_shift)) + (spot >> a.block_shift);
-        r.ks[u] = a.ks[piece];
-        r.vs[u] = a.vs[piece];
-        const int64_t row = ((line << a.page_shift) + spot) * a.D;
-        const uint8_t* kp = a.kc + row + m * a.D + 16 * g;
+        const int page = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + u);
+        const int spot = (first + i * kTile + 16 * u) & pmask;
+        const int64_t row = ((((int64_t)page * a.Hkv + head) << a.page_shift) + spot) * a.D;
+        const uint8_t* kp = a.kc + row;
+        const uint8_t* vp = a.vc + row;
 #pragma unroll
-        for (int i = 0; i < KI; ++i)
-          r.k[u][i] = 64 * i + 16 * g < a.D ? *reinterpret_cast<const uint4*>(kp + 64 * i) : make_uint4(0, 0, 0, 0);
-        const uint8_t* vp = a.vc + row + 4 * g * a.D + C * m;
+        for (int k = 0; k < KI; ++k) r.k[u][k] = ld16_stream(kp + (uint32_t)kd[k]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int w = 0; w < W; ++w) r.v[4 * u + j][w] = 0;
-          if (in_v) {
-            if constexpr (W == 1) {
-              r.v[4 * u + j][0] = *reinterpret_cast<const uint32_t*>(vp + j * a.D);
-            } else if constexpr (W == 2) {
-              const uint2 y = *reinterpret_cast<const uint2*>(vp + j * a.D);
-              r.v[4 * u + j][0] = y.x;
-              r.v[4 * u + j][1] = y.y;
-            } else {
-              const uint4 y = *reinterpret_cast<const uint4*>(vp + j * a.D);
-              r.v[4 * u + j][0] = y.x;
-              r.v[4 * u + j][1] = y.y;
-              r.v[4 * u + j][2] = y.z;
-              r.v[4 * u + j][3] = y.w;
-            }
+          const uint8_t* at = vp + j * a.D + (uint32_t)vd;
+          if constexpr (W == 1) {
+            r.v[4 * u + j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(at));
+          } else if constexpr (W == 2) {
+            const u2v y = __builtin_nontemporal_load(reinterpret_cast<const u2v*>(at));
+            r.v[4 * u + j][0] = y.x;
+            r.v[4 * u + j][1] = y.y;
+          } else {
+            const uint4 y = ld16_stream(at);
+            r.v[4 * u + j][0] = y.x;
+            r.v[4 * u + j][1] = y.y;
+            r.v[4 * u + j][2] = y.z;
+            r.v[4 * u + j][3] = y.w;
           }
         }
       }
     };
 
     // acc += V^T . P^T for the codes v of the step
-    auto accumulate = [&](const uint32_t (*v)[W], const typename Op<QT>::V* p) {
+    auto accumulate = [&](const uint32_t (*v)[W], const typename Op<QT>::V* p) __attribute__((always_inline)) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         uint32_t x0[4], x1[4];
@@ -222,8 +226,19 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
       }
     };
 
-    auto step = [&](int tok, Codes<DP>& r) {
-      if (tok >= s.len) return;
+    float kcs, evs, ivs;  // of the batch: score scale, log2 of the value scale, its reciprocal
+    uint64_t okm;
+    auto use = [&](const Batch& o) __attribute__((always_inline)) {
+      kcs = o.ok ? o.ks * a.c1 : 0.0f;  // (what was never written may hold anything)
+      evs = o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.vs), -100.0f) : 0.0f;
+      ivs = __builtin_amdgcn_exp2f(-evs);
+      okm = __ballot(o.ok);
+    };
+    auto lane_f = [&](float v, int l) { return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), l)); };
+
+    auto step = [&](int at, Codes<DP>& r) __attribute__((always_inline)) {
+      const int tok = first + at * kTile, l0 = 2 * (at & 31);
+      const uint32_t ok = (uint32_t)(okm >> l0) & 3u;
       v4f sc[NC][2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -239,7 +254,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
           }
         }
       }
-      const bool plain = tok + 32 <= all_hi && tok >= all_lo && r.ok[0] && r.ok[1];
+      const bool plain = tok + 32 <= all_hi && tok >= all_lo && ok == 3;
       uint32_t seen[NC];  // bit 4 u + i: the row sees token 16 u + 4 g + i
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -249,7 +264,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = tok + 16 * (i >> 2) + 4 * g + (i & 3);
-            if (key < hi[c] && key >= lo[c] && key < s.len && r.ok[i >> 2]) seen[c] |= 1u << i;
+            if (key < hi[c] && key >= lo[c] && key < s.len && ((ok >> (i >> 2)) & 1u)) seen[c] |= 1u << i;
           }
         }
       }
@@ -258,10 +273,9 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
       float kc[2], ev[2], iv[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bool there = r.ok[u] && tok + 16 * u < s.len;  // (else its scales may never have been written)
-        kc[u] = there ? r.ks[u] * a.c1 : 0.0f;
-        ev[u] = there ? __builtin_fmaxf(__builtin_amdgcn_logf(r.vs[u]), -100.0f) : 0.0f;
-        iv[u] = __builtin_amdgcn_exp2f(-ev[u]);
+        kc[u] = lane_f(kcs, l0 + u);
+        ev[u] = lane_f(evs, l0 + u);
+        iv[u] = lane_f(ivs, l0 + u);
       }
       typename Op<QT>::V p[NC];
 #pragma unroll
@@ -311,7 +325,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
         uint32_t nan[8][W], any = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool there = tok + 16 * (j >> 2) + 4 * g + (j & 3) < s.len && r.ok[j >> 2];
+          const bool there = tok + 16 * (j >> 2) + 4 * g + (j & 3) < s.len && ((ok >> (j >> 2)) & 1u);
 #pragma unroll
           for (int w = 0; w < W; ++w) {
             const uint32_t v = there ? r.v[j][w] : 0u;
@@ -348,15 +362,29 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
       accumulate(r.v, p);
     };
 
-    Codes<DP> r0, r1;
-    if (s.len > 0) {
-      load(first, r0);
-      for (int tok = first; tok < stop; tok += 2 * kTile) {
-        load(tok + kTile, r1);
-        step(tok, r0);
-        if (tok + kTile >= stop) break;
-        load(tok + 2 * kTile, r0);
-        step(tok + kTile, r1);
+    if (steps > 0) {
+      // The next step's codes are on their way while one is worked on (two steps ahead
+      // was no faster: 128 sequences up to 16384 keys 200 us against 197).
+      // Loads are never under a branch (behind the last step they repeat it), so that
+      // the waits count them instead of draining them.
+      Batch now = load_pages(0), ahead = load_pages(1);
+      load_scales(0, now);
+      Codes<DP> r0, r1;
+      load(0, now.page, r0);
+      use(now);
+      for (int i = 0; i < steps; i += 2) {
+        if ((i & 31) == 0 && i > 0) {
+          now = ahead;
+          use(now);
+          ahead = load_pages((i >> 5) + 1);
+        }
+        if ((i & 31) == 16) load_scales((i >> 5) + 1, ahead);
+        load(i + 1 < steps ? i + 1 : i, now.page, r1);
+        step(i, r0);
+        if (i + 1 >= steps) break;
+        const int n = i + 2 < steps ? i + 2 : i + 1;
+        load(n, (n & 31) == 0 ? ahead.page : now.page, r0);
+        step(i + 1, r1);
       }
     }
 
@@ -413,15 +441,14 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_attn_few_kernel(const Kv8Attn
         }
       }
     }
-    x += t1 - t0;
   }
 }
 
 template <int DP, int NC, int QT>
 void launch_few(const Kv8AttnArgs& a, hipStream_t st) {
-  kv8_attn_few_kernel<DP, NC, QT><<<a.wgs, 64 * kWaves, 0, st>>>(a);
+  kv8_attn_few_kernel<DP, NC, QT><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
   const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, 16 * NC);
-  kv8_merge_kernel<16 * NC, kTile, QT><<<(unsigned)items, 256, 0, st>>>(a);
+  kv8_merge_kernel<16 * NC, kTile, QT><<<(unsigned)(items * 4 * NC), 256, 0, st>>>(a);
 }
 
 template <int QT>
@@ -444,7 +471,7 @@ extern "C" {
 size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D) {
   if (T < 0 || B < 0 || Hkv < 1 || G < 1 || D < 16) return 0;
   const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, sgl::device_cu_count());
-  return (size_t)(2 * p.wgs * p.row_tile * (D + 2)) * sizeof(float);
+  return sgl::kv8_attn_workspace(p, Hkv, D);
 }
 
 int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T, int64_t B,
@@ -471,14 +498,14 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
   SGL_REQUIRE(sgl::aligned(k_codes, 16) && sgl::aligned(v_codes, 16) && sgl::aligned(out, 16),
               "kv8_attn: misaligned cache or output");
   const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, sgl::device_cu_count());
-  const size_t need = (size_t)(2 * p.wgs * p.row_tile * (D + 2)) * sizeof(float);
+  const size_t need = sgl::kv8_attn_workspace(p, Hkv, D);
   if (need && (!workspace || workspace_bytes < need)) {
     sgl::set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
     return SGL_ERR_WORKSPACE;
   }
   SGL_REQUIRE(sgl::aligned(workspace, 16), "kv8_attn: workspace must be 16-byte aligned");
   const int64_t items = sgl::kv8_attn_items(T, B, Hkv, G, p.row_tile);
-  SGL_REQUIRE_SUPPORTED(items * ((row_pages * page_size + 127) / 128) < (1ll << 31),
+  SGL_REQUIRE_SUPPORTED(items * ((row_pages * page_size + 63) / 64 + sgl::kItemCost) < (1ll << 31),
                         "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)items,
                         (long long)(row_pages * page_size));
   sgl::Kv8AttnArgs a;
@@ -506,9 +533,9 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
   a.c1 = softmax_scale * sgl::kLog2e;
   a.window = window > 0x7FFFFFFF ? 0 : (int)window;
   a.causal = causal != 0;
-  a.wgs = (int)p.wgs;
+  a.parts = (int)p.parts;
   a.ws_acc = (float*)workspace;
-  a.ws_ml = (float*)workspace + 2 * p.wgs * p.row_tile * D;
+  a.ws_ml = (float*)workspace + 2 * p.parts * Hkv * p.row_tile * D;
   if (dtype == SGL_BF16)
     sgl::launch_attn<SGL_BF16>(a, p, (hipStream_t)stream);
   else

@@ -77,50 +77,33 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
   const int c32 = lane & 31, g2 = lane >> 5;
   const float NEG_INF = -__builtin_huge_valf();
 
-  int64_t x = 0, end = 1;
-  Kv8Place at;
+  if (threadIdx.x < 2) sNan[threadIdx.x] = 0;
+  int head, part = 0;
+  Kv8Walk<RT, kKeys> walk;
+  Kv8Segment seg;
   if constexpr (SPLIT) {
-    const int64_t total = kv8_total<RT, kKeys>(a);
-    const int64_t per = (total + a.wgs - 1) / a.wgs;
-    x = (int64_t)blockIdx.x * per;
-    end = x + per < total ? x + per : total;
-    if (x >= end) return;
-    at = kv8_find<RT, kKeys, false>(a, x);
+    kv8_wg_at(a, (int)blockIdx.x, &head, &part);
+    if (!walk.start(a, part)) return;
   } else {
     // the last row tiles, which see the most keys, first; the heads go round
     // fastest, so that a head's workgroups meet on one XCD and its L2
-    x = items - 1 - (int64_t)blockIdx.x;
-    end = x + 1;
-    at = kv8_find<RT, kKeys, true>(a, x);
-    if (at.b >= a.B) return;
+    const int64_t item = items - 1 - (int64_t)blockIdx.x;
+    head = (int)(item % a.Hkv);
+    walk.c = kv8_chunk<RT, kKeys>(a, 0);
+    const Kv8Place at = kv8_find<RT, kKeys, true>(a, walk.c, item / a.Hkv);
+    if (at.l < 0) return;
+    seg.s = kv8_lane<RT, kKeys>(a, walk.c, at.l);
+    seg.b = walk.c.b0 + at.l;
+    seg.rt = (int)(item / a.Hkv - at.rts);
+    seg.t0 = 0;
+    seg.t1 = seg.s.tiles;
   }
-  if (threadIdx.x < 2) sNan[threadIdx.x] = 0;
-
-  int b = at.b;
-  int64_t base = at.before;
-  while (x < end) {
-    const Kv8Seq s = kv8_seq<RT, kKeys>(a, b);
-    int item, t0 = 0, t1 = s.tiles;
-    if constexpr (SPLIT) {
-      const int64_t mine = (int64_t)s.tiles * s.row_tiles * a.Hkv;
-      if (x >= base + mine) {
-        base += mine;
-        ++b;
-        continue;
-      }
-      const int off = (int)(x - base);
-      item = off / s.tiles;
-      t0 = off - item * s.tiles;
-      const int64_t left = end - x;
-      t1 = s.tiles - t0 < left ? s.tiles : t0 + (int)left;
-    } else {
-      item = (int)(x - at.items);
-    }
-    const int rt = item / a.Hkv, head = item - rt * a.Hkv;
+  for (bool more = SPLIT ? walk.next(a, seg) : true; more; more = SPLIT ? walk.next(a, seg) : false) {
+    const Kv8Seq& s = seg.s;
+    const int b = seg.b, rt = seg.rt, t0 = seg.t0, t1 = seg.t1;
     const int rows = s.n * a.G - rt * RT;
     const bool whole = t0 == 0 && t1 == s.tiles;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0);
-    const int64_t next = x + (t1 - t0);
 
     // this lane's row, and what it sees
     const int r = 32 * wave + c32;
@@ -451,18 +434,17 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         if (g2 == 0) *reinterpret_cast<float2*>(a.ws_ml + (slot * RT + r) * 2) = make_float2(m_run, l_run);
       }
     }
-    x = SPLIT ? next : end;
   }
 }
 
 template <int DP, int QT>
 void launch_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
   const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, 128);
-  if (p.wgs == 0) {
+  if (p.parts == 0) {
     kv8_prefill_kernel<DP, QT, 4, false><<<(unsigned)items, 256, 0, st>>>(a, items);
   } else {
-    kv8_prefill_kernel<DP, QT, 4, true><<<a.wgs, 256, 0, st>>>(a, items);
-    kv8_merge_kernel<128, kKeys, QT><<<(unsigned)items, 256, 0, st>>>(a);
+    kv8_prefill_kernel<DP, QT, 4, true><<<a.parts * a.Hkv, 256, 0, st>>>(a, items);
+    kv8_merge_kernel<128, kKeys, QT><<<(unsigned)(items * 32), 256, 0, st>>>(a);
   }
 }
 

@@ -4,14 +4,17 @@
 //
 // A sequence's n queries and the G query heads of one kv head make n G rows
 // (row r: query r / G, head r % G), cut into row tiles.  An item is (sequence,
-// row tile, kv head); its keys are cut into key tiles.  Items follow each other
-// by sequence, row tile, head; the key tiles of all items make one line, which
-// the workgroups share evenly: each takes `per` tiles of it in order.  So a
-// batch of ragged lengths keeps every CU as busy as an even one, and nothing on
-// the host needs to know the lengths.  An item inside one workgroup is written
-// out; of one that several share, each leaves its unnormalised sums, reference
-// point and weight in the workspace (at most two such parts a workgroup, one at
-// either end of its line), and the merge joins them in the order of the line.
+// row tile, kv head); its keys are cut into key tiles.  For each kv head the key
+// tiles of all items, one sequence after the other, make one line, which `parts`
+// workgroups share evenly: so a batch of ragged lengths keeps every CU as busy as
+// an even one, and nothing on the host needs to know the lengths.  An item also
+// takes kItemCost tiles' room on the line, for its start and end.  The
+// workgroups of the same part of the lines, which read the same pages, run on
+// one XCD at about the same time.
+// An item inside one workgroup is written out; of one that several share, each
+// leaves its unnormalised sums, reference point and weight in the workspace (at
+// most two such parts a workgroup, one at either end of its stretch), and the
+// merge joins them in the order of the line.
 #pragma once
 
 #include "sgl_kv8.h"
@@ -38,11 +41,14 @@ struct Kv8AttnArgs {
   float c1;     // softmax scale in log2 units
   int window;   // keys a query sees, itself included; 0: all
   bool causal;
-  int wgs;
-  float* ws_acc;  // [2 wgs][row tile][D]
-  float* ws_ml;   // [2 wgs][row tile][2]: reference point (log2 units), sum
+  int parts;      // workgroups of a kv head's line; 0: one workgroup an item
+  float* ws_acc;  // [2 parts Hkv][row tile][D]
+  float* ws_ml;   // [2 parts Hkv][row tile][2]: reference point (log2 units), sum
 };
 
+constexpr int kItemCost = 2;  // key tiles
+
+// A sequence as the line sees it.
 struct Kv8Seq {
   int row0, n, len;  // first query row, queries, keys
   int tile0, tiles;  // key tiles: first, number (at least one, so that empty rows are written)
@@ -50,128 +56,226 @@ struct Kv8Seq {
 };
 
 template <int RT, int TT>
-__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int b) {
-  const SeqRows r = seq_rows(a.cu, b, a.T);
-  const int cap = a.row_pages << a.page_shift;
-  int len = a.lens[b];
-  len = len < 0 ? 0 : len > cap ? cap : len;
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n, int len) {
   int lo = 0;
   if (a.causal && a.window > 0) {
-    const int64_t first = (int64_t)len - r.n - a.window + 1;
+    const int64_t first = (int64_t)len - n - a.window + 1;
     lo = first > 0 ? (int)first : 0;
   }
   Kv8Seq s;
-  s.row0 = r.first;
-  s.n = r.n;
+  s.row0 = row0;
+  s.n = n;
   s.len = len;
   s.tile0 = lo / TT;
   const int tiles = (len + TT - 1) / TT - s.tile0;
   s.tiles = tiles > 0 ? tiles : 1;
-  s.row_tiles = (r.n * a.G + RT - 1) / RT;
+  s.row_tiles = (n * a.G + RT - 1) / RT;
   return s;
 }
 
-// Where something lies on the line.
-struct Kv8Place {
-  int b;       // sequence; B: behind the last
-  int64_t before;  // key tiles of the sequences before
-  int items;   // items of the sequences before
+// 64 sequences from b0 on, one a lane.
+struct Kv8Chunk {
+  int b0, row0, n, len;
+  int room, rooms;  // places on the line: of this sequence, of those up to and with it
+  int rts;          // row tiles of the sequences up to and with it
 };
 
-// The line's length.
 template <int RT, int TT>
-__device__ __forceinline__ int64_t kv8_total(const Kv8AttnArgs& a) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int c = 0;
-    if (b0 + lane < a.B) {
-      const Kv8Seq s = kv8_seq<RT, TT>(a, b0 + lane);
-      c = s.tiles * s.row_tiles * a.Hkv;
-    }
-    total += __builtin_amdgcn_readlane(wave_incl_scan(c), 63);
+__device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
+  const int b = b0 + (int)(threadIdx.x & 63);
+  Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0};
+  int rts = 0;
+  if (b < a.B) {
+    const int len = a.lens[b], cap = a.row_pages << a.page_shift;
+    const SeqRows r = seq_rows(a.cu, b, a.T);
+    c.row0 = r.first;
+    c.n = r.n;
+    c.len = len < 0 ? 0 : len > cap ? cap : len;
+    const Kv8Seq s = kv8_seq<RT, TT>(a, c.row0, c.n, c.len);
+    rts = s.row_tiles;
+    c.room = rts * (s.tiles + kItemCost);
   }
+  c.rooms = wave_incl_scan(c.room);
+  c.rts = wave_incl_scan(rts);
+  return c;
+}
+
+template <int RT, int TT>
+__device__ __forceinline__ Kv8Seq kv8_lane(const Kv8AttnArgs& a, const Kv8Chunk& c, int l) {
+  return kv8_seq<RT, TT>(a, __builtin_amdgcn_readlane(c.row0, l), __builtin_amdgcn_readlane(c.n, l),
+                         __builtin_amdgcn_readlane(c.len, l));
+}
+
+// Length of a kv head's line; c: the batch's first 64 sequences.
+template <int RT, int TT>
+__device__ __forceinline__ int64_t kv8_total(const Kv8AttnArgs& a, const Kv8Chunk& c) {
+  int64_t total = __builtin_amdgcn_readlane(c.rooms, 63);
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(kv8_chunk<RT, TT>(a, b0).rooms, 63);
   return total;
 }
 
-// The sequence that holds tile x of the line (BY_ITEM: item x).
-template <int RT, int TT, bool BY_ITEM>
-__device__ __forceinline__ Kv8Place kv8_find(const Kv8AttnArgs& a, int64_t x) {
-  const int lane = threadIdx.x & 63;
-  Kv8Place at = {0, 0, 0};
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int c = 0, k = 0;
-    if (b0 + lane < a.B) {
-      const Kv8Seq s = kv8_seq<RT, TT>(a, b0 + lane);
-      k = s.row_tiles * a.Hkv;
-      c = s.tiles * k;
-    }
-    const int ci = wave_incl_scan(c), ki = wave_incl_scan(k);
-    const uint64_t past = __ballot(BY_ITEM ? at.items + ki > x : at.before + ci > x);
+// The sequence that holds place x of the line (BY_TILE: row tile x): lane `l` of
+// chunk c, and what lies before the sequence.  l < 0: behind the last.
+struct Kv8Place {
+  int l;
+  int64_t room;  // places before
+  int64_t rts;   // row tiles before
+};
+template <int RT, int TT, bool BY_TILE>
+__device__ __forceinline__ Kv8Place kv8_find(const Kv8AttnArgs& a, Kv8Chunk& c, int64_t x) {
+  Kv8Place at = {-1, 0, 0};
+  for (;;) {
+    const uint64_t past = __ballot(BY_TILE ? at.rts + c.rts > x : at.room + c.rooms > x);
     if (past) {
-      const int l = __builtin_ctzll(past);
-      at.b = b0 + l;
-      at.before += __builtin_amdgcn_readlane(ci, l) - __builtin_amdgcn_readlane(c, l);
-      at.items += __builtin_amdgcn_readlane(ki, l) - __builtin_amdgcn_readlane(k, l);
+      at.l = __builtin_ctzll(past);
+      if (at.l > 0) {
+        at.room += __builtin_amdgcn_readlane(c.rooms, at.l - 1);
+        at.rts += __builtin_amdgcn_readlane(c.rts, at.l - 1);
+      }
       return at;
     }
-    at.before += __builtin_amdgcn_readlane(ci, 63);
-    at.items += __builtin_amdgcn_readlane(ki, 63);
+    at.room += __builtin_amdgcn_readlane(c.rooms, 63);
+    at.rts += __builtin_amdgcn_readlane(c.rts, 63);
+    if (c.b0 + 64 >= a.B) return at;
+    c = kv8_chunk<RT, TT>(a, c.b0 + 64);
   }
-  at.b = a.B;
-  return at;
 }
+
+// Workgroup of a kv head's part, and back: the heads of a part follow each other
+// on one XCD (workgroups go round the eight in order; parts is a multiple of 8).
+__device__ __forceinline__ int kv8_wg(const Kv8AttnArgs& a, int head, int part) {
+  return ((part >> 3) * a.Hkv + head) * 8 + (part & 7);
+}
+__device__ __forceinline__ void kv8_wg_at(const Kv8AttnArgs& a, int wg, int* head, int* part) {
+  const int k = wg >> 3, p = k / a.Hkv;
+  *head = k - p * a.Hkv;
+  *part = 8 * p + (wg & 7);
+}
+
+// A stretch of an item's key tiles that one workgroup takes.
+struct Kv8Segment {
+  Kv8Seq s;
+  int b, rt;   // sequence, row tile
+  int t0, t1;  // key tiles, from the item's first
+};
+
+// Walks over the segments of the places [x, end) of a line.
+template <int RT, int TT>
+struct Kv8Walk {
+  Kv8Chunk c;
+  int64_t x, end, base;
+  int l;
+
+  __device__ __forceinline__ bool start(const Kv8AttnArgs& a, int part) {
+    c = kv8_chunk<RT, TT>(a, 0);
+    const int64_t total = kv8_total<RT, TT>(a, c), per = (total + a.parts - 1) / a.parts;
+    x = (int64_t)part * per;
+    end = x + per < total ? x + per : total;
+    if (x >= end) return false;
+    const Kv8Place at = kv8_find<RT, TT, false>(a, c, x);
+    base = at.room;
+    l = at.l;
+    return true;
+  }
+  // The next segment; false: none left.
+  __device__ __forceinline__ bool next(const Kv8AttnArgs& a, Kv8Segment& g) {
+    while (x < end) {
+      const int room = __builtin_amdgcn_readlane(c.room, l);
+      if (x >= base + room) {
+        base += room;
+        if (++l == 64) {
+          c = kv8_chunk<RT, TT>(a, c.b0 + 64);
+          l = 0;
+        }
+        continue;
+      }
+      g.s = kv8_lane<RT, TT>(a, c, l);
+      g.b = c.b0 + l;
+      const int size = g.s.tiles + kItemCost, off = (int)(x - base);
+      g.rt = off / size;
+      const int at = off - g.rt * size;
+      const int64_t left = end - x;
+      const int to = size - at < left ? size : at + (int)left;
+      x += to - at;
+      g.t0 = at > kItemCost ? at - kItemCost : 0;
+      g.t1 = to - kItemCost;
+      if (g.t1 > g.t0) return true;
+    }
+    return false;
+  }
+};
 
 template <int QT>
 __device__ __forceinline__ uint32_t kv8_out2(float a, float b) {
   return pack2<QT>(a, b);
 }
 
-// Items that several workgroups share, one workgroup each: 256 threads.
+// The items that several workgroups share.  One wavefront a row (four a workgroup,
+// RT / 4 workgroups an item): lane p has part p's reference and weight, then all
+// lanes go over the parts' sums, several loads in flight.
 template <int RT, int TT, int QT>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
-  const int64_t total = kv8_total<RT, TT>(a);
-  const int64_t per = (total + a.wgs - 1) / a.wgs;
-  const Kv8Place at = kv8_find<RT, TT, true>(a, (int64_t)blockIdx.x);
-  if (at.b >= a.B) return;
-  const Kv8Seq s = kv8_seq<RT, TT>(a, at.b);
-  const int item = (int)blockIdx.x - at.items;
-  const int64_t xs = at.before + (int64_t)item * s.tiles, xe = xs + s.tiles;
-  const int wa = (int)(xs / per), wb = (int)((xe - 1) / per);
-  if (wa == wb) return;
-  const int rt = item / a.Hkv, head = item - rt * a.Hkv;
-  const int rows = s.n * a.G - rt * RT;
-  const int chunks = a.D >> 3;
-  for (int i = threadIdx.x; i < RT * chunks; i += 256) {
-    const int r = i / chunks, d = (i - r * chunks) << 3;
-    if (r >= rows) return;
-    const int row = rt * RT + r, t = row / a.G, h = head * a.G + (row - t * a.G);
-    float M = -__builtin_huge_valf();
-    for (int w = wa; w <= wb; ++w) M = __builtin_fmaxf(M, a.ws_ml[((int64_t)(2 * w + (w == wa)) * RT + r) * 2]);
-    const float ref = M == -__builtin_huge_valf() ? 0.0f : M;
-    float l = a.sink ? __builtin_amdgcn_exp2f(a.sink[h] * kLog2e - ref) : 0.0f;
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-    for (int w = wa; w <= wb; ++w) {
-      const int64_t slot = (int64_t)(2 * w + (w == wa)) * RT + r;
-      const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + slot * 2);
-      const float4* p = reinterpret_cast<const float4*>(a.ws_acc + slot * a.D + d);
-      const float4 x = p[0], y = p[1];
-      const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-      l += ml.y * f;
-      acc[0] += x.x * f; acc[1] += x.y * f; acc[2] += x.z * f; acc[3] += x.w * f;
-      acc[4] += y.x * f; acc[5] += y.y * f; acc[6] += y.z * f; acc[7] += y.w * f;
-    }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  Kv8Chunk c = kv8_chunk<RT, TT>(a, 0);
+  const int64_t total = kv8_total<RT, TT>(a, c), per = (total + a.parts - 1) / a.parts;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = blockIdx.x / (RT / 4);
+  const int head = (int)(item % a.Hkv);
+  const Kv8Place at = kv8_find<RT, TT, true>(a, c, item / a.Hkv);
+  if (at.l < 0) return;
+  const Kv8Seq s = kv8_lane<RT, TT>(a, c, at.l);
+  const int rt = (int)(item / a.Hkv - at.rts);
+  const int64_t xs = at.room + (int64_t)rt * (s.tiles + kItemCost) + kItemCost;
+  const int pa = (int)(xs / per), pb = (int)((xs + s.tiles - 1) / per);
+  const int r = 4 * (int)(blockIdx.x % (RT / 4)) + wave;
+  if (pa == pb || r >= s.n * a.G - rt * RT) return;
+  const int row = rt * RT + r, t = row / a.G, h = head * a.G + (row - t * a.G);
+  const float NEG_INF = -__builtin_huge_valf();
+  auto slot = [&](int p) { return (2 * (int64_t)kv8_wg(a, head, p) + (p == pa ? 1 : 0)) * RT + r; };
+
+  float M = NEG_INF;
+  for (int p = pa + lane; p <= pb; p += 64) M = __builtin_fmaxf(M, a.ws_ml[slot(p) * 2]);
 #pragma unroll
-    for (int v = 0; v < 8; ++v) acc[v] *= inv;
-    *reinterpret_cast<uint4*>(a.o + ((int64_t)(s.row0 + t) * (a.Hkv * a.G) + h) * a.D + d) =
-        make_uint4(kv8_out2<QT>(acc[0], acc[1]), kv8_out2<QT>(acc[2], acc[3]), kv8_out2<QT>(acc[4], acc[5]),
-                   kv8_out2<QT>(acc[6], acc[7]));
+  for (int d = 32; d > 0; d >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d, 64));
+  const float ref = M == NEG_INF ? 0.0f : M;
+  float l = 0.0f, acc[4] = {0, 0, 0, 0};
+  const int d = 4 * lane;
+  for (int p0 = pa; p0 <= pb; p0 += 64) {
+    float f = 0.0f;
+    if (p0 + lane <= pb) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + slot(p0 + lane) * 2);
+      f = __builtin_amdgcn_exp2f(ml.x - ref);
+      l += ml.y * f;
+    }
+    const int n = pb - p0 < 63 ? pb - p0 + 1 : 64;
+    if (d < a.D) {
+      for (int i = 0; i < n; i += 8) {
+        float4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          x[k] = *reinterpret_cast<const float4*>(a.ws_acc + slot(p0 + (i + k < n ? i + k : n - 1)) * a.D + d);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float w = i + k < n ? bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(f), i + k)) : 0.0f;
+          if (i + k < n) {
+            acc[0] += x[k].x * w;
+            acc[1] += x[k].y * w;
+            acc[2] += x[k].z * w;
+            acc[3] += x[k].w * w;
+          }
+        }
+      }
+    }
   }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k, 64);
+  if (a.sink) l += __builtin_amdgcn_exp2f(a.sink[h] * kLog2e - ref);
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  if (d < a.D)
+    *reinterpret_cast<uint2*>(a.o + ((int64_t)(s.row0 + t) * (a.Hkv * a.G) + h) * a.D + d) =
+        make_uint2(kv8_out2<QT>(acc[0] * inv, acc[1] * inv), kv8_out2<QT>(acc[2] * inv, acc[3] * inv));
 }
 
-// kv8_prefill.hip: row tiles of 128.  plan.wgs == 0: a workgroup takes a whole item.
+// kv8_prefill.hip: row tiles of 128.
 void launch_kv8_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& plan, int dtype, hipStream_t stream);
 
 }  // namespace sgl

@@ -3,6 +3,7 @@
 // Plain C++ without HIP, so that a host test can walk over them.
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
 
 #if defined(__HIPCC__)
@@ -257,8 +258,16 @@ SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {
 // share the line of key tiles.
 struct Kv8AttnPlan {
   int64_t row_tile;  // 16 or 32: kv8_attn.hip; 128: kv8_prefill.hip
-  int64_t wgs;       // 0: a workgroup takes a whole item
+  int64_t parts;     // workgroups of a kv head's line, a multiple of 8; 0: a workgroup takes a whole item
 };
+SGL_RULE size_t kv8_attn_workspace(const Kv8AttnPlan& p, int64_t Hkv, int64_t D) {
+  return (size_t)(2 * p.parts * Hkv * p.row_tile * (D + 2)) * sizeof(float);
+}
+// parts for about so many workgroups in all
+SGL_RULE int64_t kv8_attn_parts(int64_t wgs, int64_t Hkv) {
+  const int64_t p = wgs / Hkv / 8 * 8;
+  return p < 8 ? 8 : p;
+}
 // the most items (row tile, kv head) that T queries of B sequences make
 SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t row_tile) {
   const int64_t tiles = T * G / row_tile + B, most = T * ((G + row_tile - 1) / row_tile + 1);
@@ -266,8 +275,8 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
 }
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t cus) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
-  if (rows > 32) return {128, kv8_attn_items(T, B, Hkv, G, 128) >= 2 * cus ? 0 : 2 * cus};
-  return {D <= 128 && rows > 16 ? 32 : 16, 2 * cus};
+  if (rows > 32) return {128, kv8_attn_items(T, B, Hkv, G, 128) >= 2 * cus ? 0 : kv8_attn_parts(2 * cus, Hkv)};
+  return {D <= 128 && rows > 16 ? 32 : 16, kv8_attn_parts(2 * cus, Hkv)};
 }
 
 }  // namespace sgl
