@@ -453,7 +453,7 @@ void launch_few(const Kv8AttnArgs& a, hipStream_t st) {
 
 template <int QT>
 void launch_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
-  if (p.row_tile == 128)
+  if (p.row_tile > 32)
     launch_kv8_prefill(a, p, QT, st);
   else if (a.D <= 64)
     p.row_tile == 16 ? launch_few<64, 1, QT>(a, st) : launch_few<64, 2, QT>(a, st);

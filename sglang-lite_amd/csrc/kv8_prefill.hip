@@ -1,17 +1,15 @@
 // Attention over the 8-bit paged cache: many rows a sequence and head (prompt
 // chunks).  The mathematics, and the kernel for few rows: kv8_attn.hip.
 //
-// Bound by the matrix cores and, beside them, by the softmax's VALU work (an
-// exponential is four issue slots).  Four wavefronts of 32 rows each share the
-// key tiles of 64 tokens, whose codes are converted once, on the way into LDS
+// Bound by the matrix cores and the softmax's VALU work, which take turns on a
+// SIMD.  Eight wavefronts (heads above 128: four) of 32 rows each share the key
+// tiles of 64 tokens, whose codes are converted once, on the way into LDS
 // (exact in bf16 and f16), and both products are v_mfma_f32_32x32x16:
 //   S^T = K . Q^T (Q^T fragments stay in registers), O^T += V^T . P^T, where
 //   P^T is the accumulator of S^T itself (its output layout is the B operand's)
 //   and V^T comes from the row-major tile by ds_read_b64_tr_b16.
 // Lane (row c, half g) owns row c in both: no exchange but the sum of two halves.
-// S^T of tile j + 1 is computed beside the softmax of tile j: independent work
-// that the scheduler lays between each other.  Codes are loaded two tiles ahead
-// and stored one ahead; one barrier a tile.
+// Codes are loaded two tiles ahead and stored one ahead; one barrier a tile.
 #include "sgl_kv8_attn.h"
 
 namespace sgl {
@@ -36,6 +34,11 @@ struct Wide<SGL_BF16> {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pk2_bf16(a, b); }
+  // s + the two weights as the product takes them, in one instruction
+  static __device__ __forceinline__ float add2(float s, float, float, uint32_t packed) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(sgl_bf2, packed), sgl_bf2{(__bf16)1.0f, (__bf16)1.0f}, s,
+                                           false);
+  }
 };
 template <>
 struct Wide<SGL_F16> {
@@ -47,6 +50,7 @@ struct Wide<SGL_F16> {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2<SGL_F16>(a, b); }
+  static __device__ __forceinline__ float add2(float s, float a, float b, uint32_t) { return s + a + b; }
 };
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -65,12 +69,12 @@ __device__ __forceinline__ uint32_t swt(int t) {
 template <int DP, int QT, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel(const Kv8AttnArgs a, int64_t items) {
   constexpr int RT = 32 * NW, NT = 64 * NW, ROW = 2 * DP, KS = DP / 16, DT = DP / 32;
-  constexpr int CPR = DP / 16;                  // 16-byte pieces of codes a token
-  constexpr int PIECES = kKeys * CPR / NT;      // of a thread, for K and for V each
-  constexpr int TSTEP = NT / CPR;               // tokens between a thread's pieces
+  constexpr int CPR = DP / 16;               // 16-byte pieces of codes a token
+  constexpr int SIDE = kKeys * CPR;          // pieces of K's tile, and of V's behind them
+  constexpr int PIECES = 2 * SIDE / NT;      // of a thread
+  static_assert(PIECES * NT == 2 * SIDE && SIDE % 64 == 0, "a wavefront's piece is K's or V's");
   typedef Wide<QT> O;
-  __shared__ __align__(16) uint8_t sK[2][kKeys * ROW];
-  __shared__ __align__(16) uint8_t sV[2][kKeys * ROW];
+  __shared__ __align__(16) uint8_t sK[4][kKeys * ROW];  // K, K, V, V
   __shared__ __align__(4) uint16_t sDims[2][kKeys][CPR];  // of a tile seen in part: a token's dims with NaN codes
   __shared__ int sNan[2];                                 // 1 + the last such tile in the buffer that has any
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -137,7 +141,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
-    float m_run = NEG_INF, l_run = 0.0f;
+    float m_run = live ? NEG_INF : 0.0f, l_run = 0.0f;  // (a row that is none never asks for a reference)
 
     if (j0 < j1) {
       u4v q[KS];
@@ -151,40 +155,65 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       }
       const int32_t* table = a.pages + (int64_t)b * a.row_pages;
       const int pmask = (1 << a.page_shift) - 1;
-      const int last_tok = s.len - 1;
 
-      // ---- staging: piece i of this thread is 16 codes of token ptok + i TSTEP
-      const int pc = threadIdx.x % CPR, ptok = threadIdx.x / CPR;
-      const bool in_d = 16 * pc < a.D;
-      struct Pages {
-        int p[PIECES];
+      // ---- pages and scales of 16 tiles at a time: lane l has granule l % 4 of tile
+      // l / 4, counted from j0; pages loaded a batch ahead, scales half of one
+      struct Batch {
+        int page;  // 0 where there is none
+        float k, v;
+        bool ok;  // the granule lies before the end, on a page of the cache
       };
-      auto load_pages = [&](int j) {
-        Pages o;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          int t = j * kKeys + ptok + i * TSTEP;
-          t = t < s.len ? t : last_tok;
-          o.p[i] = table[t >> a.page_shift];
-        }
+      auto load_pages = [&](int batch) __attribute__((always_inline)) {
+        Batch o;
+        const int t = (j0 + 16 * batch + (lane >> 2)) * kKeys + 16 * (lane & 3);
+        const int page = table[(t < s.len ? t : s.len - 1) >> a.page_shift];
+        o.ok = t < s.len && page >= 0 && page < a.n_pages;
+        o.page = o.ok ? page : 0;
         return o;
       };
-      auto load_codes = [&](const uint8_t* codes, int j, const Pages& pg, uint4* out) {
+      auto load_scales = [&](int batch, Batch& o) __attribute__((always_inline)) {
+        const int t = (j0 + 16 * batch + (lane >> 2)) * kKeys + 16 * (lane & 3);
+        const int64_t piece = (((int64_t)o.page * a.Hkv + head) << (a.page_shift - a.block_shift)) +
+                              ((t & pmask) >> a.block_shift);
+        o.k = a.ks[piece];
+        o.v = a.vs[piece];
+      };
+      float kcs = 0, evs = 0, ivs = 0;  // score scale, log2 of the value scale, its reciprocal
+      uint64_t okm = 0;
+      auto use = [&](const Batch& o) __attribute__((always_inline)) {
+        kcs = o.ok ? o.k * a.c1 : 1.0f;  // (what was never written may hold anything)
+        evs = o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) : 0.0f;
+        ivs = __builtin_amdgcn_exp2f(-evs);
+        okm = __ballot(o.ok);
+      };
+      auto lane_f = [&](float x, int l) __attribute__((always_inline)) {
+        return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(x), l));
+      };
+
+      // ---- staging: piece i of this thread is 16 codes of token ptok + i TSTEP.  A
+      // wavefront's piece lies in one granule, so its page is one number.
+      const int pc = threadIdx.x % CPR, ptok = threadIdx.x / CPR;
+      const int wtok = wave * (64 / CPR);
+      const uint32_t poff = (uint32_t)((ptok - wtok) * a.D + (16 * pc < a.D ? 16 * pc : 0));
+      // piece i: of V, and its token (the wavefront's first: with wtok)
+      auto is_v = [&](int i) { return wave * 64 + i * NT >= SIDE; };
+      auto tok_of = [&](int i, int t) { return (t + i * (NT / CPR)) % kKeys; };
+      auto load_codes = [&](int j, int pages, uint4* out) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          int t = j * kKeys + ptok + i * TSTEP;
-          const bool ok = t < s.len && pg.p[i] >= 0 && pg.p[i] < a.n_pages && in_d;
-          t = t < s.len ? t : last_tok;
-          const int64_t line = (int64_t)(ok ? pg.p[i] : 0) * a.Hkv + head;
-          out[i] = make_uint4(0, 0, 0, 0);
-          if (ok)
-            out[i] = *reinterpret_cast<const uint4*>(codes + ((line << a.page_shift) + (t & pmask)) * a.D + 16 * pc);
+          const int t = tok_of(i, wtok);
+          const int page = __builtin_amdgcn_readlane(pages, 4 * ((j - j0) & 15) + (t >> 4));
+          const int64_t row = (((int64_t)page * a.Hkv + head) << a.page_shift) + ((j * kKeys + t) & pmask);
+          out[i] = *reinterpret_cast<const uint4*>((is_v(i) ? a.vc : a.kc) + row * a.D + poff);
         }
       };
-      auto store_codes = [&](uint8_t* tile, const uint4* in) {
+      // (the swizzle repeats every 16 tokens: the same for all of a thread's pieces)
+      static_assert(NT / CPR % 16 == 0, "tokens between a thread's pieces");
+      const uint32_t dst0 = ptok % kKeys * ROW + (((2 * pc) ^ swt<DP>(ptok)) << 4);
+      const uint32_t dst1 = ptok % kKeys * ROW + (((2 * pc + 1) ^ swt<DP>(ptok)) << 4);
+      auto store_codes = [&](int buf, const uint4* in) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const int t = ptok + i * TSTEP;
           const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
           u4v lo, hi2;
 #pragma unroll
@@ -194,16 +223,31 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
             hi2[2 * k] = O::template cvt<false>(w[2 + k]);
             hi2[2 * k + 1] = O::template cvt<true>(w[2 + k]);
           }
-          *reinterpret_cast<u4v*>(tile + t * ROW + (((2 * pc) ^ swt<DP>(t)) << 4)) = lo;
-          *reinterpret_cast<u4v*>(tile + t * ROW + (((2 * pc + 1) ^ swt<DP>(t)) << 4)) = hi2;
+          uint8_t* to = sK[buf];
+          if constexpr (2 * SIDE == NT)
+            to += is_v(0) ? 2 * kKeys * ROW : 0;
+          else
+            to += i * NT / SIDE * (2 * kKeys * ROW) + i * NT % SIDE / CPR * ROW;
+          *reinterpret_cast<u4v*>(to + dst0) = lo;
+          *reinterpret_cast<u4v*>(to + dst1) = hi2;
+        }
+      };
+      // Values behind the last key, or on no page, were never written: zeros, which
+      // meet zeros of P.
+      auto clear_missing = [&](int j, uint32_t ok, uint4* in) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int t = tok_of(i, ptok);
+          if (is_v(i) && (j * kKeys + t >= s.len || !((ok >> (t >> 4)) & 1u))) in[i] = make_uint4(0, 0, 0, 0);
         }
       };
       // A tile that some rows see in part: its NaN codes are zeroed, so that 0 * NaN
       // reaches no row's sum, and noted, for the rows that do see them.
-      auto take_nan = [&](int j, uint4* in) {
+      auto take_nan = [&](int j, int buf, uint4* in) __attribute__((always_inline)) {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
+          if (!is_v(i)) continue;
           uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w}, dims = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -212,68 +256,40 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
             dims |= ((bad * 0x10204080u) >> 28) << (4 * k);
           }
           in[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          sDims[j & 1][ptok + i * TSTEP][pc] = (uint16_t)dims;
+          sDims[buf][tok_of(i, ptok)][pc] = (uint16_t)dims;
           any |= dims != 0;
         }
-        if (any) sNan[j & 1] = j + 1;
+        if (any) sNan[buf] = j + 1;
       };
       const int part_hi = a.causal ? s.len - s.n + (rt * RT) / a.G + 1 : s.len;  // keys that the first row sees
       const int part_lo = a.causal && a.window > 0
                               ? s.len - s.n + (rt * RT + (rows < RT ? rows : RT) - 1) / a.G - a.window + 1 : 0;
       auto partial = [&](int j) { return (j + 1) * kKeys > part_hi || j * kKeys < part_lo; };
-
-      // ---- scales: lane i < 4 has granule i of a tile
-      struct Scales {
-        float k, v;
-        bool ok;
-      };
-      auto load_scales = [&](int j) {
-        Scales o;
-        const int t = j * kKeys + 16 * (lane & 3);
-        const int u = t < s.len ? t : last_tok & ~15;
-        const int page = table[u >> a.page_shift];
-        o.ok = page >= 0 && page < a.n_pages && t < s.len;
-        const int64_t line = (int64_t)(o.ok ? page : 0) * a.Hkv + head;
-        const int64_t piece = (line << (a.page_shift - a.block_shift)) + ((u & pmask) >> a.block_shift);
-        o.k = a.ks[piece];
-        o.v = a.vs[piece];
-        return o;
+      auto stage = [&](int j, int buf, uint32_t ok, uint4* in) __attribute__((always_inline)) {
+        if ((j + 1) * kKeys > s.len || ok != 15) clear_missing(j, ok, in);
+        if (partial(j)) take_nan(j, buf, in);
+        store_codes(buf, in);
       };
 
-      // ---- S^T of tile j: lane (row c32, half g2) gets token 32 t + 8 (i / 4) + 4 g2 + i % 4 in sc[t][i]
-      uint32_t ka[DP >= 128 ? 8 : 4];
+      // ---- S^T: lane (row c32, half g2) gets token 32 t + 8 (i / 4) + 4 g2 + i % 4 in sc[t][i]
+      constexpr int NKA = DP >= 128 ? 8 : 4;
+      uint32_t ka[NKA];
 #pragma unroll
-      for (int k = 0; k < (DP >= 128 ? 8 : 4); ++k)
-        ka[k] = c32 * ROW + (((2 * k + g2) ^ swt<DP>(c32)) << 4);
-      auto scores = [&](int j, v16f* sc) {
-        const uint8_t* tile = sK[j & 1];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const u4v kf = *reinterpret_cast<const u4v*>(tile + ka[k & 7] + 32 * t * ROW + 256 * (k >> 3));
-            sc[t] = O::mfma(kf, q[k], sc[t]);
-          }
-        }
-      };
-      uint32_t va[2][DT > 4 ? 4 : DT];
+      for (int k = 0; k < NKA; ++k) ka[k] = c32 * ROW + (((2 * k + g2) ^ swt<DP>(c32)) << 4);
+      constexpr int NVA = DT > 4 ? 4 : DT;
+      uint32_t va[2][NVA];
       {
         const int G = lane >> 4, s16 = lane & 15;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int d = 0; d < (DT > 4 ? 4 : DT); ++d) {
+          for (int d = 0; d < NVA; ++d) {
             const int tok = 8 * e + 4 * (G >> 1) + (s16 >> 2);
             const int ch = 4 * d + 2 * (G & 1) + ((s16 & 3) >> 1);
             va[e][d] = tok * ROW + ((ch ^ swt<DP>(tok)) << 4) + 8 * (s16 & 1);
           }
       }
-      auto v_frag = [&](const uint8_t* tile, int s4, int d) {
+      auto v_frag = [&](const uint8_t* tile, int s4, int d) __attribute__((always_inline)) {
         const v4s l = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (lds_v4s*)(tile + va[0][d & 3] + 256 * (d >> 2) + 16 * s4 * ROW));
         const v4s h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -281,92 +297,121 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         return __builtin_bit_cast(u4v, __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7));
       };
 
-      // ---- one tile: softmax of sc (tile j), S^T of tile j + 1 into sn, O^T += V^T . P^T
-      uint4 rk[PIECES], rv[PIECES];
-      Pages pk, pv;
-      Scales sj, sj1;
-      auto tile_step = [&](int j, v16f* sc, v16f* sn) {
-        store_codes(sK[j & 1], rk);                // tile j + 2
-        if (partial(j + 1)) take_nan(j + 1, rv);
-        store_codes(sV[(j + 1) & 1], rv);          // tile j + 1
-        load_codes(a.kc, j + 3, pk, rk);
-        load_codes(a.vc, j + 2, pv, rv);
-        pv = pk;
-        pk = load_pages(j + 4);
-        // P^T = 2^(s + log2 s_v - m), so that s_v is in the exponent, and the sum takes it back
-        const float kc = sj.ok ? sj.k * a.c1 : 0.0f;
-        const float e = sj.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(sj.v), -100.0f) : 0.0f;
-        const float iv = __builtin_amdgcn_exp2f(-e);
-        const uint64_t okm = __ballot(sj.ok);
-        sj = sj1;
-        sj1 = load_scales(j + 2);
-        scores(j + 1, sn);
-        const int tok = j * kKeys;
-        const bool plain = tok + kKeys <= all_hi && tok >= all_lo && (okm & 15) == 15;
-        float mx = NEG_INF;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float kg = bits_f32(__builtin_amdgcn_readlane(f32_bits(kc), g));
-          const float eg = bits_f32(__builtin_amdgcn_readlane(f32_bits(e), g));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = 8 * (g & 1) + i;
-            sc[g >> 1][at] = __builtin_fmaf(sc[g >> 1][at], kg, eg);
-          }
+      uint4 raw[PIECES];
+      Batch now, ahead;
+      // tile j = j0 + i, whose codes are in buffer buf
+      auto tile_step = [&](int i, const int buf) __attribute__((always_inline)) {
+        const int j = j0 + i, l0 = 4 * (i & 15);
+        if ((i & 15) == 0 && i > 0) {
+          now = ahead;
+          use(now);
+          ahead = load_pages((i >> 4) + 1);
         }
+        if ((i & 15) == 4) load_scales((i >> 4) + 1, ahead);
+        const uint32_t ok = (uint32_t)(okm >> l0) & 15u;
+        const uint8_t* kt = sK[buf];
+        v16f sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
+        // fragments are read three steps ahead of their products
+        u4v kf[KS][2];
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            kf[k][t] = *reinterpret_cast<const u4v*>(kt + ka[k & 7] + 32 * t * ROW + 256 * (k >> 3));
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) sc[t] = O::mfma(kf[k][t], q[k], sc[t]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);  // LDS reads
+#pragma unroll
+        for (int k = 0; k < KS - 3; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMAs
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+        // the next tile into LDS, the one after it on its way
+        stage(j + 1, buf ^ 1, (i & 15) == 15 ? (uint32_t)__ballot(ahead.ok) & 15u : (uint32_t)(okm >> (l0 + 4)) & 15u, raw);
+        load_codes(j + 2, (i & 15) >= 14 ? ahead.page : now.page, raw);
+
+        // P^T = 2^(s + log2 s_v - m), so that s_v is in the exponent, and the sum takes it back
+        const int tok = j * kKeys;
+        const bool plain = tok + kKeys <= all_hi && tok >= all_lo && ok == 15;
         if (!plain) {
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int key = tok + 32 * t + 8 * (i >> 2) + 4 * g2 + (i & 3);
-              if (!(key < hi && key >= lo && ((okm >> (2 * t + (i >> 3))) & 1))) sc[t][i] = NEG_INF;
+              if (!(key < hi && key >= lo && ((ok >> (2 * t + (i >> 3))) & 1))) sc[t][i] = NEG_INF;
             }
         }
+        // The reference m need not be the maximum: any m gives the same softmax.  So
+        // no maximum is taken unless a row has none yet or the weights of its tile
+        // pass 2^13 (f16 holds 2^15); then it moves to the maximum and the
+        // accumulators are brought to it.
+        const uint8_t* vt = sK[2 + buf];
+        u4v vf[DT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, sc[t][i]);
-        // the reference moves only when a score exceeds it by more than 6 (log2
-        // units): the weights stay at most 64, the accumulators are rarely rescaled
-        if (__ballot(!(mx <= m_run + 6.0f) && mx != NEG_INF)) {
-          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float nx = mx <= m_run + 6.0f ? m_run : __builtin_fmaxf(m_run, mx);
-          const float alpha = nx == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - nx);
-          m_run = nx;
-          l_run *= alpha;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-        }
-        const float ref = m_run == NEG_INF ? 0.0f : m_run;
+        for (int d = 0; d < DT; ++d) vf[d] = v_frag(vt, 0, d);
         u4v p[4];
+        float sums[4];
+        bool move = __ballot(m_run == NEG_INF) != 0;
+        for (;;) {
+          if (move) {
+            asm volatile("" : "+v"(sc[0]), "+v"(sc[1]));  // (the maximum is not to be taken before the branch)
+            float mx = NEG_INF;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float ig = bits_f32(__builtin_amdgcn_readlane(f32_bits(iv), g));
-          float sum = 0.0f;
+            for (int g = 0; g < 4; ++g) {
+              float mg = sc[g >> 1][8 * (g & 1)];
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float u = __builtin_amdgcn_exp2f(sc[g >> 1][8 * (g & 1) + i] - ref);
-            const float w = __builtin_amdgcn_exp2f(sc[g >> 1][8 * (g & 1) + i + 1] - ref);
-            sum += u;
-            sum += w;
-            p[g][i >> 1] = O::pack(u, w);
+              for (int i = 1; i < 8; ++i) mg = __builtin_fmaxf(mg, sc[g >> 1][8 * (g & 1) + i]);
+              mx = __builtin_fmaxf(mx, __builtin_fmaf(mg, lane_f(kcs, l0 + g), lane_f(evs, l0 + g)));
+            }
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float nx = __builtin_fmaxf(m_run, mx);
+            const float alpha = nx == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - nx);
+            m_run = nx;
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
           }
-          l_run = __builtin_fmaf(sum, ig, l_run);
+          const float ref = m_run == NEG_INF ? 0.0f : m_run;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float kg = lane_f(kcs, l0 + g), eg = lane_f(evs, l0 + g) - ref;
+            sums[g] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i], kg, eg));
+              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i + 1], kg, eg));
+              p[g][i >> 1] = O::pack(u, w);
+              sums[g] = O::add2(sums[g], u, w, p[g][i >> 1]);
+            }
+          }
+          if (move || !__ballot(!(sums[0] + sums[1] + sums[2] + sums[3] <= 8192.0f))) break;
+          move = true;
         }
-        const uint8_t* tile = sV[j & 1];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) l_run = __builtin_fmaf(sums[g], lane_f(ivs, l0 + g), l_run);
 #pragma unroll
         for (int s4 = 0; s4 < 4; ++s4)
 #pragma unroll
-          for (int d = 0; d < DT; ++d) acc[d] = O::mfma(v_frag(tile, s4, d), p[s4], acc[d]);
-        if (partial(j) && sNan[j & 1] == j + 1) {
+          for (int d = 0; d < DT; ++d) {
+            acc[d] = O::mfma(vf[d], p[s4], acc[d]);
+            if (s4 < 3) vf[d] = v_frag(vt, s4 + 1, d);
+          }
+        if (partial(j) && sNan[buf] == j + 1) {
           for (int t = 0; t < kKeys; ++t) {
             const bool seen = tok + t < hi && tok + t >= lo;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-              const uint32_t dims = *reinterpret_cast<const uint32_t*>(&sDims[j & 1][t][2 * d]) >> (4 * g2);
+              const uint32_t dims = *reinterpret_cast<const uint32_t*>(&sDims[buf][t][2 * d]) >> (4 * g2);
 #pragma unroll
               for (int i = 0; i < 16; ++i)
                 if (seen && ((dims >> (8 * (i >> 2) + (i & 3))) & 1u)) acc[d][i] = __builtin_nanf("");
@@ -376,33 +421,21 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         lds_barrier();
       };
 
-      // ---- tiles j0, j0 + 1 into LDS, S^T of the first
       lds_barrier();  // the last segment's reads, and sNan
       {
-        const Pages p0 = load_pages(j0), p1 = load_pages(j0 + 1), p2 = load_pages(j0 + 2);
-        sj = load_scales(j0);
-        sj1 = load_scales(j0 + 1);
-        uint4 r1[PIECES];
-        load_codes(a.kc, j0, p0, rk);
-        load_codes(a.vc, j0, p0, rv);
-        load_codes(a.kc, j0 + 1, p1, r1);
-        pk = load_pages(j0 + 3);
-        store_codes(sK[j0 & 1], rk);
-        store_codes(sK[(j0 + 1) & 1], r1);
-        if (partial(j0)) take_nan(j0, rv);
-        store_codes(sV[j0 & 1], rv);
-        load_codes(a.kc, j0 + 2, p2, rk);
-        load_codes(a.vc, j0 + 1, p1, rv);
-        pv = p2;
+        now = load_pages(0);
+        ahead = load_pages(1);
+        load_scales(0, now);
+        load_codes(j0, now.page, raw);
+        use(now);
+        stage(j0, 0, (uint32_t)okm & 15u, raw);
+        load_codes(j0 + 1, now.page, raw);
       }
       lds_barrier();
-      v16f s0[2], s1[2];
-      scores(j0, s0);
-      lds_barrier();
-      for (int j = j0; j < j1; j += 2) {
-        tile_step(j, s0, s1);
-        if (j + 1 >= j1) break;
-        tile_step(j + 1, s1, s0);
+      for (int i = 0; i < j1 - j0; i += 2) {
+        tile_step(i, 0);
+        if (i + 1 >= j1 - j0) break;
+        tile_step(i + 1, 1);
       }
     }
 
@@ -439,12 +472,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 
 template <int DP, int QT>
 void launch_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
-  const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, 128);
+  constexpr int NW = DP == 128 ? 8 : 4, RT = 32 * NW;
+  static_assert(RT == kv8_chunk_rows(DP), "the plan's row tile");
+  const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, RT);
   if (p.parts == 0) {
-    kv8_prefill_kernel<DP, QT, 4, false><<<(unsigned)items, 256, 0, st>>>(a, items);
+    kv8_prefill_kernel<DP, QT, NW, false><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
   } else {
-    kv8_prefill_kernel<DP, QT, 4, true><<<a.parts * a.Hkv, 256, 0, st>>>(a, items);
-    kv8_merge_kernel<128, kKeys, QT><<<(unsigned)(items * 32), 256, 0, st>>>(a);
+    kv8_prefill_kernel<DP, QT, NW, true><<<a.parts * a.Hkv, 64 * NW, 0, st>>>(a, items);
+    kv8_merge_kernel<RT, kKeys, QT><<<(unsigned)(items * (RT / 4)), 256, 0, st>>>(a);
   }
 }
 

@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
         make_uint2(kv8_out2<QT>(acc[0] * inv, acc[1] * inv), kv8_out2<QT>(acc[2] * inv, acc[3] * inv));
 }
 
-// kv8_prefill.hip: row tiles of 128.
+// kv8_prefill.hip: row tiles of kv8_chunk_rows(D).
 void launch_kv8_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& plan, int dtype, hipStream_t stream);
 
 }  // namespace sgl

@@ -257,7 +257,7 @@ SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {
 // ---- attention over the 8-bit cache: rows of a tile, and the workgroups that
 // share the line of key tiles.
 struct Kv8AttnPlan {
-  int64_t row_tile;  // 16 or 32: kv8_attn.hip; 128: kv8_prefill.hip
+  int64_t row_tile;  // 16 or 32: kv8_attn.hip; more: kv8_prefill.hip
   int64_t parts;     // workgroups of a kv head's line, a multiple of 8; 0: a workgroup takes a whole item
 };
 SGL_RULE size_t kv8_attn_workspace(const Kv8AttnPlan& p, int64_t Hkv, int64_t D) {
@@ -273,9 +273,14 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
   const int64_t tiles = T * G / row_tile + B, most = T * ((G + row_tile - 1) / row_tile + 1);
   return Hkv * (tiles < most ? tiles : most);
 }
+constexpr int64_t kv8_chunk_rows(int64_t D) { return D > 64 && D <= 128 ? 256 : 128; }
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t cus) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
-  if (rows > 32) return {128, kv8_attn_items(T, B, Hkv, G, 128) >= 2 * cus ? 0 : kv8_attn_parts(2 * cus, Hkv)};
+  if (rows > 32) {
+    const int64_t rt = kv8_chunk_rows(D);
+    const int64_t fit = D <= 64 ? 2 * cus : cus;  // workgroups at a time
+    return {rt, kv8_attn_items(T, B, Hkv, G, rt) >= 2 * fit ? 0 : kv8_attn_parts(fit, Hkv)};
+  }
   return {D <= 128 && rows > 16 ? 32 : 16, kv8_attn_parts(2 * cus, Hkv)};
 }
 
