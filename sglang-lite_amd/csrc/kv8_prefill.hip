@@ -1,15 +1,17 @@
 // Attention over the 8-bit paged cache: many rows a sequence and head (prompt
 // chunks).  The mathematics, and the kernel for few rows: kv8_attn.hip.
 //
-// Bound by the matrix cores and the softmax's VALU work, which take turns on a
-// SIMD.  Eight wavefronts (heads above 128: four) of 32 rows each share the key
+// Bound by the matrix cores and, beside them, the softmax's VALU work.  Eight wavefronts (heads above 128: four) of 32 rows each share the key
 // tiles of 64 tokens, whose codes are converted once, on the way into LDS
 // (exact in bf16 and f16), and both products are v_mfma_f32_32x32x16:
 //   S^T = K . Q^T (Q^T fragments stay in registers), O^T += V^T . P^T, where
 //   P^T is the accumulator of S^T itself (its output layout is the B operand's)
 //   and V^T comes from the row-major tile by ds_read_b64_tr_b16.
 // Lane (row c, half g) owns row c in both: no exchange but the sum of two halves.
-// Codes are loaded two tiles ahead and stored one ahead; one barrier a tile.
+// The softmax of tile j lies, a pair of weights at a time, between the products
+// S^T of tile j + 1 and O^T of tile j - 1: VALU instructions of the same wavefront
+// run in an MFMA's shadow (32 cycles: four of them for nothing, eight for half),
+// those of another wavefront's softmax phase much less.  One barrier a tile.
 #include "sgl_kv8_attn.h"
 
 namespace sgl {
@@ -34,11 +36,6 @@ struct Wide<SGL_BF16> {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pk2_bf16(a, b); }
-  // s + the two weights as the product takes them, in one instruction
-  static __device__ __forceinline__ float add2(float s, float, float, uint32_t packed) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(sgl_bf2, packed), sgl_bf2{(__bf16)1.0f, (__bf16)1.0f}, s,
-                                           false);
-  }
 };
 template <>
 struct Wide<SGL_F16> {
@@ -50,7 +47,6 @@ struct Wide<SGL_F16> {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2<SGL_F16>(a, b); }
-  static __device__ __forceinline__ float add2(float s, float a, float b, uint32_t) { return s + a + b; }
 };
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -60,6 +56,12 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // the transpose reads (four chunks of four consecutive tokens): rows of 16
 // chunks and more rotate the token's low four bits; rows of 8 lie two to a
 // 256-byte line, so the token's lowest bit already picks the half.
+// V's tile is read by the transpose alone and rotates two bits, so that its reads 8
+// tokens on differ by a constant.
+template <int DP>
+__device__ __forceinline__ uint32_t swv(int t) {
+  return DP >= 128 ? (uint32_t)((t & 3) << 2) : (uint32_t)((t & 2) << 1);
+}
 template <int DP>
 __device__ __forceinline__ uint32_t swt(int t) {
   return DP >= 128 ? (uint32_t)(((t & 3) << 2) | ((t >> 2) & 3)) : (uint32_t)(((t & 2) << 1) | ((t >> 2) & 3));
@@ -72,10 +74,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
   constexpr int CPR = DP / 16;               // 16-byte pieces of codes a token
   constexpr int SIDE = kKeys * CPR;          // pieces of K's tile, and of V's behind them
   constexpr int PIECES = 2 * SIDE / NT;      // of a thread
-  static_assert(PIECES * NT == 2 * SIDE && SIDE % 64 == 0, "a wavefront's piece is K's or V's");
+  static_assert(PIECES * NT == 2 * SIDE && SIDE % NT == 0, "a thread's first pieces are K's, the others V's");
   typedef Wide<QT> O;
   __shared__ __align__(16) uint8_t sK[4][kKeys * ROW];  // K, K, V, V
+  // Q^T fragments: in LDS where the registers are short and LDS is not (heads of 128)
+  constexpr bool QL = DP == 128;
+  __shared__ __align__(16) u4v sQ[QL ? NW : 1][QL ? KS : 1][64];
   __shared__ __align__(4) uint16_t sDims[2][kKeys][CPR];  // of a tile seen in part: a token's dims with NaN codes
+  __shared__ __align__(8) float2 sScale[2][64];           // of a batch's granules: score scale, log2 of the value scale
   __shared__ int sNan[2];                                 // 1 + the last such tile in the buffer that has any
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, g2 = lane >> 5;
@@ -144,15 +150,25 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     float m_run = live ? NEG_INF : 0.0f, l_run = 0.0f;  // (a row that is none never asks for a reference)
 
     if (j0 < j1) {
-      u4v q[KS];
+      u4v q[QL ? 1 : KS];
       {
         const uint16_t* src = a.q + (int64_t)(s.row0 + tq) * a.qt + (int64_t)hq * a.qh + 8 * g2;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          q[k] = u4v{0, 0, 0, 0};
-          if (live && 16 * k < a.D) q[k] = *reinterpret_cast<const u4v*>(src + 16 * k);
+          u4v f = u4v{0, 0, 0, 0};
+          if (live && 16 * k < a.D) f = *reinterpret_cast<const u4v*>(src + 16 * k);
+          if constexpr (QL)
+            sQ[wave][k][lane] = f;  // (read by the lane that wrote it)
+          else
+            q[k] = f;
         }
       }
+      auto q_frag = [&](int k) __attribute__((always_inline)) {
+        if constexpr (QL)
+          return sQ[wave][k][lane];
+        else
+          return q[k];
+      };
       const int32_t* table = a.pages + (int64_t)b * a.row_pages;
       const int pmask = (1 << a.page_shift) - 1;
 
@@ -178,16 +194,15 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         o.k = a.ks[piece];
         o.v = a.vs[piece];
       };
-      float kcs = 0, evs = 0, ivs = 0;  // score scale, log2 of the value scale, its reciprocal
+      // A granule's two numbers are read back as a broadcast (v_readlane takes four
+      // times as long as a plain VALU instruction here).  Every wavefront writes the
+      // same values to the same place, and reads behind its own writes.
       uint64_t okm = 0;
-      auto use = [&](const Batch& o) __attribute__((always_inline)) {
-        kcs = o.ok ? o.k * a.c1 : 1.0f;  // (what was never written may hold anything)
-        evs = o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) : 0.0f;
-        ivs = __builtin_amdgcn_exp2f(-evs);
+      auto use = [&](int batch, const Batch& o) __attribute__((always_inline)) {
+        // (what was never written may hold anything)
+        sScale[batch & 1][lane] = make_float2(o.ok ? o.k * a.c1 : 1.0f,
+                                              o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) : 0.0f);
         okm = __ballot(o.ok);
-      };
-      auto lane_f = [&](float x, int l) __attribute__((always_inline)) {
-        return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(x), l));
       };
 
       // ---- staging: piece i of this thread is 16 codes of token ptok + i TSTEP.  A
@@ -195,42 +210,38 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       const int pc = threadIdx.x % CPR, ptok = threadIdx.x / CPR;
       const int wtok = wave * (64 / CPR);
       const uint32_t poff = (uint32_t)((ptok - wtok) * a.D + (16 * pc < a.D ? 16 * pc : 0));
-      // piece i: of V, and its token (the wavefront's first: with wtok)
-      auto is_v = [&](int i) { return wave * 64 + i * NT >= SIDE; };
+      // piece i: whether V's, and its token (the wavefront's first: with wtok)
+      auto is_v = [](int i) { return i * NT >= SIDE; };
       auto tok_of = [&](int i, int t) { return (t + i * (NT / CPR)) % kKeys; };
-      auto load_codes = [&](int j, int pages, uint4* out) __attribute__((always_inline)) {
+      // K's pieces of tile jk, V's of tile jv (pages: the lanes' pages of their batches)
+      auto load_codes = [&](int jk, int kpages, int jv, int vpages, uint4* out) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const int t = tok_of(i, wtok);
-          const int page = __builtin_amdgcn_readlane(pages, 4 * ((j - j0) & 15) + (t >> 4));
+          const int t = tok_of(i, wtok), j = is_v(i) ? jv : jk;
+          const int page = __builtin_amdgcn_readlane(is_v(i) ? vpages : kpages, 4 * ((j - j0) & 15) + (t >> 4));
           const int64_t row = (((int64_t)page * a.Hkv + head) << a.page_shift) + ((j * kKeys + t) & pmask);
           out[i] = *reinterpret_cast<const uint4*>((is_v(i) ? a.vc : a.kc) + row * a.D + poff);
         }
       };
       // (the swizzle repeats every 16 tokens: the same for all of a thread's pieces)
       static_assert(NT / CPR % 16 == 0, "tokens between a thread's pieces");
-      const uint32_t dst0 = ptok % kKeys * ROW + (((2 * pc) ^ swt<DP>(ptok)) << 4);
-      const uint32_t dst1 = ptok % kKeys * ROW + (((2 * pc + 1) ^ swt<DP>(ptok)) << 4);
-      auto store_codes = [&](int buf, const uint4* in) __attribute__((always_inline)) {
+      auto dst = [&](int i, int half) {
+        return ptok % kKeys * ROW + (((2 * pc + half) ^ (is_v(i) ? swv<DP>(ptok) : swt<DP>(ptok))) << 4);
+      };
+      const uint32_t kdst0 = dst(0, 0), kdst1 = dst(0, 1), vdst0 = dst(PIECES - 1, 0), vdst1 = dst(PIECES - 1, 1);
+      auto store_piece = [&](int i, int buf, const uint4& in) __attribute__((always_inline)) {
+        const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+        u4v lo, hi2;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
-          u4v lo, hi2;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            lo[2 * k] = O::template cvt<false>(w[k]);
-            lo[2 * k + 1] = O::template cvt<true>(w[k]);
-            hi2[2 * k] = O::template cvt<false>(w[2 + k]);
-            hi2[2 * k + 1] = O::template cvt<true>(w[2 + k]);
-          }
-          uint8_t* to = sK[buf];
-          if constexpr (2 * SIDE == NT)
-            to += is_v(0) ? 2 * kKeys * ROW : 0;
-          else
-            to += i * NT / SIDE * (2 * kKeys * ROW) + i * NT % SIDE / CPR * ROW;
-          *reinterpret_cast<u4v*>(to + dst0) = lo;
-          *reinterpret_cast<u4v*>(to + dst1) = hi2;
+        for (int k = 0; k < 2; ++k) {
+          lo[2 * k] = O::template cvt<false>(w[k]);
+          lo[2 * k + 1] = O::template cvt<true>(w[k]);
+          hi2[2 * k] = O::template cvt<false>(w[2 + k]);
+          hi2[2 * k + 1] = O::template cvt<true>(w[2 + k]);
         }
+        uint8_t* to = sK[buf] + i * NT / SIDE * (2 * kKeys * ROW) + i * NT % SIDE / CPR * ROW;
+        *reinterpret_cast<u4v*>(to + (is_v(i) ? vdst0 : kdst0)) = lo;
+        *reinterpret_cast<u4v*>(to + (is_v(i) ? vdst1 : kdst1)) = hi2;
       };
       // Values behind the last key, or on no page, were never written: zeros, which
       // meet zeros of P.
@@ -265,150 +276,35 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       const int part_lo = a.causal && a.window > 0
                               ? s.len - s.n + (rt * RT + (rows < RT ? rows : RT) - 1) / a.G - a.window + 1 : 0;
       auto partial = [&](int j) { return (j + 1) * kKeys > part_hi || j * kKeys < part_lo; };
-      auto stage = [&](int j, int buf, uint32_t ok, uint4* in) __attribute__((always_inline)) {
-        if ((j + 1) * kKeys > s.len || ok != 15) clear_missing(j, ok, in);
-        if (partial(j)) take_nan(j, buf, in);
-        store_codes(buf, in);
-      };
-
       // ---- S^T: lane (row c32, half g2) gets token 32 t + 8 (i / 4) + 4 g2 + i % 4 in sc[t][i]
       constexpr int NKA = DP >= 128 ? 8 : 4;
       uint32_t ka[NKA];
 #pragma unroll
       for (int k = 0; k < NKA; ++k) ka[k] = c32 * ROW + (((2 * k + g2) ^ swt<DP>(c32)) << 4);
       constexpr int NVA = DT > 4 ? 4 : DT;
-      uint32_t va[2][NVA];
+      uint32_t va[NVA];
       {
         const int G = lane >> 4, s16 = lane & 15;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int d = 0; d < NVA; ++d) {
-            const int tok = 8 * e + 4 * (G >> 1) + (s16 >> 2);
-            const int ch = 4 * d + 2 * (G & 1) + ((s16 & 3) >> 1);
-            va[e][d] = tok * ROW + ((ch ^ swt<DP>(tok)) << 4) + 8 * (s16 & 1);
-          }
+        for (int d = 0; d < NVA; ++d) {
+          const int tok = 4 * (G >> 1) + (s16 >> 2);
+          const int ch = 4 * d + 2 * (G & 1) + ((s16 & 3) >> 1);
+          va[d] = tok * ROW + ((ch ^ swv<DP>(tok)) << 4) + 8 * (s16 & 1);
+        }
       }
       auto v_frag = [&](const uint8_t* tile, int s4, int d) __attribute__((always_inline)) {
         const v4s l = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_v4s*)(tile + va[0][d & 3] + 256 * (d >> 2) + 16 * s4 * ROW));
+            (lds_v4s*)(tile + va[d & 3] + 256 * (d >> 2) + 16 * s4 * ROW));
         const v4s h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_v4s*)(tile + va[1][d & 3] + 256 * (d >> 2) + 16 * s4 * ROW));
+            (lds_v4s*)(tile + va[d & 3] + 256 * (d >> 2) + (16 * s4 + 8) * ROW));
         return __builtin_bit_cast(u4v, __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7));
       };
 
-      uint4 raw[PIECES];
-      Batch now, ahead;
-      // tile j = j0 + i, whose codes are in buffer buf
-      auto tile_step = [&](int i, const int buf) __attribute__((always_inline)) {
-        const int j = j0 + i, l0 = 4 * (i & 15);
-        if ((i & 15) == 0 && i > 0) {
-          now = ahead;
-          use(now);
-          ahead = load_pages((i >> 4) + 1);
-        }
-        if ((i & 15) == 4) load_scales((i >> 4) + 1, ahead);
-        const uint32_t ok = (uint32_t)(okm >> l0) & 15u;
-        const uint8_t* kt = sK[buf];
-        v16f sc[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
-        // fragments are read three steps ahead of their products
-        u4v kf[KS][2];
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            kf[k][t] = *reinterpret_cast<const u4v*>(kt + ka[k & 7] + 32 * t * ROW + 256 * (k >> 3));
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int t = 0; t < 2; ++t) sc[t] = O::mfma(kf[k][t], q[k], sc[t]);
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);  // LDS reads
-#pragma unroll
-        for (int k = 0; k < KS - 3; ++k) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMAs
-          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
-        // the next tile into LDS, the one after it on its way
-        stage(j + 1, buf ^ 1, (i & 15) == 15 ? (uint32_t)__ballot(ahead.ok) & 15u : (uint32_t)(okm >> (l0 + 4)) & 15u, raw);
-        load_codes(j + 2, (i & 15) >= 14 ? ahead.page : now.page, raw);
-
-        // P^T = 2^(s + log2 s_v - m), so that s_v is in the exponent, and the sum takes it back
-        const int tok = j * kKeys;
-        const bool plain = tok + kKeys <= all_hi && tok >= all_lo && ok == 15;
-        if (!plain) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int key = tok + 32 * t + 8 * (i >> 2) + 4 * g2 + (i & 3);
-              if (!(key < hi && key >= lo && ((ok >> (2 * t + (i >> 3))) & 1))) sc[t][i] = NEG_INF;
-            }
-        }
-        // The reference m need not be the maximum: any m gives the same softmax.  So
-        // no maximum is taken unless a row has none yet or the weights of its tile
-        // pass 2^13 (f16 holds 2^15); then it moves to the maximum and the
-        // accumulators are brought to it.
-        const uint8_t* vt = sK[2 + buf];
-        u4v vf[DT];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vf[d] = v_frag(vt, 0, d);
-        u4v p[4];
-        float sums[4];
-        bool move = __ballot(m_run == NEG_INF) != 0;
-        for (;;) {
-          if (move) {
-            asm volatile("" : "+v"(sc[0]), "+v"(sc[1]));  // (the maximum is not to be taken before the branch)
-            float mx = NEG_INF;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              float mg = sc[g >> 1][8 * (g & 1)];
-#pragma unroll
-              for (int i = 1; i < 8; ++i) mg = __builtin_fmaxf(mg, sc[g >> 1][8 * (g & 1) + i]);
-              mx = __builtin_fmaxf(mx, __builtin_fmaf(mg, lane_f(kcs, l0 + g), lane_f(evs, l0 + g)));
-            }
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float nx = __builtin_fmaxf(m_run, mx);
-            const float alpha = nx == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - nx);
-            m_run = nx;
-            l_run *= alpha;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-          }
-          const float ref = m_run == NEG_INF ? 0.0f : m_run;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float kg = lane_f(kcs, l0 + g), eg = lane_f(evs, l0 + g) - ref;
-            sums[g] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-              const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i], kg, eg));
-              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i + 1], kg, eg));
-              p[g][i >> 1] = O::pack(u, w);
-              sums[g] = O::add2(sums[g], u, w, p[g][i >> 1]);
-            }
-          }
-          if (move || !__ballot(!(sums[0] + sums[1] + sums[2] + sums[3] <= 8192.0f))) break;
-          move = true;
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) l_run = __builtin_fmaf(sums[g], lane_f(ivs, l0 + g), l_run);
-#pragma unroll
-        for (int s4 = 0; s4 < 4; ++s4)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            acc[d] = O::mfma(vf[d], p[s4], acc[d]);
-            if (s4 < 3) vf[d] = v_frag(vt, s4 + 1, d);
-          }
-        if (partial(j) && sNan[buf] == j + 1) {
+      // NaN codes of tile j, for the rows that see them
+      auto put_nan = [&](int j, int buf) __attribute__((always_inline)) {
+        if (__builtin_expect(partial(j) && sNan[buf] == j + 1, 0)) {
           for (int t = 0; t < kKeys; ++t) {
-            const bool seen = tok + t < hi && tok + t >= lo;
+            const bool seen = j * kKeys + t < hi && j * kKeys + t >= lo;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
               const uint32_t dims = *reinterpret_cast<const uint32_t*>(&sDims[buf][t][2 * d]) >> (4 * g2);
@@ -418,6 +314,143 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
             }
           }
         }
+      };
+      auto k_frag = [&](const uint8_t* kt, int n) __attribute__((always_inline)) {
+        const int k = n >> 1, t = n & 1;
+        return *reinterpret_cast<const u4v*>(kt + ka[k & 7] + 32 * t * ROW + 256 * (k >> 3));
+      };
+
+      uint4 raw[PIECES];  // K's codes of tile j + 2, V's of tile j
+      u4v p[4];           // P^T of tile j - 1
+      bool fresh = __ballot(m_run == NEG_INF) != 0;  // a row has no reference yet
+      Batch now, ahead;
+      // Tile j = j0 + i, scores in sc: its softmax, slice by slice between the products
+      // S^T of tile j + 1 (into sn) and O^T += V^T . P^T of tile j - 1.
+      auto tile_step = [&](int i, const int buf, v16f* sc, v16f* sn) __attribute__((always_inline)) {
+        const int j = j0 + i, l0 = 4 * (i & 15), tok = j * kKeys;
+        const float2* scale = &sScale[(i >> 4) & 1][l0];
+        auto top = [&]() __attribute__((always_inline)) {  // the row's largest exponent in this tile
+          float mx = NEG_INF;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float mg = sc[g >> 1][8 * (g & 1)];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mg = __builtin_fmaxf(mg, sc[g >> 1][8 * (g & 1) + e]);
+            mx = __builtin_fmaxf(mx, __builtin_fmaf(mg, scale[g].x, scale[g].y));
+          }
+          return __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+        };
+        // Everything that most tiles do not need stands behind one branch (a taken
+        // branch costs a wavefront some 50 cycles): batch borders, the end of the keys,
+        // masks, NaN codes, rows without a reference.
+        // The reference m need not be the maximum: any m gives the same softmax.  So
+        // no maximum is taken unless a row has no reference yet (its sums are zero
+        // then), or, below, the weights of its tile pass 2^13 (f16 holds 2^15).
+        const bool border = (i & 15) == 0 && i > 0;
+        const bool seen_by_all = tok + kKeys <= all_hi && tok >= all_lo;
+        if (__builtin_expect(border || (i & 15) == 4 || !seen_by_all || partial(j) || (okm >> l0 & 15u) != 15 || fresh, 0)) {
+          if (border) {
+            now = ahead;
+            use(i >> 4, now);
+            ahead = load_pages((i >> 4) + 1);
+          }
+          if ((i & 15) == 4) load_scales((i >> 4) + 1, ahead);
+          const uint32_t ok = (uint32_t)(okm >> l0) & 15u;
+          if (tok + kKeys > s.len || ok != 15) clear_missing(j, ok, raw);
+          if (partial(j)) take_nan(j, buf, raw);
+          if (!seen_by_all || ok != 15) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int key = tok + 32 * t + 8 * (e >> 2) + 4 * g2 + (e & 3);
+                if (!(key < hi && key >= lo && ((ok >> (2 * t + (e >> 3))) & 1))) sc[t][e] = NEG_INF;
+              }
+          }
+          if (fresh) {
+            const float mx = top();
+            m_run = m_run == NEG_INF ? mx : m_run;
+            fresh = __ballot(m_run == NEG_INF) != 0;
+          }
+        }
+        // P^T = 2^(s + log2 s_v - m), so that s_v is in the exponent, and the sum takes it back
+        float2 kv = scale[3], kv_next;
+        float eg = 0.0f, sum = 0.0f, most = 0.0f, l_new = l_run;
+        // The granules' order is 3, 0, 1, 2: those of the tile before are used up in the
+        // order 0, 1, 2, 3, so that all but the first of the new ones take their place.
+        u4v p3;
+        auto weigh = [&](int n) __attribute__((always_inline)) {  // two weights
+          const int g = ((n >> 2) + 3) & 3, e = 2 * (n & 3);
+          if (e == 0) {
+            if (n > 0) kv = kv_next;
+            eg = kv.y - (m_run == NEG_INF ? 0.0f : m_run);
+            sum = 0.0f;
+          }
+          if (e == 2 && n < 12) kv_next = scale[(g + 1) & 3];
+          const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + e], kv.x, eg));
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + e + 1], kv.x, eg));
+          (g == 3 ? p3 : p[g])[n & 3] = O::pack(u, w);
+          sum += u;
+          sum += w;
+          if (e == 6) {  // the sum of the probabilities takes s_v back
+            l_new = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-kv.y), l_new);
+            most += sum;
+          }
+        };
+
+        constexpr int NS = 2 * KS, AHEAD = 2;  // products of each kind; slices a fragment is read ahead
+        const uint8_t* kt = sK[buf ^ 1];
+        const uint8_t* vt = sK[2 + (buf ^ 1)];
+        u4v kf[AHEAD + 1], vf[AHEAD + 1], qf[2];
+        qf[0] = q_frag(0);
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+          kf[n] = k_frag(kt, n);
+          vf[n] = v_frag(vt, n / DT, n % DT);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sn[t][e] = 0.0f;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          if (n + AHEAD < NS) {
+            kf[(n + AHEAD) % (AHEAD + 1)] = k_frag(kt, n + AHEAD);
+            vf[(n + AHEAD) % (AHEAD + 1)] = v_frag(vt, (n + AHEAD) / DT, (n + AHEAD) % DT);
+          }
+          if (n % 2 == 0 && n + 2 < NS) qf[(n / 2 + 1) & 1] = q_frag(n / 2 + 1);
+          sn[n & 1] = O::mfma(kf[n % (AHEAD + 1)], qf[(n >> 1) & 1], sn[n & 1]);
+#pragma unroll
+          for (int w = n * 16 / NS; w < (2 * n + 1) * 16 / (2 * NS); ++w) weigh(w);
+          acc[n % DT] = O::mfma(vf[n % (AHEAD + 1)], p[n / DT], acc[n % DT]);
+#pragma unroll
+          for (int w = (2 * n + 1) * 16 / (2 * NS); w < (n + 1) * 16 / NS; ++w) weigh(w);
+          // (one piece of the next codes into LDS every few slices, then the loads)
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c)
+            if (n == (c + 1) * NS / (PIECES + 2)) store_piece(c, buf, raw[c]);
+          if (n == (PIECES + 1) * NS / (PIECES + 2))
+            load_codes(j + 3, (i & 15) >= 13 ? ahead.page : now.page, j + 1, (i & 15) == 15 ? ahead.page : now.page, raw);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_expect(__ballot(!(most <= 8192.0f)) != 0, 0)) {
+          asm volatile("" : "+v"(sc[0]), "+v"(sc[1]));  // (nothing of this is to be done before the branch)
+          const float nx = __builtin_fmaxf(m_run, top());
+          const float alpha = nx == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - nx);
+          m_run = nx;
+          l_new = l_run * alpha;
+          kv = scale[3];
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
+#pragma unroll
+          for (int n = 0; n < 16; ++n) weigh(n);
+        }
+        l_run = l_new;
+        p[3] = p3;
+        if (__builtin_expect(i > 0 && partial(j - 1), 0)) put_nan(j - 1, buf ^ 1);
         lds_barrier();
       };
 
@@ -426,17 +459,40 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         now = load_pages(0);
         ahead = load_pages(1);
         load_scales(0, now);
-        load_codes(j0, now.page, raw);
-        use(now);
-        stage(j0, 0, (uint32_t)okm & 15u, raw);
-        load_codes(j0 + 1, now.page, raw);
+        uint4 first[PIECES];
+        load_codes(j0, now.page, j0, now.page, first);
+        load_codes(j0 + 1, now.page, j0, now.page, raw);
+        use(0, now);
+        // (V's buffer of the tile before the first: zeros)
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+          if (!is_v(c)) store_piece(c, 0, first[c]);
+          store_piece(c, 1, is_v(c) ? make_uint4(0, 0, 0, 0) : raw[c]);
+        }
+        load_codes(j0 + 2, now.page, j0, now.page, raw);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) p[g] = u4v{0, 0, 0, 0};
       }
       lds_barrier();
-      for (int i = 0; i < j1 - j0; i += 2) {
-        tile_step(i, 0);
-        if (i + 1 >= j1 - j0) break;
-        tile_step(i + 1, 1);
+      v16f s0[2], s1[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s0[t][e] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 2 * KS; ++n) s0[n & 1] = O::mfma(k_frag(sK[0], n), q_frag(n >> 1), s0[n & 1]);
+      lds_barrier();
+      const int n_tiles = j1 - j0;
+      for (int i = 0; i < n_tiles; i += 2) {
+        tile_step(i, 0, s0, s1);
+        if (i + 1 >= n_tiles) break;
+        tile_step(i + 1, 1, s1, s0);
       }
+      const int lb = (n_tiles - 1) & 1;
+#pragma unroll
+      for (int n = 0; n < 2 * KS; ++n)
+        acc[n % DT] = O::mfma(v_frag(sK[2] + lb * kKeys * ROW, n / DT, n % DT), p[n / DT], acc[n % DT]);
+      put_nan(j1 - 1, lb);
     }
 
     // ---- out
