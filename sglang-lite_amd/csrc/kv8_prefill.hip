@@ -150,17 +150,13 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     float m_run = live ? NEG_INF : 0.0f, l_run = 0.0f;  // (a row that is none never asks for a reference)
 
     if (j0 < j1) {
-      u4v q[QL ? 1 : KS];
+      u4v q[KS];  // (with QL only until they are in LDS)
       {
         const uint16_t* src = a.q + (int64_t)(s.row0 + tq) * a.qt + (int64_t)hq * a.qh + 8 * g2;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          u4v f = u4v{0, 0, 0, 0};
-          if (live && 16 * k < a.D) f = *reinterpret_cast<const u4v*>(src + 16 * k);
-          if constexpr (QL)
-            sQ[wave][k][lane] = f;  // (read by the lane that wrote it)
-          else
-            q[k] = f;
+          q[k] = u4v{0, 0, 0, 0};
+          if (live && 16 * k < a.D) q[k] = *reinterpret_cast<const u4v*>(src + 16 * k);
         }
       }
       auto q_frag = [&](int k) __attribute__((always_inline)) {
@@ -462,6 +458,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         uint4 first[PIECES];
         load_codes(j0, now.page, j0, now.page, first);
         load_codes(j0 + 1, now.page, j0, now.page, raw);
+        if constexpr (QL) {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) sQ[wave][k][lane] = q[k];  // (read by the lane that wrote it)
+        }
         use(0, now);
         // (V's buffer of the tile before the first: zeros)
 #pragma unroll
