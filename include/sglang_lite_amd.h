@@ -564,8 +564,9 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
                  float softmax_scale, int causal, int64_t window, const float* sink, void* out,
                  void* workspace, size_t workspace_bytes, sgl_stream_t stream);
 
-/* Workspace bytes of sgl_kv8_attn on the current device. */
-size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D);
+/* Workspace bytes of sgl_kv8_attn on the current device (0: none); max_tokens:
+ * row_pages * page_size, what the block table can hold of a sequence. */
+size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens);
 
 /* ------------------------------------------------- host-side self checks */
 

@@ -83,8 +83,9 @@ struct Codes {
 };
 
 // DP: head dim rounded up to 64, 128 or 256; NC: 16-row column tiles
-template <int DP, int NC, int QT>
-__global__ __launch_bounds__(64 * kWaves, 2) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
+// SPLIT: workgroups share the lines, else a workgroup takes a whole item
+template <int DP, int NC, int QT, bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
   constexpr int RT = 16 * NC, KI = DP / 64, C = DP / 16, W = C / 4;
   __shared__ __align__(16) float sAcc[kWaves][16][DP + 4];
   __shared__ float sM[kWaves][16], sL[kWaves][16];
@@ -92,12 +93,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attn_few_kernel(const Kv8A
   const int m = lane & 15, g = lane >> 4;
   const float NEG_INF = -__builtin_huge_valf();
 
-  int head, part;
-  kv8_wg_at(a, (int)blockIdx.x, &head, &part);
+  int head, part = 0;
   Kv8Walk<RT, kTile> walk;
-  if (!walk.start(a, part)) return;
   Kv8Segment seg;
-  while (walk.next(a, seg)) {
+  if constexpr (SPLIT) {
+    kv8_wg_at(a, (int)blockIdx.x, &head, &part);
+    if (!walk.start(a, part)) return;
+  } else {
+    if (!kv8_item<RT, kTile>(a, (int64_t)blockIdx.x, &head, seg)) return;
+  }
+  for (bool more = SPLIT ? walk.next(a, seg) : true; more; more = SPLIT ? walk.next(a, seg) : false) {
     const Kv8Seq& s = seg.s;
     const int b = seg.b, rt = seg.rt, t0 = seg.t0, t1 = seg.t1;
     const int rows = s.n * a.G - rt * RT;  // valid rows of the tile (may be more than RT)
@@ -446,8 +451,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_attn_few_kernel(const Kv8A
 
 template <int DP, int NC, int QT>
 void launch_few(const Kv8AttnArgs& a, hipStream_t st) {
-  kv8_attn_few_kernel<DP, NC, QT><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
   const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, 16 * NC);
+  if (a.parts == 0) {
+    kv8_attn_few_kernel<DP, NC, QT, false><<<(unsigned)items, 64 * kWaves, 0, st>>>(a);
+    return;
+  }
+  kv8_attn_few_kernel<DP, NC, QT, true><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
   kv8_merge_kernel<16 * NC, kTile, QT><<<(unsigned)(items * 4 * NC), 256, 0, st>>>(a);
 }
 
@@ -468,9 +477,9 @@ void launch_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
 
 extern "C" {
 
-size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D) {
-  if (T < 0 || B < 0 || Hkv < 1 || G < 1 || D < 16) return 0;
-  const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, sgl::device_cu_count());
+size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens) {
+  if (T < 0 || B < 0 || Hkv < 1 || G < 1 || D < 16 || max_tokens < 0) return 0;
+  const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, max_tokens, sgl::device_cu_count());
   return sgl::kv8_attn_workspace(p, Hkv, D);
 }
 
@@ -497,7 +506,7 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
               "kv8_attn: q and its strides must be 16-byte aligned");
   SGL_REQUIRE(sgl::aligned(k_codes, 16) && sgl::aligned(v_codes, 16) && sgl::aligned(out, 16),
               "kv8_attn: misaligned cache or output");
-  const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, sgl::device_cu_count());
+  const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, row_pages * page_size, sgl::device_cu_count());
   const size_t need = sgl::kv8_attn_workspace(p, Hkv, D);
   if (need && (!workspace || workspace_bytes < need)) {
     sgl::set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
@@ -505,7 +514,7 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
   }
   SGL_REQUIRE(sgl::aligned(workspace, 16), "kv8_attn: workspace must be 16-byte aligned");
   const int64_t items = sgl::kv8_attn_items(T, B, Hkv, G, p.row_tile);
-  SGL_REQUIRE_SUPPORTED(items * ((row_pages * page_size + 63) / 64 + sgl::kItemCost) < (1ll << 31),
+  SGL_REQUIRE_SUPPORTED(items * ((row_pages * page_size + 31) / 32 + sgl::kItemCost) < (1ll << 31),
                         "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)items,
                         (long long)(row_pages * page_size));
   sgl::Kv8AttnArgs a;

@@ -22,7 +22,8 @@ typedef short v8s __attribute__((ext_vector_type(8)));
 typedef v4s __attribute__((address_space(3))) lds_v4s;
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
-constexpr int kKeys = 64;  // tokens of a key tile
+// Tokens of a key tile: 64; 32 of heads above 128, whose accumulators leave less room.
+constexpr int chunk_keys(int DP) { return DP == 256 ? 32 : 64; }
 
 template <int QT>
 struct Wide;
@@ -70,15 +71,19 @@ __device__ __forceinline__ uint32_t swt(int t) {
 // DP: head dim rounded up to 64, 128 or 256; NW wavefronts
 template <int DP, int QT, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel(const Kv8AttnArgs a, int64_t items) {
+  constexpr int kKeys = chunk_keys(DP), NG = kKeys / 16, NH = kKeys / 32;  // granules, halves of 32 tokens
   constexpr int RT = 32 * NW, NT = 64 * NW, ROW = 2 * DP, KS = DP / 16, DT = DP / 32;
+  constexpr int NS = KS * NH;   // products of each kind in a tile
+  constexpr int TB = 64 / NG;   // tiles whose granules' scales and pages the lanes hold
+  static_assert(NS == NG * DT, "as many of S as of O");
   constexpr int CPR = DP / 16;               // 16-byte pieces of codes a token
   constexpr int SIDE = kKeys * CPR;          // pieces of K's tile, and of V's behind them
   constexpr int PIECES = 2 * SIDE / NT;      // of a thread
   static_assert(PIECES * NT == 2 * SIDE && SIDE % NT == 0, "a thread's first pieces are K's, the others V's");
   typedef Wide<QT> O;
   __shared__ __align__(16) uint8_t sK[4][kKeys * ROW];  // K, K, V, V
-  // Q^T fragments: in LDS where the registers are short and LDS is not (heads of 128)
-  constexpr bool QL = DP == 128;
+  // Q^T fragments: in LDS where the registers are short
+  constexpr bool QL = DP >= 128;
   __shared__ __align__(16) u4v sQ[QL ? NW : 1][QL ? KS : 1][64];
   __shared__ __align__(4) uint16_t sDims[2][kKeys][CPR];  // of a tile seen in part: a token's dims with NaN codes
   __shared__ __align__(8) float2 sScale[2][64];           // of a batch's granules: score scale, log2 of the value scale
@@ -97,16 +102,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
   } else {
     // the last row tiles, which see the most keys, first; the heads go round
     // fastest, so that a head's workgroups meet on one XCD and its L2
-    const int64_t item = items - 1 - (int64_t)blockIdx.x;
-    head = (int)(item % a.Hkv);
-    walk.c = kv8_chunk<RT, kKeys>(a, 0);
-    const Kv8Place at = kv8_find<RT, kKeys, true>(a, walk.c, item / a.Hkv);
-    if (at.l < 0) return;
-    seg.s = kv8_lane<RT, kKeys>(a, walk.c, at.l);
-    seg.b = walk.c.b0 + at.l;
-    seg.rt = (int)(item / a.Hkv - at.rts);
-    seg.t0 = 0;
-    seg.t1 = seg.s.tiles;
+    if (!kv8_item<RT, kKeys>(a, items - 1 - (int64_t)blockIdx.x, &head, seg)) return;
   }
   for (bool more = SPLIT ? walk.next(a, seg) : true; more; more = SPLIT ? walk.next(a, seg) : false) {
     const Kv8Seq& s = seg.s;
@@ -168,8 +164,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       const int32_t* table = a.pages + (int64_t)b * a.row_pages;
       const int pmask = (1 << a.page_shift) - 1;
 
-      // ---- pages and scales of 16 tiles at a time: lane l has granule l % 4 of tile
-      // l / 4, counted from j0; pages loaded a batch ahead, scales half of one
+      // ---- pages and scales of TB tiles at a time: lane l has granule l % NG of tile
+      // l / NG, counted from j0; pages loaded a batch ahead, scales most of one
       struct Batch {
         int page;  // 0 where there is none
         float k, v;
@@ -177,14 +173,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       };
       auto load_pages = [&](int batch) __attribute__((always_inline)) {
         Batch o;
-        const int t = (j0 + 16 * batch + (lane >> 2)) * kKeys + 16 * (lane & 3);
+        const int t = (j0 + TB * batch + lane / NG) * kKeys + 16 * (lane % NG);
         const int page = table[(t < s.len ? t : s.len - 1) >> a.page_shift];
         o.ok = t < s.len && page >= 0 && page < a.n_pages;
         o.page = o.ok ? page : 0;
         return o;
       };
       auto load_scales = [&](int batch, Batch& o) __attribute__((always_inline)) {
-        const int t = (j0 + 16 * batch + (lane >> 2)) * kKeys + 16 * (lane & 3);
+        const int t = (j0 + TB * batch + lane / NG) * kKeys + 16 * (lane % NG);
         const int64_t piece = (((int64_t)o.page * a.Hkv + head) << (a.page_shift - a.block_shift)) +
                               ((t & pmask) >> a.block_shift);
         o.k = a.ks[piece];
@@ -214,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int t = tok_of(i, wtok), j = is_v(i) ? jv : jk;
-          const int page = __builtin_amdgcn_readlane(is_v(i) ? vpages : kpages, 4 * ((j - j0) & 15) + (t >> 4));
+          const int page = __builtin_amdgcn_readlane(is_v(i) ? vpages : kpages, NG * ((j - j0) & (TB - 1)) + (t >> 4));
           const int64_t row = (((int64_t)page * a.Hkv + head) << a.page_shift) + ((j * kKeys + t) & pmask);
           out[i] = *reinterpret_cast<const uint4*>((is_v(i) ? a.vc : a.kc) + row * a.D + poff);
         }
@@ -312,23 +308,24 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         }
       };
       auto k_frag = [&](const uint8_t* kt, int n) __attribute__((always_inline)) {
-        const int k = n >> 1, t = n & 1;
+        const int k = n / NH, t = n % NH;
         return *reinterpret_cast<const u4v*>(kt + ka[k & 7] + 32 * t * ROW + 256 * (k >> 3));
       };
 
       uint4 raw[PIECES];  // K's codes of tile j + 2, V's of tile j
-      u4v p[4];           // P^T of tile j - 1
+      u4v p[NG];          // P^T of tile j - 1
+      constexpr uint32_t kAll = (1u << NG) - 1;
       bool fresh = __ballot(m_run == NEG_INF) != 0;  // a row has no reference yet
       Batch now, ahead;
       // Tile j = j0 + i, scores in sc: its softmax, slice by slice between the products
       // S^T of tile j + 1 (into sn) and O^T += V^T . P^T of tile j - 1.
       auto tile_step = [&](int i, const int buf, v16f* sc, v16f* sn) __attribute__((always_inline)) {
-        const int j = j0 + i, l0 = 4 * (i & 15), tok = j * kKeys;
-        const float2* scale = &sScale[(i >> 4) & 1][l0];
+        const int j = j0 + i, l0 = NG * (i & (TB - 1)), tok = j * kKeys;
+        const float2* scale = &sScale[(i / TB) & 1][l0];
         auto top = [&]() __attribute__((always_inline)) {  // the row's largest exponent in this tile
           float mx = NEG_INF;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < NG; ++g) {
             float mg = sc[g >> 1][8 * (g & 1)];
 #pragma unroll
             for (int e = 1; e < 8; ++e) mg = __builtin_fmaxf(mg, sc[g >> 1][8 * (g & 1) + e]);
@@ -342,21 +339,21 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         // The reference m need not be the maximum: any m gives the same softmax.  So
         // no maximum is taken unless a row has no reference yet (its sums are zero
         // then), or, below, the weights of its tile pass 2^13 (f16 holds 2^15).
-        const bool border = (i & 15) == 0 && i > 0;
+        const bool border = (i & (TB - 1)) == 0 && i > 0;
         const bool seen_by_all = tok + kKeys <= all_hi && tok >= all_lo;
-        if (__builtin_expect(border || (i & 15) == 4 || !seen_by_all || partial(j) || (okm >> l0 & 15u) != 15 || fresh, 0)) {
+        if (__builtin_expect(border || (i & (TB - 1)) == 4 || !seen_by_all || partial(j) || (okm >> l0 & kAll) != kAll || fresh, 0)) {
           if (border) {
             now = ahead;
-            use(i >> 4, now);
-            ahead = load_pages((i >> 4) + 1);
+            use(i / TB, now);
+            ahead = load_pages(i / TB + 1);
           }
-          if ((i & 15) == 4) load_scales((i >> 4) + 1, ahead);
-          const uint32_t ok = (uint32_t)(okm >> l0) & 15u;
-          if (tok + kKeys > s.len || ok != 15) clear_missing(j, ok, raw);
+          if ((i & (TB - 1)) == 4) load_scales(i / TB + 1, ahead);
+          const uint32_t ok = (uint32_t)(okm >> l0) & kAll;
+          if (tok + kKeys > s.len || ok != kAll) clear_missing(j, ok, raw);
           if (partial(j)) take_nan(j, buf, raw);
-          if (!seen_by_all || ok != 15) {
+          if (!seen_by_all || ok != kAll) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < NH; ++t)
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 const int key = tok + 32 * t + 8 * (e >> 2) + 4 * g2 + (e & 3);
@@ -370,22 +367,22 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           }
         }
         // P^T = 2^(s + log2 s_v - m), so that s_v is in the exponent, and the sum takes it back
-        float2 kv = scale[3], kv_next;
+        float2 kv = scale[NG - 1], kv_next;
         float eg = 0.0f, sum = 0.0f, most = 0.0f, l_new = l_run;
-        // The granules' order is 3, 0, 1, 2: those of the tile before are used up in the
-        // order 0, 1, 2, 3, so that all but the first of the new ones take their place.
-        u4v p3;
+        // The granules' order is NG - 1, 0, 1, ...: those of the tile before are used up in
+        // the order 0, 1, ..., so that all but the first of the new ones take their place.
+        u4v p_last;
         auto weigh = [&](int n) __attribute__((always_inline)) {  // two weights
-          const int g = ((n >> 2) + 3) & 3, e = 2 * (n & 3);
+          const int g = ((n >> 2) + NG - 1) % NG, e = 2 * (n & 3);
           if (e == 0) {
             if (n > 0) kv = kv_next;
             eg = kv.y - (m_run == NEG_INF ? 0.0f : m_run);
             sum = 0.0f;
           }
-          if (e == 2 && n < 12) kv_next = scale[(g + 1) & 3];
+          if (e == 2 && n < 4 * NG - 4) kv_next = scale[(g + 1) % NG];
           const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + e], kv.x, eg));
           const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + e + 1], kv.x, eg));
-          (g == 3 ? p3 : p[g])[n & 3] = O::pack(u, w);
+          (g == NG - 1 ? p_last : p[g])[n & 3] = O::pack(u, w);
           sum += u;
           sum += w;
           if (e == 6) {  // the sum of the probabilities takes s_v back
@@ -394,7 +391,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           }
         };
 
-        constexpr int NS = 2 * KS, AHEAD = 2;  // products of each kind; slices a fragment is read ahead
+        constexpr int NP = 4 * NG, AHEAD = 2;  // pairs of weights; slices a fragment is read ahead
         const uint8_t* kt = sK[buf ^ 1];
         const uint8_t* vt = sK[2 + (buf ^ 1)];
         u4v kf[AHEAD + 1], vf[AHEAD + 1], qf[2];
@@ -405,7 +402,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           vf[n] = v_frag(vt, n / DT, n % DT);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NH; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) sn[t][e] = 0.0f;
         __builtin_amdgcn_sched_barrier(0);
@@ -415,37 +412,38 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
             kf[(n + AHEAD) % (AHEAD + 1)] = k_frag(kt, n + AHEAD);
             vf[(n + AHEAD) % (AHEAD + 1)] = v_frag(vt, (n + AHEAD) / DT, (n + AHEAD) % DT);
           }
-          if (n % 2 == 0 && n + 2 < NS) qf[(n / 2 + 1) & 1] = q_frag(n / 2 + 1);
-          sn[n & 1] = O::mfma(kf[n % (AHEAD + 1)], qf[(n >> 1) & 1], sn[n & 1]);
+          if (n % NH == 0 && n + NH < NS) qf[(n / NH + 1) & 1] = q_frag(n / NH + 1);
+          sn[n % NH] = O::mfma(kf[n % (AHEAD + 1)], qf[(n / NH) & 1], sn[n % NH]);
 #pragma unroll
-          for (int w = n * 16 / NS; w < (2 * n + 1) * 16 / (2 * NS); ++w) weigh(w);
+          for (int w = n * NP / NS; w < (2 * n + 1) * NP / (2 * NS); ++w) weigh(w);
           acc[n % DT] = O::mfma(vf[n % (AHEAD + 1)], p[n / DT], acc[n % DT]);
 #pragma unroll
-          for (int w = (2 * n + 1) * 16 / (2 * NS); w < (n + 1) * 16 / NS; ++w) weigh(w);
+          for (int w = (2 * n + 1) * NP / (2 * NS); w < (n + 1) * NP / NS; ++w) weigh(w);
           // (one piece of the next codes into LDS every few slices, then the loads)
 #pragma unroll
           for (int c = 0; c < PIECES; ++c)
             if (n == (c + 1) * NS / (PIECES + 2)) store_piece(c, buf, raw[c]);
           if (n == (PIECES + 1) * NS / (PIECES + 2))
-            load_codes(j + 3, (i & 15) >= 13 ? ahead.page : now.page, j + 1, (i & 15) == 15 ? ahead.page : now.page, raw);
+            load_codes(j + 3, (i & (TB - 1)) >= TB - 3 ? ahead.page : now.page, j + 1, (i & (TB - 1)) == TB - 1 ? ahead.page : now.page, raw);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_expect(__ballot(!(most <= 8192.0f)) != 0, 0)) {
-          asm volatile("" : "+v"(sc[0]), "+v"(sc[1]));  // (nothing of this is to be done before the branch)
+#pragma unroll
+          for (int t = 0; t < NH; ++t) asm volatile("" : "+v"(sc[t]));  // (nothing of this is to be done before the branch)
           const float nx = __builtin_fmaxf(m_run, top());
           const float alpha = nx == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - nx);
           m_run = nx;
           l_new = l_run * alpha;
-          kv = scale[3];
+          kv = scale[NG - 1];
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
 #pragma unroll
-          for (int n = 0; n < 16; ++n) weigh(n);
+          for (int n = 0; n < NP; ++n) weigh(n);
         }
         l_run = l_new;
-        p[3] = p3;
+        p[NG - 1] = p_last;
         if (__builtin_expect(i > 0 && partial(j - 1), 0)) put_nan(j - 1, buf ^ 1);
         lds_barrier();
       };
@@ -471,16 +469,16 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         }
         load_codes(j0 + 2, now.page, j0, now.page, raw);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) p[g] = u4v{0, 0, 0, 0};
+        for (int g = 0; g < NG; ++g) p[g] = u4v{0, 0, 0, 0};
       }
       lds_barrier();
-      v16f s0[2], s1[2];
+      v16f s0[NH], s1[NH];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NH; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s0[t][e] = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 2 * KS; ++n) s0[n & 1] = O::mfma(k_frag(sK[0], n), q_frag(n >> 1), s0[n & 1]);
+      for (int n = 0; n < NS; ++n) s0[n % NH] = O::mfma(k_frag(sK[0], n), q_frag(n / NH), s0[n % NH]);
       lds_barrier();
       const int n_tiles = j1 - j0;
       for (int i = 0; i < n_tiles; i += 2) {
@@ -490,7 +488,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       }
       const int lb = (n_tiles - 1) & 1;
 #pragma unroll
-      for (int n = 0; n < 2 * KS; ++n)
+      for (int n = 0; n < NS; ++n)
         acc[n % DT] = O::mfma(v_frag(sK[2] + lb * kKeys * ROW, n / DT, n % DT), p[n / DT], acc[n % DT]);
       put_nan(j1 - 1, lb);
     }
@@ -535,7 +533,7 @@ void launch_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) 
     kv8_prefill_kernel<DP, QT, NW, false><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
   } else {
     kv8_prefill_kernel<DP, QT, NW, true><<<a.parts * a.Hkv, 64 * NW, 0, st>>>(a, items);
-    kv8_merge_kernel<RT, kKeys, QT><<<(unsigned)(items * (RT / 4)), 256, 0, st>>>(a);
+    kv8_merge_kernel<RT, chunk_keys(DP), QT><<<(unsigned)(items * (RT / 4)), 256, 0, st>>>(a);
   }
 }
 

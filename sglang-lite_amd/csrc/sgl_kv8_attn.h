@@ -210,6 +210,22 @@ __device__ __forceinline__ uint32_t kv8_out2(float a, float b) {
   return pack2<QT>(a, b);
 }
 
+// Item x of the batch (row tiles in order, the heads of each together) as one segment.
+template <int RT, int TT>
+__device__ __forceinline__ bool kv8_item(const Kv8AttnArgs& a, int64_t x, int* head, Kv8Segment& g) {
+  const int64_t tile = x / a.Hkv;
+  *head = (int)(x - tile * a.Hkv);
+  Kv8Chunk c = kv8_chunk<RT, TT>(a, 0);
+  const Kv8Place at = kv8_find<RT, TT, true>(a, c, tile);
+  if (at.l < 0) return false;
+  g.s = kv8_lane<RT, TT>(a, c, at.l);
+  g.b = c.b0 + at.l;
+  g.rt = (int)(tile - at.rts);
+  g.t0 = 0;
+  g.t1 = g.s.tiles;
+  return true;
+}
+
 // The items that several workgroups share.  One wavefront a row (four a workgroup,
 // RT / 4 workgroups an item): lane p has part p's reference and weight, then all
 // lanes go over the parts' sums, several loads in flight.

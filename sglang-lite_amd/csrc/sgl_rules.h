@@ -273,15 +273,26 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
   const int64_t tiles = T * G / row_tile + B, most = T * ((G + row_tile - 1) / row_tile + 1);
   return Hkv * (tiles < most ? tiles : most);
 }
+// Few rows: whether a workgroup reads a whole item, with no merge behind.  By what
+// the block table can hold of a sequence, as the lengths are not known here: 32
+// query heads on 8 kv heads of 128, lengths up to that, whole / shared, us: 1
+// sequence 500 10.4 / 15.6, 1000 11.3 / 15.7, 2000 17.8 / 15.8; 16: 500 10.4 / 16.9,
+// 1000 12.7 / 17.6, 2000 20.1 / 19.7, 4000 34.0 / 25.6; 64: 500 14.4 / 26.4, 1000 21.6 /
+// 32.6, 2000 36.7 / 42.5, 4000 65.3 / 64.1.
+SGL_RULE bool kv8_attn_whole(int64_t capacity, int64_t items, int64_t cus) {
+  return capacity <= 1024 || (capacity <= 2048 && items >= 2 * cus);
+}
 constexpr int64_t kv8_chunk_rows(int64_t D) { return D > 64 && D <= 128 ? 256 : 128; }
-SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t cus) {
+SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
+                                   int64_t cus) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
   if (rows > 32) {
     const int64_t rt = kv8_chunk_rows(D);
     const int64_t fit = D <= 64 ? 2 * cus : cus;  // workgroups at a time
     return {rt, kv8_attn_items(T, B, Hkv, G, rt) >= 2 * fit ? 0 : kv8_attn_parts(fit, Hkv)};
   }
-  return {D <= 128 && rows > 16 ? 32 : 16, kv8_attn_parts(2 * cus, Hkv)};
+  const int64_t rt = D <= 128 && rows > 16 ? 32 : 16;
+  return {rt, kv8_attn_whole(capacity, kv8_attn_items(T, B, Hkv, G, rt), cus) ? 0 : kv8_attn_parts(2 * cus, Hkv)};
 }
 
 }  // namespace sgl

@@ -125,7 +125,7 @@ SIGNATURES = {
         [P, I64, I64, c_int, I64, I64, c_int, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P, P, P,
          P, c_float, c_int, I64, P, P, P, c_size_t, P],
     ),
-    "sgl_kv8_attn_workspace_size": (c_size_t, [I64, I64, c_int, c_int, c_int]),
+    "sgl_kv8_attn_workspace_size": (c_size_t, [I64, I64, c_int, c_int, c_int, I64]),
     "sgl_host_f32_to_e4m3": (c_int, [P, P, I64]),
     "sgl_host_e4m3_to_f32": (c_int, [P, P, I64]),
     "sgl_host_group_scale": (c_int, [c_int, P, P, I64]),
@@ -135,6 +135,7 @@ SIGNATURES = {
 _LIB: Optional[ctypes.CDLL] = None
 _FN: dict = {}         # the bound functions of _LIB by name
 _RAW_STREAM = None     # torch's raw current-stream getter, by device index
+_GET_DEVICE = None     # torch's current device index
 
 
 class SglError(RuntimeError):
@@ -256,35 +257,35 @@ def require_device(*tensors, what: str) -> None:
             )
 
 
-def require_same_device(*tensors, what: str) -> None:
-    """One call's tensors lie on one GPU."""
-    at = None
-    for t in tensors:
-        if t is not None:
-            d = t.get_device()
-            if at is None:
-                at = d
-            elif d != at:
-                raise ValueError(f"{what}: tensors on devices {at} and {d}")
+def device_of(what: str, first, *others) -> int:
+    """The one GPU that a call's tensors (None: left out) lie on."""
+    d = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
+            d = -1
+            break
+    if d < 0:
+        require_device(first, *others, what=what)
+        raise ValueError(f"{what}: tensors on devices "
+                         f"{sorted({t.get_device() for t in (first, *others) if t is not None})}")
+    return d
 
 
-class _Here:
-    """The context of :func:`on_device` where nothing has to change."""
+def call_on(d: int, name: str, *args) -> None:
+    """:func:`call` with device ``d`` the current one, on torch's stream there (the
+    last argument): a launch goes to the current device, whatever device its
+    pointers belong to."""
+    global _RAW_STREAM, _GET_DEVICE
+    if _GET_DEVICE is None:
+        import torch
 
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def on_device(t):
-    """A context in which ``t``'s device is the current one: a launch goes to the
-    current device, whatever device its stream and pointers belong to."""
+        _GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        _RAW_STREAM = _RAW_STREAM or getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+    if _GET_DEVICE() == d:
+        call(name, *args, _RAW_STREAM(d))
+        return
     import torch
 
-    d = t.get_device()
-    return _HERE if torch._C._cuda_getDevice() == d else torch.cuda.device(d)
+    with torch.cuda.device(d):
+        call(name, *args, _RAW_STREAM(d))

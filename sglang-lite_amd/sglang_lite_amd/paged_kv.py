@@ -16,6 +16,7 @@ a HIP graph and replayed with other lengths.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -59,45 +60,56 @@ def _check_sizes(pages, heads, page, dim, block, what):
 
 def _check_cache(cache: PagedKV, what: str):
     k, v, ks, vs = cache
-    if k.dim() != 4 or k.dtype != FP8 or v.dtype != FP8 or v.shape != k.shape:
+    shape, scales = k.shape, ks.shape
+    if len(shape) != 4 or k.dtype is not FP8 or v.dtype is not FP8 or v.shape != shape:
         raise ValueError(f"{what}: cache codes must be float8_e4m3fn [pages, Hkv, page, D], got "
-                         f"{k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    pages, heads, page, dim = k.shape
-    if ks.dim() != 3 or ks.shape != vs.shape or ks.shape[0] != pages or ks.shape[1] != heads or \
-            ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape[2] < 1 or \
-            page % ks.shape[2]:
+                         f"{k.dtype} {tuple(shape)} and {v.dtype} {tuple(v.shape)}")
+    pages, heads, page, dim = shape
+    if len(scales) != 3 or vs.shape != scales or scales[0] != pages or scales[1] != heads or \
+            ks.dtype is not torch.float32 or vs.dtype is not torch.float32 or scales[2] < 1 or \
+            page % scales[2]:
         raise ValueError(f"{what}: cache scales must be float32 [{pages}, {heads}, page / block], got "
-                         f"{ks.dtype} {tuple(ks.shape)} and {vs.dtype} {tuple(vs.shape)}")
+                         f"{ks.dtype} {tuple(scales)} and {vs.dtype} {tuple(vs.shape)}")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f"{what}: the cache's tensors must be contiguous")
-    return pages, heads, page, dim, page // ks.shape[2]
+    return pages, heads, page, dim, page // scales[2]
 
 
 def _check_batch(rows: int, block_table: torch.Tensor, lens: torch.Tensor,
-                 cu_tokens: Optional[torch.Tensor], name: str, what: str) -> int:
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or not block_table.is_contiguous():
+                 cu_tokens: Optional[torch.Tensor], name: str, what: str):
+    shape = block_table.shape
+    if len(shape) != 2 or block_table.dtype is not torch.int32 or not block_table.is_contiguous():
         raise ValueError(f"{what}: block_table must be a contiguous int32 [B, pages], got "
-                         f"{block_table.dtype} {tuple(block_table.shape)}")
-    B = block_table.shape[0]
-    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+                         f"{block_table.dtype} {tuple(shape)}")
+    B = shape[0]
+    if lens.dtype is not torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous int32 [{B}], got {lens.dtype} "
                          f"{tuple(lens.shape)}")
     if cu_tokens is None:
         if rows != B:
             raise ValueError(f"{what}: {rows} rows for {B} sequences of one token each; pass cu_tokens")
-    elif cu_tokens.dtype != torch.int32 or cu_tokens.shape != (B + 1,) or \
+    elif cu_tokens.dtype is not torch.int32 or cu_tokens.shape != (B + 1,) or \
             not cu_tokens.is_contiguous():
         raise ValueError(f"{what}: cu_tokens must be a contiguous int32 [{B + 1}], got "
                          f"{cu_tokens.dtype} {tuple(cu_tokens.shape)}")
-    return B
+    return shape
 
 
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """``x`` itself where its rows can be read 16 bytes at a time, else a copy."""
-    n = 16 // x.element_size()
-    if x.stride(2) == 1 and x.stride(0) % n == 0 and x.stride(1) % n == 0 and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)  # (a fresh buffer, which is aligned)
+def _rows16(x: torch.Tensor, n: int):
+    """``x`` and its strides where its rows can be read 16 bytes (``n`` elements) at a
+    time, else those of a copy."""
+    s = x.stride()
+    if s[2] == 1 and s[0] % n == 0 and s[1] % n == 0 and x.data_ptr() % 16 == 0:
+        return x, s
+    x = x.clone(memory_format=torch.contiguous_format)  # (a fresh buffer, which is aligned)
+    return x, x.stride()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(device: int, *sizes: int) -> int:
+    """Bytes for the attention of these sizes: a function of them and of the device's CUs."""
+    with torch.cuda.device(device):
+        return _lib.size_of("sgl_kv8_attn_workspace_size", *sizes)
 
 
 def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -120,15 +132,16 @@ def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: tor
     must belong to one sequence of the call; pages that are only read (the full
     pages of a common prefix) may be shared."""
     pages, heads, page, dim, block = _check_cache(cache, "append_kv")
-    if k.dim() != 3 or k.shape[1] != heads or k.shape[2] != dim or v.shape != k.shape:
-        raise ValueError(f"append_kv: expected k and v [T, {heads}, {dim}], got {tuple(k.shape)} and "
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape:
+        raise ValueError(f"append_kv: expected k and v [T, {heads}, {dim}], got {tuple(shape)} and "
                          f"{tuple(v.shape)}")
     dt = DTYPES.get(k.dtype)
-    if dt is None or v.dtype != k.dtype:
+    if dt is None or v.dtype is not k.dtype:
         raise TypeError(f"append_kv: k and v must be bfloat16, float16 or float32, got {k.dtype} and "
                         f"{v.dtype}")
-    T = k.shape[0]
-    B = _check_batch(T, block_table, start, cu_tokens, "start", "append_kv")
+    T = shape[0]
+    B, columns = _check_batch(T, block_table, start, cu_tokens, "start", "append_kv")
     rot = n_positions = 0
     if table is not None:
         rot = check_table(table, offset, dim, "append_kv")
@@ -136,26 +149,23 @@ def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: tor
         if rot % 16 or offset % 8:
             raise ValueError(f"append_kv: rotated elements must be a multiple of 16 at an offset that is "
                              f"one of 8, got {rot} at {offset}")
-        if positions is not None and (positions.dtype != torch.int32 or positions.shape != (T,)
+        if positions is not None and (positions.dtype is not torch.int32 or positions.shape != (T,)
                                       or not positions.is_contiguous()):
             raise ValueError(f"append_kv: positions must be a contiguous int32 [{T}], got "
                              f"{positions.dtype} {tuple(positions.shape)}")
     elif positions is not None:
         raise ValueError("append_kv: positions without a rotary table")
-    _lib.require_device(k, v, block_table, start, cu_tokens, table, positions, *cache,
-                        what="append_kv")
-    _lib.require_same_device(k, v, block_table, start, cu_tokens, table, positions, *cache,
-                             what="append_kv")
+    kc, vc, ks, vs = cache
+    d = _lib.device_of("append_kv", k, v, block_table, start, cu_tokens, table, positions, kc, vc, ks, vs)
     if T == 0 or B == 0:
         return
-    k, v = _rows16(k), _rows16(v)
-    with _lib.on_device(k):
-        _lib.call("sgl_kv8_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                  v.stride(1), dt, T, B, heads, dim, _lib.ptr(cu_tokens), start.data_ptr(),
-                  block_table.data_ptr(), block_table.shape[1], page, block, pages, _lib.ptr(table),
-                  n_positions, rot, offset, _lib.ptr(positions), interleaved, cache.k.data_ptr(),
-                  cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-                  _lib.stream_of(k))
+    n = 4 if dt == _lib.SGL_F32 else 8
+    k, sk = _rows16(k, n)
+    v, sv = _rows16(v, n)
+    _lib.call_on(d, "sgl_kv8_append", k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], dt, T, B,
+                 heads, dim, _lib.ptr(cu_tokens), start.data_ptr(), block_table.data_ptr(), columns,
+                 page, block, pages, _lib.ptr(table), n_positions, rot, offset, _lib.ptr(positions),
+                 interleaved, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr())
 
 
 def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens: torch.Tensor, *,
@@ -172,38 +182,38 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     ``softmax_scale``: ``D ** -0.5`` by default.  A row that sees no key is zero;
     rows of ``out`` behind the last sequence are left as they are."""
     pages, heads, page, dim, block = _check_cache(cache, "paged_attn")
-    if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % heads:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dim or shape[1] < 1 or shape[1] % heads:
         raise ValueError(f"paged_attn: expected q [T, Hq, {dim}] with Hq a multiple of {heads}, got "
-                         f"{tuple(q.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+                         f"{tuple(shape)}")
+    dt = DTYPES.get(q.dtype)
+    if dt is None or dt == _lib.SGL_F32:
         raise TypeError(f"paged_attn: q must be bfloat16 or float16, got {q.dtype}")
-    T, hq, _ = q.shape
-    B = _check_batch(T, block_table, lens, cu_tokens, "lens", "paged_attn")
-    if sink is not None and (sink.dtype != torch.float32 or sink.shape != (hq,)
+    T, hq, _ = shape
+    B, columns = _check_batch(T, block_table, lens, cu_tokens, "lens", "paged_attn")
+    if sink is not None and (sink.dtype is not torch.float32 or sink.shape != (hq,)
                              or not sink.is_contiguous()):
         raise ValueError(f"paged_attn: sink must be a contiguous float32 [{hq}], got {sink.dtype} "
                          f"{tuple(sink.shape)}")
     if window < 0 or (window and not causal):
         raise ValueError(f"paged_attn: window ({window}) must not be negative and is for causal attention")
-    _lib.require_device(q, block_table, lens, cu_tokens, sink, out, *cache, what="paged_attn")
-    _lib.require_same_device(q, block_table, lens, cu_tokens, sink, out, *cache, what="paged_attn")
+    kc, vc, ks, vs = cache
+    d = _lib.device_of("paged_attn", q, block_table, lens, cu_tokens, sink, out, kc, vc, ks, vs)
     if out is None:
-        out = torch.empty((T, hq, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError(f"paged_attn: out must be a contiguous {q.dtype} {tuple(q.shape)}, got "
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous():
+        raise ValueError(f"paged_attn: out must be a contiguous {q.dtype} {tuple(shape)}, got "
                          f"{out.dtype} {tuple(out.shape)}")
     if T == 0 or B == 0:
         return out
-    q = _rows16(q)
-    with _lib.on_device(q):
-        nws = _lib.size_of("sgl_kv8_attn_workspace_size", T, B, heads, hq // heads, dim)
-        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
-        _lib.call("sgl_kv8_attn", q.data_ptr(), q.stride(0), q.stride(1), DTYPES[q.dtype], T, B, heads,
-                  hq // heads, dim, _lib.ptr(cu_tokens), lens.data_ptr(), block_table.data_ptr(),
-                  block_table.shape[1], page, block, pages, cache.k.data_ptr(), cache.v.data_ptr(),
-                  cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-                  dim ** -0.5 if softmax_scale is None else float(softmax_scale), causal, int(window),
-                  _lib.ptr(sink), out.data_ptr(), ws.data_ptr(), nws, _lib.stream_of(q))
+    q, sq = _rows16(q, 8)
+    nws = _workspace(d, T, B, heads, hq // heads, dim, columns * page)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    _lib.call_on(d, "sgl_kv8_attn", q.data_ptr(), sq[0], sq[1], dt, T, B, heads, hq // heads, dim,
+                 _lib.ptr(cu_tokens), lens.data_ptr(), block_table.data_ptr(), columns, page, block,
+                 pages, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+                 dim ** -0.5 if softmax_scale is None else softmax_scale, causal, window,
+                 _lib.ptr(sink), out.data_ptr(), _lib.ptr(ws), nws)
     return out
 
 

@@ -80,19 +80,18 @@ def rotary_table(n_positions: int, rot_dim: int, base: float = 10000.0, *,
                            "(there is no CPU path)")
     freq = freq.to(device)
     table = torch.empty(n_positions, rot_dim // 2, 2, dtype=torch.float32, device=freq.device)
-    with _lib.on_device(freq):
-        _lib.call("sgl_rotary_table", freq.data_ptr(), length, n_positions, rot_dim, table.data_ptr(),
-                  _lib.stream_of(freq))
+    _lib.call_on(freq.get_device(), "sgl_rotary_table", freq.data_ptr(), length, n_positions, rot_dim,
+                 table.data_ptr())
     return table
 
 
 def check_table(table: torch.Tensor, offset: int, dim: int, what: str) -> int:
     """rot_dim of a table that fits into heads of ``dim`` elements at ``offset``."""
-    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or \
-            not table.is_contiguous():
+    shape = table.shape
+    if len(shape) != 3 or shape[2] != 2 or table.dtype is not torch.float32 or not table.is_contiguous():
         raise ValueError(f"{what}: table must be a contiguous float32 [positions, pairs, 2], got "
-                         f"{table.dtype} {tuple(table.shape)}")
-    rot = 2 * table.shape[1]
+                         f"{table.dtype} {tuple(shape)}")
+    rot = 2 * shape[1]
     if offset < 0 or offset + rot > dim:
         raise ValueError(f"{what}: {rot} rotated elements at offset {offset} do not fit into {dim}")
     return rot
@@ -107,36 +106,37 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     ``i + rot_dim / 2`` of them, or ``2 i`` and ``2 i + 1`` with ``interleaved``.
     A negative position (a padding row) leaves its row as it is, one behind the
     table gives NaN.  ``out`` may be ``x`` itself."""
-    if x.dim() != 3:
-        raise ValueError(f"rotary: expected x [T, H, D], got {tuple(x.shape)}")
-    T, H, D = x.shape
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"rotary: expected x [T, H, D], got {tuple(shape)}")
+    T, H, D = shape
     dt = DTYPES.get(x.dtype)
     if dt is None:
         raise TypeError(f"rotary: x must be bfloat16, float16 or float32, got {x.dtype}")
     rot = check_table(table, offset, D, "rotary")
-    if positions.dim() != 1 or positions.shape[0] != T:
+    if positions.shape != (T,):
         raise ValueError(f"rotary: expected positions [{T}], got {tuple(positions.shape)}")
-    if positions.dtype not in (torch.int32, torch.int64):
+    wide = positions.dtype is torch.int64
+    if not wide and positions.dtype is not torch.int32:
         raise TypeError(f"rotary: positions must be int32 or int64, got {positions.dtype}")
-    _lib.require_device(x, table, positions, out, what="rotary")
-    _lib.require_same_device(x, table, positions, out, what="rotary")
-    if x.stride(2) != 1 and D > 1:
+    d = _lib.device_of("rotary", x, table, positions, out)
+    xs = x.stride()
+    if xs[2] != 1 and D > 1:
         x = x.contiguous()
+        xs = x.stride()
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-    else:
-        if out.shape != x.shape or out.dtype != x.dtype or (out.stride(2) != 1 and D > 1):
-            raise ValueError(f"rotary: out must be {x.dtype} {tuple(x.shape)} with a dense last "
-                             f"dimension, got {out.dtype} {tuple(out.shape)}")
-        if (T > 1 and abs(out.stride(0)) < D) or (H > 1 and abs(out.stride(1)) < D):
-            raise ValueError("rotary: rows of out overlap")
-    if positions.stride(0) != 1:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype is not x.dtype or (out.stride(2) != 1 and D > 1):
+        raise ValueError(f"rotary: out must be {x.dtype} {tuple(shape)} with a dense last "
+                         f"dimension, got {out.dtype} {tuple(out.shape)}")
+    elif (T > 1 and abs(out.stride(0)) < D) or (H > 1 and abs(out.stride(1)) < D):
+        raise ValueError("rotary: rows of out overlap")
+    os = out.stride()
+    if not positions.is_contiguous():
         positions = positions.contiguous()
-    with _lib.on_device(x):
-        _lib.call("sgl_rotary", x.data_ptr(), dt, T, H, D, x.stride(0), x.stride(1), table.data_ptr(),
-                  table.shape[0], rot, offset, positions.data_ptr(), positions.dtype == torch.int64,
-                  interleaved, inverse, out.data_ptr(), out.stride(0), out.stride(1),
-                  _lib.stream_of(x))
+    _lib.call_on(d, "sgl_rotary", x.data_ptr(), dt, T, H, D, xs[0], xs[1], table.data_ptr(),
+                 table.shape[0], rot, offset, positions.data_ptr(), wide, interleaved, inverse,
+                 out.data_ptr(), os[0], os[1])
     return out
 
 

@@ -243,10 +243,10 @@ def test_the_library_refuses_before_any_launch():
         with pytest.raises(ValueError, match="kv8_attn"):
             L.call("sgl_kv8_attn", *attn(**kw))
     with pytest.raises(L.SglError, match="workspace") as e:
-        L.call("sgl_kv8_attn", *attn())
+        L.call("sgl_kv8_attn", *attn(cols=1000))
     assert e.value.status == L.SGL_ERR_WORKSPACE
     L.call("sgl_kv8_attn", *attn(T=0, cu=p, q=None))
-    assert L.load().sgl_kv8_attn_workspace_size(-1, 1, 1, 1, 64) == 0
+    assert L.load().sgl_kv8_attn_workspace_size(-1, 1, 1, 1, 64, 4096) == 0
 
 
 def test_oracle_attention_is_a_softmax():
