@@ -283,13 +283,28 @@ SGL_RULE bool kv8_attn_whole(int64_t capacity, int64_t items, int64_t cus) {
   return capacity <= 1024 || (capacity <= 2048 && items >= 2 * cus);
 }
 constexpr int64_t kv8_chunk_rows(int64_t D) { return D > 64 && D <= 128 ? 256 : 128; }
+// Few rows or a chunk, by a sequence's rows on a kv head (few / chunk, us, 4 query heads
+// to each of 8 kv heads; 1 sequence of 16000 tokens and 8 of 4000).  Heads of 128: 64 rows
+// 32 / 34 and 43 / 47, 96 rows 38 / 35 and 56 / 51, 128 rows 40 / 36 and 66 / 56.  Of 64: 64 rows
+// 23 / 26 and 29 / 31, 96 rows 25 / 27 and 37 / 35.  Of 256: 16 rows 40 / 39 and 36 / 50, 32
+// rows 46 / 39 and 62 / 52, 64 rows 60 / 42 and 97 / 62.
+SGL_RULE bool kv8_attn_chunk(int64_t rows, int64_t D) { return rows > (D <= 128 ? 64 : 16); }
+// A chunk's row tiles go to workgroups whole where there are two for every workgroup
+// at a time (fit), or few keys to divide: up to 4096 at one item a place, half of that
+// at half of the items.  Whole / shared, us, 32 query heads on 8 kv heads of 128:
+// 1 x 512 queries on 512 keys 26 / 38, 1500 keys 54 / 47, 3000 96 / 58; 1 x 1024 on 2000 72 / 82, on
+// 3500 111 / 103; 1 x 2560 on 5000 212 / 258, on 8500 408 / 394; 16 x 64 on 2500 86 / 103, on 6000
+// 178 / 161; 1 x 8192 on 8192 563 / 1030.
+SGL_RULE bool kv8_chunk_whole(int64_t capacity, int64_t items, int64_t fit) {
+  return items >= 2 * fit || capacity <= 1024 || capacity * fit <= 4096 * items;
+}
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
                                    int64_t cus) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
-  if (rows > 32) {
+  if (kv8_attn_chunk(rows, D)) {
     const int64_t rt = kv8_chunk_rows(D);
-    const int64_t fit = D <= 64 ? 2 * cus : cus;  // workgroups at a time
-    return {rt, kv8_attn_items(T, B, Hkv, G, rt) >= 2 * fit ? 0 : kv8_attn_parts(fit, Hkv)};
+    const int64_t fit = D <= 64 ? 2 * cus : cus;
+    return {rt, kv8_chunk_whole(capacity, kv8_attn_items(T, B, Hkv, G, rt), fit) ? 0 : kv8_attn_parts(fit, Hkv)};
   }
   const int64_t rt = D <= 128 && rows > 16 ? 32 : 16;
   return {rt, kv8_attn_whole(capacity, kv8_attn_items(T, B, Hkv, G, rt), cus) ? 0 : kv8_attn_parts(2 * cus, Hkv)};
