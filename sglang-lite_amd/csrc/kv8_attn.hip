@@ -18,9 +18,10 @@
 //     holds the A operands of C tiles of 16 dims (row m of tile j: dim C m + j).
 // A conversion e4m3 -> bf16 (exact) is one instruction for two codes.  The
 // scales are one number for 16 tokens: s_k multiplies the score, log2 s_v is added
-// to it, so that P carries s_v.  P is rounded to q's type (half a step: 2^-9
-// relative in bf16, 2^-12 in f16), the only rounding between the codes and the
-// output's own.
+// to it, so that P carries s_v.  P and the codes of V are f16 for every type of q: a
+// code is exact there, a weight is rounded by at most 2^-12 of itself (bf16: 2^-9) or
+// 2^-25 of the row's reference, and that is the only rounding between the codes and
+// the output's own.
 #include "sgl_kv8_attn.h"
 
 namespace sgl {
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void kv8_attn_few_k
     };
 
     // acc += V^T . P^T for the codes v of the step
-    auto accumulate = [&](const uint32_t (*v)[W], const typename Op<QT>::V* p) __attribute__((always_inline)) {
+    auto accumulate = [&](const uint32_t (*v)[W], const v8h* p) __attribute__((always_inline)) {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         uint32_t x0[4], x1[4];
@@ -224,9 +225,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void kv8_attn_few_k
         transpose4(v[4][w], v[5][w], v[6][w], v[7][w], x1);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const typename Op<QT>::V f = cvt8<QT>(x0[k], x1[k]);
+          const v8h f = cvt8<SGL_F16>(x0[k], x1[k]);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) acc[c][4 * w + k] = Op<QT>::mfma(f, p[c], acc[c][4 * w + k]);
+          for (int c = 0; c < NC; ++c) acc[c][4 * w + k] = Op<SGL_F16>::mfma(f, p[c], acc[c][4 * w + k]);
         }
       }
     };
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void kv8_attn_few_k
         ev[u] = lane_f(evs, l0 + u);
         iv[u] = lane_f(ivs, l0 + u);
       }
-      typename Op<QT>::V p[NC];
+      v8h p[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         float f[8];
@@ -320,8 +321,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void kv8_attn_few_k
         }
         l_run[c] += l;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2<QT>(f[2 * i], f[2 * i + 1]);
-        p[c] = __builtin_bit_cast(typename Op<QT>::V, u4v{w[0], w[1], w[2], w[3]});
+        for (int i = 0; i < 4; ++i) w[i] = pack2<SGL_F16>(f[2 * i], f[2 * i + 1]);
+        p[c] = __builtin_bit_cast(v8h, u4v{w[0], w[1], w[2], w[3]});
       }
       if (!plain) {
         // What no row sees must not reach the product: keys behind the last

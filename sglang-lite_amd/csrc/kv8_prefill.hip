@@ -36,7 +36,6 @@ struct Wide<SGL_BF16> {
   static __device__ __forceinline__ uint32_t cvt(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
   }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pk2_bf16(a, b); }
 };
 template <>
 struct Wide<SGL_F16> {
@@ -80,7 +79,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
   constexpr int SIDE = kKeys * CPR;          // pieces of K's tile, and of V's behind them
   constexpr int PIECES = 2 * SIDE / NT;      // of a thread
   static_assert(PIECES * NT == 2 * SIDE && SIDE % NT == 0, "a thread's first pieces are K's, the others V's");
-  typedef Wide<QT> O;
+  typedef Wide<QT> O;       // K's codes, as q
+  typedef Wide<SGL_F16> F;  // V's codes and the weights
   __shared__ __align__(16) uint8_t sK[4][kKeys * ROW];  // K, K, V, V
   // Q^T fragments: in LDS where the registers are short
   constexpr bool QL = DP >= 128;
@@ -226,10 +226,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         u4v lo, hi2;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          lo[2 * k] = O::template cvt<false>(w[k]);
-          lo[2 * k + 1] = O::template cvt<true>(w[k]);
-          hi2[2 * k] = O::template cvt<false>(w[2 + k]);
-          hi2[2 * k + 1] = O::template cvt<true>(w[2 + k]);
+          lo[2 * k] = is_v(i) ? F::template cvt<false>(w[k]) : O::template cvt<false>(w[k]);
+          lo[2 * k + 1] = is_v(i) ? F::template cvt<true>(w[k]) : O::template cvt<true>(w[k]);
+          hi2[2 * k] = is_v(i) ? F::template cvt<false>(w[2 + k]) : O::template cvt<false>(w[2 + k]);
+          hi2[2 * k + 1] = is_v(i) ? F::template cvt<true>(w[2 + k]) : O::template cvt<true>(w[2 + k]);
         }
         uint8_t* to = sK[buf] + i * NT / SIDE * (2 * kKeys * ROW) + i * NT % SIDE / CPR * ROW;
         *reinterpret_cast<u4v*>(to + (is_v(i) ? vdst0 : kdst0)) = lo;
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           if (e == 2 && n < 4 * NG - 4) kv_next = scale[(g + 1) % NG];
           const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + e], kv.x, eg));
           const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + e + 1], kv.x, eg));
-          (g == NG - 1 ? p_last : p[g])[n & 3] = O::pack(u, w);
+          (g == NG - 1 ? p_last : p[g])[n & 3] = F::pack(u, w);
           sum += u;
           sum += w;
           if (e == 6) {  // the sum of the probabilities takes s_v back
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           sn[n % NH] = O::mfma(kf[n % (AHEAD + 1)], qf[(n / NH) & 1], sn[n % NH]);
 #pragma unroll
           for (int w = n * NP / NS; w < (2 * n + 1) * NP / (2 * NS); ++w) weigh(w);
-          acc[n % DT] = O::mfma(vf[n % (AHEAD + 1)], p[n / DT], acc[n % DT]);
+          acc[n % DT] = F::mfma(vf[n % (AHEAD + 1)], p[n / DT], acc[n % DT]);
 #pragma unroll
           for (int w = (2 * n + 1) * NP / (2 * NS); w < (n + 1) * NP / NS; ++w) weigh(w);
           // (one piece of the next codes into LDS every few slices, then the loads)
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       const int lb = (n_tiles - 1) & 1;
 #pragma unroll
       for (int n = 0; n < NS; ++n)
-        acc[n % DT] = O::mfma(v_frag(sK[2] + lb * kKeys * ROW, n / DT, n % DT), p[n / DT], acc[n % DT]);
+        acc[n % DT] = F::mfma(v_frag(sK[2] + lb * kKeys * ROW, n / DT, n % DT), p[n / DT], acc[n % DT]);
       put_nan(j1 - 1, lb);
     }
 
