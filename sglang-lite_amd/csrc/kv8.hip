@@ -30,6 +30,7 @@ struct AppendArgs {
   int64_t n_positions;
   int64_t n_pages;
   int T, B, Hkv, D, row_pages, page_shift, block_shift;
+  int per_magic;  // i / (D / 16) = i per_magic >> 16 for i < 4096
   int rot, offset;
   bool interleaved;
 };
@@ -82,9 +83,33 @@ __device__ __forceinline__ Unit find_unit(const AppendArgs& a, int u) {
   return {r.first + (int)(lo - st), (int)(hi - lo), (int)lo, page};
 }
 
+// 4 values by 1 / s, a power of two, to codes (v_cvt_scalef32_pk_fp8: scaled and
+// rounded in one); finite ones alone, at most 448 s.
+typedef short s2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float s) {
+  s2v o = {0, 0};
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, a, b, s, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, c, d, s, true));
+}
+// the same of packed 16-bit values
+template <int DT>
+__device__ __forceinline__ uint32_t codes4(uint32_t ab, uint32_t cd, float s) {
+  s2v o = {0, 0};
+  if constexpr (DT == SGL_BF16) {
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(sgl_bf2, ab), s, false);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(sgl_bf2, cd), s, true);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(h2, ab), s, false);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(h2, cd), s, true);
+  }
+  return __builtin_bit_cast(uint32_t, o);
+}
+
 // NT threads, IT units of 16 elements a thread
 template <int DT, int NT, int IT>
 __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
+  constexpr int RW = DT == SGL_F32 ? 2 : 1;  // 16-byte words of 8 elements
   const int head = (int)blockIdx.y >> 1;
   const bool keys = (blockIdx.y & 1) == 0;
   const Unit w = find_unit(a, (int)blockIdx.x);
@@ -94,16 +119,22 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
   const int rot = keys ? a.rot : 0;
   const int per = a.D >> 4, rot_units = rot >> 4;
   const int count = w.n * per;
+  // What is not rotated stays packed: its largest by integers, its codes in one
+  // instruction for two.
+  const bool packed = DT != SGL_F32 && rot == 0;
 
+  uint4 raw[IT][2 * RW];
   float x[IT][16];
   int e0[IT], e1[IT], tok[IT];
+  bool odd[IT];  // a NaN or an infinity among them
   float amax = 0.0f;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int i = it * NT + (int)threadIdx.x;
     tok[it] = -1;
+    odd[it] = false;
     if (i < count) {
-      const int t = i / per, u = i - t * per;
+      const int t = i * a.per_magic >> 16, u = i - t * per;
       int p0, p1;  // two chunks of 8 elements: those of 8 pairs, or two of the others
       if (u < rot_units) {
         p0 = a.offset + (a.interleaved ? 16 : 8) * u;
@@ -114,37 +145,70 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
         p1 = c + 8 < off ? c + 8 : c + 8 + rot;
       }
       const int64_t at = (int64_t)(w.row0 + t) * st + (int64_t)head * sh;
-      load8<DT>(src, at + p0, x[it]);
-      load8<DT>(src, at + p1, x[it] + 8);
+      load_raw8<DT>(src, at + p0, raw[it]);
+      load_raw8<DT>(src, at + p1, raw[it] + RW);
       tok[it] = t;
       e0[it] = p0;
       e1[it] = p1;
-      if (u < rot_units) {
-        float cs[8], sn[8];
-        const int64_t pos = a.positions ? a.positions[w.row0 + t] : w.at + t;
-        load_turn<8>(a.table, a.n_positions, a.rot >> 1, pos, 8 * u, false, cs, sn);
-        if (a.interleaved) {
-          float p[8], q[8];
+      float top;
+      if (packed) {
+        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+        us2 m = {0, 0};
 #pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            p[v] = x[it][2 * v];
-            q[v] = x[it][2 * v + 1];
-          }
-          rotate_pairs<8>(p, q, cs, sn);
+        for (int v = 0; v < 2 * RW; ++v) {
+          const uint32_t q[4] = {raw[it][v].x, raw[it][v].y, raw[it][v].z, raw[it][v].w};
 #pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            x[it][2 * v] = p[v];
-            x[it][2 * v + 1] = q[v];
+          for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, q[j] & 0x7FFF7FFFu));
+        }
+        const uint32_t most = m.x > m.y ? m.x : m.y;
+        odd[it] = most >= (DT == SGL_BF16 ? 0x7F80u : 0x7C00u);
+        top = DT == SGL_BF16 ? bits_f32(most << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)most);
+      } else {
+        widen8<DT>(raw[it], x[it]);
+        widen8<DT>(raw[it] + RW, x[it] + 8);
+        if (u < rot_units) {
+          float cs[8], sn[8];
+          const int64_t pos = a.positions ? a.positions[w.row0 + t] : w.at + t;
+          load_turn<8>(a.table, a.n_positions, a.rot >> 1, pos, 8 * u, false, cs, sn);
+          if (a.interleaved) {
+            float p[8], q[8];
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              p[v] = x[it][2 * v];
+              q[v] = x[it][2 * v + 1];
+            }
+            rotate_pairs<8>(p, q, cs, sn);
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              x[it][2 * v] = p[v];
+              x[it][2 * v + 1] = q[v];
+            }
+          } else {
+            rotate_pairs<8>(x[it], x[it] + 8, cs, sn);
           }
-        } else {
-          rotate_pairs<8>(x[it], x[it] + 8, cs, sn);
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const uint32_t m = f32_bits(x[it][v]) & 0x7FFFFFFFu;
+          most = m > most ? m : most;
+        }
+        odd[it] = most >= 0x7F800000u;
+        top = bits_f32(most);
+      }
+      if (__builtin_expect(odd[it], 0)) {  // finite values alone
+        if (packed) {
+          widen8<DT>(raw[it], x[it]);
+          widen8<DT>(raw[it] + RW, x[it] + 8);
+        }
+        top = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float m = __builtin_fabsf(x[it][v]);
+          top = m < __builtin_huge_valf() && m > top ? m : top;
         }
       }
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const float m = __builtin_fabsf(x[it][v]);
-        amax = m < __builtin_huge_valf() ? __builtin_fmaxf(amax, m) : amax;  // finite values alone
-      }
+      amax = top > amax ? top : amax;
     }
   }
 #pragma unroll
@@ -185,19 +249,35 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
       *at = make_uint4(q[0], q[1], q[2], q[3]);
     }
   }
-  const float inv = 1.0f / s;  // exact for the powers of two that this kernel writes
   if (threadIdx.x == 0) *scale = s;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     if (tok[it] >= 0) {
       uint8_t* row = codes + (int64_t)(spot + tok[it]) * a.D;
-      float* f = x[it];
+      uint32_t c[4];
+      if (__builtin_expect(odd[it], 0)) {  // an infinity becomes the NaN code, a NaN keeps its sign
+        const float inv = 1.0f / s;        // exact for the powers of two that this kernel writes
+        const float* f = x[it];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) f[v] *= inv;  // at most 448; an infinity becomes the NaN code
-      *reinterpret_cast<uint2*>(row + e0[it]) =
-          make_uint2(pk4_e4m3_exact(f[0], f[1], f[2], f[3]), pk4_e4m3_exact(f[4], f[5], f[6], f[7]));
-      *reinterpret_cast<uint2*>(row + e1[it]) =
-          make_uint2(pk4_e4m3_exact(f[8], f[9], f[10], f[11]), pk4_e4m3_exact(f[12], f[13], f[14], f[15]));
+        for (int j = 0; j < 4; ++j)
+          c[j] = pk4_e4m3_exact(f[4 * j] * inv, f[4 * j + 1] * inv, f[4 * j + 2] * inv, f[4 * j + 3] * inv);
+      } else if (packed) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          c[2 * v] = codes4<DT>(raw[it][v].x, raw[it][v].y, s);
+          c[2 * v + 1] = codes4<DT>(raw[it][v].z, raw[it][v].w, s);
+        }
+      } else {
+        const float* f = x[it];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = codes4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3], s);
+      }
+      if (rot == 0) {  // the two chunks lie side by side
+        *reinterpret_cast<uint4*>(row + e0[it]) = make_uint4(c[0], c[1], c[2], c[3]);
+      } else {
+        *reinterpret_cast<uint2*>(row + e0[it]) = make_uint2(c[0], c[1]);
+        *reinterpret_cast<uint2*>(row + e1[it]) = make_uint2(c[2], c[3]);
+      }
     }
   }
 }
@@ -274,6 +354,7 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
   a.row_pages = (int)row_pages;
   a.page_shift = __builtin_ctz((unsigned)page_size);
   a.block_shift = __builtin_ctz((unsigned)block);
+  a.per_magic = 65536 / (D / 16) + 1;
   a.rot = table ? rot_dim : 0;
   a.offset = table ? offset : 0;
   a.interleaved = interleaved != 0;

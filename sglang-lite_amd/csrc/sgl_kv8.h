@@ -27,17 +27,19 @@ inline int kv8_check_cache(const char* what, int Hkv, int D, int page, int block
   return SGL_OK;
 }
 
-// Eight consecutive elements of a row as fp32.
+// Eight elements of a row as fp32.
 template <int DT>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float* f) {
+__device__ __forceinline__ void widen8(const uint4* raw, float* f) {
   if constexpr (DT == SGL_F32) {
-    const float4* p = reinterpret_cast<const float4*>((const float*)base + at);
-    const float4 a = p[0], b = p[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[4 * i] = bits_f32(raw[i].x);
+      f[4 * i + 1] = bits_f32(raw[i].y);
+      f[4 * i + 2] = bits_f32(raw[i].z);
+      f[4 * i + 3] = bits_f32(raw[i].w);
+    }
   } else {
-    const uint4 w = *reinterpret_cast<const uint4*>((const uint16_t*)base + at);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t v[4] = {raw->x, raw->y, raw->z, raw->w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (DT == SGL_BF16) {
@@ -51,6 +53,23 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, float* f) {
       }
     }
   }
+}
+// Eight consecutive ones as they lie: 16 or 32 bytes.
+template <int DT>
+__device__ __forceinline__ void load_raw8(const void* base, int64_t at, uint4* raw) {
+  if constexpr (DT == SGL_F32) {
+    const uint4* p = reinterpret_cast<const uint4*>((const float*)base + at);
+    raw[0] = p[0];
+    raw[1] = p[1];
+  } else {
+    *raw = *reinterpret_cast<const uint4*>((const uint16_t*)base + at);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void load8(const void* base, int64_t at, float* f) {
+  uint4 raw[DT == SGL_F32 ? 2 : 1];
+  load_raw8<DT>(base, at, raw);
+  widen8<DT>(raw, f);
 }
 
 // fp32 values rounded once to the output type: torch's casts, NaN kept.
@@ -98,8 +117,15 @@ __device__ __forceinline__ void load_turn(const float* table, int64_t n_position
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float2 t = row[i];
-    cos[i] = in ? t.x : p < 0 ? 1.0f : __builtin_nanf("");
-    sin[i] = in ? (inverse ? -t.y : t.y) : p < 0 ? 0.0f : __builtin_nanf("");
+    cos[i] = t.x;
+    sin[i] = inverse ? -t.y : t.y;
+  }
+  if (__builtin_expect(!in, 0)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      cos[i] = p < 0 ? 1.0f : __builtin_nanf("");
+      sin[i] = p < 0 ? 0.0f : __builtin_nanf("");
+    }
   }
 }
 
