@@ -123,8 +123,7 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
   // instruction for two.
   const bool packed = DT != SGL_F32 && rot == 0;
 
-  uint4 raw[IT][2 * RW];
-  float x[IT][16];
+  uint32_t kept[IT][16];  // packed as they lie, or fp32
   int e0[IT], e1[IT], tok[IT];
   bool odd[IT];  // a NaN or an infinity among them
   float amax = 0.0f;
@@ -145,18 +144,21 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
         p1 = c + 8 < off ? c + 8 : c + 8 + rot;
       }
       const int64_t at = (int64_t)(w.row0 + t) * st + (int64_t)head * sh;
-      load_raw8<DT>(src, at + p0, raw[it]);
-      load_raw8<DT>(src, at + p1, raw[it] + RW);
+      uint4 raw[2 * RW];
+      load_raw8<DT>(src, at + p0, raw);
+      load_raw8<DT>(src, at + p1, raw + RW);
       tok[it] = t;
       e0[it] = p0;
       e1[it] = p1;
-      float top;
+      float top, x[16];
       if (packed) {
         typedef uint16_t us2 __attribute__((ext_vector_type(2)));
         us2 m = {0, 0};
 #pragma unroll
         for (int v = 0; v < 2 * RW; ++v) {
-          const uint32_t q[4] = {raw[it][v].x, raw[it][v].y, raw[it][v].z, raw[it][v].w};
+          const uint32_t q[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kept[it][4 * v + j] = q[j];
 #pragma unroll
           for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, q[j] & 0x7FFF7FFFu));
         }
@@ -164,8 +166,8 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
         odd[it] = most >= (DT == SGL_BF16 ? 0x7F80u : 0x7C00u);
         top = DT == SGL_BF16 ? bits_f32(most << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)most);
       } else {
-        widen8<DT>(raw[it], x[it]);
-        widen8<DT>(raw[it] + RW, x[it] + 8);
+        widen8<DT>(raw, x);
+        widen8<DT>(raw + RW, x + 8);
         if (u < rot_units) {
           float cs[8], sn[8];
           const int64_t pos = a.positions ? a.positions[w.row0 + t] : w.at + t;
@@ -174,23 +176,24 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
             float p[8], q[8];
 #pragma unroll
             for (int v = 0; v < 8; ++v) {
-              p[v] = x[it][2 * v];
-              q[v] = x[it][2 * v + 1];
+              p[v] = x[2 * v];
+              q[v] = x[2 * v + 1];
             }
             rotate_pairs<8>(p, q, cs, sn);
 #pragma unroll
             for (int v = 0; v < 8; ++v) {
-              x[it][2 * v] = p[v];
-              x[it][2 * v + 1] = q[v];
+              x[2 * v] = p[v];
+              x[2 * v + 1] = q[v];
             }
           } else {
-            rotate_pairs<8>(x[it], x[it] + 8, cs, sn);
+            rotate_pairs<8>(x, x + 8, cs, sn);
           }
         }
         uint32_t most = 0;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const uint32_t m = f32_bits(x[it][v]) & 0x7FFFFFFFu;
+          kept[it][v] = f32_bits(x[v]);
+          const uint32_t m = kept[it][v] & 0x7FFFFFFFu;
           most = m > most ? m : most;
         }
         odd[it] = most >= 0x7F800000u;
@@ -198,13 +201,13 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
       }
       if (__builtin_expect(odd[it], 0)) {  // finite values alone
         if (packed) {
-          widen8<DT>(raw[it], x[it]);
-          widen8<DT>(raw[it] + RW, x[it] + 8);
+          widen8<DT>(raw, x);
+          widen8<DT>(raw + RW, x + 8);
         }
         top = 0.0f;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const float m = __builtin_fabsf(x[it][v]);
+          const float m = __builtin_fabsf(x[v]);
           top = m < __builtin_huge_valf() && m > top ? m : top;
         }
       }
@@ -257,20 +260,27 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
       uint32_t c[4];
       if (__builtin_expect(odd[it], 0)) {  // an infinity becomes the NaN code, a NaN keeps its sign
         const float inv = 1.0f / s;        // exact for the powers of two that this kernel writes
-        const float* f = x[it];
+        float f[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) f[v] = bits_f32(kept[it][v]);
+        if (packed) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const uint4 raw = make_uint4(kept[it][4 * v], kept[it][4 * v + 1], kept[it][4 * v + 2], kept[it][4 * v + 3]);
+            widen8<DT == SGL_F32 ? SGL_BF16 : DT>(&raw, f + 8 * v);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           c[j] = pk4_e4m3_exact(f[4 * j] * inv, f[4 * j + 1] * inv, f[4 * j + 2] * inv, f[4 * j + 3] * inv);
       } else if (packed) {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          c[2 * v] = codes4<DT>(raw[it][v].x, raw[it][v].y, s);
-          c[2 * v + 1] = codes4<DT>(raw[it][v].z, raw[it][v].w, s);
-        }
+        for (int j = 0; j < 4; ++j) c[j] = codes4<DT>(kept[it][2 * j], kept[it][2 * j + 1], s);
       } else {
-        const float* f = x[it];
+        const uint32_t* f = kept[it];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = codes4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3], s);
+        for (int j = 0; j < 4; ++j)
+          c[j] = codes4(bits_f32(f[4 * j]), bits_f32(f[4 * j + 1]), bits_f32(f[4 * j + 2]), bits_f32(f[4 * j + 3]), s);
       }
       if (rot == 0) {  // the two chunks lie side by side
         *reinterpret_cast<uint4*>(row + e0[it]) = make_uint4(c[0], c[1], c[2], c[3]);
@@ -290,11 +300,11 @@ void launch_append(const AppendArgs& a, int64_t units, int64_t per_unit, hipStre
   else if (per_unit <= 256)
     append_kernel<DT, 256, 1><<<grid, 256, 0, st>>>(a);
   else if (per_unit <= 512)
-    append_kernel<DT, 256, 2><<<grid, 256, 0, st>>>(a);
+    append_kernel<DT, 512, 1><<<grid, 512, 0, st>>>(a);
   else if (per_unit <= 1024)
-    append_kernel<DT, 256, 4><<<grid, 256, 0, st>>>(a);
+    append_kernel<DT, 512, 2><<<grid, 512, 0, st>>>(a);
   else
-    append_kernel<DT, 256, 8><<<grid, 256, 0, st>>>(a);
+    append_kernel<DT, 512, 4><<<grid, 512, 0, st>>>(a);
 }
 
 }  // namespace
