@@ -541,7 +541,7 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
   a.page_shift = __builtin_ctz((unsigned)page_size);
   a.block_shift = __builtin_ctz((unsigned)block);
   a.c1 = softmax_scale * sgl::kLog2e;
-  a.window = window > 0x7FFFFFFF ? 0 : (int)window;
+  a.window = window >= row_pages * page_size ? 0 : (int)window;  // (as long as the table: all keys)
   a.causal = causal != 0;
   a.parts = (int)p.parts;
   a.ws_acc = (float*)workspace;

@@ -184,6 +184,7 @@ struct Kv8Walk {
       if (x >= base + room) {
         base += room;
         if (++l == 64) {
+          if (c.b0 + 64 >= a.B) return false;
           c = kv8_chunk<RT, TT>(a, c.b0 + 64);
           l = 0;
         }

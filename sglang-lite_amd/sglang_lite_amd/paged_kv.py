@@ -9,7 +9,7 @@ page / block]``.  A layer's step is
     o = paged_attn(q, cache, block_table, start + new, cu_tokens=cu)
 
 with the tokens of a batch's sequences one after the other, ``cu_tokens``
-(int32 ``[B + 1]``) saying where each begins; without it every sequence has one
+(int32 ``[B + 1]``, never falling) saying where each begins; without it every sequence has one
 token (decode).  All lengths stay on the device, so a step can be captured into
 a HIP graph and replayed with other lengths.
 """
@@ -129,7 +129,7 @@ def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: tor
     rounded again where it grew.  A NaN or an infinity is stored as NaN.  Rows
     behind the last sequence, tokens behind the block table, and table entries
     that are no page of the cache are skipped.  Every page that is written to
-    must belong to one sequence of the call; pages that are only read (the full
+    must belong to one sequence of the call, at one place of its row; pages that are only read (the full
     pages of a common prefix) may be shared."""
     pages, heads, page, dim, block = _check_cache(cache, "append_kv")
     shape = k.shape
@@ -180,7 +180,8 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     of them if that is not 0; otherwise all.  ``sink`` (float32 ``[Hq]``): a
     logit of each head that takes part in the softmax and has no value.
     ``softmax_scale``: ``D ** -0.5`` by default.  A row that sees no key is zero;
-    rows of ``out`` behind the last sequence are left as they are."""
+    rows behind the last sequence are not written (of a new tensor: they hold
+    anything)."""
     pages, heads, page, dim, block = _check_cache(cache, "paged_attn")
     shape = q.shape
     if len(shape) != 3 or shape[2] != dim or shape[1] < 1 or shape[1] % heads:

@@ -97,6 +97,11 @@ def check_table(table: torch.Tensor, offset: int, dim: int, what: str) -> int:
     return rot
 
 
+def _apart(outer: int, so: int, inner: int, si: int, D: int) -> bool:
+    """Whether ``outer`` groups of ``inner`` rows of ``D`` elements, at these strides, lie apart."""
+    return (inner <= 1 or si >= D) and (outer <= 1 or so >= (inner - 1) * si + D)
+
+
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
            interleaved: bool = False, offset: int = 0, inverse: bool = False,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -129,9 +134,9 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     elif out.shape != shape or out.dtype is not x.dtype or (out.stride(2) != 1 and D > 1):
         raise ValueError(f"rotary: out must be {x.dtype} {tuple(shape)} with a dense last "
                          f"dimension, got {out.dtype} {tuple(out.shape)}")
-    elif (T > 1 and abs(out.stride(0)) < D) or (H > 1 and abs(out.stride(1)) < D):
-        raise ValueError("rotary: rows of out overlap")
     os = out.stride()
+    if not (_apart(T, os[0], H, os[1], D) or _apart(H, os[1], T, os[0], D)):
+        raise ValueError("rotary: rows of out overlap")
     if not positions.is_contiguous():
         positions = positions.contiguous()
     _lib.call_on(d, "sgl_rotary", x.data_ptr(), dt, T, H, D, xs[0], xs[1], table.data_ptr(),

@@ -477,6 +477,80 @@ def test_nan_and_infinity_reach_only_the_rows_that_see_them(gpu, new, window):
     _check_attn(c, q, [L], [0, n], window=window)
 
 
+def _widen(c, tokens):
+    """A block table for so many tokens a sequence, the new entries no page: long tables have
+    the keys of an item shared between workgroups, short ones do not."""
+    B, old = c.table.shape
+    t = np.full((B, max(old, -(-tokens // c.k.shape[2]))), -1, dtype=c.table.dtype)
+    t[:, :old] = c.table
+    c.table, c.bt = t, torch.from_numpy(t).to(c.dev)
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hkv,D,page,block,dtype,causal,window,sink", CHUNKS + [
+    ([1] * len(lens), lens, Hq, Hkv, D, page, block, dtype, True, window, sink)
+    for lens, Hq, Hkv, D, page, block, dtype, window, sink in DECODE])
+def test_attention_shared_between_workgroups(gpu, new, lens, Hq, Hkv, D, page, block, dtype, causal, window, sink):
+    print(f"shared new={new} lens={lens} Hq={Hq} Hkv={Hkv} D={D} page={page}", flush=True)
+    c = _filled(gpu, lens, Hkv, D, page, block, seed=D + Hq)
+    _widen(c, 16384)
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], Hq, D, dtype, 8)
+    s = (np.random.default_rng(2).standard_normal(Hq) * 2).astype(np.float32) if sink else None
+    _check_attn(c, q, lens, cu, causal=causal, window=window, sink=s)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,new", [(128, 8, 2, 16), (128, 8, 2, 17), (64, 4, 1, 16), (64, 4, 1, 17),
+                                          (256, 8, 4, 8), (256, 8, 4, 9), (128, 4, 1, 64), (128, 4, 1, 65)])
+@pytest.mark.parametrize("tokens", [1024, 1040, 2048, 2064, 4200])
+def test_attention_on_both_sides_of_its_choices(gpu, D, Hq, Hkv, new, tokens):
+    """The most rows that count as few and one token more, one row tile and two; tables that
+    hold as much as an item that is not shared, and a page more."""
+    lens = [tokens // 4, 70, 333]
+    c = _filled(gpu, lens, Hkv, D, 16, 16, seed=D)
+    _widen(c, tokens)
+    cu = [0, new, 2 * new, 3 * new]
+    q = _queries(gpu, cu[-1], Hq, D, torch.bfloat16, 6)
+    _check_attn(c, q, lens, cu)
+
+
+@pytest.mark.parametrize("tokens", [0, 16384])
+@pytest.mark.parametrize("new", [1, 3])
+def test_attention_of_many_short_sequences(gpu, new, tokens):
+    """More sequences than a wavefront has lanes, some without keys or queries."""
+    rng = np.random.default_rng(6)
+    lens = rng.integers(0, 200, 150).tolist()
+    n = [new if i % 7 else 0 for i in range(150)]
+    c = _filled(gpu, lens, 2, 64, 16, 16, seed=12)
+    _widen(c, tokens)
+    cu = [0] + np.cumsum(n).tolist()
+    q = _queries(gpu, cu[-1] + 3, 8, 64, torch.float16, 6)
+    _check_attn(c, q, lens, cu)
+
+
+@pytest.mark.parametrize("new", [2, 150])
+def test_windows_past_every_length(gpu, new):
+    """A window of 2^31 - 1 and more, with more queries than keys."""
+    lens = [new // 2, new + 30]
+    c = _filled(gpu, lens, 1, 128, 16, 16, seed=13)
+    q = _queries(gpu, 2 * new, 4, 128, torch.bfloat16, 6)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        _check_attn(c, q, lens, [0, new, 2 * new], window=window)
+
+
+@pytest.mark.parametrize("D,new,window,tokens", [(64, 150, 60, 0), (256, 150, 60, 0), (256, 5, 0, 4096),
+                                                 (64, 4, 0, 4096), (128, 150, 60, 16384), (256, 40, 60, 16384)])
+def test_nan_stays_with_its_rows_at_every_width(gpu, D, new, window, tokens):
+    L = 200
+    c = _filled(gpu, [L], 2, D, 64, 16, seed=11)
+    for t, h, d in ((L - 1, 0, 3), (L - new // 2 - 1, 1, D - 6), (100, 0, 9)):
+        p, spot = int(c.table[0, t // 64]), t % 64
+        c.kv.v.view(torch.uint8)[p, h, spot, d] = 0x7F
+        c.v[p, h, spot, d] = 0x7F
+    _widen(c, tokens)
+    q = _queries(gpu, new, 8, D, torch.bfloat16, 5)
+    _check_attn(c, q, [L], [0, new], window=window)
+
+
 def test_attention_of_large_scores_and_few_survivors(gpu):
     """Scores of hundreds, so that one key takes all and the reference moves often; a query of
     zeros; a scale of its own; a query row that is not finite."""

@@ -25,6 +25,12 @@ int64_t append_units(int64_t T, int64_t B, int64_t block) { return kv8_append_un
 int64_t attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t rows) { return kv8_attn_items(T, B, Hkv, G, rows); }
 int head_threads(int64_t T, int64_t H, int64_t units, int64_t cus) { return rotary_head_threads(T, H, units, cus); }
 float block_scale(float amax) { return kv8_scale(amax); }
+void attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity, int64_t cus, int64_t* o) {
+  const Kv8AttnPlan p = kv8_attn_plan(T, B, Hkv, G, D, capacity, cus);
+  o[0] = p.row_tile;
+  o[1] = p.parts;
+  o[2] = (int64_t)kv8_attn_workspace(p, Hkv, D);
+}
 }
 """
 
@@ -41,6 +47,7 @@ def rules(tmp_path_factory):
     lib.append_units.restype, lib.append_units.argtypes = i64, [i64] * 3
     lib.attn_items.restype, lib.attn_items.argtypes = i64, [i64] * 5
     lib.head_threads.argtypes = [i64] * 4
+    lib.attn_plan.argtypes = [i64] * 7 + [ctypes.c_void_p]
     lib.block_scale.restype, lib.block_scale.argtypes = ctypes.c_float, [ctypes.c_float]
     return lib
 
@@ -58,6 +65,42 @@ def test_grids_cover_every_block_and_row_tile(rules, seed):
     for G, rows in ((1, 16), (4, 16), (5, 32), (64, 16), (8, 128), (48, 32)):
         tiles = sum(-(-int(n) * G // rows) for n in new)
         assert tiles * 3 <= rules.attn_items(T, B, 3, G, rows)
+
+
+def test_attention_plans(rules):
+    o = (ctypes.c_int64 * 3)()
+
+    def plan(T, B, Hkv, G, D, capacity, cus=256):
+        rules.attn_plan(T, B, Hkv, G, D, capacity, cus, o)
+        return o[0], o[1], o[2]
+
+    rng = np.random.default_rng(0)
+    for _ in range(2000):
+        B, Hkv, G = (int(rng.integers(1, n)) for n in (200, 70, 70))
+        T, D = B * int(rng.integers(1, 300)), 16 * int(rng.integers(1, 17))
+        rt, parts, ws = plan(T, B, Hkv, G, D, 16 << int(rng.integers(0, 14)), int(rng.integers(8, 400)))
+        assert rt in (16, 32, 128, 256) and parts % 8 == 0 and parts >= 0
+        assert (rt > 32) == (T * G // B > (64 if D <= 128 else 16))
+        assert ws == parts * 2 * Hkv * rt * (D + 2) * 4  # two stretches a workgroup
+    # a short table: no sharing, no workspace; few rows up to 2048 tokens where items are many
+    assert plan(1, 1, 8, 4, 128, 1024)[1:] == (0, 0) and plan(1, 1, 8, 4, 128, 1040)[1] == 64
+    # (the items are a bound, T G / 16 + B row tiles for each of 8 heads: 52 sequences 520, 51 504)
+    assert plan(52, 52, 8, 4, 128, 2048)[1] == 0 and plan(51, 51, 8, 4, 128, 2048)[1] == 64
+    # a chunk's row tiles: two a workgroup are not shared, fewer by how much there is to share
+    assert plan(8192, 1, 8, 4, 128, 1 << 17)[1] == 0 and plan(512, 1, 8, 4, 128, 1 << 13)[1] == 32
+    assert plan(2048, 1, 8, 4, 128, 4096)[1] == 0 and plan(2048, 1, 8, 4, 128, 8192)[1] == 32
+
+
+def test_rows_that_overlap():
+    from sglang_lite_amd.rotary import _apart
+
+    rng = np.random.default_rng(1)
+    for _ in range(3000):
+        T, H, D = (int(rng.integers(1, 4)) for _ in range(3))
+        s0, s1 = int(rng.integers(0, 14)), int(rng.integers(0, 14))
+        at = [t * s0 + h * s1 + d for t in range(T) for h in range(H) for d in range(D)]
+        if _apart(T, s0, H, s1, D) or _apart(H, s1, T, s0, D):
+            assert len(set(at)) == len(at)
 
 
 def test_head_threads(rules):
