@@ -36,4 +36,8 @@ Pinning (what checks each function against something other than itself):
 * ``kv``: the reference's tests (tests/test_dsv4_kv_pack.py:16-65,
   tests/test_v4_dual_pool.py:57-75) and closed forms of the footer layout.
   Layout B has no reference producer: parity unpinned beyond its closed form.
+* ``paged``: no reference counterpart.  The codes are ``quant.f32_to_e4m3``'s;
+  the scales against brute force over the powers of two; the attention, written
+  from the softmax in 64 bits, against a second form of it
+  (tests/test_paged_kv.py).
 """

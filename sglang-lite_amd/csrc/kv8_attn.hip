@@ -451,8 +451,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 256 ? 1 : 2) void kv8_attn_few_k
 }
 
 template <int DP, int NC, int QT>
-void launch_few(const Kv8AttnArgs& a, hipStream_t st) {
-  const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, 16 * NC);
+void launch_few(const Kv8AttnArgs& a, int64_t items, hipStream_t st) {
   if (a.parts == 0) {
     kv8_attn_few_kernel<DP, NC, QT, false><<<(unsigned)items, 64 * kWaves, 0, st>>>(a);
     return;
@@ -462,15 +461,19 @@ void launch_few(const Kv8AttnArgs& a, hipStream_t st) {
 }
 
 template <int QT>
-void launch_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
+void launch_attn(Kv8AttnArgs a, const Kv8AttnPlan& p, hipStream_t st) {
+  a.parts = (int)p.parts;
+  a.above = (int)p.above;
+  a.upto = (int)p.upto;
+  a.ws_ml = a.ws_acc + 2 * p.parts * a.Hkv * p.row_tile * a.D;
   if (p.row_tile > 32)
     launch_kv8_prefill(a, p, QT, st);
   else if (a.D <= 64)
-    p.row_tile == 16 ? launch_few<64, 1, QT>(a, st) : launch_few<64, 2, QT>(a, st);
+    p.row_tile == 16 ? launch_few<64, 1, QT>(a, p.items, st) : launch_few<64, 2, QT>(a, p.items, st);
   else if (a.D <= 128)
-    p.row_tile == 16 ? launch_few<128, 1, QT>(a, st) : launch_few<128, 2, QT>(a, st);
+    p.row_tile == 16 ? launch_few<128, 1, QT>(a, p.items, st) : launch_few<128, 2, QT>(a, p.items, st);
   else
-    launch_few<256, 1, QT>(a, st);
+    launch_few<256, 1, QT>(a, p.items, st);
 }
 
 }  // namespace
@@ -480,8 +483,13 @@ extern "C" {
 
 size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens) {
   if (T < 0 || B < 0 || Hkv < 1 || G < 1 || D < 16 || max_tokens < 0) return 0;
-  const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, max_tokens, sgl::device_cu_count());
-  return sgl::kv8_attn_workspace(p, Hkv, D);
+  size_t bytes = 0;
+  for (const sgl::Kv8AttnPlan& p : {sgl::kv8_attn_plan(T, B, Hkv, G, D, max_tokens, sgl::device_cu_count()),
+                                    sgl::kv8_attn_rest(T, B, Hkv, G, D, max_tokens, sgl::device_cu_count())}) {
+    const size_t b = sgl::kv8_attn_workspace(p, Hkv, D);
+    bytes = b > bytes ? b : bytes;
+  }
+  return bytes;
 }
 
 int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T, int64_t B,
@@ -507,17 +515,22 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
               "kv8_attn: q and its strides must be 16-byte aligned");
   SGL_REQUIRE(sgl::aligned(k_codes, 16) && sgl::aligned(v_codes, 16) && sgl::aligned(out, 16),
               "kv8_attn: misaligned cache or output");
-  const sgl::Kv8AttnPlan p = sgl::kv8_attn_plan(T, B, Hkv, G, D, row_pages * page_size, sgl::device_cu_count());
-  const size_t need = sgl::kv8_attn_workspace(p, Hkv, D);
-  if (need && (!workspace || workspace_bytes < need)) {
-    sgl::set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
-    return SGL_ERR_WORKSPACE;
+  // one launch, or (chunks and few rows in one batch) two, one after the other on the same workspace
+  const int64_t tokens = row_pages * page_size;
+  const sgl::Kv8AttnPlan plans[2] = {sgl::kv8_attn_plan(T, B, Hkv, G, D, tokens, sgl::device_cu_count()),
+                                     sgl::kv8_attn_rest(T, B, Hkv, G, D, tokens, sgl::device_cu_count())};
+  for (const sgl::Kv8AttnPlan& p : plans) {
+    const size_t need = sgl::kv8_attn_workspace(p, Hkv, D);
+    if (need && (!workspace || workspace_bytes < need)) {
+      sgl::set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
+      return SGL_ERR_WORKSPACE;
+    }
+    SGL_REQUIRE_SUPPORTED(p.items * ((tokens + 31) / 32 + sgl::kItemCost) < (1ll << 31) &&
+                              p.items * p.row_tile / 4 < (1ll << 31),
+                          "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)p.items,
+                          (long long)tokens);
   }
   SGL_REQUIRE(sgl::aligned(workspace, 16), "kv8_attn: workspace must be 16-byte aligned");
-  const int64_t items = sgl::kv8_attn_items(T, B, Hkv, G, p.row_tile);
-  SGL_REQUIRE_SUPPORTED(items * ((row_pages * page_size + 31) / 32 + sgl::kItemCost) < (1ll << 31),
-                        "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)items,
-                        (long long)(row_pages * page_size));
   sgl::Kv8AttnArgs a;
   a.q = (const uint16_t*)q;
   a.qt = q_token_stride;
@@ -541,15 +554,16 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
   a.page_shift = __builtin_ctz((unsigned)page_size);
   a.block_shift = __builtin_ctz((unsigned)block);
   a.c1 = softmax_scale * sgl::kLog2e;
-  a.window = window >= row_pages * page_size ? 0 : (int)window;  // (as long as the table: all keys)
+  a.window = window >= tokens ? 0 : (int)window;  // (as long as the table: all keys)
   a.causal = causal != 0;
-  a.parts = (int)p.parts;
   a.ws_acc = (float*)workspace;
-  a.ws_ml = (float*)workspace + 2 * p.parts * Hkv * p.row_tile * D;
-  if (dtype == SGL_BF16)
-    sgl::launch_attn<SGL_BF16>(a, p, (hipStream_t)stream);
-  else
-    sgl::launch_attn<SGL_F16>(a, p, (hipStream_t)stream);
+  for (const sgl::Kv8AttnPlan& p : plans) {
+    if (p.items == 0) continue;
+    if (dtype == SGL_BF16)
+      sgl::launch_attn<SGL_BF16>(a, p, (hipStream_t)stream);
+    else
+      sgl::launch_attn<SGL_F16>(a, p, (hipStream_t)stream);
+  }
   return sgl::check_launch("kv8_attn");
 }
 

@@ -528,7 +528,7 @@ template <int DP, int QT>
 void launch_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
   constexpr int NW = DP == 128 ? 8 : 4, RT = 32 * NW;
   static_assert(RT == kv8_chunk_rows(DP), "the plan's row tile");
-  const int64_t items = kv8_attn_items(a.T, a.B, a.Hkv, a.G, RT);
+  const int64_t items = p.items;
   if (p.parts == 0) {
     kv8_prefill_kernel<DP, QT, NW, false><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
   } else {

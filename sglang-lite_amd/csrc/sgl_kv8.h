@@ -22,7 +22,7 @@ inline int kv8_check_cache(const char* what, int Hkv, int D, int page, int block
   SGL_REQUIRE(block >= 16 && block <= 128 && block <= page && (block & (block - 1)) == 0,
               "%s: block=%d must be a power of two, 16 to 128, and at most the page (%d)", what, block, page);
   SGL_REQUIRE(n_pages >= 1 && n_pages <= 0x7FFFFFFF, "%s: n_pages=%lld out of range", what, (long long)n_pages);
-  SGL_REQUIRE(row_pages >= 1 && row_pages * page <= 0x7FFFFFFF, "%s: %lld pages of %d tokens a sequence: too many",
+  SGL_REQUIRE(row_pages >= 1 && row_pages * page <= (1 << 30), "%s: %lld pages of %d tokens a sequence: too many",
               what, (long long)row_pages, page);
   return SGL_OK;
 }

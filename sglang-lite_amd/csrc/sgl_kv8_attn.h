@@ -42,6 +42,7 @@ struct Kv8AttnArgs {
   int window;   // keys a query sees, itself included; 0: all
   bool causal;
   int parts;      // workgroups of a kv head's line; 0: one workgroup an item
+  int above, upto;  // takes the sequences of more than `above` rows a kv head, and up to `upto`
   float* ws_acc;  // [2 parts Hkv][row tile][D]
   float* ws_ml;   // [2 parts Hkv][row tile][2]: reference point (log2 units), sum
 };
@@ -92,7 +93,8 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
     c.n = r.n;
     c.len = len < 0 ? 0 : len > cap ? cap : len;
     const Kv8Seq s = kv8_seq<RT, TT>(a, c.row0, c.n, c.len);
-    rts = s.row_tiles;
+    const int rows = r.n * a.G;
+    rts = rows > a.above && rows <= a.upto ? s.row_tiles : 0;
     c.room = rts * (s.tiles + kItemCost);
   }
   c.rooms = wave_incl_scan(c.room);

@@ -259,6 +259,8 @@ SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {
 struct Kv8AttnPlan {
   int64_t row_tile;  // 16 or 32: kv8_attn.hip; more: kv8_prefill.hip
   int64_t parts;     // workgroups of a kv head's line, a multiple of 8; 0: a workgroup takes a whole item
+  int64_t items;     // at most; 0: nothing to launch
+  int64_t above, upto;  // rows of the sequences that it takes: more than, and up to
 };
 SGL_RULE size_t kv8_attn_workspace(const Kv8AttnPlan& p, int64_t Hkv, int64_t D) {
   return (size_t)(2 * p.parts * Hkv * p.row_tile * (D + 2)) * sizeof(float);
@@ -288,7 +290,15 @@ constexpr int64_t kv8_chunk_rows(int64_t D) { return D > 64 && D <= 128 ? 256 : 
 // 32 / 34 and 43 / 47, 96 rows 38 / 35 and 56 / 51, 128 rows 40 / 36 and 66 / 56.  Of 64: 64 rows
 // 23 / 26 and 29 / 31, 96 rows 25 / 27 and 37 / 35.  Of 256: 16 rows 40 / 39 and 36 / 50, 32
 // rows 46 / 39 and 62 / 52, 64 rows 60 / 42 and 97 / 62.
-SGL_RULE bool kv8_attn_chunk(int64_t rows, int64_t D) { return rows > (D <= 128 ? 64 : 16); }
+SGL_RULE int64_t kv8_few_rows(int64_t D) { return D <= 128 ? 64 : 16; }
+// A batch of chunks may hold single tokens too, for which a chunk's tiles cost many
+// times the few rows' kernel: from 8 sequences on, each kernel takes those of its own.
+// 32 query heads on 8 kv heads of 128, two launches / the chunk's alone, us: 63 x 1 query on
+// 4000 keys + 2000 on 2000 162 / 297, 15 x 1 on 8000 + 512 on 8000 155 / 214, 7 x 1 + 512
+// on 8000 132 / 151; where there are no few rows after all 16 x 128 54 / 52, 8 x 512 198 / 192.
+SGL_RULE bool kv8_attn_mixed(int64_t T, int64_t B, int64_t G, int64_t D) {
+  return B >= 8 && T * G / B > kv8_few_rows(D) && T > B;
+}
 // A chunk's row tiles go to workgroups whole where there are two for every workgroup
 // at a time (fit), or few keys to divide: up to 4096 at one item a place, half of that
 // at half of the items.  Whole / shared, us, 32 query heads on 8 kv heads of 128:
@@ -301,13 +311,22 @@ SGL_RULE bool kv8_chunk_whole(int64_t capacity, int64_t items, int64_t fit) {
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
                                    int64_t cus) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
-  if (kv8_attn_chunk(rows, D)) {
-    const int64_t rt = kv8_chunk_rows(D);
+  if (rows > kv8_few_rows(D)) {
+    const int64_t rt = kv8_chunk_rows(D), items = kv8_attn_items(T, B, Hkv, G, rt);
     const int64_t fit = D <= 64 ? 2 * cus : cus;
-    return {rt, kv8_chunk_whole(capacity, kv8_attn_items(T, B, Hkv, G, rt), fit) ? 0 : kv8_attn_parts(fit, Hkv)};
+    return {rt, kv8_chunk_whole(capacity, items, fit) ? 0 : kv8_attn_parts(fit, Hkv), items,
+            kv8_attn_mixed(T, B, G, D) ? kv8_few_rows(D) : 0, 0x7FFFFFFF};
   }
-  const int64_t rt = D <= 128 && rows > 16 ? 32 : 16;
-  return {rt, kv8_attn_whole(capacity, kv8_attn_items(T, B, Hkv, G, rt), cus) ? 0 : kv8_attn_parts(2 * cus, Hkv)};
+  const int64_t rt = D <= 128 && rows > 16 ? 32 : 16, items = kv8_attn_items(T, B, Hkv, G, rt);
+  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_attn_parts(2 * cus, Hkv), items, 0, 0x7FFFFFFF};
+}
+// The second launch of a batch of chunks: its sequences of few rows.
+SGL_RULE Kv8AttnPlan kv8_attn_rest(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
+                                   int64_t cus) {
+  if (!kv8_attn_mixed(T, B, G, D)) return {16, 0, 0, 0, 0};
+  const int64_t rt = D <= 128 && G > 16 ? 32 : 16, upto = kv8_few_rows(D);
+  const int64_t items = B * ((upto + rt - 1) / rt) * Hkv;
+  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_attn_parts(2 * cus, Hkv), items, 0, upto};
 }
 
 }  // namespace sgl

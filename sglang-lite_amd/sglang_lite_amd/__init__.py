@@ -8,6 +8,11 @@ A drop-in for the reference's (ParaTensor/sglang-lite) hot path:
 * ``v4_deep_gemm``  -- FP8 GEMM call-site adapter: probe, attach, scale caches
 * ``dsv4_kv_pack``  -- FP8 KV row pack / paging / gather-dequant / index split
 
+and, for ordinary attention heads:
+
+* ``rotary``        -- rotary tables and rotations
+* ``paged_kv``      -- 8-bit block-scaled paged KV cache: append, attention
+
 All compute runs in hand-written HIP kernels of ``lib/libsglang_lite_amd.so``
 (C ABI: ``include/sglang_lite_amd.h``); torch only provides device memory and
 the current stream.  There is no CPU fallback.

@@ -527,6 +527,23 @@ def test_attention_of_many_short_sequences(gpu, new, tokens):
     _check_attn(c, q, lens, cu)
 
 
+@pytest.mark.parametrize("tokens", [0, 1500, 16384])
+@pytest.mark.parametrize("D,Hq,Hkv,dtype", [(128, 8, 2, torch.bfloat16), (64, 40, 2, torch.float16),
+                                            (256, 6, 2, torch.bfloat16)])
+def test_single_tokens_beside_prompts(gpu, D, Hq, Hkv, dtype, tokens):
+    """Chunks and few rows in one batch: no row is missed or taken twice, whichever kernel is its."""
+    new = [1, 300, 0, 1, 16, 17, 1, 2, 0, 130, 1, 3]
+    lens = [700, 300, 50, 0, 16, 400, 65, 1, 0, 290, 513, 40]
+    c = _filled(gpu, lens, Hkv, D, 32, 16, seed=D)
+    _widen(c, tokens)
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1] + 2, Hq, D, dtype, 4)
+    s = (np.random.default_rng(2).standard_normal(Hq) * 2).astype(np.float32)
+    out = torch.full_like(q, 7.0)
+    _check_attn(c, q, lens, cu, sink=s, window=450, out=out)
+    assert bool((out[cu[-1]:] == 7.0).all())
+
+
 @pytest.mark.parametrize("new", [2, 150])
 def test_windows_past_every_length(gpu, new):
     """A window of 2^31 - 1 and more, with more queries than keys."""

@@ -30,6 +30,11 @@ void attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t 
   o[0] = p.row_tile;
   o[1] = p.parts;
   o[2] = (int64_t)kv8_attn_workspace(p, Hkv, D);
+  const Kv8AttnPlan r = kv8_attn_rest(T, B, Hkv, G, D, capacity, cus);
+  o[3] = r.row_tile;
+  o[4] = r.items;
+  o[5] = p.above;
+  o[6] = r.upto;
 }
 }
 """
@@ -68,7 +73,7 @@ def test_grids_cover_every_block_and_row_tile(rules, seed):
 
 
 def test_attention_plans(rules):
-    o = (ctypes.c_int64 * 3)()
+    o = (ctypes.c_int64 * 7)()
 
     def plan(T, B, Hkv, G, D, capacity, cus=256):
         rules.attn_plan(T, B, Hkv, G, D, capacity, cus, o)
@@ -82,6 +87,10 @@ def test_attention_plans(rules):
         assert rt in (16, 32, 128, 256) and parts % 8 == 0 and parts >= 0
         assert (rt > 32) == (T * G // B > (64 if D <= 128 else 16))
         assert ws == parts * 2 * Hkv * rt * (D + 2) * 4  # two stretches a workgroup
+        # a second launch takes exactly the sequences that the first leaves, all their row tiles
+        few = 64 if D <= 128 else 16
+        assert o[5] == o[6] == (few if rt > 32 and B >= 8 and T > B else 0)
+        assert o[4] == (B * -(-few // o[3]) * Hkv if o[5] else 0)
     # a short table: no sharing, no workspace; few rows up to 2048 tokens where items are many
     assert plan(1, 1, 8, 4, 128, 1024)[1:] == (0, 0) and plan(1, 1, 8, 4, 128, 1040)[1] == 64
     # (the items are a bound, T G / 16 + B row tiles for each of 8 heads: 52 sequences 520, 51 504)
