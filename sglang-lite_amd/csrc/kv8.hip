@@ -9,7 +9,8 @@
 // grew: a power of two, so nothing but codes near the smallest are rounded.
 //
 // Bound by HBM (6 bytes for an element of k and of v: 2 x 2 read, 2 x 1
-// written); for single tokens by the chain table entry -> old scale -> codes.
+// written), and beside it by the conversion (16384 tokens of 8 heads of 128: 28 us at
+// 3.8 TB/s); for single tokens by the chain table entry -> old scale -> codes.
 // One workgroup takes one block, head and side (keys or values), so that the
 // scale is one reduction in registers and LDS and no block has two writers.
 #include "sgl_kv8.h"
@@ -292,6 +293,8 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
   }
 }
 
+// By a unit's 16 elements: a thread each up to 512 (256 threads with two each: 31.3 us
+// against 30.4 for 16384 tokens of 8 heads of 128), the small ones in small workgroups.
 template <int DT>
 void launch_append(const AppendArgs& a, int64_t units, int64_t per_unit, hipStream_t st) {
   const dim3 grid((unsigned)units, (unsigned)(2 * a.Hkv));

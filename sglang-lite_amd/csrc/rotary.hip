@@ -8,7 +8,8 @@
 // Bound by HBM: an element is read and written once, the table's row once for
 // all heads of a token.  A thread takes 2 x 8 elements (16-byte accesses; both
 // chunks of its pairs, so that the rotation may be done in place) of several
-// heads with the same cos and sin in registers.
+// heads with the same cos and sin in registers.  16384 tokens of 32 heads of 128:
+// 51 to 54 us, 5.2 TB/s, a large copy's rate.
 #include "sgl_kv8.h"
 
 namespace sgl {

@@ -242,7 +242,8 @@ SGL_RULE int permute_rounds(int E, bool table) {
 
 // ---- rotary positions: threads that share the heads of a token's unit, each
 // with four heads in flight at a time.  One head a thread while that leaves CUs
-// without a full round of wavefronts.
+// without a full round of wavefronts.  One head / four, us, 32 heads of 128: 512 tokens
+// 7.9 / 8.1, 2048 9.0 / 9.3, 4096 14.9 / 13.2, 16384 64 / 53.
 SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cus) {
   return T * units * ((H + 3) / 4) < cus * 1024 ? (int)H : (int)((H + 3) / 4);
 }
@@ -270,6 +271,14 @@ SGL_RULE int64_t kv8_attn_parts(int64_t wgs, int64_t Hkv) {
   const int64_t p = wgs / Hkv / 8 * 8;
   return p < 8 ? 8 : p;
 }
+// Few rows: two workgroups a CU for heads of 64, else one, which has fewer starts and
+// joins.  One / two a CU, us: heads of 64, 64 sequences up to 8000 67.5 / 59.9; of 128, 64
+// up to 4000 59.8 / 63.2, 3 up to 131072 92.9 / 97.8, 128 up to 16384 (4 heads) 185.8 /
+// 194.6, 32 x 4 queries up to 6000 48.5 / 51.4, 16 up to 2000 20.1 / 19.5; of 256, 32 up to
+// 8000 96 / 103.
+SGL_RULE int64_t kv8_few_parts(int64_t D, int64_t Hkv, int64_t cus) {
+  return kv8_attn_parts(D <= 64 ? 2 * cus : cus, Hkv);
+}
 // the most items (row tile, kv head) that T queries of B sequences make
 SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t row_tile) {
   const int64_t tiles = T * G / row_tile + B, most = T * ((G + row_tile - 1) / row_tile + 1);
@@ -278,24 +287,24 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
 // Few rows: whether a workgroup reads a whole item, with no merge behind.  By what
 // the block table can hold of a sequence, as the lengths are not known here: 32
 // query heads on 8 kv heads of 128, lengths up to that, whole / shared, us: 1
-// sequence 500 10.4 / 15.6, 1000 11.3 / 15.7, 2000 17.8 / 15.8; 16: 500 10.4 / 16.9,
-// 1000 12.7 / 17.6, 2000 20.1 / 19.7, 4000 34.0 / 25.6; 64: 500 14.4 / 26.4, 1000 21.6 /
-// 32.6, 2000 36.7 / 42.5, 4000 65.3 / 64.1.
+// sequence 500 11.5 / 16.9, 1000 11.7 / 16.9, 2000 17.4 / 16.8; 16: 500 11.5 / 16.9,
+// 1000 13.1 / 18.4, 2000 20.2 / 20.2, 4000 34.2 / 25.4; 64: 500 14.7 / 26.3, 1000 21.7 /
+// 32.2, 2000 36.3 / 41.4, 4000 65.0 / 60.4.
 SGL_RULE bool kv8_attn_whole(int64_t capacity, int64_t items, int64_t cus) {
   return capacity <= 1024 || (capacity <= 2048 && items >= 2 * cus);
 }
 constexpr int64_t kv8_chunk_rows(int64_t D) { return D > 64 && D <= 128 ? 256 : 128; }
 // Few rows or a chunk, by a sequence's rows on a kv head (few / chunk, us, 4 query heads
 // to each of 8 kv heads; 1 sequence of 16000 tokens and 8 of 4000).  Heads of 128: 64 rows
-// 32 / 34 and 43 / 47, 96 rows 38 / 35 and 56 / 51, 128 rows 40 / 36 and 66 / 56.  Of 64: 64 rows
-// 23 / 26 and 29 / 31, 96 rows 25 / 27 and 37 / 35.  Of 256: 16 rows 40 / 39 and 36 / 50, 32
-// rows 46 / 39 and 62 / 52, 64 rows 60 / 42 and 97 / 62.
-SGL_RULE int64_t kv8_few_rows(int64_t D) { return D <= 128 ? 64 : 16; }
+// 25 / 35 and 39 / 46, 96 rows 32 / 35 and 50 / 50, 128 rows 36 / 36 and 62 / 56.  Of 64: 64 rows
+// 22 / 25 and 28 / 30, 96 rows 24 / 27 and 34 / 35, 128 rows 40 / 37 (8 sequences).  Of 256: 16
+// rows 26 / 39 and 27 / 50, 32 rows 33 / 39 and 52 / 52.
+SGL_RULE int64_t kv8_few_rows(int64_t D) { return D <= 128 ? 96 : 32; }
 // A batch of chunks may hold single tokens too, for which a chunk's tiles cost many
 // times the few rows' kernel: from 8 sequences on, each kernel takes those of its own.
 // 32 query heads on 8 kv heads of 128, two launches / the chunk's alone, us: 63 x 1 query on
-// 4000 keys + 2000 on 2000 162 / 297, 15 x 1 on 8000 + 512 on 8000 155 / 214, 7 x 1 + 512
-// on 8000 132 / 151; where there are no few rows after all 16 x 128 54 / 52, 8 x 512 198 / 192.
+// 4000 keys + 2000 on 2000 168 / 298, 15 x 1 on 8000 + 512 on 8000 152 / 215, 7 x 1 + 512
+// on 8000 129 / 151; where there are no few rows after all 16 x 128 54 / 52, 8 x 512 198 / 192.
 SGL_RULE bool kv8_attn_mixed(int64_t T, int64_t B, int64_t G, int64_t D) {
   return B >= 8 && T * G / B > kv8_few_rows(D) && T > B;
 }
@@ -308,6 +317,11 @@ SGL_RULE bool kv8_attn_mixed(int64_t T, int64_t B, int64_t G, int64_t D) {
 SGL_RULE bool kv8_chunk_whole(int64_t capacity, int64_t items, int64_t fit) {
   return items >= 2 * fit || capacity <= 1024 || capacity * fit <= 4096 * items;
 }
+// Rows of a tile of few rows: 32, where there are more than 16, read the keys half as
+// often.  16 / 32, us, heads of 128, 1 sequence of 16000 and 8 of 4000: 16 rows 20 / 21, 32
+// rows 21 / 22 and 32 / 30, 48 rows 27 / 25 and 43 / 35, 64 rows 28 / 25 and 54 / 39; 32
+// sequences of 16 rows up to 6000 49 / 57.  Heads above 128 have no room for 32.
+SGL_RULE int64_t kv8_few_tile(int64_t rows, int64_t D) { return D <= 128 && rows > 16 ? 32 : 16; }
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
                                    int64_t cus) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
@@ -317,16 +331,16 @@ SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G,
     return {rt, kv8_chunk_whole(capacity, items, fit) ? 0 : kv8_attn_parts(fit, Hkv), items,
             kv8_attn_mixed(T, B, G, D) ? kv8_few_rows(D) : 0, 0x7FFFFFFF};
   }
-  const int64_t rt = D <= 128 && rows > 16 ? 32 : 16, items = kv8_attn_items(T, B, Hkv, G, rt);
-  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_attn_parts(2 * cus, Hkv), items, 0, 0x7FFFFFFF};
+  const int64_t rt = kv8_few_tile(rows, D), items = kv8_attn_items(T, B, Hkv, G, rt);
+  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, 0x7FFFFFFF};
 }
 // The second launch of a batch of chunks: its sequences of few rows.
 SGL_RULE Kv8AttnPlan kv8_attn_rest(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
                                    int64_t cus) {
   if (!kv8_attn_mixed(T, B, G, D)) return {16, 0, 0, 0, 0};
-  const int64_t rt = D <= 128 && G > 16 ? 32 : 16, upto = kv8_few_rows(D);
+  const int64_t rt = kv8_few_tile(G, D), upto = kv8_few_rows(D);
   const int64_t items = B * ((upto + rt - 1) / rt) * Hkv;
-  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_attn_parts(2 * cus, Hkv), items, 0, upto};
+  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, upto};
 }
 
 }  // namespace sgl

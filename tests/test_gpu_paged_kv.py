@@ -500,7 +500,9 @@ def test_attention_shared_between_workgroups(gpu, new, lens, Hq, Hkv, D, page, b
 
 
 @pytest.mark.parametrize("D,Hq,Hkv,new", [(128, 8, 2, 16), (128, 8, 2, 17), (64, 4, 1, 16), (64, 4, 1, 17),
-                                          (256, 8, 4, 8), (256, 8, 4, 9), (128, 4, 1, 64), (128, 4, 1, 65)])
+                                          (256, 8, 4, 8), (256, 8, 4, 9), (128, 4, 1, 64), (128, 4, 1, 65),
+                                          (128, 8, 2, 24), (128, 8, 2, 25), (64, 4, 1, 24), (64, 4, 1, 25),
+                                          (256, 8, 4, 16), (256, 8, 4, 17)])
 @pytest.mark.parametrize("tokens", [1024, 1040, 2048, 2064, 4200])
 def test_attention_on_both_sides_of_its_choices(gpu, D, Hq, Hkv, new, tokens):
     """The most rows that count as few and one token more, one row tile and two; tables that

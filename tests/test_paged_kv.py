@@ -85,16 +85,16 @@ def test_attention_plans(rules):
         T, D = B * int(rng.integers(1, 300)), 16 * int(rng.integers(1, 17))
         rt, parts, ws = plan(T, B, Hkv, G, D, 16 << int(rng.integers(0, 14)), int(rng.integers(8, 400)))
         assert rt in (16, 32, 128, 256) and parts % 8 == 0 and parts >= 0
-        assert (rt > 32) == (T * G // B > (64 if D <= 128 else 16))
+        assert (rt > 32) == (T * G // B > (96 if D <= 128 else 32))
         assert ws == parts * 2 * Hkv * rt * (D + 2) * 4  # two stretches a workgroup
         # a second launch takes exactly the sequences that the first leaves, all their row tiles
-        few = 64 if D <= 128 else 16
+        few = 96 if D <= 128 else 32
         assert o[5] == o[6] == (few if rt > 32 and B >= 8 and T > B else 0)
         assert o[4] == (B * -(-few // o[3]) * Hkv if o[5] else 0)
     # a short table: no sharing, no workspace; few rows up to 2048 tokens where items are many
-    assert plan(1, 1, 8, 4, 128, 1024)[1:] == (0, 0) and plan(1, 1, 8, 4, 128, 1040)[1] == 64
+    assert plan(1, 1, 8, 4, 128, 1024)[1:] == (0, 0) and plan(1, 1, 8, 4, 128, 1040)[1] == 32
     # (the items are a bound, T G / 16 + B row tiles for each of 8 heads: 52 sequences 520, 51 504)
-    assert plan(52, 52, 8, 4, 128, 2048)[1] == 0 and plan(51, 51, 8, 4, 128, 2048)[1] == 64
+    assert plan(52, 52, 8, 4, 128, 2048)[1] == 0 and plan(51, 51, 8, 4, 128, 2048)[1] == 32 and plan(9, 9, 8, 4, 64, 4096)[1] == 64
     # a chunk's row tiles: two a workgroup are not shared, fewer by how much there is to share
     assert plan(8192, 1, 8, 4, 128, 1 << 17)[1] == 0 and plan(512, 1, 8, 4, 128, 1 << 13)[1] == 32
     assert plan(2048, 1, 8, 4, 128, 4096)[1] == 0 and plan(2048, 1, 8, 4, 128, 8192)[1] == 32
