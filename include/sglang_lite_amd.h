@@ -522,9 +522,11 @@ int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_toke
  * `block` tokens of a page and head; a stored value is code * scale.  D a
  * multiple of 16 up to 256; page_size a power of two from 16 to 1024, block
  * one from 16 to 128 and at most page_size.  block_table int32 [B, row_pages]:
- * the pages of each sequence in order, token p in entry p / page_size.
+ * the pages of each sequence in order, token p in entry p / page_size (2^30 tokens
+ * at most).
  * Sequence b's rows of the token-major inputs are [cu_tokens[b],
- * cu_tokens[b + 1]) (int32 [B + 1], device), or row b with cu_tokens NULL.
+ * cu_tokens[b + 1]) (int32 [B + 1], device, never falling), or row b with
+ * cu_tokens NULL.
  *
  * Appends k and v [T, Hkv, D] (sgl_dtype, 16-byte aligned strides): row i of
  * sequence b becomes token start[b] + i.  With a table the keys are rotated
@@ -536,7 +538,8 @@ int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_toke
  * grew.  code = e4m3(x / scale), round to nearest even; NaN and infinities
  * become the NaN code.  Rows behind cu_tokens[B], tokens that the table does not
  * reach, entries outside [0, n_pages) and sequences with a negative start are
- * skipped.  Every page that is written to must belong to one sequence of the call. */
+ * skipped.  Every page that is written to must belong to one sequence of the call,
+ * at one place of its row. */
 int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                    int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv,
                    int D, const int32_t* cu_tokens, const int32_t* start, const int32_t* block_table,
@@ -554,7 +557,7 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
  * gives zeros.  Keys behind lens[b], and those on entries outside [0, n_pages),
  * are not seen, whatever their codes and scales hold; a lens[b] past the block
  * table is cut to it.  out [T, Hkv * G, D] dense, in q's type; rows behind
- * cu_tokens[B] are left as they are.  The workspace has
+ * cu_tokens[B] are left as they are.  One or two launches and their merges.  The workspace has
  * sgl_kv8_attn_workspace_size bytes, 16-byte aligned; calls that overlap need
  * their own. */
 int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T,

@@ -328,7 +328,8 @@ def _attention(c, q, lens, cu, scale, **kw):
         vr, _ = OP.rows(c.v, c.vs, c.table[b], L)
         y, size, reach = OP.attention(q[r0:r1], kr, vr, there, L - (r1 - r0), scale, **kw)
         o[r0:r1] = y
-        # a weight: rounded to bf16 for the product (2^-8 relative at most), its score an fp32 sum
+        # a weight: rounded to f16 for the product (2^-11 relative at most, or 2^-25 of the row's
+        # reference; 2^-8 is what bf16 would take), its score an fp32 sum
         # of D products (a step of 2^-23 each at most), then in log2 units and through exp2
         # (2^-20 with the sums over keys); normaliser and numerator both carry the score's error
         score = 2 * (D + 8) * 2.0 ** -23 * reach
@@ -544,6 +545,20 @@ def test_single_tokens_beside_prompts(gpu, D, Hq, Hkv, dtype, tokens):
     out = torch.full_like(q, 7.0)
     _check_attn(c, q, lens, cu, sink=s, window=450, out=out)
     assert bool((out[cu[-1]:] == 7.0).all())
+
+
+def test_many_single_tokens_beside_prompts(gpu):
+    """More sequences than a wavefront has lanes, prompts among the first, the last and between."""
+    rng = np.random.default_rng(3)
+    new = [400 if b in (0, 70, 139) else int(rng.integers(0, 3)) for b in range(140)]
+    lens = [n + int(rng.integers(0, 90)) for n in new]
+    assert sum(new) * 16 // 140 > 96  # (rows on average: a batch of chunks)
+    c = _filled(gpu, lens, 1, 128, 16, 16, seed=21)
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], 16, 128, torch.bfloat16, 4)
+    for tokens in (0, 16384):
+        _widen(c, tokens)
+        _check_attn(c, q, lens, cu)
 
 
 @pytest.mark.parametrize("new", [2, 150])
