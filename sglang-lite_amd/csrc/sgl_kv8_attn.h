@@ -230,8 +230,8 @@ __device__ __forceinline__ bool kv8_item(const Kv8AttnArgs& a, int64_t x, int* h
 }
 
 // The items that several workgroups share.  One wavefront a row (four a workgroup,
-// RT / 4 workgroups an item): lane p has part p's reference and weight, then all
-// lanes go over the parts' sums, several loads in flight.
+// RT / 4 workgroups an item): lane p has part p's reference and weight, and all lanes
+// go over the parts' sums.
 template <int RT, int TT, int QT>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
   Kv8Chunk c = kv8_chunk<RT, TT>(a, 0);
@@ -251,13 +251,21 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
   const float NEG_INF = -__builtin_huge_valf();
   auto slot = [&](int p) { return (2 * (int64_t)kv8_wg(a, head, p) + (p == pa ? 1 : 0)) * RT + r; };
 
+  // sums of 8 parts from p on, on their way while the references (or the last 8) are worked on
+  const int d = 4 * lane;
+  auto fetch = [&](int p, float4* x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = *reinterpret_cast<const float4*>(a.ws_acc + slot(p + k < pb ? p + k : pb) * a.D + (d < a.D ? d : 0));
+  };
+  float4 x[8];
+  fetch(pa, x);
   float M = NEG_INF;
   for (int p = pa + lane; p <= pb; p += 64) M = __builtin_fmaxf(M, a.ws_ml[slot(p) * 2]);
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d, 64));
+  for (int k = 32; k > 0; k >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, k, 64));
   const float ref = M == NEG_INF ? 0.0f : M;
   float l = 0.0f, acc[4] = {0, 0, 0, 0};
-  const int d = 4 * lane;
   for (int p0 = pa; p0 <= pb; p0 += 64) {
     float f = 0.0f;
     if (p0 + lane <= pb) {
@@ -266,23 +274,21 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
       l += ml.y * f;
     }
     const int n = pb - p0 < 63 ? pb - p0 + 1 : 64;
-    if (d < a.D) {
-      for (int i = 0; i < n; i += 8) {
-        float4 x[8];
+    for (int i = 0; i < n; i += 8) {
+      float4 y[8];
+      if (p0 + i + 8 <= pb) fetch(p0 + i + 8, y);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          x[k] = *reinterpret_cast<const float4*>(a.ws_acc + slot(p0 + (i + k < n ? i + k : n - 1)) * a.D + d);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float w = i + k < n ? bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(f), i + k)) : 0.0f;
-          if (i + k < n) {
-            acc[0] += x[k].x * w;
-            acc[1] += x[k].y * w;
-            acc[2] += x[k].z * w;
-            acc[3] += x[k].w * w;
-          }
+      for (int k = 0; k < 8; ++k) {
+        if (i + k < n) {
+          const float w = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(f), i + k));
+          acc[0] += x[k].x * w;
+          acc[1] += x[k].y * w;
+          acc[2] += x[k].z * w;
+          acc[3] += x[k].w * w;
         }
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = y[k];
     }
   }
 #pragma unroll
