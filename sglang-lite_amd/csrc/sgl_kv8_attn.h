@@ -47,7 +47,9 @@ struct Kv8AttnArgs {
   float* ws_ml;   // [2 parts Hkv][row tile][2]: reference point (log2 units), sum
 };
 
-constexpr int kItemCost = 2;  // key tiles
+// Key tiles.  1 / 2 / 3 / 5, us: 32 sequences of 4 queries up to 6000 keys 49.3 / 48.2 / 46.1 /
+// 47.2, 16 single ones up to 4000 25.6 / 24.8 / 23.3 / 23.5, 512 queries on 2000 57.0 / 55.2 / 51.8 / 53.8.
+constexpr int kItemCost = 3;
 
 // A sequence as the line sees it.
 struct Kv8Seq {

@@ -304,7 +304,8 @@ SGL_RULE int64_t kv8_few_rows(int64_t D) { return D <= 128 ? 96 : 32; }
 // times the few rows' kernel: from 8 sequences on, each kernel takes those of its own.
 // 32 query heads on 8 kv heads of 128, two launches / the chunk's alone, us: 63 x 1 query on
 // 4000 keys + 2000 on 2000 168 / 298, 15 x 1 on 8000 + 512 on 8000 152 / 215, 7 x 1 + 512
-// on 8000 129 / 151; where there are no few rows after all 16 x 128 54 / 52, 8 x 512 198 / 192.
+// on 8000 129 / 151; where there are no few rows after all 16 x 128 54 / 52, 8 x 512 198 / 192,
+// 8 x 64 on 4000 87 / 77.
 SGL_RULE bool kv8_attn_mixed(int64_t T, int64_t B, int64_t G, int64_t D) {
   return B >= 8 && T * G / B > kv8_few_rows(D) && T > B;
 }
