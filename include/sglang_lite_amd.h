@@ -553,8 +553,10 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
  * Causal: a query sees the keys up to its own position, with window > 0 the last
  * `window` of them; otherwise all lens[b].
  *   o = sum_j e^(s_j) v_j / (sum_j e^(s_j) + e^(sink[h])),  s_j = softmax_scale q . k_j
- * (sink fp32 [Hkv * G] or NULL: no such term).  fp32 sums; a row that sees no key
- * gives zeros.  Keys behind lens[b], and those on entries outside [0, n_pages),
+ * (sink fp32 [Hkv * G] or NULL: no such term).  fp32 sums, the normaliser's of fp32
+ * weights; the weights that meet the values are f16, rounded by at most 2^-11 of
+ * themselves, or 2^-35 of the row's largest (each times its value's scale).  A row
+ * that sees no key gives zeros.  Keys behind lens[b], and those on entries outside [0, n_pages),
  * are not seen, whatever their codes and scales hold; a lens[b] past the block
  * table is cut to it.  out [T, Hkv * G, D] dense, in q's type; rows behind
  * cu_tokens[B] are left as they are.  One or two launches and their merges.  The workspace has

@@ -20,9 +20,9 @@
 // A conversion e4m3 -> bf16 (exact) is one instruction for two codes.  The
 // scales are one number for 16 tokens: s_k multiplies the score, log2 s_v is added
 // to it, so that P carries s_v.  P and the codes of V are f16 for every type of q: a
-// code is exact there, a weight is rounded by at most 2^-12 of itself (bf16: 2^-9) or
-// 2^-25 of the row's reference, and that is the only rounding between the codes and
-// the output's own.
+// code is exact there, a weight is rounded by at most 2^-11 of itself (bf16: 2^-8) or
+// 2^-35 of the row's largest (kLift), and that is the only rounding between the codes
+// and the output's own.
 #include "sgl_kv8_attn.h"
 
 namespace sgl {
@@ -233,11 +233,11 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       }
     };
 
-    float kcs, evs, ivs;  // of the batch: score scale, log2 of the value scale, its reciprocal
+    float kcs, evs, ivs;  // of the batch: score scale, kLift + log2 of the value scale, 2^-that
     uint64_t okm;
     auto use = [&](const Batch& o) __attribute__((always_inline)) {
       kcs = o.ok ? o.ks * a.c1 : 0.0f;  // (what was never written may hold anything)
-      evs = o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.vs), -100.0f) : 0.0f;
+      evs = o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.vs), -100.0f) + kLift : 0.0f;
       ivs = __builtin_amdgcn_exp2f(-evs);
       okm = __ballot(o.ok);
     };
@@ -275,8 +275,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
           }
         }
       }
-      // P^T = 2^(s + log2 s_v - m): the value's scale is part of the exponent, so that
-      // P fits f16 as well, and the sum of the probabilities takes it back
+      // P^T = 2^(s + log2 s_v + kLift - m): the value's scale is part of the exponent, so
+      // that P fits f16 as well, and the sum of the probabilities takes both back
       float kc[2], ev[2], iv[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -297,13 +297,13 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         float mx = f[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = __builtin_fmaxf(mx, f[i]);
-        // The reference moves only when a weight's exponent exceeds it by more than 6
-        // (log2 units): any reference gives the same softmax, the weights stay at
-        // most 64, and the accumulators are rarely rescaled.
-        if (__ballot(!(mx <= m_run[c] + 6.0f) && mx != NEG_INF)) {
+        // The reference moves only when a weight's exponent exceeds it by more than 15.5
+        // (log2 units), to kLift below: any reference gives the same softmax, the
+        // weights fit f16, and the accumulators are rarely rescaled.
+        if (__ballot(!(mx <= m_run[c] + 15.5f) && mx != NEG_INF)) {
           mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
           mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float next = mx <= m_run[c] + 6.0f ? m_run[c] : __builtin_fmaxf(m_run[c], mx);
+          const float next = mx <= m_run[c] + 15.5f ? m_run[c] : __builtin_fmaxf(m_run[c], mx - kLift);
           const float alpha = next == m_run[c] ? 1.0f : __builtin_amdgcn_exp2f(m_run[c] - next);
           m_run[c] = next;
           l_run[c] *= alpha;
@@ -429,7 +429,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
           const float f = __builtin_amdgcn_exp2f(sM[w][n] - ref);
           sum += sL[w][n] * f;
 #pragma unroll
-          for (int v = 0; v < 8; ++v) y[v] += sAcc[w][n][d + v] * f;
+          for (int v = 0; v < 8; ++v) y[v] += sAcc[w][n][d + v] * (f * kUnlift);
         }
         if (whole) {
           const int row = rt * RT + r, t = row / a.G, h = head * a.G + (row - t * a.G);

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
   constexpr bool QL = DP >= 128;
   __shared__ __align__(16) u4v sQ[QL ? NW : 1][QL ? KS : 1][64];
   __shared__ __align__(4) uint16_t sDims[2][kKeys][CPR];  // of a tile seen in part: a token's dims with NaN codes
-  __shared__ __align__(8) float2 sScale[2][64];           // of a batch's granules: score scale, log2 of the value scale
+  __shared__ __align__(8) float2 sScale[2][64];           // of a batch's granules: score scale, kLift + log2 of the value scale
   __shared__ int sNan[2];                                 // 1 + the last such tile in the buffer that has any
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c32 = lane & 31, g2 = lane >> 5;
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
-    float m_run = live ? NEG_INF : 0.0f, l_run = 0.0f;  // (a row that is none never asks for a reference)
+    float m_run = live ? NEG_INF : 1e30f, l_run = 0.0f;  // (a row that is none never asks for a reference)
 
     if (j0 < j1) {
       u4v q[KS];  // (with QL only until they are in LDS)
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       auto use = [&](int batch, const Batch& o) __attribute__((always_inline)) {
         // (what was never written may hold anything)
         sScale[batch & 1][lane] = make_float2(o.ok ? o.k * a.c1 : 1.0f,
-                                              o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) : 0.0f);
+                                              o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) + kLift : 0.0f);
         okm = __ballot(o.ok);
       };
 
@@ -343,7 +343,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         // masks, NaN codes, rows without a reference.
         // The reference m need not be the maximum: any m gives the same softmax.  So
         // no maximum is taken unless a row has no reference yet (its sums are zero
-        // then), or, below, the weights of its tile pass 2^13 (f16 holds 2^15).
+        // then), or, below, eight weights pass what one f16 holds.  It lies kLift
+        // below the maximum that it was taken from.
         const bool border = (i & (TB - 1)) == 0 && i > 0;
         const bool seen_by_all = tok + kKeys <= all_hi && tok >= all_lo;
         if (__builtin_expect(border || (i & (TB - 1)) == 4 || !seen_by_all || partial(j) || (okm >> l0 & kAll) != kAll || fresh, 0)) {
@@ -367,11 +368,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           }
           if (fresh) {
             const float mx = top();
-            m_run = m_run == NEG_INF ? mx : m_run;
+            m_run = m_run == NEG_INF ? mx - kLift : m_run;
             fresh = __ballot(m_run == NEG_INF) != 0;
           }
         }
-        // P^T = 2^(s + log2 s_v - m), so that s_v is in the exponent, and the sum takes it back
+        // P^T = 2^(s + log2 s_v + kLift - m), so that s_v is in the exponent, and the sum takes it back
         float2 kv = scale[NG - 1], kv_next;
         float eg = 0.0f, sum = 0.0f, most = 0.0f, l_new = l_run;
         // The granules' order is NG - 1, 0, 1, ...: those of the tile before are used up in
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           sum += w;
           if (e == 6) {  // the sum of the probabilities takes s_v back
             l_new = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-kv.y), l_new);
-            most += sum;
+            most = __builtin_fmaxf(most, sum);
           }
         };
 
@@ -432,10 +433,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
             load_codes(j + 3, (i & (TB - 1)) >= TB - 3 ? ahead.page : now.page, j + 1, (i & (TB - 1)) == TB - 1 ? ahead.page : now.page, raw);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (__builtin_expect(__ballot(!(most <= 8192.0f)) != 0, 0)) {
+        if (__builtin_expect(__ballot(most > 60000.0f) != 0, 0)) {
 #pragma unroll
           for (int t = 0; t < NH; ++t) asm volatile("" : "+v"(sc[t]));  // (nothing of this is to be done before the branch)
-          const float nx = __builtin_fmaxf(m_run, top());
+          const float nx = __builtin_fmaxf(m_run, top() - kLift);
           const float alpha = nx == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - nx);
           m_run = nx;
           l_new = l_run * alpha;
@@ -504,7 +505,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       if (whole) {
         const float ref = m_run == NEG_INF ? 0.0f : m_run;
         const float sum = a.sink ? l_run + __builtin_amdgcn_exp2f(a.sink[hq] * kLog2e - ref) : l_run;
-        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        const float inv = sum > 0.0f || sum != sum ? kUnlift / sum : 0.0f;
         uint16_t* o = a.o + ((int64_t)(s.row0 + tq) * (a.Hkv * a.G) + hq) * a.D + 4 * g2;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -522,7 +523,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           for (int k = 0; k < 4; ++k)
             if (32 * d + 8 * k < a.D)
               *reinterpret_cast<float4*>(o + 32 * d + 8 * k) =
-                  make_float4(acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]);
+                  make_float4(acc[d][4 * k] * kUnlift, acc[d][4 * k + 1] * kUnlift, acc[d][4 * k + 2] * kUnlift,
+                              acc[d][4 * k + 3] * kUnlift);
         if (g2 == 0) *reinterpret_cast<float2*>(a.ws_ml + (slot * RT + r) * 2) = make_float2(m_run, l_run);
       }
     }

@@ -28,6 +28,14 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The products take weights as f16, 2^kLift times what the reference point makes of them: an
+// f16 reaches 2^16 above 1 but loses bits from 2^-14 on and is 0 from 2^-25 on, and small weights
+// are all that a row has where the keys above them have no value.  So a key's weight keeps 11
+// bits down to 2^-24 of the row's largest (each times its value's scale) and counts down to 2^-35
+// of it, about 24 in the exponent of e.  2^kLift is in the exponent beside the value's scale, so it
+// costs nothing but the room for a maximum to grow before a reference has to move.
+constexpr float kLift = 10.0f, kUnlift = 0x1p-10f;
+
 struct Kv8AttnArgs {
   const uint16_t* q;
   int64_t qt, qh;  // elements between tokens, heads

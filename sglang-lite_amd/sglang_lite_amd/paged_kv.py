@@ -179,7 +179,9 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     ``causal``: a query sees the keys up to its own position, the last ``window``
     of them if that is not 0; otherwise all.  ``sink`` (float32 ``[Hq]``): a
     logit of each head that takes part in the softmax and has no value.
-    ``softmax_scale``: ``D ** -0.5`` by default.  A row that sees no key is zero;
+    ``softmax_scale``: ``D ** -0.5`` by default.  The weights that meet the values
+    are rounded by at most 2^-11 of themselves, or 2^-35 of the row's largest (each
+    times its value's scale).  A row that sees no key is zero;
     rows behind the last sequence are not written (of a new tensor: they hold
     anything)."""
     pages, heads, page, dim, block = _check_cache(cache, "paged_attn")
