@@ -109,3 +109,67 @@ def test_small_weights_under_a_dominant_key_without_a_value(gpu, tokens, D, new,
     q = _queries(gpu, new, Hq, D, dtype, 5)
     q[..., 0] = 8.0
     _check_sharp(c, q, [L], [0, new])
+
+
+CASES = [
+    # new, lens, Hq, Hkv, D, page, block, dtype, window, sink
+    ([1], [5000], 8, 2, 128, 64, 64, torch.float16, 0, False),
+    ([1, 1, 1], [700, 2000, 33], 16, 2, 64, 16, 16, torch.float16, 0, True),
+    ([4, 2], [2000, 900], 8, 2, 128, 64, 32, torch.float16, 500, False),
+    ([1], [1500], 8, 1, 256, 128, 128, torch.bfloat16, 0, False),
+    ([40, 3], [2000, 260], 4, 1, 256, 64, 64, torch.float16, 0, False),
+    ([150, 30], [1500, 700], 8, 2, 128, 32, 16, torch.float16, 0, True),
+    ([200], [2000], 8, 2, 64, 64, 64, torch.float16, 600, False),
+    ([130], [900], 4, 1, 96, 64, 64, torch.bfloat16, 0, False),
+]
+
+
+@pytest.mark.parametrize("tokens", [0, 16384])
+@pytest.mark.parametrize("new,lens,Hq,Hkv,D,page,block,dtype,window,sink", CASES)
+def test_attention_within_the_roundings_of_its_weights(gpu, tokens, new, lens, Hq, Hkv, D, page, block, dtype,
+                                                       window, sink):
+    c = _filled(gpu, lens, Hkv, D, page, block, seed=D + Hq)
+    _widen(c, tokens)
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], Hq, D, dtype, 9)
+    s = (np.random.default_rng(2).standard_normal(Hq) * 2).astype(np.float32) if sink else None
+    _check_sharp(c, q, lens, cu, window=window, sink=s)
+
+
+@pytest.mark.parametrize("tokens", [0, 16384])
+@pytest.mark.parametrize("new,L,H,D,page,window,dtype", [
+    (1, 4500, 8, 128, 64, 0, torch.float16),
+    (1, 2300, 4, 64, 16, 1000, torch.float16),
+    (1, 2100, 2, 256, 128, 0, torch.bfloat16),
+    (20, 1500, 8, 128, 32, 0, torch.float16),    # 32 rows a tile
+    (130, 1300, 8, 128, 64, 0, torch.float16),   # chunks
+    (150, 1300, 8, 64, 16, 700, torch.float16),
+    (40, 700, 4, 256, 64, 0, torch.bfloat16),
+])
+def test_every_key_counts_once(gpu, tokens, new, L, H, D, page, window, dtype):
+    """Values of zero but for one key in each dim of a kv head: the output is that key's weight.
+    As many rounds as it takes for every key to have had its dim."""
+    c = Cache(gpu, 1, L, H, D, page, 16, seed=4)
+    _widen(c, tokens)
+    g = torch.Generator(device=gpu).manual_seed(L)
+    k = 0.5 * torch.randn(L, H, D, generator=g, device=gpu)
+    q = _queries(gpu, new, 2 * H, D, dtype, 11)
+    for base in range(0, L, H * D):
+        v = torch.zeros(L, H, D, device=gpu)
+        t = base + torch.arange(H * D, device=gpu)
+        t = t[t < L]
+        v[t, (t - base) // D, (t - base) % D] = 1.0 + (t % 7) / 8.0
+        _append(c, k, v, [0], [0, L])
+        _check_sharp(c, q, [L], [0, new], window=window, rms=False)
+
+
+@pytest.mark.parametrize("new", [1, 130])
+def test_a_sequence_beside_others_of_other_lengths(gpu, new):
+    """The seams between workgroups move with the batch; the result stays within its bounds."""
+    for others in ([], [40], [3000, 10], [9000], [500] * 30):
+        lens = [2500] + others
+        c = _filled(gpu, lens, 2, 128, 64, 64, seed=15)
+        _widen(c, 16384)
+        cu = [0] + np.cumsum([new] + [1] * len(others)).tolist()
+        q = _queries(gpu, cu[-1], 8, 128, torch.float16, 12)
+        _check_sharp(c, q, lens, cu)
