@@ -196,8 +196,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       // same values to the same place, and reads behind its own writes.
       uint64_t okm = 0;
       auto use = [&](int batch, const Batch& o) __attribute__((always_inline)) {
-        // (what was never written may hold anything)
-        sScale[batch & 1][lane] = make_float2(o.ok ? o.k * a.c1 : 1.0f,
+        // (what was never written may hold anything).  A score of -inf, a key not seen,
+        // has to stay one: a scale of 0 becomes the smallest above it.
+        const float k = o.k * a.c1;
+        sScale[batch & 1][lane] = make_float2(!o.ok ? 1.0f : k == 0.0f ? 0x1p-149f : k,
                                               o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) + kLift : 0.0f);
         okm = __ballot(o.ok);
       };

@@ -1,0 +1,51 @@
+"""Caches whose scales the append would not write: zero, tiny, not a power of two, not finite.  A
+stored value is code * scale whatever the scale is; a token is seen by those that may see it."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_paged_kv import _check_attn, _filled, _queries, _widen
+
+pytestmark = pytest.mark.gpu
+
+KERNELS = [(1, 128), (30, 64), (30, 256), (150, 64), (150, 128), (150, 256)]  # queries, head dim
+FEW_AND_CHUNKS = pytest.mark.parametrize("new,D", KERNELS)
+TOKENS = pytest.mark.parametrize("tokens", [0, 16384])
+
+
+def _set(c, side, token, value, head=slice(None)):
+    """The scale of a token's block (sequence 0)."""
+    page, block = c.k.shape[2], c.k.shape[2] // c.ks.shape[2]
+    p, piece = int(c.table[0, token // page]), token % page // block
+    ours, theirs = ((c.kv.k_scale, c.ks), (c.kv.v_scale, c.vs))[side]
+    ours[p, head, piece] = value
+    theirs[p, head, piece] = value
+
+
+@TOKENS
+@FEW_AND_CHUNKS
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_of_keys_whose_scale_is_zero(gpu, tokens, new, D, window):
+    """Scores of zero for those who see them, nothing for the others: the last block, one that the
+    rows see in part, one at a window's edge."""
+    L = 200
+    c = _filled(gpu, [L], 2, D, 64, 16, seed=3)
+    for t in (L - 1, L - new // 2 - 1, 100, max(0, L - new - 20)):
+        _set(c, 0, t, 0.0, head=t % 2)
+    _widen(c, tokens)
+    _check_attn(c, _queries(gpu, new, 4, D, torch.bfloat16, 5), [L], [0, new], window=window)
+
+
+@TOKENS
+@FEW_AND_CHUNKS
+def test_a_softmax_scale_that_takes_scores_below_the_smallest_float(gpu, tokens, new, D):
+    """Keys of zero have the scale 2^-100, and with 1e-25 before it 0 in fp32: equal weights."""
+    L = 200
+    c = _filled(gpu, [L], 2, D, 64, 16, seed=3)
+    for t in range(0, L, 16):
+        _set(c, 0, t, 2.0 ** -100)
+    _widen(c, tokens)
+    _check_attn(c, _queries(gpu, new, 4, D, torch.bfloat16, 5), [L], [0, new], softmax_scale=1e-25)
