@@ -234,12 +234,14 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
     };
 
     float kcs, evs, ivs;  // of the batch: score scale, kLift + log2 of the value scale, 2^-that
-    uint64_t okm;
+    uint64_t okm;  // granules that are there, with scales as they should be
     auto use = [&](const Batch& o) __attribute__((always_inline)) {
-      kcs = o.ok ? o.ks * a.c1 : 0.0f;  // (what was never written may hold anything)
-      evs = o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.vs), -100.0f) + kLift : 0.0f;
+      // (what was never written may hold anything)
+      const bool good = kv8_scale_ok(o.ks) && kv8_scale_ok(o.vs);
+      kcs = !o.ok ? 0.0f : good ? o.ks * a.c1 : __builtin_nanf("");
+      evs = !o.ok ? kNoToken : good ? __builtin_fmaxf(__builtin_amdgcn_logf(o.vs), -100.0f) + kLift : kBadScale;
       ivs = __builtin_amdgcn_exp2f(-evs);
-      okm = __ballot(o.ok);
+      okm = __ballot(o.ok && good);
     };
     auto lane_f = [&](float v, int l) { return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), l)); };
 
@@ -262,6 +264,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         }
       }
       const bool plain = tok + 32 <= all_hi && tok >= all_lo && ok == 3;
+      const uint32_t here = plain ? 3u : (uint32_t)(__ballot(evs != kNoToken) >> l0) & 3u;
       uint32_t seen[NC];  // bit 4 u + i: the row sees token 16 u + 4 g + i
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = tok + 16 * (i >> 2) + 4 * g + (i & 3);
-            if (key < hi[c] && key >= lo[c] && key < s.len && ((ok >> (i >> 2)) & 1u)) seen[c] |= 1u << i;
+            if (key < hi[c] && key >= lo[c] && key < s.len && ((here >> (i >> 2)) & 1u)) seen[c] |= 1u << i;
           }
         }
       }
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         uint32_t nan[8][W], any = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool there = tok + 16 * (j >> 2) + 4 * g + (j & 3) < s.len && ((ok >> (j >> 2)) & 1u);
+          const bool there = tok + 16 * (j >> 2) + 4 * g + (j & 3) < s.len && ((here >> (j >> 2)) & 1u);
 #pragma unroll
           for (int w = 0; w < W; ++w) {
             const uint32_t v = there ? r.v[j][w] : 0u;

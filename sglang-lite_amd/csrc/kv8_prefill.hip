@@ -194,14 +194,18 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       // A granule's two numbers are read back as a broadcast (v_readlane takes four
       // times as long as a plain VALU instruction here).  Every wavefront writes the
       // same values to the same place, and reads behind its own writes.
-      uint64_t okm = 0;
+      uint64_t okm = 0;  // granules that are there, with scales as they should be
       auto use = [&](int batch, const Batch& o) __attribute__((always_inline)) {
         // (what was never written may hold anything).  A score of -inf, a key not seen,
         // has to stay one: a scale of 0 becomes the smallest above it.
+        const bool good = kv8_scale_ok(o.k) && kv8_scale_ok(o.v);
         const float k = o.k * a.c1;
-        sScale[batch & 1][lane] = make_float2(!o.ok ? 1.0f : k == 0.0f ? 0x1p-149f : k,
-                                              o.ok ? __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) + kLift : 0.0f);
-        okm = __ballot(o.ok);
+        sScale[batch & 1][lane] =
+            make_float2(!o.ok || !good ? 1.0f : k == 0.0f ? 0x1p-149f : k,
+                        !o.ok   ? kNoToken
+                        : !good ? kBadScale
+                                : __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) + kLift);
+        okm = __ballot(o.ok && good);
       };
 
       // ---- staging: piece i of this thread is 16 codes of token ptok + i TSTEP.  A
@@ -244,11 +248,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       };
       // Values behind the last key, or on no page, were never written: zeros, which
       // meet zeros of P.
-      auto clear_missing = [&](int j, uint32_t ok, uint4* in) __attribute__((always_inline)) {
+      auto clear_missing = [&](int j, uint32_t here, uint4* in) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int t = tok_of(i, ptok);
-          if (is_v(i) && (j * kKeys + t >= s.len || !((ok >> (t >> 4)) & 1u))) in[i] = make_uint4(0, 0, 0, 0);
+          if (is_v(i) && (j * kKeys + t >= s.len || !((here >> (t >> 4)) & 1u))) in[i] = make_uint4(0, 0, 0, 0);
         }
       };
       // A tile that some rows see in part: its NaN codes are zeroed, so that 0 * NaN
@@ -357,15 +361,26 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           }
           if ((i & (TB - 1)) == 4) load_scales(i / TB + 1, ahead);
           const uint32_t ok = (uint32_t)(okm >> l0) & kAll;
-          if (tok + kKeys > s.len || ok != kAll) clear_missing(j, ok, raw);
+          uint32_t here = kAll;
+          if (__builtin_expect(ok != kAll, 0)) {
+            here = (uint32_t)(__ballot(sScale[(i / TB) & 1][lane].y != kNoToken) >> l0) & kAll;
+            if (here != ok) {
+#pragma unroll
+              for (int t = 0; t < NH; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  if (((here & ~ok) >> (2 * t + (e >> 3))) & 1) sc[t][e] = __builtin_nanf("");
+            }
+          }
+          if (tok + kKeys > s.len || here != kAll) clear_missing(j, here, raw);
           if (partial(j)) take_nan(j, buf, raw);
-          if (!seen_by_all || ok != kAll) {
+          if (!seen_by_all || here != kAll) {
 #pragma unroll
             for (int t = 0; t < NH; ++t)
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 const int key = tok + 32 * t + 8 * (e >> 2) + 4 * g2 + (e & 3);
-                if (!(key < hi && key >= lo && ((ok >> (2 * t + (e >> 3))) & 1))) sc[t][e] = NEG_INF;
+                if (!(key < hi && key >= lo && ((here >> (2 * t + (e >> 3))) & 1))) sc[t][e] = NEG_INF;
               }
           }
           if (fresh) {

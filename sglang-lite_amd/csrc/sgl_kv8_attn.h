@@ -59,6 +59,11 @@ struct Kv8AttnArgs {
 // 47.2, 16 single ones up to 4000 25.6 / 24.8 / 23.3 / 23.5, 512 queries on 2000 57.0 / 55.2 / 51.8 / 53.8.
 constexpr int kItemCost = 3;
 
+// In the place of a granule's exponent (kLift + log2 of its value scale, -90 to 138): there is no
+// such token; a scale of it is negative or not finite, which makes NaN of its keys and values.
+constexpr float kNoToken = 1000.0f, kBadScale = 2000.0f;
+__device__ __forceinline__ bool kv8_scale_ok(float s) { return s >= 0.0f && s < __builtin_huge_valf(); }
+
 // A sequence as the line sees it.
 struct Kv8Seq {
   int row0, n, len;  // first query row, queries, keys

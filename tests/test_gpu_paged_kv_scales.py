@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged_kv import _check_attn, _filled, _queries, _widen
+from test_gpu_paged_kv import _check_attn, _filled, _host, _queries, _widen
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,36 @@ def test_a_softmax_scale_that_takes_scores_below_the_smallest_float(gpu, tokens,
         _set(c, 0, t, 2.0 ** -100)
     _widen(c, tokens)
     _check_attn(c, _queries(gpu, new, 4, D, torch.bfloat16, 5), [L], [0, new], softmax_scale=1e-25)
+
+
+@TOKENS
+@FEW_AND_CHUNKS
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("window", [0, 40])
+def test_a_scale_that_is_not_finite_reaches_the_rows_that_see_its_tokens(gpu, tokens, new, D, side, value, window):
+    """As NaN, and no other row: those before the block, those whose window is behind it."""
+    L = 200
+    c = _filled(gpu, [L], 2, D, 64, 16, seed=3)
+    c.kv.k.view(torch.uint8)[:, :, :, 0] = 0  # (a code of zero times an infinity is NaN)
+    _set(c, side, 180, value, head=0)          # rows from token 176 on
+    if window:
+        _set(c, side, 100, value, head=1)      # rows up to token 111 + 39
+    _widen(c, tokens)
+    q = _queries(gpu, new, 4, D, torch.bfloat16, 5)
+    lens = torch.tensor([L], dtype=torch.int32, device=gpu)
+    cu = torch.tensor([0, new], dtype=torch.int32, device=gpu)
+    o = _host(c.P.paged_attn(q, c.kv, c.bt, lens, cu_tokens=cu, window=window))
+    good = _filled(gpu, [L], 2, D, 64, 16, seed=3)
+    good.kv.k.view(torch.uint8)[:, :, :, 0] = 0
+    _widen(good, tokens)
+    want = _host(good.P.paged_attn(q, good.kv, good.bt, lens, cu_tokens=cu, window=window))
+    pos = L - new + np.arange(new)
+    bad = np.zeros((new, 4), bool)
+    bad[:, :2] = (pos >= 176)[:, None]
+    if window:
+        bad[:, 2:] = ((pos >= 96) & (pos - window + 1 <= 111))[:, None]
+    assert np.isnan(o[bad]).all()
+    assert np.isfinite(o[~bad]).all()
+    # (the same sums but for where a reference was taken: a rounding of the output and of weights)
+    np.testing.assert_allclose(o[~bad], want[~bad], rtol=2.0 ** -6, atol=2.0 ** -8)
