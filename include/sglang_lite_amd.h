@@ -520,7 +520,8 @@ int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_toke
 /* The 8-bit paged cache: e4m3 codes [n_pages, Hkv, page_size, D] of keys and of
  * values, and fp32 scales [n_pages, Hkv, page_size / block], one for every
  * `block` tokens of a page and head; a stored value is code * scale.  Scales are
- * finite and not negative; tokens of one that is not are NaN.  D a
+ * finite and not negative; tokens of one that is not are NaN, and the attention
+ * takes values of a scale below 2^-100 as zero.  D a
  * multiple of 16 up to 256; page_size a power of two from 16 to 1024, block
  * one from 16 to 128 and at most page_size.  block_table int32 [B, row_pages]:
  * the pages of each sequence in order, token p in entry p / page_size (2^30 tokens

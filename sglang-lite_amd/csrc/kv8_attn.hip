@@ -239,9 +239,9 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       // (what was never written may hold anything)
       const bool good = kv8_scale_ok(o.ks) && kv8_scale_ok(o.vs);
       kcs = !o.ok ? 0.0f : good ? o.ks * a.c1 : __builtin_nanf("");
-      evs = !o.ok ? kNoToken : good ? __builtin_fmaxf(__builtin_amdgcn_logf(o.vs), -100.0f) + kLift : kBadScale;
+      evs = kv8_exponent(o.ok, good, o.vs);
       ivs = __builtin_amdgcn_exp2f(-evs);
-      okm = __ballot(o.ok && good);
+      okm = __ballot(evs < kNoToken && evs != kNoValue);
     };
     auto lane_f = [&](float v, int l) { return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), l)); };
 
@@ -332,6 +332,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         // What no row sees must not reach the product: keys behind the last
         // (never written) are zeroed.  A NaN code that some rows see and others
         // do not is zeroed too and put back into the sums of those that do.
+        const uint32_t none = (uint32_t)(__ballot(evs == kNoValue) >> l0) & 3u;
         uint32_t nan[8][W], any = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
             const uint32_t bad = (((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
             any |= bad;
             nan[j][w] = bad * 0x38u;  // 1.0
-            r.v[j][w] = v & ~(bad * 0xFFu);
+            r.v[j][w] = (none >> (j >> 2)) & 1u ? 0u : v & ~(bad * 0xFFu);
           }
         }
         if (__ballot(any != 0)) {

@@ -201,11 +201,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         const bool good = kv8_scale_ok(o.k) && kv8_scale_ok(o.v);
         const float k = o.k * a.c1;
         sScale[batch & 1][lane] =
-            make_float2(!o.ok || !good ? 1.0f : k == 0.0f ? 0x1p-149f : k,
-                        !o.ok   ? kNoToken
-                        : !good ? kBadScale
-                                : __builtin_fmaxf(__builtin_amdgcn_logf(o.v), -100.0f) + kLift);
-        okm = __ballot(o.ok && good);
+            make_float2(!o.ok || !good ? 1.0f : k == 0.0f ? 0x1p-149f : k, kv8_exponent(o.ok, good, o.v));
+        okm = __ballot(o.ok && good && o.v >= 0x1p-100f);
       };
 
       // ---- staging: piece i of this thread is 16 codes of token ptok + i TSTEP.  A
@@ -254,6 +251,16 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           const int t = tok_of(i, ptok);
           if (is_v(i) && (j * kKeys + t >= s.len || !((here >> (t >> 4)) & 1u))) in[i] = make_uint4(0, 0, 0, 0);
         }
+      };
+      // Values that count as zero: only NaN codes are left of them.
+      auto clear_values = [&](uint32_t none, uint4* in) __attribute__((always_inline)) {
+        auto nan_alone = [](uint32_t w) {
+          return w & ((((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xFFu;
+        };
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+          if (is_v(i) && ((none >> (tok_of(i, ptok) >> 4)) & 1u))
+            in[i] = make_uint4(nan_alone(in[i].x), nan_alone(in[i].y), nan_alone(in[i].z), nan_alone(in[i].w));
       };
       // A tile that some rows see in part: its NaN codes are zeroed, so that 0 * NaN
       // reaches no row's sum, and noted, for the rows that do see them.
@@ -363,13 +370,16 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           const uint32_t ok = (uint32_t)(okm >> l0) & kAll;
           uint32_t here = kAll;
           if (__builtin_expect(ok != kAll, 0)) {
-            here = (uint32_t)(__ballot(sScale[(i / TB) & 1][lane].y != kNoToken) >> l0) & kAll;
+            const float mark = sScale[(i / TB) & 1][lane].y;
+            here = (uint32_t)(__ballot(mark != kNoToken) >> l0) & kAll;
             if (here != ok) {
+              const uint32_t bad = (uint32_t)(__ballot(mark == kBadScale) >> l0);
 #pragma unroll
               for (int t = 0; t < NH; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                  if (((here & ~ok) >> (2 * t + (e >> 3))) & 1) sc[t][e] = __builtin_nanf("");
+                  if ((bad >> (2 * t + (e >> 3))) & 1) sc[t][e] = __builtin_nanf("");
+              clear_values((uint32_t)(__ballot(mark == kNoValue) >> l0), raw);
             }
           }
           if (tok + kKeys > s.len || here != kAll) clear_missing(j, here, raw);

@@ -60,9 +60,15 @@ struct Kv8AttnArgs {
 constexpr int kItemCost = 3;
 
 // In the place of a granule's exponent (kLift + log2 of its value scale, -90 to 138): there is no
-// such token; a scale of it is negative or not finite, which makes NaN of its keys and values.
-constexpr float kNoToken = 1000.0f, kBadScale = 2000.0f;
+// such token; a scale of it is negative or not finite, which makes NaN of its keys and values;
+// its values count as zero (NaN codes as NaN).  The last is for value scales below 2^-100, whose
+// reciprocal times the weights of a long sequence would not fit fp32: no value of theirs reaches
+// 2^-91.  The append writes 2^-100 at least.
+constexpr float kNoToken = 1000.0f, kBadScale = 2000.0f, kNoValue = -91.0f;
 __device__ __forceinline__ bool kv8_scale_ok(float s) { return s >= 0.0f && s < __builtin_huge_valf(); }
+__device__ __forceinline__ float kv8_exponent(bool there, bool good, float vs) {
+  return !there ? kNoToken : !good ? kBadScale : vs < 0x1p-100f ? kNoValue : __builtin_amdgcn_logf(vs) + kLift;
+}
 
 // A sequence as the line sees it.
 struct Kv8Seq {

@@ -3,7 +3,8 @@
 The cache (:class:`PagedKV`) keeps keys and values as e4m3 codes ``[pages, Hkv,
 page, D]`` with one fp32 scale for each block of tokens and head ``[pages, Hkv,
 page / block]``: a stored value is code * scale (finite, not negative; tokens of a scale
-that is not are NaN).  A layer's step is
+that is not are NaN, and the attention takes values of one below 2^-100 as zero).  A
+layer's step is
 
     q = rotary(q, table, positions)
     append_kv(cache, k, v, block_table, start, cu_tokens=cu, table=table)

@@ -82,3 +82,19 @@ def test_a_scale_that_is_not_finite_reaches_the_rows_that_see_its_tokens(gpu, to
     assert np.isfinite(o[~bad]).all()
     # (the same sums but for where a reference was taken: a rounding of the output and of weights)
     np.testing.assert_allclose(o[~bad], want[~bad], rtol=2.0 ** -6, atol=2.0 ** -8)
+
+
+@TOKENS
+@FEW_AND_CHUNKS
+def test_values_whose_scale_is_zero_are_zero(gpu, tokens, new, D):
+    """Also alone, where nothing is added to hide them; beside others they take their weight."""
+    L = 200
+    c = _filled(gpu, [L], 2, D, 64, 16, seed=3)
+    for t in range(0, L, 16):
+        _set(c, 1, t, 0.0, head=0)  # all of head 0
+    _set(c, 1, 40, 0.0, head=1)
+    _set(c, 1, L - 1, 0.0, head=1)
+    _set(c, 1, 100, 2.0 ** -110, head=1)  # (values below 2^-101: nothing beside the others)
+    _widen(c, tokens)
+    o = _check_attn(c, _queries(gpu, new, 4, D, torch.bfloat16, 5), [L], [0, new])
+    assert bool((o[:, :2] == 0).all())
