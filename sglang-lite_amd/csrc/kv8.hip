@@ -254,13 +254,15 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
     }
   }
   if (threadIdx.x == 0) *scale = s;
+  // An old scale that this kernel did not write may be no power of two, and the packed
+  // conversions take an exponent alone.
+  const bool uneven = (f32_bits(s) & 0x7FFFFFu) != 0;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     if (tok[it] >= 0) {
       uint8_t* row = codes + (int64_t)(spot + tok[it]) * a.D;
       uint32_t c[4];
-      if (__builtin_expect(odd[it], 0)) {  // an infinity becomes the NaN code, a NaN keeps its sign
-        const float inv = 1.0f / s;        // exact for the powers of two that this kernel writes
+      if (__builtin_expect(odd[it] || uneven, 0)) {  // an infinity becomes the NaN code, a NaN keeps its sign
         float f[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) f[v] = bits_f32(kept[it][v]);
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          c[j] = pk4_e4m3_exact(f[4 * j] * inv, f[4 * j + 1] * inv, f[4 * j + 2] * inv, f[4 * j + 3] * inv);
+          c[j] = pk4_e4m3_exact(f[4 * j] / s, f[4 * j + 1] / s, f[4 * j + 2] / s, f[4 * j + 3] / s);
       } else if (packed) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) c[j] = codes4<DT>(kept[it][2 * j], kept[it][2 * j + 1], s);

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged_kv import _check_attn, _filled, _host, _queries, _widen
+from test_gpu_paged_kv import Cache, _check_attn, _filled, _host, _new, _queries, _widen
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,28 @@ def test_values_whose_scale_is_zero_are_zero(gpu, tokens, new, D):
     _widen(c, tokens)
     o = _check_attn(c, _queries(gpu, new, 4, D, torch.bfloat16, 5), [L], [0, new])
     assert bool((o[:, :2] == 0).all())
+
+
+@pytest.mark.parametrize("dtype,rot", [(torch.bfloat16, 0), (torch.float16, 0), (torch.float32, 0),
+                                       (torch.bfloat16, 32), (torch.float32, 32)])
+@pytest.mark.parametrize("factor", [1.3, 0.7])
+def test_append_beside_a_scale_that_is_no_power_of_two(gpu, dtype, rot, factor):
+    """Tokens that fit under it, tokens that it grows for, a NaN and an infinity among them."""
+    from sglang_lite_amd import rotary as R
+
+    c = Cache(gpu, 2, 64, 2, 64, 16, 16, seed=8)
+    kw = dict(table=R.rotary_table(100, rot, device=gpu)) if rot else {}
+    k, v = _new(gpu, 10, 2, 64, dtype, 1, spread=0.0)
+    c.append(k, v, [0, 0], [0, 5, 10], **kw)
+    for t in (c.kv.k_scale, c.kv.v_scale):
+        t.mul_(factor)
+    c.ks *= np.float32(factor)
+    c.vs *= np.float32(factor)
+    k, v = _new(gpu, 8, 2, 64, dtype, 2, spread=0.0)
+    k, v = k * 0.25, v * 0.25
+    k[2, 0, 50], v[1, 1, 7] = float("nan"), float("inf")
+    c.append(k, v, [5, 5], [0, 3, 8], **kw)
+    c.check()
+    k, v = _new(gpu, 2, 2, 64, dtype, 3, spread=0.0)
+    c.append(k * 9, v * 9, [8, 10], None, **kw)
+    c.check()
