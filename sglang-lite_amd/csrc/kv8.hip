@@ -6,7 +6,8 @@
 // finite ones, and not below the scale that the block had if it holds earlier
 // tokens of the sequence; code = e4m3(x / s), NaN for a NaN or an infinity.
 // Earlier tokens are written again, e4m3(code s_old / s), only where the scale
-// grew: a power of two, so nothing but codes near the smallest are rounded.
+// grew: a power of two, so nothing but codes near the smallest are rounded.  Of an
+// old scale that is negative or not finite they are NaN.
 //
 // Bound by HBM (6 bytes for an element of k and of v: 2 x 2 read, 2 x 1
 // written), and beside it by the conversion (16384 tokens of 8 heads of 128: 28 us at
@@ -233,10 +234,11 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
     for (int i = 0; i < NT / 64; ++i) amax = __builtin_fmaxf(amax, part[i]);
   }
   float s = kv8_scale(amax);
-  if (was >= s) {
+  if (was >= s && was < __builtin_huge_valf()) {
     s = was;
-  } else if (was > 0.0f) {
+  } else if (spot > begin) {
     const float inv = 1.0f / s;  // exact
+    const float old = was >= 0.0f ? was : __builtin_nanf("");  // (an infinity makes NaN codes of itself)
     const int bytes = (spot - begin) * a.D;
     for (int i = 16 * (int)threadIdx.x; i < bytes; i += 16 * NT) {
       uint4* at = reinterpret_cast<uint4*>(codes + (int64_t)begin * a.D + i);
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
         float f[4];
         unpack4_e4m3(q[j], f);
         const uint32_t keep = ((((q[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xFFu;  // NaN codes
-        const uint32_t r = pk4_e4m3(f[0] * was * inv, f[1] * was * inv, f[2] * was * inv, f[3] * was * inv);
+        const uint32_t r = pk4_e4m3(f[0] * old * inv, f[1] * old * inv, f[2] * old * inv, f[3] * old * inv);
         q[j] = (q[j] & keep) | (r & ~keep);
       }
       *at = make_uint4(q[0], q[1], q[2], q[3]);

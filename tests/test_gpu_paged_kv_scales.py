@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged_kv import Cache, _check_attn, _filled, _host, _new, _queries, _widen
+from oracle import quant as Q
+from test_gpu_paged_kv import Cache, _bytes, _check_attn, _filled, _host, _new, _queries, _widen
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +124,25 @@ def test_append_beside_a_scale_that_is_no_power_of_two(gpu, dtype, rot, factor):
     k, v = _new(gpu, 2, 2, 64, dtype, 3, spread=0.0)
     c.append(k * 9, v * 9, [8, 10], None, **kw)
     c.check()
+
+
+@pytest.mark.parametrize("value", [0.0, float("nan"), float("inf"), -1.0])
+def test_append_beside_a_scale_of_zero_or_none(gpu, value):
+    """The earlier tokens' values were zero, or NaN, and stay so when the block gets a scale."""
+    c = Cache(gpu, 1, 32, 2, 64, 16, 16, seed=8)
+    k, v = _new(gpu, 6, 2, 64, torch.bfloat16, 1)
+    c.append(k, v, [0], [0, 6])
+    c.kv.k_scale.fill_(value)
+    c.kv.v_scale.fill_(value)
+    p = int(c.table[0, 0])
+    k, v = _new(gpu, 4, 2, 64, torch.bfloat16, 2)
+    st, cu = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([6], [0, 4]))
+    c.P.append_kv(c.kv, k, v, c.bt, st, cu_tokens=cu)
+    for codes, scale, x in ((c.kv.k, c.kv.k_scale, k), (c.kv.v, c.kv.v_scale, v)):
+        s = _host(scale)[p, :, 0]
+        got = Q.e4m3_to_f32(_bytes(codes)[p]) * s[:, None, None]
+        assert (s > 0).all() and np.isfinite(s).all()
+        assert (got[:, :6] == 0).all() if value == 0 else np.isnan(got[:, :6]).all()
+        want = _host(x).transpose(1, 0, 2)
+        # e4m3: half a step is 2^-4 of a normal value, 2^-10 of the scale below them
+        assert (np.abs(got[:, 6:10] - want) <= np.maximum(2.0 ** -4 * np.abs(want), 2.0 ** -10 * s[:, None, None])).all()
