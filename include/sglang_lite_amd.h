@@ -533,7 +533,7 @@ int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_toke
  * Appends k and v [T, Hkv, D] (sgl_dtype, 16-byte aligned strides): row i of
  * sequence b becomes token start[b] + i.  With a table the keys are rotated
  * first (arguments as for sgl_rotary, 16-byte aligned; positions int32 [T], NULL
- * for the token's own place).  A block's scale is the smallest power of two,
+ * for the token's own place, negative ones leave their key as it is).  A block's scale is the smallest power of two,
  * 2^-100 at least, that brings the largest finite magnitude among its new values
  * down to 448, and not below the scale it had where it holds earlier tokens of
  * the sequence (block start <= p < start[b]); those are rounded again where it

@@ -170,9 +170,9 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
       } else {
         widen8<DT>(raw, x);
         widen8<DT>(raw + RW, x + 8);
-        if (u < rot_units) {
+        const int64_t pos = u >= rot_units ? -1 : a.positions ? a.positions[w.row0 + t] : w.at + t;
+        if (pos >= 0) {
           float cs[8], sn[8];
-          const int64_t pos = a.positions ? a.positions[w.row0 + t] : w.at + t;
           load_turn<8>(a.table, a.n_positions, a.rot >> 1, pos, 8 * u, false, cs, sn);
           if (a.interleaved) {
             float p[8], q[8];

@@ -62,9 +62,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     two = c + VEC < rest;
   }
   float cs[VEC], sn[VEC];
+  bool turn = false;
   if (u < rot_units) {
     const int64_t p = a.pos64 ? ((const int64_t*)a.positions)[t] : ((const int32_t*)a.positions)[t];
-    load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, VEC * u, a.inverse, cs, sn);
+    turn = p >= 0;
+    if (turn) load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, VEC * u, a.inverse, cs, sn);
   }
   auto load = [&](int64_t at, float* f) {
     if constexpr (VEC == 8) {
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     for (int k = 0; k < kHeads; ++k) {
       const int h = h0 + k * a.hsplit;
       if (h < a.H) {
-        if (u < rot_units) {
+        if (turn) {
           if (VEC == 8 && a.interleaved) {
             float p[VEC], q[VEC];
 #pragma unroll

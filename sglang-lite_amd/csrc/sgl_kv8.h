@@ -107,12 +107,13 @@ __device__ __forceinline__ void rotate_pairs(float* a, float* b, const float* co
   }
 }
 
-// cos and sin of N pairs of position p.  Behind the table's last position there
-// is no rotation to give: NaN.  Before the first (the marker of a padding row): none.
+// cos and sin of N pairs of position p >= 0.  Behind the table's last position there
+// is no rotation to give: NaN.  (A negative one marks a padding row, which is not
+// turned at all: by 1 and 0 an infinity would make NaN of its partner.)
 template <int N>
 __device__ __forceinline__ void load_turn(const float* table, int64_t n_positions, int pairs, int64_t p,
                                           int pair, bool inverse, float* cos, float* sin) {
-  const bool in = p >= 0 && p < n_positions;
+  const bool in = p < n_positions;
   const float2* row = reinterpret_cast<const float2*>(table) + (in ? p : 0) * pairs + pair;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -123,8 +124,8 @@ __device__ __forceinline__ void load_turn(const float* table, int64_t n_position
   if (__builtin_expect(!in, 0)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      cos[i] = p < 0 ? 1.0f : __builtin_nanf("");
-      sin[i] = p < 0 ? 0.0f : __builtin_nanf("");
+      cos[i] = __builtin_nanf("");
+      sin[i] = __builtin_nanf("");
     }
   }
 }

@@ -146,3 +146,45 @@ def test_append_beside_a_scale_of_zero_or_none(gpu, value):
         want = _host(x).transpose(1, 0, 2)
         # e4m3: half a step is 2^-4 of a normal value, 2^-10 of the scale below them
         assert (np.abs(got[:, 6:10] - want) <= np.maximum(2.0 ** -4 * np.abs(want), 2.0 ** -10 * s[:, None, None])).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,rot,offset", [(64, 32, 16), (33, 10, 1)])
+def test_rotary_leaves_padding_rows_whatever_they_hold(gpu, dtype, interleaved, D, rot, offset):
+    """Infinities, NaN, zeros of either sign in a row without a position."""
+    from sglang_lite_amd import rotary as R
+
+    table = R.rotary_table(16, rot, scaling={"type": "yarn", "factor": 4.0, "original": 64}, device=gpu)
+    x = torch.randn(6, 3, D, device=gpu).to(dtype)
+    x[1, :, offset] = float("inf")
+    x[1, :, offset + 1] = -0.0
+    x[3, 1, offset:offset + rot] = -0.0
+    x[3, 2, offset + 2] = float("nan")
+    x[4] = float("-inf")
+    for at in (torch.tensor([2, -1, 3, -7, -2 ** 31, 5], device=gpu), torch.tensor([2, -1, 3, -7, -3, 5], device=gpu).int()):
+        for inverse in (False, True):
+            y = R.rotary(x, table, at, interleaved=interleaved, offset=offset, inverse=inverse)
+            for r in (1, 3, 4):
+                nan = torch.isnan(x[r])
+                assert torch.equal(torch.isnan(y[r]), nan)
+                assert torch.equal(y[r][~nan], x[r][~nan])
+                assert torch.equal(torch.signbit(y[r][~nan]), torch.signbit(x[r][~nan]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_leaves_keys_without_a_position(gpu, dtype, interleaved):
+    """As if there were no table: an infinity turns no other element into NaN."""
+    from sglang_lite_amd import rotary as R
+
+    table = R.rotary_table(100, 64, device=gpu)
+    k, v = _new(gpu, 4, 2, 64, dtype, 4)
+    k[1, 0, 3], k[1, 1, 40], k[2, 0, 5] = float("inf"), float("nan"), -0.0
+    at = torch.full((4,), -1, dtype=torch.int32, device=gpu)
+    one, two = (Cache(gpu, 1, 16, 2, 64, 16, 16, seed=6) for _ in range(2))
+    st, cu = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0], [0, 4]))
+    one.P.append_kv(one.kv, k, v, one.bt, st, cu_tokens=cu, table=table, positions=at, interleaved=interleaved)
+    two.P.append_kv(two.kv, k, v, two.bt, st, cu_tokens=cu)
+    for a, b in zip(one.kv, two.kv):
+        np.testing.assert_array_equal(_bytes(a), _bytes(b))
