@@ -24,7 +24,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .rotary import DTYPES, check_table
+from .rotary import DTYPES, check_apart, check_table
 
 FP8 = torch.float8_e4m3fn
 MAX_DIM = 256
@@ -185,7 +185,7 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     are rounded by at most 2^-11 of themselves, or 2^-35 of the row's largest (each
     times its value's scale).  A row that sees no key is zero;
     rows behind the last sequence are not written (of a new tensor: they hold
-    anything)."""
+    anything).  ``out`` may be ``q`` itself, or share no memory with its rows."""
     pages, heads, page, dim, block = _check_cache(cache, "paged_attn")
     shape = q.shape
     if len(shape) != 3 or shape[2] != dim or shape[1] < 1 or shape[1] % heads:
@@ -204,7 +204,8 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
         raise ValueError(f"paged_attn: window ({window}) must not be negative and is for causal attention")
     kc, vc, ks, vs = cache
     d = _lib.device_of("paged_attn", q, block_table, lens, cu_tokens, sink, out, kc, vc, ks, vs)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous():
         raise ValueError(f"paged_attn: out must be a contiguous {q.dtype} {tuple(shape)}, got "
@@ -212,6 +213,8 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     if T == 0 or B == 0:
         return out
     q, sq = _rows16(q, 8)
+    if given and out is not q:
+        check_apart(q, out, "paged_attn")
     nws = _workspace(d, T, B, heads, hq // heads, dim, columns * page)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
     _lib.call_on(d, "sgl_kv8_attn", q.data_ptr(), sq[0], sq[1], dt, T, B, heads, hq // heads, dim,

@@ -102,6 +102,36 @@ def _apart(outer: int, so: int, inner: int, si: int, D: int) -> bool:
     return (inner <= 1 or si >= D) and (outer <= 1 or so >= (inner - 1) * si + D)
 
 
+def check_apart(x: torch.Tensor, out: torch.Tensor, what: str) -> None:
+    """Refuse an ``out`` whose rows (none on another) share memory with ``x`` ``[T, H, D]`` and are
+    not its very rows: one workgroup would overwrite what another is still to read."""
+    n, D = out.shape[:2], out.shape[2]
+    if 0 in out.shape:
+        return
+    a, b, size = x.data_ptr(), out.data_ptr(), out.element_size()
+
+    def end(t):  # bytes from its first element to behind its last
+        return (sum((m - 1) * s for m, s in zip(t.shape, t.stride())) + 1) * size
+
+    if a + end(x) <= b or b + end(out) <= a:
+        return
+    d, rest = divmod(b - a, size)
+    axes = [(s, m, r) for m, s, r in zip(n, out.stride(), x.stride()) if m > 1]
+    if not rest and all(s == r for s, _, r in axes):
+        if d == 0:
+            return
+        # rows (i, j) of x and (i', j') of out meet where d + (i' - i) s0 + (j' - j) s1 is less than D
+        near = [d]
+        axes.sort(reverse=True)
+        for k, (s, m, _) in enumerate(axes):
+            reach = sum((m2 - 1) * s2 for s2, m2, _ in axes[k + 1:]) + D - 1
+            near = [v - i * s for v in near
+                    for i in range(max(1 - m, -((reach - v) // s)), min(m - 1, (v + reach) // s) + 1)]
+        if all(abs(v) >= D for v in near):
+            return
+    raise ValueError(f"{what}: out overlaps the input without being it")
+
+
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
            interleaved: bool = False, offset: int = 0, inverse: bool = False,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -110,7 +140,7 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     by ``positions`` (int32 or int64 ``[T]``): pair ``i`` is elements ``i`` and
     ``i + rot_dim / 2`` of them, or ``2 i`` and ``2 i + 1`` with ``interleaved``.
     A negative position (a padding row) leaves its row as it is, one behind the
-    table gives NaN.  ``out`` may be ``x`` itself."""
+    table gives NaN.  ``out`` may be ``x`` itself, or share no memory with its rows."""
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"rotary: expected x [T, H, D], got {tuple(shape)}")
@@ -129,7 +159,8 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     if xs[2] != 1 and D > 1:
         x = x.contiguous()
         xs = x.stride()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not x.dtype or (out.stride(2) != 1 and D > 1):
         raise ValueError(f"rotary: out must be {x.dtype} {tuple(shape)} with a dense last "
@@ -137,6 +168,8 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     os = out.stride()
     if not (_apart(T, os[0], H, os[1], D) or _apart(H, os[1], T, os[0], D)):
         raise ValueError("rotary: rows of out overlap")
+    if given and out is not x:
+        check_apart(x, out, "rotary")
     if not positions.is_contiguous():
         positions = positions.contiguous()
     _lib.call_on(d, "sgl_rotary", x.data_ptr(), dt, T, H, D, xs[0], xs[1], table.data_ptr(),
