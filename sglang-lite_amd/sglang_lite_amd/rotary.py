@@ -39,7 +39,7 @@ def frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = N
                     (1 + 0.1 ln factor) multiplies the elements."""
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError(f"rot_dim must be even and at least 2, got {rot_dim}")
-    if not base > 1.0:
+    if not 1.0 < base < math.inf:
         raise ValueError(f"base must be greater than 1, got {base}")
     i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
     if scaling is None:
@@ -47,7 +47,7 @@ def frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = N
     kind, factor = scaling.get("type"), float(scaling.get("factor", 0.0))
     if kind not in ("linear", "ntk", "yarn"):
         raise ValueError(f"scaling type must be linear, ntk or yarn, got {kind!r}")
-    if not factor >= 1.0:
+    if not 1.0 <= factor < math.inf:
         raise ValueError(f"scaling factor must be at least 1, got {factor}")
     if kind == "linear":
         return base ** (-i / rot_dim) / factor, 1.0
@@ -55,14 +55,18 @@ def frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[dict] = N
         if rot_dim == 2:
             return base ** (-i / rot_dim), 1.0
         return (base * factor ** (rot_dim / (rot_dim - 2))) ** (-i / rot_dim), 1.0
-    original = float(scaling["original"])
+    original = float(scaling.get("original", 0.0))
+    fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+    if not 1.0 <= original < math.inf or not 0.0 < slow <= fast < math.inf:
+        raise ValueError(f"yarn scaling needs original positions and 0 < beta_slow <= beta_fast, got "
+                         f"{scaling.get('original')}, {slow} and {fast}")
     freq = base ** (-i / rot_dim)
 
     def pair(turns: float) -> float:  # the pair that makes so many turns over `original` positions
         return rot_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    lo = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
-    hi = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+    lo = max(math.floor(pair(fast)), 0)
+    hi = min(math.ceil(pair(slow)), rot_dim - 1)
     ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
     length = scaling.get("length")
     return freq / factor * ramp + freq * (1 - ramp), \
