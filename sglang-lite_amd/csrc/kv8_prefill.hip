@@ -2,7 +2,7 @@
 // chunks).  The mathematics, and the kernel for few rows: kv8_attn.hip.
 //
 // Bound by the matrix cores and, beside them, the softmax's VALU work (8192 queries
-// of 32 heads of 128 on 8 kv heads: 565 us, 0.98 PFLOP/s; MFMA 47 %, VALU 44 % busy).
+// of 32 heads of 128 on 8 kv heads: 560 us, 0.98 PFLOP/s; MFMA 47 %, VALU 45 % busy).
 // Eight wavefronts (heads up to 64 and above 128: four) of 32 rows each share the key
 // tiles of 64 tokens (heads above 128: 32), whose codes are converted once, on the
 // way into LDS (exact in bf16 and f16), and both products are v_mfma_f32_32x32x16:
@@ -15,8 +15,9 @@
 // run in an MFMA's shadow (32 cycles: four of them for nothing, eight for half),
 // those of another wavefront's softmax phase much less.  One barrier a tile.
 // Wavefronts of 64 rows halve the LDS reads, but not the time: 690 us with tiles of 32
-// tokens, 830 with 64, which spill.  Heads of 256, 4096 queries of 16 heads: 209 us;
-// 612 with tiles of 64 tokens and Q in registers, which spill.
+// tokens, 830 with 64, which spill.  Heads of 256, 4096 queries of 16 heads: 214 us
+// (MFMA 28 %, VALU 26 %, LDS 36 %: one wavefront a SIMD waits for itself); 612 with tiles of
+// 64 tokens and Q in registers, which spill.
 #include "sgl_kv8_attn.h"
 
 namespace sgl {

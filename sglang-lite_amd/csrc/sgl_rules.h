@@ -256,7 +256,8 @@ SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {
 }
 
 // ---- attention over the 8-bit cache: rows of a tile, and the workgroups that
-// share the line of key tiles.
+// share the line of key tiles.  The lengths are not known here, only the block table's
+// width; but where a wider one is named, the figures are of tables as wide as the longest sequence.
 struct Kv8AttnPlan {
   int64_t row_tile;  // 16 or 32: kv8_attn.hip; more: kv8_prefill.hip
   int64_t parts;     // workgroups of a kv head's line, a multiple of 8; 0: a workgroup takes a whole item
@@ -289,7 +290,9 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
 // query heads on 8 kv heads of 128, lengths up to that, whole / shared, us: 1
 // sequence 500 11.5 / 16.9, 1000 11.7 / 16.9, 2000 17.4 / 16.8; 16: 500 11.5 / 16.9,
 // 1000 13.1 / 18.4, 2000 20.2 / 20.2, 4000 34.2 / 25.4; 64: 500 14.7 / 26.3, 1000 21.7 /
-// 32.2, 2000 36.3 / 41.4, 4000 65.0 / 60.4.
+// 32.2, 2000 36.3 / 41.4, 4000 65.0 / 60.4.  So a table of 32768 tokens costs short sequences the
+// difference: 1 of 500 12 / 17, 64 of 500 17 / 25, a prompt of 512 (kv8_chunk_whole) 26 / 40; and a window
+// counts for nothing here: 16 x 1 on 20000 with a window of 128 16.6, on 128 keys 12.5.
 SGL_RULE bool kv8_attn_whole(int64_t capacity, int64_t items, int64_t cus) {
   return capacity <= 1024 || (capacity <= 2048 && items >= 2 * cus);
 }
@@ -305,7 +308,9 @@ SGL_RULE int64_t kv8_few_rows(int64_t D) { return D <= 128 ? 96 : 32; }
 // 32 query heads on 8 kv heads of 128, two launches / the chunk's alone, us: 63 x 1 query on
 // 4000 keys + 2000 on 2000 168 / 298, 15 x 1 on 8000 + 512 on 8000 152 / 215, 7 x 1 + 512
 // on 8000 129 / 151; where there are no few rows after all 16 x 128 54 / 52, 8 x 512 198 / 192,
-// 8 x 64 on 4000 87 / 77.
+// 8 x 64 on 4000 87 / 77.  The average decides: 127 x 1 on 2000 + 2048 on 2048 have 67 rows and go
+// to the few rows' kernel together, 267 (the two apart 87 and 71), 255 x 1 + 4096 1620 (172
+// and 157), and 6 x 1 on 100000 + 2048, fewer than 8, to the chunk's, 618 (193 and 71).
 SGL_RULE bool kv8_attn_mixed(int64_t T, int64_t B, int64_t G, int64_t D) {
   return B >= 8 && T * G / B > kv8_few_rows(D) && T > B;
 }

@@ -12,7 +12,7 @@ from test_gpu_paged_kv import Cache, _bytes, _check_attn, _filled, _host, _new, 
 
 pytestmark = pytest.mark.gpu
 
-KERNELS = [(1, 128), (30, 64), (30, 256), (150, 64), (150, 128), (150, 256)]  # queries, head dim
+KERNELS = [(1, 128), (8, 256), (20, 128), (30, 64), (30, 256), (150, 64), (150, 128), (150, 256)]  # queries, head dim
 FEW_AND_CHUNKS = pytest.mark.parametrize("new,D", KERNELS)
 TOKENS = pytest.mark.parametrize("tokens", [0, 16384])
 
