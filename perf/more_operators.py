@@ -500,8 +500,9 @@ def _run_own(s):
         return R.rotary(s["x"], s["table"], s["positions"], axes=s["axes8"],
                         interleaved=c["layout"] == "interleaved")
     if c["kind"] == "norm":
-        return N.residual_norm(s["x"], s["residual"], s["before"], after=s["after"], gate=s["gate"],
+        h, y = N.residual_norm(s["x"], s["residual"], s["before"], after=s["after"], gate=s["gate"],
                                scale=c["scale"], eps=EPS, quant=c["quant"])
+        return (h, *y) if c["quant"] else (h, y)
     cache = P.PagedKV(s["kc"], s["vc"], s["ks"], s["vs"])
     if c["kind"] == "append":
         P.append_kv(cache, s["k"], s["v"], s["pages"], s["have"], cu_tokens=s["cu"], table=s["table"],
