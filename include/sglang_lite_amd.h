@@ -517,6 +517,16 @@ int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_toke
                const void* positions, int positions_int64, int interleaved, int inverse, void* out,
                int64_t out_token_stride, int64_t out_head_stride, sgl_stream_t stream);
 
+/* sgl_rotary with several axes (time, height, width): positions [n_axes, T]
+ * (1 to 4 axes), and pair i turns by its token's position on axis pair_axes[i]
+ * (uint8 [rot_dim / 2], device).  A token with a negative position on any axis is
+ * left as it is; a pair whose axis is n_axes or more gives NaN.  n_positions below 2^31. */
+int sgl_rotary_axes(const void* x, int dtype, int64_t T, int H, int D, int64_t x_token_stride,
+                    int64_t x_head_stride, const float* table, int64_t n_positions, int rot_dim, int offset,
+                    const void* positions, int positions_int64, int n_axes, const uint8_t* pair_axes,
+                    int interleaved, int inverse, void* out, int64_t out_token_stride,
+                    int64_t out_head_stride, sgl_stream_t stream);
+
 /* The 8-bit paged cache: e4m3 codes [n_pages, Hkv, page_size, D] of keys and of
  * values, and fp32 scales [n_pages, Hkv, page_size / block], one for every
  * `block` tokens of a page and head; a stored value is code * scale.  Scales are
@@ -549,6 +559,16 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
                    int64_t n_positions, int rot_dim, int offset, const int32_t* positions, int interleaved,
                    void* k_codes, void* v_codes, float* k_scale, float* v_scale, sgl_stream_t stream);
 
+/* sgl_kv8_append with keys turned by positions of several axes: positions
+ * int32 [n_axes, T] and pair_axes as for sgl_rotary_axes, both and the table given. */
+int sgl_kv8_append_axes(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                        int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B,
+                        int Hkv, int D, const int32_t* cu_tokens, const int32_t* start,
+                        const int32_t* block_table, int64_t row_pages, int page_size, int block,
+                        int64_t n_pages, const float* table, int64_t n_positions, int rot_dim, int offset,
+                        const int32_t* positions, int n_axes, const uint8_t* pair_axes, int interleaved,
+                        void* k_codes, void* v_codes, float* k_scale, float* v_scale, sgl_stream_t stream);
+
 /* Attention of q [T, Hkv * G, D] (bf16 or f16, 16-byte aligned strides; query
  * head h reads kv head h / G) over the cache: lens[b] keys of sequence b, its n
  * queries being the last n of them (query i at position lens[b] - n + i).
@@ -574,6 +594,28 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
 /* Workspace bytes of sgl_kv8_attn on the current device (0: none); max_tokens:
  * row_pages * page_size, what the block table can hold of a sequence. */
 size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens);
+
+/* ------------------------------------------------- between two blocks */
+
+/* One pass over T rows of H (at most 16384) elements, H dense, rows at the
+ * given strides:
+ *   u = x                                      x of `dtype`
+ *   u = u / sqrt(mean u^2 + eps) * after[H]    unless after is NULL
+ *   h = residual + scale * gate * u            gate NULL: 1; [H], or with gate_rows [T, H]
+ *   y = h / sqrt(mean h^2 + eps) * before[H]   unless before is NULL
+ * in fp32; h is rounded to residual_dtype (dtype or SGL_F32), y, of the unrounded h,
+ * to dtype (rows of H).  The weights and the gate have any sgl_dtype.  With quant y is e4m3
+ * [T, H] (8-byte aligned) and scales one for each `group` (32, 64 or 128) elements, fp32 or, with a
+ * power-of-two scale_mode, e8m0 bytes: sgl_act_quant's formulas on the fp32 y.  h
+ * may be residual, x or gate itself at the same stride and type; other overlaps are not allowed.
+ * No counterpart in the reference, whose norms and sums are torch calls
+ * (deepseek_infer/model.py). */
+int sgl_residual_norm(const void* x, int dtype, int64_t T, int64_t H, int64_t x_stride, const void* residual,
+                      int residual_dtype, int64_t residual_stride, const void* after, int after_dtype,
+                      const void* gate, int gate_dtype, int gate_rows, int64_t gate_stride, float scale,
+                      const void* before, int before_dtype, float eps, void* h, int64_t h_stride, void* y,
+                      int quant, void* scales, int group, int scale_mode, int scale_e8m0,
+                      sgl_stream_t stream);
 
 /* ------------------------------------------------- host-side self checks */
 

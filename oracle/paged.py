@@ -137,3 +137,16 @@ def attention(q, k_rows, v_rows, there, first, scale, causal=True, window=0, sin
                 size[i, h] = w @ np.abs(vv) / den
                 reach[i, h] = (np.abs(kk) @ np.abs(q[i, h])).max() * scale
     return o, size, reach
+
+
+def rotate_axes(x, positions, axes, freq, length=1.0, offset=0, interleaved=False, inverse=False):
+    """x [T, H, D] -> float64: pair i turned by its axis' position, positions [A, T], axes [pairs]."""
+    y = np.array(x, dtype=np.float64)
+    a, b = pairs(2 * len(freq), offset, interleaved)
+    angle = np.asarray(positions, np.float64)[np.asarray(axes)].T * np.asarray(freq, np.float64)
+    c, s = (length * np.cos(angle))[:, None], (length * np.sin(angle))[:, None]
+    if inverse:
+        s = -s
+    u, w = y[..., a].copy(), y[..., b].copy()
+    y[..., a], y[..., b] = u * c - w * s, w * c + u * s
+    return y

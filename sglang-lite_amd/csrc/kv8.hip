@@ -28,7 +28,9 @@ struct AppendArgs {
   const int32_t* start;  // [B]
   const int32_t* cu;     // [B + 1] or null: one token each
   const float* table;    // or null: no rotation
-  const int32_t* positions;
+  const int32_t* positions;  // [T], or of several axes [n_axes][T]; null: a token's place
+  const uint8_t* axes;       // the axis of each pair, or null: one position for all
+  int n_axes;
   int64_t n_positions;
   int64_t n_pages;
   int T, B, Hkv, D, row_pages, page_shift, block_shift;
@@ -109,7 +111,7 @@ __device__ __forceinline__ uint32_t codes4(uint32_t ab, uint32_t cd, float s) {
 }
 
 // NT threads, IT units of 16 elements a thread
-template <int DT, int NT, int IT>
+template <int DT, int NT, int IT, bool AXES>
 __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
   constexpr int RW = DT == SGL_F32 ? 2 : 1;  // 16-byte words of 8 elements
   const int head = (int)blockIdx.y >> 1;
@@ -170,10 +172,21 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
       } else {
         widen8<DT>(raw, x);
         widen8<DT>(raw + RW, x + 8);
-        const int64_t pos = u >= rot_units ? -1 : a.positions ? a.positions[w.row0 + t] : w.at + t;
-        if (pos >= 0) {
-          float cs[8], sn[8];
-          load_turn<8>(a.table, a.n_positions, a.rot >> 1, pos, 8 * u, false, cs, sn);
+        float cs[8], sn[8];
+        bool turn = u < rot_units;
+        if constexpr (AXES) {
+          if (turn) {
+            const AxisPositions at =
+                load_axis_positions<false>(a.positions, a.n_axes, a.T, w.row0 + t, (int)a.n_positions);
+            turn = at.turn;
+            if (turn) load_turn_axes<8>(a.table, (int)a.n_positions, a.rot >> 1, at, a.axes, 8 * u, false, cs, sn);
+          }
+        } else {
+          const int64_t pos = !turn ? -1 : a.positions ? a.positions[w.row0 + t] : w.at + t;
+          turn = pos >= 0;
+          if (turn) load_turn<8>(a.table, a.n_positions, a.rot >> 1, pos, 8 * u, false, cs, sn);
+        }
+        if (turn) {
           if (a.interleaved) {
             float p[8], q[8];
 #pragma unroll
@@ -299,34 +312,30 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
 
 // By a unit's 16 elements: a thread each up to 512 (256 threads with two each: 31.3 us
 // against 30.4 for 16384 tokens of 8 heads of 128), the small ones in small workgroups.
-template <int DT>
+template <int DT, bool AXES>
 void launch_append(const AppendArgs& a, int64_t units, int64_t per_unit, hipStream_t st) {
   const dim3 grid((unsigned)units, (unsigned)(2 * a.Hkv));
   if (per_unit <= 64)
-    append_kernel<DT, 64, 1><<<grid, 64, 0, st>>>(a);
+    append_kernel<DT, 64, 1, AXES><<<grid, 64, 0, st>>>(a);
   else if (per_unit <= 256)
-    append_kernel<DT, 256, 1><<<grid, 256, 0, st>>>(a);
+    append_kernel<DT, 256, 1, AXES><<<grid, 256, 0, st>>>(a);
   else if (per_unit <= 512)
-    append_kernel<DT, 512, 1><<<grid, 512, 0, st>>>(a);
+    append_kernel<DT, 512, 1, AXES><<<grid, 512, 0, st>>>(a);
   else if (per_unit <= 1024)
-    append_kernel<DT, 512, 2><<<grid, 512, 0, st>>>(a);
+    append_kernel<DT, 512, 2, AXES><<<grid, 512, 0, st>>>(a);
   else
-    append_kernel<DT, 512, 4><<<grid, 512, 0, st>>>(a);
+    append_kernel<DT, 512, 4, AXES><<<grid, 512, 0, st>>>(a);
 }
 
-}  // namespace
-}  // namespace sgl
-
-extern "C" {
-
-int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
-                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv, int D,
-                   const int32_t* cu_tokens, const int32_t* start, const int32_t* block_table, int64_t row_pages,
-                   int page_size, int block, int64_t n_pages, const float* table, int64_t n_positions, int rot_dim,
-                   int offset, const int32_t* positions, int interleaved, void* k_codes, void* v_codes,
-                   float* k_scale, float* v_scale, sgl_stream_t stream) {
+template <bool AXES>
+int append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+           int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv, int D, const int32_t* cu_tokens,
+           const int32_t* start, const int32_t* block_table, int64_t row_pages, int page_size, int block,
+           int64_t n_pages, const float* table, int64_t n_positions, int rot_dim, int offset,
+           const int32_t* positions, int n_axes, const uint8_t* axes, int interleaved, void* k_codes, void* v_codes,
+           float* k_scale, float* v_scale, sgl_stream_t stream) {
   SGL_REQUIRE(dtype == SGL_BF16 || dtype == SGL_F16 || dtype == SGL_F32, "kv8_append: dtype %d", dtype);
-  const int rc = sgl::kv8_check_cache("kv8_append", Hkv, D, page_size, block, n_pages, row_pages);
+  const int rc = kv8_check_cache("kv8_append", Hkv, D, page_size, block, n_pages, row_pages);
   if (rc != SGL_OK) return rc;
   SGL_REQUIRE(T >= 0 && T <= (1 << 30) && B >= 0 && B <= (1 << 24), "kv8_append: T=%lld B=%lld out of range",
               (long long)T, (long long)B);
@@ -336,17 +345,22 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
     SGL_REQUIRE(rot_dim >= 16 && rot_dim % 16 == 0 && offset >= 0 && offset % 8 == 0 && offset + rot_dim <= D,
                 "kv8_append: rot_dim=%d must be a multiple of 16 and fit at offset %d (a multiple of 8) into D=%d",
                 rot_dim, offset, D);
-    SGL_REQUIRE(n_positions >= 1 && sgl::aligned(table, 16), "kv8_append: bad rotary table");
+    SGL_REQUIRE(n_positions >= 1 && aligned(table, 16), "kv8_append: bad rotary table");
+  }
+  if (AXES) {
+    SGL_REQUIRE(n_axes >= 1 && n_axes <= kMaxAxes, "kv8_append: n_axes=%d must be 1 to %d", n_axes, kMaxAxes);
+    SGL_REQUIRE(n_positions <= 0x7FFFFFFF, "kv8_append: n_positions=%lld out of range", (long long)n_positions);
   }
   if (T == 0 || B == 0) return SGL_OK;
   SGL_REQUIRE(k && v && start && block_table && k_codes && v_codes && k_scale && v_scale,
               "kv8_append: null pointer");
+  SGL_REQUIRE(!AXES || (table && positions && axes), "kv8_append: axes need a table and positions");
   const int size = dtype == SGL_F32 ? 4 : 2;
-  SGL_REQUIRE(sgl::aligned(k, 16) && sgl::aligned(v, 16) && k_token_stride * size % 16 == 0 &&
+  SGL_REQUIRE(aligned(k, 16) && aligned(v, 16) && k_token_stride * size % 16 == 0 &&
                   k_head_stride * size % 16 == 0 && v_token_stride * size % 16 == 0 && v_head_stride * size % 16 == 0,
               "kv8_append: k and v and their strides must be 16-byte aligned");
-  SGL_REQUIRE(sgl::aligned(k_codes, 16) && sgl::aligned(v_codes, 16), "kv8_append: misaligned cache");
-  sgl::AppendArgs a;
+  SGL_REQUIRE(aligned(k_codes, 16) && aligned(v_codes, 16), "kv8_append: misaligned cache");
+  AppendArgs a;
   a.k = k;
   a.v = v;
   a.kt = k_token_stride;
@@ -362,6 +376,8 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
   a.cu = cu_tokens;
   a.table = table;
   a.positions = positions;
+  a.axes = axes;
+  a.n_axes = n_axes;
   a.n_positions = n_positions;
   a.n_pages = n_pages;
   a.T = (int)T;
@@ -375,15 +391,45 @@ int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
   a.rot = table ? rot_dim : 0;
   a.offset = table ? offset : 0;
   a.interleaved = interleaved != 0;
-  const int64_t units = cu_tokens ? sgl::kv8_append_units(T, B, block) : B;
+  const int64_t units = cu_tokens ? kv8_append_units(T, B, block) : B;
   const int64_t per_unit = (cu_tokens ? (int64_t)block : 1) * (D / 16);
   if (dtype == SGL_BF16)
-    sgl::launch_append<SGL_BF16>(a, units, per_unit, (hipStream_t)stream);
+    launch_append<SGL_BF16, AXES>(a, units, per_unit, (hipStream_t)stream);
   else if (dtype == SGL_F16)
-    sgl::launch_append<SGL_F16>(a, units, per_unit, (hipStream_t)stream);
+    launch_append<SGL_F16, AXES>(a, units, per_unit, (hipStream_t)stream);
   else
-    sgl::launch_append<SGL_F32>(a, units, per_unit, (hipStream_t)stream);
-  return sgl::check_launch("kv8_append");
+    launch_append<SGL_F32, AXES>(a, units, per_unit, (hipStream_t)stream);
+  return check_launch("kv8_append");
+}
+
+}  // namespace
+}  // namespace sgl
+
+extern "C" {
+
+int sgl_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv, int D,
+                   const int32_t* cu_tokens, const int32_t* start, const int32_t* block_table, int64_t row_pages,
+                   int page_size, int block, int64_t n_pages, const float* table, int64_t n_positions, int rot_dim,
+                   int offset, const int32_t* positions, int interleaved, void* k_codes, void* v_codes,
+                   float* k_scale, float* v_scale, sgl_stream_t stream) {
+  return sgl::append<false>(k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, T, B, Hkv, D,
+                            cu_tokens, start, block_table, row_pages, page_size, block, n_pages, table, n_positions,
+                            rot_dim, offset, positions, 1, nullptr, interleaved, k_codes, v_codes, k_scale, v_scale,
+                            stream);
+}
+
+int sgl_kv8_append_axes(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                        int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t T, int64_t B, int Hkv, int D,
+                        const int32_t* cu_tokens, const int32_t* start, const int32_t* block_table, int64_t row_pages,
+                        int page_size, int block, int64_t n_pages, const float* table, int64_t n_positions,
+                        int rot_dim, int offset, const int32_t* positions, int n_axes, const uint8_t* pair_axes,
+                        int interleaved, void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                        sgl_stream_t stream) {
+  return sgl::append<true>(k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, T, B, Hkv, D,
+                           cu_tokens, start, block_table, row_pages, page_size, block, n_pages, table, n_positions,
+                           rot_dim, offset, positions, n_axes, pair_axes, interleaved, k_codes, v_codes, k_scale,
+                           v_scale, stream);
 }
 
 }  // extern "C"

@@ -32,7 +32,9 @@ struct RotaryArgs {
   int64_t xt, xh, ot, oh;  // elements between tokens, heads
   const float* table;
   int64_t n_positions;
-  const void* positions;
+  const void* positions;  // [T], or of several axes [n_axes][T]
+  const uint8_t* axes;    // the axis of each pair
+  int n_axes;
   int T, H, D, rot, offset;
   int units;    // a head's units of 2 VEC elements that there is work on
   int hsplit;   // threads that share a unit's heads
@@ -41,7 +43,7 @@ struct RotaryArgs {
 
 constexpr int kHeads = 4;  // heads of a thread in flight
 
-template <int DT, int VEC>
+template <int DT, int VEC, bool AXES>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   const uint32_t per = (uint32_t)(a.units * a.hsplit);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -63,7 +65,13 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   }
   float cs[VEC], sn[VEC];
   bool turn = false;
-  if (u < rot_units) {
+  if (AXES && u < rot_units) {
+    const AxisPositions at = a.pos64 ? load_axis_positions<true>(a.positions, a.n_axes, a.T, t, (int)a.n_positions)
+                                     : load_axis_positions<false>(a.positions, a.n_axes, a.T, t, (int)a.n_positions);
+    turn = at.turn;
+    if (turn)
+      load_turn_axes<VEC>(a.table, (int)a.n_positions, a.rot / 2, at, a.axes, VEC * u, a.inverse, cs, sn);
+  } else if (u < rot_units) {
     const int64_t p = a.pos64 ? ((const int64_t*)a.positions)[t] : ((const int32_t*)a.positions)[t];
     turn = p >= 0;
     if (turn) load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, VEC * u, a.inverse, cs, sn);
@@ -126,14 +134,74 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   }
 }
 
-template <int DT>
+template <int DT, bool AXES>
 void launch_rotary(const RotaryArgs& a, bool vec, hipStream_t st) {
   const int64_t threads = (int64_t)a.T * a.units * a.hsplit;
   const dim3 grid((unsigned)ceil_div(threads, 256));
   if (vec)
-    rotary_kernel<DT, 8><<<grid, 256, 0, st>>>(a);
+    rotary_kernel<DT, 8, AXES><<<grid, 256, 0, st>>>(a);
   else
-    rotary_kernel<DT, 1><<<grid, 256, 0, st>>>(a);
+    rotary_kernel<DT, 1, AXES><<<grid, 256, 0, st>>>(a);
+}
+
+template <bool AXES>
+int rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_token_stride, int64_t x_head_stride,
+           const float* table, int64_t n_positions, int rot_dim, int offset, const void* positions,
+           int positions_int64, int n_axes, const uint8_t* axes, int interleaved, int inverse, void* out,
+           int64_t out_token_stride, int64_t out_head_stride, sgl_stream_t stream) {
+  SGL_REQUIRE(dtype == SGL_BF16 || dtype == SGL_F16 || dtype == SGL_F32, "rotary: dtype %d", dtype);
+  SGL_REQUIRE(T >= 0 && T <= 0x7FFFFFFF && H >= 0 && H <= 65536 && D >= 1 && D <= 65536,
+              "rotary: T=%lld H=%d D=%d out of range", (long long)T, H, D);
+  SGL_REQUIRE(rot_dim >= 2 && rot_dim % 2 == 0 && offset >= 0 && offset + rot_dim <= D,
+              "rotary: rot_dim=%d must be even and fit at offset %d into D=%d", rot_dim, offset, D);
+  SGL_REQUIRE(n_positions >= 1, "rotary: the table has no positions");
+  if (AXES) {
+    SGL_REQUIRE(n_axes >= 1 && n_axes <= kMaxAxes, "rotary: n_axes=%d must be 1 to %d", n_axes, kMaxAxes);
+    SGL_REQUIRE(n_positions <= 0x7FFFFFFF, "rotary: n_positions=%lld out of range", (long long)n_positions);
+  }
+  if (T == 0 || H == 0) return SGL_OK;
+  SGL_REQUIRE(x && table && positions && out && (axes || !AXES), "rotary: null pointer");
+  SGL_REQUIRE(aligned(table, 8), "rotary: table must be 8-byte aligned");
+  const int size = dtype == SGL_F32 ? 4 : 2;
+  SGL_REQUIRE(aligned(x, size) && aligned(out, size), "rotary: misaligned pointer");
+  const bool in_place = x == out;
+  SGL_REQUIRE(!in_place || (x_token_stride == out_token_stride && x_head_stride == out_head_stride),
+              "rotary: in place the strides of x and out must be the same");
+  const bool vec = rot_dim % 16 == 0 && offset % 8 == 0 && D % 8 == 0 && aligned(x, 16) &&
+                   aligned(out, 16) && aligned(table, 16) && x_token_stride * size % 16 == 0 &&
+                   x_head_stride * size % 16 == 0 && out_token_stride * size % 16 == 0 &&
+                   out_head_stride * size % 16 == 0;
+  RotaryArgs a;
+  a.x = x;
+  a.out = out;
+  a.xt = x_token_stride;
+  a.xh = x_head_stride;
+  a.ot = out_token_stride;
+  a.oh = out_head_stride;
+  a.table = table;
+  a.n_positions = n_positions;
+  a.positions = positions;
+  a.axes = axes;
+  a.n_axes = n_axes;
+  a.T = (int)T;
+  a.H = H;
+  a.D = D;
+  a.rot = rot_dim;
+  a.offset = offset;
+  a.pos64 = positions_int64 != 0;
+  a.interleaved = interleaved != 0;
+  a.inverse = inverse != 0;
+  const int width = vec ? 16 : 2;
+  a.units = rot_dim / width + (in_place ? 0 : (D - rot_dim + width - 1) / width);
+  a.hsplit = rotary_head_threads(T, H, a.units, device_cu_count());
+  SGL_REQUIRE((int64_t)a.T * a.units * a.hsplit <= 256ll * 0x7FFFFFFF, "rotary: too large");
+  if (dtype == SGL_BF16)
+    launch_rotary<SGL_BF16, AXES>(a, vec, (hipStream_t)stream);
+  else if (dtype == SGL_F16)
+    launch_rotary<SGL_F16, AXES>(a, vec, (hipStream_t)stream);
+  else
+    launch_rotary<SGL_F32, AXES>(a, vec, (hipStream_t)stream);
+  return check_launch("rotary");
 }
 
 }  // namespace
@@ -161,53 +229,18 @@ int sgl_rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_toke
                const float* table, int64_t n_positions, int rot_dim, int offset, const void* positions,
                int positions_int64, int interleaved, int inverse, void* out, int64_t out_token_stride,
                int64_t out_head_stride, sgl_stream_t stream) {
-  SGL_REQUIRE(dtype == SGL_BF16 || dtype == SGL_F16 || dtype == SGL_F32, "rotary: dtype %d", dtype);
-  SGL_REQUIRE(T >= 0 && T <= 0x7FFFFFFF && H >= 0 && H <= 65536 && D >= 1 && D <= 65536,
-              "rotary: T=%lld H=%d D=%d out of range", (long long)T, H, D);
-  SGL_REQUIRE(rot_dim >= 2 && rot_dim % 2 == 0 && offset >= 0 && offset + rot_dim <= D,
-              "rotary: rot_dim=%d must be even and fit at offset %d into D=%d", rot_dim, offset, D);
-  SGL_REQUIRE(n_positions >= 1, "rotary: the table has no positions");
-  if (T == 0 || H == 0) return SGL_OK;
-  SGL_REQUIRE(x && table && positions && out, "rotary: null pointer");
-  SGL_REQUIRE(sgl::aligned(table, 8), "rotary: table must be 8-byte aligned");
-  const int size = dtype == SGL_F32 ? 4 : 2;
-  SGL_REQUIRE(sgl::aligned(x, size) && sgl::aligned(out, size), "rotary: misaligned pointer");
-  const bool in_place = x == out;
-  SGL_REQUIRE(!in_place || (x_token_stride == out_token_stride && x_head_stride == out_head_stride),
-              "rotary: in place the strides of x and out must be the same");
-  const bool vec = rot_dim % 16 == 0 && offset % 8 == 0 && D % 8 == 0 && sgl::aligned(x, 16) &&
-                   sgl::aligned(out, 16) && sgl::aligned(table, 16) && x_token_stride * size % 16 == 0 &&
-                   x_head_stride * size % 16 == 0 && out_token_stride * size % 16 == 0 &&
-                   out_head_stride * size % 16 == 0;
-  sgl::RotaryArgs a;
-  a.x = x;
-  a.out = out;
-  a.xt = x_token_stride;
-  a.xh = x_head_stride;
-  a.ot = out_token_stride;
-  a.oh = out_head_stride;
-  a.table = table;
-  a.n_positions = n_positions;
-  a.positions = positions;
-  a.T = (int)T;
-  a.H = H;
-  a.D = D;
-  a.rot = rot_dim;
-  a.offset = offset;
-  a.pos64 = positions_int64 != 0;
-  a.interleaved = interleaved != 0;
-  a.inverse = inverse != 0;
-  const int width = vec ? 16 : 2;
-  a.units = rot_dim / width + (in_place ? 0 : (D - rot_dim + width - 1) / width);
-  a.hsplit = sgl::rotary_head_threads(T, H, a.units, sgl::device_cu_count());
-  SGL_REQUIRE((int64_t)a.T * a.units * a.hsplit <= 256ll * 0x7FFFFFFF, "rotary: too large");
-  if (dtype == SGL_BF16)
-    sgl::launch_rotary<SGL_BF16>(a, vec, (hipStream_t)stream);
-  else if (dtype == SGL_F16)
-    sgl::launch_rotary<SGL_F16>(a, vec, (hipStream_t)stream);
-  else
-    sgl::launch_rotary<SGL_F32>(a, vec, (hipStream_t)stream);
-  return sgl::check_launch("rotary");
+  return sgl::rotary<false>(x, dtype, T, H, D, x_token_stride, x_head_stride, table, n_positions, rot_dim, offset,
+                            positions, positions_int64, 1, nullptr, interleaved, inverse, out, out_token_stride,
+                            out_head_stride, stream);
+}
+
+int sgl_rotary_axes(const void* x, int dtype, int64_t T, int H, int D, int64_t x_token_stride, int64_t x_head_stride,
+                    const float* table, int64_t n_positions, int rot_dim, int offset, const void* positions,
+                    int positions_int64, int n_axes, const uint8_t* pair_axes, int interleaved, int inverse, void* out,
+                    int64_t out_token_stride, int64_t out_head_stride, sgl_stream_t stream) {
+  return sgl::rotary<true>(x, dtype, T, H, D, x_token_stride, x_head_stride, table, n_positions, rot_dim, offset,
+                           positions, positions_int64, n_axes, pair_axes, interleaved, inverse, out, out_token_stride,
+                           out_head_stride, stream);
 }
 
 }  // extern "C"

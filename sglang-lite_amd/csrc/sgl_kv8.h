@@ -130,6 +130,49 @@ __device__ __forceinline__ void load_turn(const float* table, int64_t n_position
   }
 }
 
+// A token's positions on up to four axes, and cos and sin of N pairs that turn by one of
+// them each (`axes`: a byte for each pair).  The positions are loaded beside the pairs' axes and
+// chosen in registers, so that the chain to the table is no longer than with one position.
+// Behind the table, and for an axis that there is none of: NaN, as above.  `turn` is false, and
+// nothing is loaded, where any of them is negative.
+constexpr int kMaxAxes = 4;
+struct AxisPositions {
+  int p[kMaxAxes];  // at most n_positions, which is behind the table
+  bool turn;
+};
+template <bool POS64>
+__device__ __forceinline__ AxisPositions load_axis_positions(const void* positions, int n_axes, int64_t T, int64_t t,
+                                                             int n_positions) {
+  AxisPositions o;
+  o.turn = true;
+#pragma unroll
+  for (int a = 0; a < kMaxAxes; ++a) {
+    int64_t p = n_positions;
+    if (a < n_axes) p = POS64 ? ((const int64_t*)positions)[a * T + t] : ((const int32_t*)positions)[a * T + t];
+    o.turn = o.turn && p >= 0;
+    o.p[a] = p < n_positions ? (int)p : n_positions;
+  }
+  return o;
+}
+template <int N>
+__device__ __forceinline__ void load_turn_axes(const float* table, int n_positions, int pairs, const AxisPositions& at,
+                                               const uint8_t* axes, int pair, bool inverse, float* cos, float* sin) {
+  uint8_t axis[N];
+  __builtin_memcpy(axis, axes + pair, N);
+  bool same = true;
+#pragma unroll
+  for (int i = 1; i < N; ++i) same = same && axis[i] == axis[0];
+  auto place = [&](int a) {
+    return a == 0 ? at.p[0] : a == 1 ? at.p[1] : a == 2 ? at.p[2] : a == 3 ? at.p[3] : n_positions;
+  };
+  if (same) {  // sections of whole chunks: consecutive entries of one row, in 16-byte loads
+    load_turn<N>(table, n_positions, pairs, place(axis[0]), pair, inverse, cos, sin);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) load_turn<1>(table, n_positions, pairs, place(axis[i]), pair + i, inverse, cos + i, sin + i);
+}
+
 // Sum over the lanes up to and with this one, by DPP moves: within rows of 16,
 // then each row's last lane to the row behind it, then lane 31 to the upper half.
 __device__ __forceinline__ int wave_incl_scan(int v) {

@@ -248,6 +248,19 @@ SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cu
   return T * units * ((H + 3) / 4) < cus * 1024 ? (int)H : (int)((H + 3) / 4);
 }
 
+// ---- norms between blocks: threads of a row's workgroup, units of 8 elements a
+// thread, and workgroups.
+constexpr int64_t kNormMost = 16384;  // elements of a row: 1024 threads of two units
+struct NormPlan {
+  int64_t threads, units, grid;
+};
+SGL_RULE NormPlan norm_plan(int64_t T, int64_t row_units, int64_t cus) {
+  const int64_t units = row_units <= 256 ? 1 : 2;
+  const int64_t threads = ((row_units + units - 1) / units + 63) / 64 * 64;
+  const int64_t most = cus * (1024 / threads < 1 ? 1 : 1024 / threads);
+  return {threads, units, T < most ? T : most};
+}
+
 // ---- append to the 8-bit cache: the most blocks that T tokens of B sequences
 // touch.  n tokens touch at most (n - 2) / block + 2, and no more than n.
 SGL_RULE int64_t kv8_append_units(int64_t T, int64_t B, int64_t block) {

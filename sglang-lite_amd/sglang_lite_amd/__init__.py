@@ -12,6 +12,7 @@ and, for ordinary attention heads:
 
 * ``rotary``        -- rotary tables and rotations
 * ``paged_kv``      -- 8-bit block-scaled paged KV cache: append, attention
+* ``norms``         -- norms, gate and residual sum between two blocks
 
 All compute runs in hand-written HIP kernels of ``lib/libsglang_lite_amd.so``
 (C ABI: ``include/sglang_lite_amd.h``); torch only provides device memory and

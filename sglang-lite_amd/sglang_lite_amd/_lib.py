@@ -120,6 +120,21 @@ SIGNATURES = {
         [P, I64, I64, P, I64, I64, c_int, I64, I64, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P,
          I64, c_int, c_int, P, c_int, P, P, P, P, P],
     ),
+    "sgl_rotary_axes": (
+        c_int,
+        [P, c_int, I64, c_int, c_int, I64, I64, P, I64, c_int, c_int, P, c_int, c_int, P, c_int, c_int, P,
+         I64, I64, P],
+    ),
+    "sgl_kv8_append_axes": (
+        c_int,
+        [P, I64, I64, P, I64, I64, c_int, I64, I64, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P,
+         I64, c_int, c_int, P, c_int, P, c_int, P, P, P, P, P],
+    ),
+    "sgl_residual_norm": (
+        c_int,
+        [P, c_int, I64, I64, I64, P, c_int, I64, P, c_int, P, c_int, c_int, I64, c_float, P, c_int, c_float,
+         P, I64, P, c_int, P, c_int, c_int, c_int, P],
+    ),
     "sgl_kv8_attn": (
         c_int,
         [P, I64, I64, c_int, I64, I64, c_int, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P, P, P,

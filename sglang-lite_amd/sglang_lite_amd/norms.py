@@ -1,0 +1,156 @@
+"""What stands between two blocks of a layer, on gfx950, in one launch.
+
+``residual_norm(x, residual, before, ...)``: the norm behind the block that made
+``x``, its gate and residual scale, the sum with the residual stream, and the
+norm before the next block, whose result may come as the e4m3 codes and scales
+that ``kernel.fp8_gemm`` reads::
+
+    h, y = residual_norm(x, residual, w)                       # sum and norm
+    h, (codes, s) = residual_norm(x, residual, w, quant=True)  # and act_quant
+    h, y = residual_norm(x, residual, w, after=v, gate=g, scale=0.5)
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .kernel import E8M0, FP8, scale_mode_for
+from .rotary import DTYPES
+
+MAX_DIM = 16384
+
+
+def _weight(w: Optional[torch.Tensor], H: int, name: str) -> Optional[int]:
+    if w is None:
+        return 0
+    dt = DTYPES.get(w.dtype)
+    if dt is None:
+        raise TypeError(f"residual_norm: {name} must be bfloat16, float16 or float32, got {w.dtype}")
+    if w.shape != (H,) or not w.is_contiguous():
+        raise ValueError(f"residual_norm: {name} must be a contiguous [{H}], got {tuple(w.shape)}")
+    return dt
+
+
+def _rows(t: torch.Tensor, H: int) -> torch.Tensor:
+    """``t`` as rows of ``H`` elements, each dense (a copy where its strides do not allow it)."""
+    t = t if t.dim() == 2 else t.reshape(-1, H)
+    return t if t.stride(1) == 1 or H == 1 else t.contiguous()
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torch.Tensor] = None, *,
+                  after: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  scale: float = 1.0, eps: float = 1e-6, inplace: bool = False, quant: bool = False,
+                  block_size: int = 128, scale_fmt: Optional[str] = None,
+                  scale_dtype: torch.dtype = torch.float32):
+    """``(h, y)`` of ``x`` and ``residual`` ``[..., H]``::
+
+        u = rms(x) * after            (without ``after``: u = x)
+        h = residual + scale * gate * u
+        y = rms(h) * before           (without ``before``: y is None)
+
+    with ``rms(v) = v / sqrt(mean(v^2) + eps)``.  ``x`` is bf16, f16 or f32,
+    ``residual`` of the same type or f32, the weights ``[H]`` and the gate
+    (``[H]``, or a shape of x's that broadcasts) any of the three.  ``h`` has residual's type,
+    or is ``residual`` itself with ``inplace``; ``y`` has x's.  Everything is
+    computed in fp32 and each output rounded once (``y`` is of the unrounded ``h``);
+    squares that pass fp32 make zeros and NaN of their row.
+
+    ``quant``: ``y`` is ``(codes, scales)`` as ``act_quant`` gives them of the
+    fp32 ``y``: e4m3 ``[..., H]`` and one scale for ``block_size`` elements, by the
+    formula of ``scale_fmt`` in ``scale_dtype``."""
+    shape = x.shape
+    dt = DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"residual_norm: x must be bfloat16, float16 or float32, got {x.dtype}")
+    if len(shape) < 1 or residual.shape != shape:
+        raise ValueError(f"residual_norm: expected x and residual of one shape [..., H], got {tuple(shape)} and "
+                         f"{tuple(residual.shape)}")
+    H = shape[-1]
+    if not 1 <= H <= MAX_DIM:
+        raise ValueError(f"residual_norm: rows of 1 to {MAX_DIM} elements, got {H}")
+    rdt = DTYPES.get(residual.dtype)
+    if rdt is None or (rdt != dt and rdt != _lib.SGL_F32):
+        raise TypeError(f"residual_norm: residual must be {x.dtype} or float32, got {residual.dtype}")
+    bdt, adt = _weight(before, H, "before"), _weight(after, H, "after")
+    gdt = gs = 0
+    gate_rows = False
+    if gate is not None:
+        gdt = DTYPES.get(gate.dtype)
+        if gdt is None:
+            raise TypeError(f"residual_norm: gate must be bfloat16, float16 or float32, got {gate.dtype}")
+    mode = 0
+    if quant:
+        if before is None:
+            raise ValueError("residual_norm: codes are of the norm before the next block, which is missing")
+        if block_size not in (32, 64, 128) or H % block_size:
+            raise ValueError(f"residual_norm: block_size must be 32, 64 or 128 and divide {H}, got {block_size}")
+        if scale_dtype not in (torch.float32, E8M0):
+            raise TypeError(f"residual_norm: scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
+        mode = scale_mode_for(scale_fmt)
+        if scale_dtype is E8M0 and scale_fmt is None:
+            raise ValueError("residual_norm: float8_e8m0fnu scales need a scale_fmt (powers of two)")
+    d = _lib.device_of("residual_norm", x, residual, before, after, gate)
+    if gate is not None:
+        if gate.shape == (H,):
+            gate = gate if gate.is_contiguous() else gate.contiguous()
+        else:
+            if gate.shape != shape:
+                try:
+                    gate = gate.expand(shape)
+                except RuntimeError as e:
+                    raise ValueError(f"residual_norm: a gate {tuple(gate.shape)} does not broadcast to "
+                                     f"{tuple(shape)}") from e
+            gate_rows = True
+            gate = _rows(gate, H)
+            gs = gate.stride(0)
+    xr = _rows(x, H)
+    T = xr.shape[0]
+    if inplace:
+        try:
+            rr = h = residual.view(-1, H)
+        except RuntimeError as e:
+            raise ValueError("residual_norm: inplace needs a residual whose rows lie at one stride") from e
+        if (H > 1 and rr.stride(1) != 1) or (T > 1 and rr.stride(0) < H):
+            raise ValueError("residual_norm: inplace needs dense rows that do not overlap")
+        _check_apart(xr, rr, "x")
+        if gate_rows:
+            _check_apart(gate, rr, "the gate")
+        out = residual
+    else:
+        rr = _rows(residual, H)
+        out = torch.empty(shape, dtype=residual.dtype, device=x.device)
+        h = out
+    y = scales = None
+    if quant:
+        y = torch.empty(shape, dtype=FP8, device=x.device)
+        scales = torch.empty((*shape[:-1], H // block_size), dtype=scale_dtype, device=x.device)
+    elif before is not None:
+        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if T:
+        _lib.call_on(d, "sgl_residual_norm", xr.data_ptr(), dt, T, H, xr.stride(0), rr.data_ptr(), rdt, rr.stride(0),
+                     _lib.ptr(after), adt, _lib.ptr(gate), gdt, gate_rows, gs, scale, _lib.ptr(before), bdt, eps,
+                     h.data_ptr(), rr.stride(0) if inplace else H, _lib.ptr(y), quant, _lib.ptr(scales), block_size,
+                     mode, quant and scale_dtype is E8M0)
+    return out, (y, scales) if quant else y
+
+
+def _check_apart(x: torch.Tensor, h: torch.Tensor, name: str) -> None:
+    """Refuse an in-place residual that shares memory with ``x`` and is not its very rows."""
+    if x.numel() == 0:
+        return
+    a, b = x.data_ptr(), h.data_ptr()
+
+    def end(t):
+        return ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+
+    if a + end(x) <= b or b + end(h) <= a:
+        return
+    if a == b and x.dtype is h.dtype and x.stride(0) == h.stride(0):
+        return
+    raise ValueError(f"residual_norm: the residual written in place overlaps {name} without being it")
+
+
+__all__ = ["residual_norm"]

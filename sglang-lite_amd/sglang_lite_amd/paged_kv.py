@@ -24,7 +24,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .rotary import DTYPES, check_apart, check_table
+from .rotary import DTYPES, check_apart, check_axes, check_table
 
 FP8 = torch.float8_e4m3fn
 MAX_DIM = 256
@@ -117,13 +117,13 @@ def _workspace(device: int, *sizes: int) -> int:
 def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
               start: torch.Tensor, *, cu_tokens: Optional[torch.Tensor] = None,
               table: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
-              interleaved: bool = False, offset: int = 0) -> None:
+              axes: Optional[torch.Tensor] = None, interleaved: bool = False, offset: int = 0) -> None:
     """Write ``k`` and ``v`` ``[T, Hkv, D]`` (bf16, f16 or f32) into the cache.
 
     Row ``i`` of sequence ``b`` becomes token ``start[b] + i`` (``start`` int32
     ``[B]``: the tokens it has), in page ``block_table[b, token // page]``.  With
     ``table`` the keys are rotated first, as :func:`rotary.rotary` does, by their
-    token's place or by ``positions`` (int32 ``[T]``).
+    token's place or by ``positions`` (int32 ``[T]``; with ``axes`` ``[axes, T]``).
 
     A block of tokens and head has one scale: the smallest power of two that
     brings the largest finite magnitude of its new values down to 448, and not
@@ -151,19 +151,31 @@ def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: tor
         if rot % 16 or offset % 8:
             raise ValueError(f"append_kv: rotated elements must be a multiple of 16 at an offset that is "
                              f"one of 8, got {rot} at {offset}")
-        if positions is not None and (positions.dtype is not torch.int32 or positions.shape != (T,)
-                                      or not positions.is_contiguous()):
+        if axes is not None:
+            if positions is None:
+                raise ValueError("append_kv: axes without positions")
+            n_axes = check_axes(axes, rot, positions, T, "append_kv")
+            if positions.dtype is not torch.int32 or not positions.is_contiguous():
+                raise ValueError(f"append_kv: positions must be contiguous int32, got {positions.dtype}")
+        elif positions is not None and (positions.dtype is not torch.int32 or positions.shape != (T,)
+                                        or not positions.is_contiguous()):
             raise ValueError(f"append_kv: positions must be a contiguous int32 [{T}], got "
                              f"{positions.dtype} {tuple(positions.shape)}")
-    elif positions is not None:
+    elif positions is not None or axes is not None:
         raise ValueError("append_kv: positions without a rotary table")
     kc, vc, ks, vs = cache
-    d = _lib.device_of("append_kv", k, v, block_table, start, cu_tokens, table, positions, kc, vc, ks, vs)
+    d = _lib.device_of("append_kv", k, v, block_table, start, cu_tokens, table, positions, axes, kc, vc, ks, vs)
     if T == 0 or B == 0:
         return
     n = 4 if dt == _lib.SGL_F32 else 8
     k, sk = _rows16(k, n)
     v, sv = _rows16(v, n)
+    if axes is not None:
+        _lib.call_on(d, "sgl_kv8_append_axes", k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], dt, T, B,
+                     heads, dim, _lib.ptr(cu_tokens), start.data_ptr(), block_table.data_ptr(), columns, page,
+                     block, pages, table.data_ptr(), n_positions, rot, offset, positions.data_ptr(), n_axes,
+                     axes.data_ptr(), interleaved, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr())
+        return
     _lib.call_on(d, "sgl_kv8_append", k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], dt, T, B,
                  heads, dim, _lib.ptr(cu_tokens), start.data_ptr(), block_table.data_ptr(), columns,
                  page, block, pages, _lib.ptr(table), n_positions, rot, offset, _lib.ptr(positions),

@@ -5,7 +5,10 @@
   angles in 64 bits; plain, or scaled for long contexts.
 * ``rotary(x, table, positions, ...)`` -- ``x`` ``[T, H, D]`` with the pairs of
   ``rot_dim`` elements of each head turned by their row's position; ``inverse``
-  turns them back, which is also the gradient with respect to ``x``.
+  turns them back, which is also the gradient with respect to ``x``.  With
+  ``axes`` a token has a position on each of several axes (time, height, width)
+  and every pair turns by one of them.
+* ``rotary_axes(sections)`` -- the axis of each pair, made once.
 
 ``paged_kv.append_kv`` takes the same table and turns the keys on their way
 into the cache.
@@ -14,7 +17,7 @@ into the cache.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -101,6 +104,34 @@ def check_table(table: torch.Tensor, offset: int, dim: int, what: str) -> int:
     return rot
 
 
+MAX_AXES = 4
+
+
+def rotary_axes(sections: Sequence[int], *, spread: bool = False, device="cuda") -> torch.Tensor:
+    """uint8 ``[rot_dim / 2]``: the axis that each pair turns by, ``sections[a]`` pairs for axis
+    ``a`` (up to four): one section after the other, or, ``spread``, the axes in turn for as long as
+    they have pairs left (``[2, 3, 1]``: 0 1 2 0 1 1)."""
+    sizes = [int(n) for n in sections]
+    if not 1 <= len(sizes) <= MAX_AXES or min(sizes) < 0 or sum(sizes) < 1:
+        raise ValueError(f"rotary_axes: sections must be one to {MAX_AXES} numbers of pairs, got {sections}")
+    if spread:
+        axis = [a for turn in range(max(sizes)) for a, n in enumerate(sizes) if turn < n]
+    else:
+        axis = [a for a, n in enumerate(sizes) for _ in range(n)]
+    return torch.tensor(axis, dtype=torch.uint8, device=device)
+
+
+def check_axes(axes: torch.Tensor, rot: int, positions: torch.Tensor, T: int, what: str) -> int:
+    """The number of axes of ``positions`` ``[axes, T]`` for pairs that turn by ``axes``."""
+    if axes.dtype is not torch.uint8 or axes.shape != (rot // 2,) or not axes.is_contiguous():
+        raise ValueError(f"{what}: axes must be a contiguous uint8 [{rot // 2}], got {axes.dtype} "
+                         f"{tuple(axes.shape)}")
+    shape = positions.shape
+    if len(shape) != 2 or not 1 <= shape[0] <= MAX_AXES or shape[1] != T:
+        raise ValueError(f"{what}: with axes, expected positions [1 to {MAX_AXES} axes, {T}], got {tuple(shape)}")
+    return shape[0]
+
+
 def _apart(outer: int, so: int, inner: int, si: int, D: int) -> bool:
     """Whether ``outer`` groups of ``inner`` rows of ``D`` elements, at these strides, lie apart."""
     return (inner <= 1 or si >= D) and (outer <= 1 or so >= (inner - 1) * si + D)
@@ -137,14 +168,16 @@ def check_apart(x: torch.Tensor, out: torch.Tensor, what: str) -> None:
 
 
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
-           interleaved: bool = False, offset: int = 0, inverse: bool = False,
-           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+           axes: Optional[torch.Tensor] = None, interleaved: bool = False, offset: int = 0,
+           inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` ``[T, H, D]`` (bf16, f16 or f32; any strides with a dense last
     dimension) with elements ``[offset, offset + rot_dim)`` of every head turned
     by ``positions`` (int32 or int64 ``[T]``): pair ``i`` is elements ``i`` and
     ``i + rot_dim / 2`` of them, or ``2 i`` and ``2 i + 1`` with ``interleaved``.
     A negative position (a padding row) leaves its row as it is, one behind the
-    table gives NaN.  ``out`` may be ``x`` itself, or share no memory with its rows."""
+    table gives NaN.  With ``axes`` (:func:`rotary_axes`) positions are ``[axes, T]`` and pair ``i``
+    turns by its token's position on axis ``axes[i]``; a token with a negative position on any axis
+    is left as it is, and a pair of an axis that there is none of gives NaN.  ``out`` may be ``x`` itself, or share no memory with its rows."""
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"rotary: expected x [T, H, D], got {tuple(shape)}")
@@ -153,12 +186,15 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
     if dt is None:
         raise TypeError(f"rotary: x must be bfloat16, float16 or float32, got {x.dtype}")
     rot = check_table(table, offset, D, "rotary")
-    if positions.shape != (T,):
+    n_axes = 1
+    if axes is not None:
+        n_axes = check_axes(axes, rot, positions, T, "rotary")
+    elif positions.shape != (T,):
         raise ValueError(f"rotary: expected positions [{T}], got {tuple(positions.shape)}")
     wide = positions.dtype is torch.int64
     if not wide and positions.dtype is not torch.int32:
         raise TypeError(f"rotary: positions must be int32 or int64, got {positions.dtype}")
-    d = _lib.device_of("rotary", x, table, positions, out)
+    d = _lib.device_of("rotary", x, table, positions, axes, out)
     xs = x.stride()
     if xs[2] != 1 and D > 1:
         x = x.contiguous()
@@ -176,10 +212,15 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
         check_apart(x, out, "rotary")
     if not positions.is_contiguous():
         positions = positions.contiguous()
+    if axes is not None:
+        _lib.call_on(d, "sgl_rotary_axes", x.data_ptr(), dt, T, H, D, xs[0], xs[1], table.data_ptr(),
+                     table.shape[0], rot, offset, positions.data_ptr(), wide, n_axes, axes.data_ptr(),
+                     interleaved, inverse, out.data_ptr(), os[0], os[1])
+        return out
     _lib.call_on(d, "sgl_rotary", x.data_ptr(), dt, T, H, D, xs[0], xs[1], table.data_ptr(),
                  table.shape[0], rot, offset, positions.data_ptr(), wide, interleaved, inverse,
                  out.data_ptr(), os[0], os[1])
     return out
 
 
-__all__ = ["frequencies", "rotary", "rotary_table"]
+__all__ = ["frequencies", "rotary", "rotary_axes", "rotary_table"]
