@@ -591,6 +591,41 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
                  float softmax_scale, int causal, int64_t window, const float* sink, void* out,
                  void* workspace, size_t workspace_bytes, sgl_stream_t stream);
 
+/* sgl_kv8_attn with a window (above 0 unless `first` is 0) beside which every query
+ * sees the sequence's first `first` tokens, up to its own position: key j of query
+ * position p where j <= p and (p - j < window or j < first). */
+int sgl_kv8_attn_first(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T,
+                       int64_t B, int Hkv, int G, int D, const int32_t* cu_tokens, const int32_t* lens,
+                       const int32_t* block_table, int64_t row_pages, int page_size, int block,
+                       int64_t n_pages, const void* k_codes, const void* v_codes, const float* k_scale,
+                       const float* v_scale, float softmax_scale, int causal, int64_t window, int64_t first,
+                       const float* sink, void* out, void* workspace, size_t workspace_bytes,
+                       sgl_stream_t stream);
+
+/* Workspace bytes of sgl_kv8_attn_first. */
+size_t sgl_kv8_attn_first_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens,
+                                         int64_t window, int64_t first);
+
+/* sgl_kv8_attn without a window, for sequences that begin alike: those of group g
+ * are [cu_groups[g], cu_groups[g + 1]) (int32 [n_groups + 1], device, never falling;
+ * sequences outside of all groups are allowed), and the full pages among the first shared[g]
+ * tokens (int32 [n_groups], device) are the same in each of their block table rows.  Those
+ * keys are read once for all queries of the group; the result is that of sgl_kv8_attn but for the
+ * order of its sums.  What is taken together is cut to whole pages, whole 128 tokens and to the
+ * tokens before each sequence's first query; the pages are those of the group's first row.
+ * Its workspace has sgl_kv8_attn_shared_workspace_size bytes. */
+int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T,
+                        int64_t B, int Hkv, int G, int D, const int32_t* cu_tokens, const int32_t* lens,
+                        const int32_t* block_table, int64_t row_pages, int page_size, int block,
+                        int64_t n_pages, const void* k_codes, const void* v_codes, const float* k_scale,
+                        const float* v_scale, float softmax_scale, int causal, const float* sink,
+                        int64_t n_groups, const int32_t* cu_groups, const int32_t* shared, void* out,
+                        void* workspace, size_t workspace_bytes, sgl_stream_t stream);
+
+/* Workspace bytes of sgl_kv8_attn_shared. */
+size_t sgl_kv8_attn_shared_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens,
+                                          int64_t n_groups);
+
 /* Workspace bytes of sgl_kv8_attn on the current device (0: none); max_tokens:
  * row_pages * page_size, what the block table can hold of a sequence. */
 size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens);

@@ -107,8 +107,9 @@ def rows(codes, scales, table_row, n):
     return out, there
 
 
-def attention(q, k_rows, v_rows, there, first, scale, causal=True, window=0, sink=None):
-    """One sequence: q [n, Hq, D] at positions first, first + 1, ...; k_rows, v_rows [L, Hkv, D].
+def attention(q, k_rows, v_rows, there, first, scale, causal=True, window=0, sink=None, kept=0):
+    """One sequence: q [n, Hq, D] at positions first, first + 1, ...; k_rows, v_rows [L, Hkv, D];
+    the window does not hide the sequence's `kept` first tokens.
     Returns o [n, Hq, D] float64 and, per element, sum_j w_j |v_j| and the largest
     sum_i |q_i k_i| scale among the keys seen (what rounding errors go by)."""
     n, Hq, D = q.shape
@@ -122,7 +123,7 @@ def attention(q, k_rows, v_rows, there, first, scale, causal=True, window=0, sin
         if causal:
             seen &= key <= p
             if window:
-                seen &= key > p - window
+                seen &= (key > p - window) | (key < kept)
         if not seen.any():
             continue
         for h in range(Hq):

@@ -86,7 +86,8 @@ struct Codes {
 
 // DP: head dim rounded up to 64, 128 or 256; NC: 16-row column tiles
 // SPLIT: workgroups share the lines, else a workgroup takes a whole item
-template <int DP, int NC, int QT, bool SPLIT>
+// FIRST: the sequence's first tokens are seen beside the window
+template <int DP, int NC, int QT, bool SPLIT, bool FIRST>
 __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
   constexpr int RT = 16 * NC, KI = DP / 64, C = DP / 16, W = C / 4;
   __shared__ __align__(16) float sAcc[kWaves][16][DP + 4];
@@ -151,12 +152,11 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       for (int j = 0; j < C; ++j) acc[c][j] = v4f{0, 0, 0, 0};
     }
 
-    const int32_t* table = a.pages + (int64_t)b * a.row_pages;
+    const int32_t* table = a.pages + (int64_t)(a.table_row ? a.table_row[b] : b) * a.row_pages;
     const int pmask = (1 << a.page_shift) - 1;
-    const int first = (s.tile0 + t0) * kTile + 32 * wave;
-    int stop = (s.tile0 + t1) * kTile;
-    stop = stop < s.len ? stop : s.len;
-    const int steps = first < stop ? (stop - first + kTile - 1) / kTile : 0;  // step i: tokens first + i kTile on
+    // the wavefront's first token in step i; only the last tile's may lie behind the end
+    auto token = [&](int i) __attribute__((always_inline)) { return s.template tile<FIRST>(t0 + i) * kTile + 32 * wave; };
+    const int steps = t1 - t0 - (token(t1 - t0 - 1) < s.len ? 0 : 1);
 
     // Pages and scales of 32 steps at a time: lane l has granule l & 1 of step l >> 1.
     // Loaded a batch ahead, so that no step waits for its table entry.
@@ -167,14 +167,14 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
     };
     auto load_pages = [&](int batch) __attribute__((always_inline)) {
       Batch o;
-      const int t = first + (32 * batch + (lane >> 1)) * kTile + 16 * (lane & 1);
+      const int t = token(32 * batch + (lane >> 1)) + 16 * (lane & 1);
       const int page = table[(t < s.len ? t : s.len - 1) >> a.page_shift];
       o.ok = t < s.len && page >= 0 && page < a.n_pages;
       o.page = o.ok ? page : 0;
       return o;
     };
     auto load_scales = [&](int batch, Batch& o) __attribute__((always_inline)) {
-      const int t = first + (32 * batch + (lane >> 1)) * kTile + 16 * (lane & 1);
+      const int t = token(32 * batch + (lane >> 1)) + 16 * (lane & 1);
       const int64_t piece = (((int64_t)o.page * a.Hkv + head) << (a.page_shift - a.block_shift)) +
                             ((t & pmask) >> a.block_shift);
       o.ks = a.ks[piece];
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int page = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + u);
-        const int spot = (first + i * kTile + 16 * u) & pmask;
+        const int spot = (token(i) + 16 * u) & pmask;
         const int64_t row = ((((int64_t)page * a.Hkv + head) << a.page_shift) + spot) * a.D;
         const uint8_t* kp = a.kc + row;
         const uint8_t* vp = a.vc + row;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
     auto lane_f = [&](float v, int l) { return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), l)); };
 
     auto step = [&](int at, Codes<DP>& r) __attribute__((always_inline)) {
-      const int tok = first + at * kTile, l0 = 2 * (at & 31);
+      const int tok = token(at), l0 = 2 * (at & 31);
       const uint32_t ok = (uint32_t)(okm >> l0) & 3u;
       v4f sc[NC][2];
 #pragma unroll
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
           }
         }
       }
-      const bool plain = tok + 32 <= all_hi && tok >= all_lo && ok == 3;
+      const bool plain = tok + 32 <= all_hi && (tok >= all_lo || (FIRST && tok + 32 <= a.first)) && ok == 3;
       const uint32_t here = plain ? 3u : (uint32_t)(__ballot(evs != kNoToken) >> l0) & 3u;
       uint32_t seen[NC];  // bit 4 u + i: the row sees token 16 u + 4 g + i
 #pragma unroll
@@ -274,7 +274,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = tok + 16 * (i >> 2) + 4 * g + (i & 3);
-            if (key < hi[c] && key >= lo[c] && key < s.len && ((here >> (i >> 2)) & 1u)) seen[c] |= 1u << i;
+            const bool in = FIRST ? (uint32_t)(key - a.first) >= (uint32_t)(lo[c] > a.first ? lo[c] - a.first : 0) : key >= lo[c];
+            if (key < hi[c] && in && key < s.len && ((here >> (i >> 2)) & 1u)) seen[c] |= 1u << i;
           }
         }
       }
@@ -437,13 +438,21 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         }
         if (whole) {
           const int row = rt * RT + r, t = row / a.G, h = head * a.G + (row - t * a.G);
-          if (a.sink) sum += __builtin_amdgcn_exp2f(a.sink[h] * kLog2e - ref);
-          const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-          for (int v = 0; v < 8; ++v) y[v] *= inv;
-          *reinterpret_cast<uint4*>(a.o + ((int64_t)(s.row0 + t) * (a.Hkv * a.G) + h) * a.D + d) =
-              make_uint4(kv8_out2<QT>(y[0], y[1]), kv8_out2<QT>(y[2], y[3]), kv8_out2<QT>(y[4], y[5]),
-                         kv8_out2<QT>(y[6], y[7]));
+          const int64_t at = (int64_t)(s.row0 + t) * (a.Hkv * a.G) + h;
+          float4 y0 = make_float4(y[0], y[1], y[2], y[3]), y1 = make_float4(y[4], y[5], y[6], y[7]);
+          if (a.raw) {
+            float4* out = reinterpret_cast<float4*>(a.prior_acc + at * a.D + d);
+            out[0] = y0;
+            out[1] = y1;
+            if (d == 0) *reinterpret_cast<float2*>(a.prior_ml + 2 * at) = make_float2(M, sum);
+          } else {
+            const Kv8Join join = kv8_join(a, s, at, h, M, sum);
+            y0 = kv8_joined(a, join, at, d, y0);
+            y1 = kv8_joined(a, join, at, d + 4, y1);
+            *reinterpret_cast<uint4*>(a.o + at * a.D + d) =
+                make_uint4(kv8_out2<QT>(y0.x, y0.y), kv8_out2<QT>(y0.z, y0.w), kv8_out2<QT>(y1.x, y1.y),
+                           kv8_out2<QT>(y1.z, y1.w));
+          }
         } else {
           float4* out = reinterpret_cast<float4*>(a.ws_acc + (slot * RT + r) * a.D + d);
           out[0] = make_float4(y[0], y[1], y[2], y[3]);
@@ -455,14 +464,22 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
   }
 }
 
-template <int DP, int NC, int QT>
-void launch_few(const Kv8AttnArgs& a, int64_t items, hipStream_t st) {
+template <int DP, int NC, int QT, bool FIRST>
+void launch_few_as(const Kv8AttnArgs& a, int64_t items, hipStream_t st) {
   if (a.parts == 0) {
-    kv8_attn_few_kernel<DP, NC, QT, false><<<(unsigned)items, 64 * kWaves, 0, st>>>(a);
+    kv8_attn_few_kernel<DP, NC, QT, false, FIRST><<<(unsigned)items, 64 * kWaves, 0, st>>>(a);
     return;
   }
-  kv8_attn_few_kernel<DP, NC, QT, true><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
+  kv8_attn_few_kernel<DP, NC, QT, true, FIRST><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
   kv8_merge_kernel<16 * NC, kTile, QT><<<(unsigned)(items * 4 * NC), 256, 0, st>>>(a);
+}
+
+template <int DP, int NC, int QT>
+void launch_few(const Kv8AttnArgs& a, int64_t items, hipStream_t st) {
+  if (a.first > 0)
+    launch_few_as<DP, NC, QT, true>(a, items, st);
+  else
+    launch_few_as<DP, NC, QT, false>(a, items, st);
 }
 
 template <int QT>
@@ -481,20 +498,210 @@ void launch_attn(Kv8AttnArgs a, const Kv8AttnPlan& p, hipStream_t st) {
     launch_few<256, 1, QT>(a, p.items, st);
 }
 
+struct AttnPlans {
+  Kv8AttnPlan p[2];  // one launch, or (chunks and few rows in one batch) two, one after the other on the same workspace
+};
+AttnPlans attn_plans(int64_t T, int64_t B, int Hkv, int G, int D, int64_t tokens) {
+  const int cus = device_cu_count();
+  return {{kv8_attn_plan(T, B, Hkv, G, D, tokens, cus), kv8_attn_rest(T, B, Hkv, G, D, tokens, cus)}};
+}
+size_t attn_workspace(const AttnPlans& plans, int Hkv, int D) {
+  const size_t x = kv8_attn_workspace(plans.p[0], Hkv, D), y = kv8_attn_workspace(plans.p[1], Hkv, D);
+  return x > y ? x : y;
+}
+bool attn_sizes_ok(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens) {
+  return T >= 0 && B >= 0 && Hkv >= 1 && G >= 1 && D >= 16 && max_tokens >= 0;
+}
+
+// Checks a call's arguments and lays them out; `nothing`: there is no row to write.
+struct AttnCall {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  int dtype;
+  int64_t T, B;
+  int Hkv, G, D;
+  const int32_t *cu_tokens, *lens, *block_table;
+  int64_t row_pages;
+  int page_size, block;
+  int64_t n_pages;
+  const void *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  float softmax_scale;
+  int causal;
+  int64_t window;
+  const float* sink;
+  void* out;
+  void* workspace;
+};
+int attn_args(const AttnCall& c, Kv8AttnArgs& a, bool& nothing) {
+  const int64_t T = c.T, B = c.B;
+  SGL_REQUIRE(c.dtype == SGL_BF16 || c.dtype == SGL_F16, "kv8_attn: dtype %d (bf16 or f16)", c.dtype);
+  const int rc = kv8_check_cache("kv8_attn", c.Hkv, c.D, c.page_size, c.block, c.n_pages, c.row_pages);
+  if (rc != SGL_OK) return rc;
+  SGL_REQUIRE(c.G >= 1 && (int64_t)c.G * c.Hkv <= 65536, "kv8_attn: G=%d query heads for each of %d kv heads", c.G, c.Hkv);
+  SGL_REQUIRE(T >= 0 && B >= 0 && B <= (1 << 24) && T * c.G < (1ll << 31), "kv8_attn: T=%lld B=%lld out of range",
+              (long long)T, (long long)B);
+  SGL_REQUIRE(c.cu_tokens || T == B, "kv8_attn: without cu_tokens every sequence has one token (T=%lld, B=%lld)",
+              (long long)T, (long long)B);
+  SGL_REQUIRE(c.window >= 0 && (c.causal || c.window == 0), "kv8_attn: a window (%lld) is for causal attention",
+              (long long)c.window);
+  SGL_REQUIRE(c.softmax_scale > 0.0f && c.softmax_scale < 1e30f, "kv8_attn: softmax_scale must be positive");
+  nothing = T == 0 || B == 0;
+  if (nothing) return SGL_OK;
+  SGL_REQUIRE(c.q && c.lens && c.block_table && c.k_codes && c.v_codes && c.k_scale && c.v_scale && c.out,
+              "kv8_attn: null pointer");
+  SGL_REQUIRE(aligned(c.q, 16) && c.q_token_stride % 8 == 0 && c.q_head_stride % 8 == 0,
+              "kv8_attn: q and its strides must be 16-byte aligned");
+  SGL_REQUIRE(aligned(c.k_codes, 16) && aligned(c.v_codes, 16) && aligned(c.out, 16),
+              "kv8_attn: misaligned cache or output");
+  const int64_t tokens = c.row_pages * c.page_size;
+  a = Kv8AttnArgs{};
+  a.q = (const uint16_t*)c.q;
+  a.qt = c.q_token_stride;
+  a.qh = c.q_head_stride;
+  a.o = (uint16_t*)c.out;
+  a.kc = (const uint8_t*)c.k_codes;
+  a.vc = (const uint8_t*)c.v_codes;
+  a.ks = c.k_scale;
+  a.vs = c.v_scale;
+  a.pages = c.block_table;
+  a.lens = c.lens;
+  a.cu = c.cu_tokens;
+  a.sink = c.sink;
+  a.n_pages = c.n_pages;
+  a.T = (int)T;
+  a.B = (int)B;
+  a.Hkv = c.Hkv;
+  a.G = c.G;
+  a.D = c.D;
+  a.row_pages = (int)c.row_pages;
+  a.page_shift = __builtin_ctz((unsigned)c.page_size);
+  a.block_shift = __builtin_ctz((unsigned)c.block);
+  a.c1 = c.softmax_scale * kLog2e;
+  a.window = c.window >= tokens ? 0 : (int)c.window;  // (as long as the table: all keys)
+  a.causal = c.causal != 0;
+  a.ws_acc = (float*)c.workspace;
+  return SGL_OK;
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need)) {
+    set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? bytes : 0, need);
+    return SGL_ERR_WORKSPACE;
+  }
+  SGL_REQUIRE(aligned(workspace, 16), "kv8_attn: workspace must be 16-byte aligned");
+  return SGL_OK;
+}
+int check_plans(const AttnPlans& plans, int64_t tokens) {
+  for (const Kv8AttnPlan& p : plans.p)
+    SGL_REQUIRE_SUPPORTED(p.items * ((tokens + 31) / 32 + kItemCost) < (1ll << 31) &&
+                              p.items * p.row_tile / 4 < (1ll << 31),
+                          "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)p.items,
+                          (long long)tokens);
+  return SGL_OK;
+}
+void launch_plans(const Kv8AttnArgs& a, int dtype, const AttnPlans& plans, hipStream_t st) {
+  for (const Kv8AttnPlan& p : plans.p) {
+    if (p.items == 0) continue;
+    if (dtype == SGL_BF16)
+      launch_attn<SGL_BF16>(a, p, st);
+    else
+      launch_attn<SGL_F16>(a, p, st);
+  }
+}
+
+// ---- a common prefix.  A group's queries all see the keys [0, covered), so that pass takes
+// the group as one sequence, whose rows meet the keys' tiles together; the second pass
+// takes every sequence from there on.  `covered` is what the caller says, cut to whole
+// pages and key tiles (of every kernel: 128 tokens), and to what lies before the first query of
+// each sequence of the group that has any; 0 for a group of fewer than two such.
+constexpr int kPrefixTile = 128;
+struct PrefixPlan {
+  int32_t *cu, *lens, *row;  // of the groups: first token rows [n + 1], covered tokens, a row of the block table
+  int32_t* skip;             // of the sequences: covered tokens
+};
+// Workgroup g takes group g; the last one the sequences of no group.
+__global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, const int32_t* cu_groups,
+                                                         const int32_t* shared, int n, PrefixPlan o) {
+  const int g = (int)blockIdx.x;
+  auto edge = [&](int i) {
+    const int b = cu_groups[i];
+    return b < 0 ? 0 : b > a.B ? a.B : b;
+  };
+  auto row_of = [&](int b) {  // the first token row of sequence b, or of what lies behind the last
+    if (b < a.B) return seq_rows(a.cu, b, a.T).first;
+    const SeqRows last = seq_rows(a.cu, a.B - 1, a.T);
+    return last.first + last.n;
+  };
+  if (g == n) {
+    const int lo = edge(0), hi = edge(n);
+    for (int b = (int)threadIdx.x; b < a.B; b += 256)
+      if (b < lo || b >= hi) o.skip[b] = 0;
+    if (threadIdx.x == 0) o.cu[n] = row_of(hi);
+    return;
+  }
+  const int b0 = edge(g), b1 = edge(g + 1), cap = a.row_pages << a.page_shift;
+  int most = shared[g], with = 0;
+  for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) {
+    const SeqRows r = seq_rows(a.cu, b, a.T);
+    if (r.n == 0) continue;
+    const int len = a.lens[b] < cap ? a.lens[b] : cap;
+    most = len - r.n < most ? len - r.n : most;
+    ++with;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const int other = __shfl_xor(most, d, 64);
+    most = other < most ? other : most;
+    with += __shfl_xor(with, d, 64);
+  }
+  __shared__ int part[4][2];
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6][0] = most;
+    part[threadIdx.x >> 6][1] = with;
+  }
+  __syncthreads();
+  with = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    most = part[i][0] < most ? part[i][0] : most;
+    with += part[i][1];
+  }
+  const int unit = kPrefixTile > (1 << a.page_shift) ? kPrefixTile : 1 << a.page_shift;
+  const int covered = with < 2 || most < unit ? 0 : most & ~(unit - 1);
+  for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) o.skip[b] = covered;
+  if (threadIdx.x == 0) {
+    o.cu[g] = row_of(b0);
+    o.lens[g] = covered;
+    o.row[g] = b0 < a.B ? b0 : 0;
+  }
+}
+
+// The workspace: the plan's numbers, the first pass' sums, then what either pass needs for itself.
+struct PrefixSpace {
+  size_t plan, acc, ml, rest, total;
+};
+PrefixSpace prefix_space(int64_t T, int64_t B, int Hkv, int G, int D, int64_t tokens, int64_t n) {
+  auto round = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t first = attn_workspace(attn_plans(T, n, Hkv, G, D, tokens), Hkv, D);
+  const size_t second = attn_workspace(attn_plans(T, B, Hkv, G, D, tokens), Hkv, D);
+  PrefixSpace s;
+  s.plan = 0;
+  s.acc = round((size_t)(3 * n + 1 + B) * 4);
+  s.ml = s.acc + round((size_t)T * Hkv * G * D * 4);
+  s.rest = s.ml + round((size_t)T * Hkv * G * 8);
+  s.total = s.rest + (first > second ? first : second);
+  return s;
+}
+
 }  // namespace
 }  // namespace sgl
 
 extern "C" {
 
 size_t sgl_kv8_attn_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens) {
-  if (T < 0 || B < 0 || Hkv < 1 || G < 1 || D < 16 || max_tokens < 0) return 0;
-  size_t bytes = 0;
-  for (const sgl::Kv8AttnPlan& p : {sgl::kv8_attn_plan(T, B, Hkv, G, D, max_tokens, sgl::device_cu_count()),
-                                    sgl::kv8_attn_rest(T, B, Hkv, G, D, max_tokens, sgl::device_cu_count())}) {
-    const size_t b = sgl::kv8_attn_workspace(p, Hkv, D);
-    bytes = b > bytes ? b : bytes;
-  }
-  return bytes;
+  if (!sgl::attn_sizes_ok(T, B, Hkv, G, D, max_tokens)) return 0;
+  return sgl::attn_workspace(sgl::attn_plans(T, B, Hkv, G, D, max_tokens), Hkv, D);
 }
 
 int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T, int64_t B,
@@ -503,72 +710,94 @@ int sgl_kv8_attn(const void* q, int64_t q_token_stride, int64_t q_head_stride, i
                  const void* v_codes, const float* k_scale, const float* v_scale, float softmax_scale, int causal,
                  int64_t window, const float* sink, void* out, void* workspace, size_t workspace_bytes,
                  sgl_stream_t stream) {
-  SGL_REQUIRE(dtype == SGL_BF16 || dtype == SGL_F16, "kv8_attn: dtype %d (bf16 or f16)", dtype);
-  const int rc = sgl::kv8_check_cache("kv8_attn", Hkv, D, page_size, block, n_pages, row_pages);
-  if (rc != SGL_OK) return rc;
-  SGL_REQUIRE(G >= 1 && (int64_t)G * Hkv <= 65536, "kv8_attn: G=%d query heads for each of %d kv heads", G, Hkv);
-  SGL_REQUIRE(T >= 0 && B >= 0 && B <= (1 << 24) && T * G < (1ll << 31), "kv8_attn: T=%lld B=%lld out of range",
-              (long long)T, (long long)B);
-  SGL_REQUIRE(cu_tokens || T == B, "kv8_attn: without cu_tokens every sequence has one token (T=%lld, B=%lld)",
-              (long long)T, (long long)B);
-  SGL_REQUIRE(window >= 0 && (causal || window == 0), "kv8_attn: a window (%lld) is for causal attention",
-              (long long)window);
-  SGL_REQUIRE(softmax_scale > 0.0f && softmax_scale < 1e30f, "kv8_attn: softmax_scale must be positive");
-  if (T == 0 || B == 0) return SGL_OK;
-  SGL_REQUIRE(q && lens && block_table && k_codes && v_codes && k_scale && v_scale && out, "kv8_attn: null pointer");
-  SGL_REQUIRE(sgl::aligned(q, 16) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
-              "kv8_attn: q and its strides must be 16-byte aligned");
-  SGL_REQUIRE(sgl::aligned(k_codes, 16) && sgl::aligned(v_codes, 16) && sgl::aligned(out, 16),
-              "kv8_attn: misaligned cache or output");
-  // one launch, or (chunks and few rows in one batch) two, one after the other on the same workspace
-  const int64_t tokens = row_pages * page_size;
-  const sgl::Kv8AttnPlan plans[2] = {sgl::kv8_attn_plan(T, B, Hkv, G, D, tokens, sgl::device_cu_count()),
-                                     sgl::kv8_attn_rest(T, B, Hkv, G, D, tokens, sgl::device_cu_count())};
-  for (const sgl::Kv8AttnPlan& p : plans) {
-    const size_t need = sgl::kv8_attn_workspace(p, Hkv, D);
-    if (need && (!workspace || workspace_bytes < need)) {
-      sgl::set_error("kv8_attn: workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : 0, need);
-      return SGL_ERR_WORKSPACE;
-    }
-    SGL_REQUIRE_SUPPORTED(p.items * ((tokens + 31) / 32 + sgl::kItemCost) < (1ll << 31) &&
-                              p.items * p.row_tile / 4 < (1ll << 31),
-                          "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)p.items,
-                          (long long)tokens);
-  }
-  SGL_REQUIRE(sgl::aligned(workspace, 16), "kv8_attn: workspace must be 16-byte aligned");
+  return sgl_kv8_attn_first(q, q_token_stride, q_head_stride, dtype, T, B, Hkv, G, D, cu_tokens, lens, block_table,
+                            row_pages, page_size, block, n_pages, k_codes, v_codes, k_scale, v_scale, softmax_scale,
+                            causal, window, 0, sink, out, workspace, workspace_bytes, stream);
+}
+
+size_t sgl_kv8_attn_first_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens,
+                                         int64_t window, int64_t first) {
+  if (!sgl::attn_sizes_ok(T, B, Hkv, G, D, max_tokens) || window < 0 || first < 0) return 0;
+  return sgl::attn_workspace(
+      sgl::attn_plans(T, B, Hkv, G, D, sgl::kv8_attn_reach(T, B, max_tokens, window, first)), Hkv, D);
+}
+
+int sgl_kv8_attn_first(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T, int64_t B,
+                       int Hkv, int G, int D, const int32_t* cu_tokens, const int32_t* lens,
+                       const int32_t* block_table, int64_t row_pages, int page_size, int block, int64_t n_pages,
+                       const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                       float softmax_scale, int causal, int64_t window, int64_t first, const float* sink, void* out,
+                       void* workspace, size_t workspace_bytes, sgl_stream_t stream) {
+  const sgl::AttnCall call = {q, q_token_stride, q_head_stride, dtype, T, B, Hkv, G, D, cu_tokens, lens, block_table,
+                              row_pages, page_size, block, n_pages, k_codes, v_codes, k_scale, v_scale, softmax_scale,
+                              causal, window, sink, out, workspace};
   sgl::Kv8AttnArgs a;
-  a.q = (const uint16_t*)q;
-  a.qt = q_token_stride;
-  a.qh = q_head_stride;
-  a.o = (uint16_t*)out;
-  a.kc = (const uint8_t*)k_codes;
-  a.vc = (const uint8_t*)v_codes;
-  a.ks = k_scale;
-  a.vs = v_scale;
-  a.pages = block_table;
-  a.lens = lens;
-  a.cu = cu_tokens;
-  a.sink = sink;
-  a.n_pages = n_pages;
-  a.T = (int)T;
-  a.B = (int)B;
-  a.Hkv = Hkv;
-  a.G = G;
-  a.D = D;
-  a.row_pages = (int)row_pages;
-  a.page_shift = __builtin_ctz((unsigned)page_size);
-  a.block_shift = __builtin_ctz((unsigned)block);
-  a.c1 = softmax_scale * sgl::kLog2e;
-  a.window = window >= tokens ? 0 : (int)window;  // (as long as the table: all keys)
-  a.causal = causal != 0;
-  a.ws_acc = (float*)workspace;
-  for (const sgl::Kv8AttnPlan& p : plans) {
-    if (p.items == 0) continue;
-    if (dtype == SGL_BF16)
-      sgl::launch_attn<SGL_BF16>(a, p, (hipStream_t)stream);
-    else
-      sgl::launch_attn<SGL_F16>(a, p, (hipStream_t)stream);
-  }
+  bool nothing;
+  SGL_REQUIRE(first >= 0 && (first == 0 || window > 0), "kv8_attn: first tokens (%lld) are for a window", (long long)first);
+  int rc = sgl::attn_args(call, a, nothing);
+  if (rc != SGL_OK || nothing) return rc;
+  const int64_t tokens = row_pages * page_size, reach = sgl::kv8_attn_reach(T, B, tokens, window, first);
+  a.first = a.window == 0 ? 0 : (int)(first < tokens ? first : tokens);
+  const sgl::AttnPlans plans = sgl::attn_plans(T, B, Hkv, G, D, reach);
+  rc = sgl::check_workspace(workspace, workspace_bytes, sgl::attn_workspace(plans, Hkv, D));
+  if (rc == SGL_OK) rc = sgl::check_plans(plans, tokens);
+  if (rc != SGL_OK) return rc;
+  sgl::launch_plans(a, dtype, plans, (hipStream_t)stream);
+  return sgl::check_launch("kv8_attn");
+}
+
+size_t sgl_kv8_attn_shared_workspace_size(int64_t T, int64_t B, int Hkv, int G, int D, int64_t max_tokens,
+                                          int64_t n_groups) {
+  if (!sgl::attn_sizes_ok(T, B, Hkv, G, D, max_tokens) || n_groups < 1) return 0;
+  return sgl::prefix_space(T, B, Hkv, G, D, max_tokens, n_groups).total;
+}
+
+int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T, int64_t B,
+                        int Hkv, int G, int D, const int32_t* cu_tokens, const int32_t* lens,
+                        const int32_t* block_table, int64_t row_pages, int page_size, int block, int64_t n_pages,
+                        const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                        float softmax_scale, int causal, const float* sink, int64_t n_groups,
+                        const int32_t* cu_groups, const int32_t* shared, void* out, void* workspace,
+                        size_t workspace_bytes, sgl_stream_t stream) {
+  const sgl::AttnCall call = {q, q_token_stride, q_head_stride, dtype, T, B, Hkv, G, D, cu_tokens, lens, block_table,
+                              row_pages, page_size, block, n_pages, k_codes, v_codes, k_scale, v_scale, softmax_scale,
+                              causal, 0, sink, out, workspace};
+  sgl::Kv8AttnArgs a;
+  bool nothing;
+  SGL_REQUIRE(n_groups >= 1 && n_groups <= (1 << 24), "kv8_attn: n_groups=%lld out of range", (long long)n_groups);
+  int rc = sgl::attn_args(call, a, nothing);
+  if (rc != SGL_OK || nothing) return rc;
+  SGL_REQUIRE(cu_groups && shared, "kv8_attn: null pointer");
+  const int64_t tokens = row_pages * page_size, n = n_groups;
+  const sgl::AttnPlans first = sgl::attn_plans(T, n, Hkv, G, D, tokens);
+  const sgl::AttnPlans second = sgl::attn_plans(T, B, Hkv, G, D, tokens);
+  const sgl::PrefixSpace space = sgl::prefix_space(T, B, Hkv, G, D, tokens, n);
+  rc = sgl::check_workspace(workspace, workspace_bytes, space.total);
+  if (rc == SGL_OK) rc = sgl::check_plans(first, tokens);
+  if (rc == SGL_OK) rc = sgl::check_plans(second, tokens);
+  if (rc != SGL_OK) return rc;
+  char* base = (char*)workspace;
+  sgl::PrefixPlan plan;
+  plan.cu = (int32_t*)(base + space.plan);
+  plan.lens = plan.cu + n + 1;
+  plan.row = plan.lens + n;
+  plan.skip = plan.row + n;
+  a.ws_acc = (float*)(base + space.rest);
+  a.prior_acc = (float*)(base + space.acc);
+  a.prior_ml = (float*)(base + space.ml);
+  const hipStream_t st = (hipStream_t)stream;
+  sgl::kv8_prefix_kernel<<<(unsigned)(n + 1), 256, 0, st>>>(a, cu_groups, shared, (int)n, plan);
+  sgl::Kv8AttnArgs g = a;
+  g.B = (int)n;
+  g.cu = plan.cu;
+  g.lens = plan.lens;
+  g.table_row = plan.row;
+  g.causal = false;
+  g.sink = nullptr;
+  g.raw = true;
+  sgl::launch_plans(g, dtype, first, st);
+  a.skip = plan.skip;
+  sgl::launch_plans(a, dtype, second, st);
   return sgl::check_launch("kv8_attn");
 }
 

@@ -73,8 +73,9 @@ __device__ __forceinline__ uint32_t swt(int t) {
   return DP >= 128 ? (uint32_t)(((t & 3) << 2) | ((t >> 2) & 3)) : (uint32_t)(((t & 2) << 1) | ((t >> 2) & 3));
 }
 
-// DP: head dim rounded up to 64, 128 or 256; NW wavefronts
-template <int DP, int QT, int NW, bool SPLIT>
+// DP: head dim rounded up to 64, 128 or 256; NW wavefronts; FIRST: the sequence's first
+// tokens are seen beside the window
+template <int DP, int QT, int NW, bool SPLIT, bool FIRST>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel(const Kv8AttnArgs a, int64_t items) {
   constexpr int kKeys = chunk_keys(DP), NG = kKeys / 16, NH = kKeys / 32;  // granules, halves of 32 tokens
   constexpr int RT = 32 * NW, NT = 64 * NW, ROW = 2 * DP, KS = DP / 16, DT = DP / 32;
@@ -124,6 +125,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     const int pos = s.len - s.n + tq;
     const int hi = !live ? 0 : a.causal && pos + 1 < s.len ? pos + 1 : s.len;
     const int lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
+    // (without branches: of an `or` in the masks below the compiler makes wrong code)
+    const uint32_t hidden = lo > a.first ? (uint32_t)(lo - a.first) : 0u;  // keys between the first tokens and the window
+    auto sees = [&](int key) __attribute__((always_inline)) {
+      if constexpr (FIRST)
+        return (key < hi) & ((uint32_t)(key - a.first) >= hidden);
+      else
+        return key < hi && key >= lo;
+    };
     // what all rows of the wavefront see, and what any row of the tile sees
     int all_hi = s.len, all_lo = 0, any_lo = 0, any_hi = s.len;
     if (a.causal) {
@@ -138,11 +147,21 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         any_lo = any_lo < 0 ? 0 : any_lo;
       }
     }
-    int j0 = s.tile0 + t0, j1 = s.tile0 + t1;
-    if (any_lo / kKeys > j0) j0 = any_lo / kKeys;
+    // The tiles to go over: of the first tokens those from t0 on, `front` of them, then
+    // from j0 on, where the windows of these rows begin.
+    int front = 0, j0 = t0, j1 = s.tile0 + t1;
     const int jh = any_hi <= 0 ? 0 : (any_hi + kKeys - 1) / kKeys;
+    if (FIRST && t0 < s.kept) {
+      front = (t1 < s.kept ? t1 : s.kept) < jh ? (t1 < s.kept ? t1 : s.kept) - t0 : jh - t0;
+      front = front > 0 ? front : 0;
+      if (t1 <= s.kept) j1 = 0;  // (nothing behind them)
+      j0 = s.kept;
+    }
+    j0 += s.tile0;
+    if (any_lo / kKeys > j0) j0 = any_lo / kKeys;
     if (jh < j1) j1 = jh;
-    if (s.len == 0) j1 = j0;
+    const int n_tiles = s.len == 0 ? 0 : front + (j1 > j0 ? j1 - j0 : 0);
+    auto tile_at = [&](int i) __attribute__((always_inline)) { return FIRST && i < front ? t0 + i : i + (FIRST ? j0 - front : j0); };
 
     v16f acc[DT];
 #pragma unroll
@@ -151,7 +170,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
     float m_run = live ? NEG_INF : 1e30f, l_run = 0.0f;  // (a row that is none never asks for a reference)
 
-    if (j0 < j1) {
+    if (n_tiles > 0) {
       u4v q[KS];  // (with QL only until they are in LDS)
       {
         const uint16_t* src = a.q + (int64_t)(s.row0 + tq) * a.qt + (int64_t)hq * a.qh + 8 * g2;
@@ -167,11 +186,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         else
           return q[k];
       };
-      const int32_t* table = a.pages + (int64_t)b * a.row_pages;
+      const int32_t* table = a.pages + (int64_t)(a.table_row ? a.table_row[b] : b) * a.row_pages;
       const int pmask = (1 << a.page_shift) - 1;
 
       // ---- pages and scales of TB tiles at a time: lane l has granule l % NG of tile
-      // l / NG, counted from j0; pages loaded a batch ahead, scales most of one
+      // l / NG, in their order; pages loaded a batch ahead, scales most of one
       struct Batch {
         int page;  // 0 where there is none
         float k, v;
@@ -179,14 +198,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       };
       auto load_pages = [&](int batch) __attribute__((always_inline)) {
         Batch o;
-        const int t = (j0 + TB * batch + lane / NG) * kKeys + 16 * (lane % NG);
+        const int t = tile_at(TB * batch + lane / NG) * kKeys + 16 * (lane % NG);
         const int page = table[(t < s.len ? t : s.len - 1) >> a.page_shift];
         o.ok = t < s.len && page >= 0 && page < a.n_pages;
         o.page = o.ok ? page : 0;
         return o;
       };
       auto load_scales = [&](int batch, Batch& o) __attribute__((always_inline)) {
-        const int t = (j0 + TB * batch + lane / NG) * kKeys + 16 * (lane % NG);
+        const int t = tile_at(TB * batch + lane / NG) * kKeys + 16 * (lane % NG);
         const int64_t piece = (((int64_t)o.page * a.Hkv + head) << (a.page_shift - a.block_shift)) +
                               ((t & pmask) >> a.block_shift);
         o.k = a.ks[piece];
@@ -214,12 +233,13 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       // piece i: whether V's, and its token (the wavefront's first: with wtok)
       auto is_v = [](int i) { return i * NT >= SIDE; };
       auto tok_of = [&](int i, int t) { return (t + i * (NT / CPR)) % kKeys; };
-      // K's pieces of tile jk, V's of tile jv (pages: the lanes' pages of their batches)
-      auto load_codes = [&](int jk, int kpages, int jv, int vpages, uint4* out) __attribute__((always_inline)) {
+      // K's pieces of the ik-th tile, V's of the iv-th (pages: the lanes' pages of their batches)
+      auto load_codes = [&](int ik, int kpages, int iv, int vpages, uint4* out) __attribute__((always_inline)) {
+        const int jk = tile_at(ik), jv = tile_at(iv);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int t = tok_of(i, wtok), j = is_v(i) ? jv : jk;
-          const int page = __builtin_amdgcn_readlane(is_v(i) ? vpages : kpages, NG * ((j - j0) & (TB - 1)) + (t >> 4));
+          const int page = __builtin_amdgcn_readlane(is_v(i) ? vpages : kpages, NG * ((is_v(i) ? iv : ik) & (TB - 1)) + (t >> 4));
           const int64_t row = (((int64_t)page * a.Hkv + head) << a.page_shift) + ((j * kKeys + t) & pmask);
           out[i] = *reinterpret_cast<const uint4*>((is_v(i) ? a.vc : a.kc) + row * a.D + poff);
         }
@@ -286,7 +306,9 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       const int part_hi = a.causal ? s.len - s.n + (rt * RT) / a.G + 1 : s.len;  // keys that the first row sees
       const int part_lo = a.causal && a.window > 0
                               ? s.len - s.n + (rt * RT + (rows < RT ? rows : RT) - 1) / a.G - a.window + 1 : 0;
-      auto partial = [&](int j) { return (j + 1) * kKeys > part_hi || j * kKeys < part_lo; };
+      auto partial = [&](int j) {
+        return (j + 1) * kKeys > part_hi || (j * kKeys < part_lo && !(FIRST && (j + 1) * kKeys <= a.first));
+      };
       // ---- S^T: lane (row c32, half g2) gets token 32 t + 8 (i / 4) + 4 g2 + i % 4 in sc[t][i]
       constexpr int NKA = DP >= 128 ? 8 : 4;
       uint32_t ka[NKA];
@@ -315,7 +337,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       auto put_nan = [&](int j, int buf) __attribute__((always_inline)) {
         if (__builtin_expect(partial(j) && sNan[buf] == j + 1, 0)) {
           for (int t = 0; t < kKeys; ++t) {
-            const bool seen = j * kKeys + t < hi && j * kKeys + t >= lo;
+            const bool seen = sees(j * kKeys + t);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
               const uint32_t dims = *reinterpret_cast<const uint32_t*>(&sDims[buf][t][2 * d]) >> (4 * g2);
@@ -336,10 +358,10 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
       constexpr uint32_t kAll = (1u << NG) - 1;
       bool fresh = __ballot(m_run == NEG_INF) != 0;  // a row has no reference yet
       Batch now, ahead;
-      // Tile j = j0 + i, scores in sc: its softmax, slice by slice between the products
+      // The i-th tile j, scores in sc: its softmax, slice by slice between the products
       // S^T of tile j + 1 (into sn) and O^T += V^T . P^T of tile j - 1.
       auto tile_step = [&](int i, const int buf, v16f* sc, v16f* sn) __attribute__((always_inline)) {
-        const int j = j0 + i, l0 = NG * (i & (TB - 1)), tok = j * kKeys;
+        const int j = tile_at(i), l0 = NG * (i & (TB - 1)), tok = j * kKeys;
         const float2* scale = &sScale[(i / TB) & 1][l0];
         auto top = [&]() __attribute__((always_inline)) {  // the row's largest exponent in this tile
           float mx = NEG_INF;
@@ -360,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         // then), or, below, eight weights pass what one f16 holds.  It lies kLift
         // below the maximum that it was taken from.
         const bool border = (i & (TB - 1)) == 0 && i > 0;
-        const bool seen_by_all = tok + kKeys <= all_hi && tok >= all_lo;
+        const bool seen_by_all = tok + kKeys <= all_hi && (tok >= all_lo || (FIRST && tok + kKeys <= a.first));
         if (__builtin_expect(border || (i & (TB - 1)) == 4 || !seen_by_all || partial(j) || (okm >> l0 & kAll) != kAll || fresh, 0)) {
           if (border) {
             now = ahead;
@@ -391,7 +413,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 const int key = tok + 32 * t + 8 * (e >> 2) + 4 * g2 + (e & 3);
-                if (!(key < hi && key >= lo && ((here >> (2 * t + (e >> 3))) & 1))) sc[t][e] = NEG_INF;
+                if (!(sees(key) && ((here >> (2 * t + (e >> 3))) & 1))) sc[t][e] = NEG_INF;
               }
           }
           if (fresh) {
@@ -458,7 +480,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           for (int c = 0; c < PIECES; ++c)
             if (n == (c + 1) * NS / (PIECES + 2)) store_piece(c, buf, raw[c]);
           if (n == (PIECES + 1) * NS / (PIECES + 2))
-            load_codes(j + 3, (i & (TB - 1)) >= TB - 3 ? ahead.page : now.page, j + 1, (i & (TB - 1)) == TB - 1 ? ahead.page : now.page, raw);
+            load_codes(i + 3, (i & (TB - 1)) >= TB - 3 ? ahead.page : now.page, i + 1, (i & (TB - 1)) == TB - 1 ? ahead.page : now.page, raw);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_expect(__ballot(most > 60000.0f) != 0, 0)) {
@@ -478,7 +500,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         }
         l_run = l_new;
         p[NG - 1] = p_last;
-        if (__builtin_expect(i > 0 && partial(j - 1), 0)) put_nan(j - 1, buf ^ 1);
+        if (__builtin_expect(i > 0 && partial(tile_at(i - 1)), 0)) put_nan(tile_at(i - 1), buf ^ 1);
         lds_barrier();
       };
 
@@ -488,8 +510,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         ahead = load_pages(1);
         load_scales(0, now);
         uint4 first[PIECES];
-        load_codes(j0, now.page, j0, now.page, first);
-        load_codes(j0 + 1, now.page, j0, now.page, raw);
+        load_codes(0, now.page, 0, now.page, first);
+        load_codes(1, now.page, 0, now.page, raw);
         if constexpr (QL) {
 #pragma unroll
           for (int k = 0; k < KS; ++k) sQ[wave][k][lane] = q[k];  // (read by the lane that wrote it)
@@ -501,7 +523,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
           if (!is_v(c)) store_piece(c, 0, first[c]);
           store_piece(c, 1, is_v(c) ? make_uint4(0, 0, 0, 0) : raw[c]);
         }
-        load_codes(j0 + 2, now.page, j0, now.page, raw);
+        load_codes(2, now.page, 0, now.page, raw);
 #pragma unroll
         for (int g = 0; g < NG; ++g) p[g] = u4v{0, 0, 0, 0};
       }
@@ -514,7 +536,6 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 #pragma unroll
       for (int n = 0; n < NS; ++n) s0[n % NH] = O::mfma(k_frag(sK[0], n), q_frag(n / NH), s0[n % NH]);
       lds_barrier();
-      const int n_tiles = j1 - j0;
       for (int i = 0; i < n_tiles; i += 2) {
         tile_step(i, 0, s0, s1);
         if (i + 1 >= n_tiles) break;
@@ -524,27 +545,28 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 #pragma unroll
       for (int n = 0; n < NS; ++n)
         acc[n % DT] = F::mfma(v_frag(sK[2] + lb * kKeys * ROW, n / DT, n % DT), p[n / DT], acc[n % DT]);
-      put_nan(j1 - 1, lb);
+      put_nan(tile_at(n_tiles - 1), lb);
     }
 
     // ---- out
     l_run += __shfl_xor(l_run, 32, 64);
     if (live) {
-      if (whole) {
-        const float ref = m_run == NEG_INF ? 0.0f : m_run;
-        const float sum = a.sink ? l_run + __builtin_amdgcn_exp2f(a.sink[hq] * kLog2e - ref) : l_run;
-        const float inv = sum > 0.0f || sum != sum ? kUnlift / sum : 0.0f;
-        uint16_t* o = a.o + ((int64_t)(s.row0 + tq) * (a.Hkv * a.G) + hq) * a.D + 4 * g2;
+      const int64_t at = (int64_t)(s.row0 + tq) * (a.Hkv * a.G) + hq;
+      if (whole && !a.raw) {
+        Kv8Join join = kv8_join(a, s, at, hq, m_run, l_run);
+        join.own *= kUnlift;
+        uint16_t* o = a.o + at * a.D + 4 * g2;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (32 * d + 8 * k < a.D)
-              *reinterpret_cast<uint2*>(o + 32 * d + 8 * k) =
-                  make_uint2(kv8_out2<QT>(acc[d][4 * k] * inv, acc[d][4 * k + 1] * inv),
-                             kv8_out2<QT>(acc[d][4 * k + 2] * inv, acc[d][4 * k + 3] * inv));
+            if (32 * d + 8 * k < a.D) {
+              const float4 y = kv8_joined(a, join, at, 32 * d + 8 * k + 4 * g2,
+                                          make_float4(acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]));
+              *reinterpret_cast<uint2*>(o + 32 * d + 8 * k) = make_uint2(kv8_out2<QT>(y.x, y.y), kv8_out2<QT>(y.z, y.w));
+            }
       } else {
-        float* o = a.ws_acc + (slot * RT + r) * a.D + 4 * g2;
+        float* o = (whole ? a.prior_acc + at * a.D : a.ws_acc + (slot * RT + r) * a.D) + 4 * g2;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -553,42 +575,43 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
               *reinterpret_cast<float4*>(o + 32 * d + 8 * k) =
                   make_float4(acc[d][4 * k] * kUnlift, acc[d][4 * k + 1] * kUnlift, acc[d][4 * k + 2] * kUnlift,
                               acc[d][4 * k + 3] * kUnlift);
-        if (g2 == 0) *reinterpret_cast<float2*>(a.ws_ml + (slot * RT + r) * 2) = make_float2(m_run, l_run);
+        if (g2 == 0)
+          *reinterpret_cast<float2*>(whole ? a.prior_ml + 2 * at : a.ws_ml + (slot * RT + r) * 2) = make_float2(m_run, l_run);
       }
     }
   }
 }
 
-template <int DP, int QT>
+template <int DP, int QT, bool FIRST>
 void launch_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
   constexpr int NW = DP == 128 ? 8 : 4, RT = 32 * NW;
   static_assert(RT == kv8_chunk_rows(DP), "the plan's row tile");
   const int64_t items = p.items;
   if (p.parts == 0) {
-    kv8_prefill_kernel<DP, QT, NW, false><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
+    kv8_prefill_kernel<DP, QT, NW, false, FIRST><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
   } else {
-    kv8_prefill_kernel<DP, QT, NW, true><<<a.parts * a.Hkv, 64 * NW, 0, st>>>(a, items);
+    kv8_prefill_kernel<DP, QT, NW, true, FIRST><<<a.parts * a.Hkv, 64 * NW, 0, st>>>(a, items);
     kv8_merge_kernel<RT, chunk_keys(DP), QT><<<(unsigned)(items * (RT / 4)), 256, 0, st>>>(a);
   }
 }
 
-template <int QT>
+template <int QT, bool FIRST>
 void launch_prefill_as(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
   if (a.D <= 64)
-    launch_prefill<64, QT>(a, p, st);
+    launch_prefill<64, QT, FIRST>(a, p, st);
   else if (a.D <= 128)
-    launch_prefill<128, QT>(a, p, st);
+    launch_prefill<128, QT, FIRST>(a, p, st);
   else
-    launch_prefill<256, QT>(a, p, st);
+    launch_prefill<256, QT, FIRST>(a, p, st);
 }
 
 }  // namespace
 
 void launch_kv8_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, int dtype, hipStream_t st) {
   if (dtype == SGL_BF16)
-    launch_prefill_as<SGL_BF16>(a, p, st);
+    a.first > 0 ? launch_prefill_as<SGL_BF16, true>(a, p, st) : launch_prefill_as<SGL_BF16, false>(a, p, st);
   else
-    launch_prefill_as<SGL_F16>(a, p, st);
+    a.first > 0 ? launch_prefill_as<SGL_F16, true>(a, p, st) : launch_prefill_as<SGL_F16, false>(a, p, st);
 }
 
 }  // namespace sgl

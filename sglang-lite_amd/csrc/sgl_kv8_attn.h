@@ -50,11 +50,19 @@ struct Kv8AttnArgs {
   int T, B, Hkv, G, D, row_pages, page_shift, block_shift;
   float c1;     // softmax scale in log2 units
   int window;   // keys a query sees, itself included; 0: all
+  int first;    // and the sequence's first tokens, which the window does not hide
   bool causal;
   int parts;      // workgroups of a kv head's line; 0: one workgroup an item
   int above, upto;  // takes the sequences of more than `above` rows a kv head, and up to `upto`
   float* ws_acc;  // [2 parts Hkv][row tile][D]
   float* ws_ml;   // [2 parts Hkv][row tile][2]: reference point (log2 units), sum
+  // A common prefix: its groups are the sequences of a first pass, whose unnormalised sums go
+  // to `prior` (`raw`); the second pass begins behind what they cover, and joins the two.
+  const int32_t* table_row;  // first pass: the row of the block table of each group; null: its own
+  const int32_t* skip;       // second pass: tokens that the first has covered; null: none
+  float* prior_acc;          // [T Hkv G][D]
+  float* prior_ml;           // [T Hkv G][2]
+  bool raw;
 };
 
 // Key tiles.  1 / 2 / 3 / 5, us: 32 sequences of 4 queries up to 6000 keys 49.3 / 48.2 / 46.1 /
@@ -75,13 +83,21 @@ __device__ __forceinline__ float kv8_exponent(bool there, bool good, float vs) {
 // A sequence as the line sees it.
 struct Kv8Seq {
   int row0, n, len;  // first query row, queries, keys
-  int tile0, tiles;  // key tiles: first, number (at least one, so that empty rows are written)
+  int tile0, tiles;  // key tiles: hidden ones in front, number (at least one, so that empty rows are written)
+  int kept;          // tiles of the first tokens, which lie before the hidden ones
   int row_tiles;
+  int skip;
+
+  // the key tile that tile i of the item is
+  template <bool FIRST>
+  __device__ __forceinline__ int tile(int i) const {
+    return FIRST && i < kept ? i : i + tile0;
+  }
 };
 
 template <int RT, int TT>
-__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n, int len) {
-  int lo = 0;
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n, int len, int skip) {
+  int lo = skip;
   if (a.causal && a.window > 0) {
     const int64_t first = (int64_t)len - n - a.window + 1;
     lo = first > 0 ? (int)first : 0;
@@ -90,7 +106,9 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n,
   s.row0 = row0;
   s.n = n;
   s.len = len;
-  s.tile0 = lo / TT;
+  s.skip = skip;
+  s.kept = (a.first + TT - 1) / TT;
+  s.tile0 = lo / TT > s.kept ? lo / TT - s.kept : 0;
   const int tiles = (len + TT - 1) / TT - s.tile0;
   s.tiles = tiles > 0 ? tiles : 1;
   s.row_tiles = (n * a.G + RT - 1) / RT;
@@ -99,7 +117,7 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n,
 
 // 64 sequences from b0 on, one a lane.
 struct Kv8Chunk {
-  int b0, row0, n, len;
+  int b0, row0, n, len, skip;
   int room, rooms;  // places on the line: of this sequence, of those up to and with it
   int rts;          // row tiles of the sequences up to and with it
 };
@@ -107,7 +125,7 @@ struct Kv8Chunk {
 template <int RT, int TT>
 __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
   const int b = b0 + (int)(threadIdx.x & 63);
-  Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0};
+  Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0, 0};
   int rts = 0;
   if (b < a.B) {
     const int len = a.lens[b], cap = a.row_pages << a.page_shift;
@@ -115,9 +133,10 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
     c.row0 = r.first;
     c.n = r.n;
     c.len = len < 0 ? 0 : len > cap ? cap : len;
-    const Kv8Seq s = kv8_seq<RT, TT>(a, c.row0, c.n, c.len);
+    if (a.skip) c.skip = a.skip[b];
+    const Kv8Seq s = kv8_seq<RT, TT>(a, c.row0, c.n, c.len, c.skip);
     const int rows = r.n * a.G;
-    rts = rows > a.above && rows <= a.upto ? s.row_tiles : 0;
+    rts = rows > a.above && rows <= a.upto && !(a.raw && c.len == 0) ? s.row_tiles : 0;
     c.room = rts * (s.tiles + kItemCost);
   }
   c.rooms = wave_incl_scan(c.room);
@@ -128,7 +147,7 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
 template <int RT, int TT>
 __device__ __forceinline__ Kv8Seq kv8_lane(const Kv8AttnArgs& a, const Kv8Chunk& c, int l) {
   return kv8_seq<RT, TT>(a, __builtin_amdgcn_readlane(c.row0, l), __builtin_amdgcn_readlane(c.n, l),
-                         __builtin_amdgcn_readlane(c.len, l));
+                         __builtin_amdgcn_readlane(c.len, l), __builtin_amdgcn_readlane(c.skip, l));
 }
 
 // Length of a kv head's line; c: the batch's first 64 sequences.
@@ -236,6 +255,44 @@ __device__ __forceinline__ uint32_t kv8_out2(float a, float b) {
   return pack2<QT>(a, b);
 }
 
+// What is to be done with the sums of a row (reference point M, sum) that all of its keys have
+// gone into: the first pass keeps them; the others join the first's, take the sink
+// and divide.  `own` and `before` are the factors of the sums and of the prior ones.
+struct Kv8Join {
+  float own, before;
+  bool prior;
+};
+__device__ __forceinline__ Kv8Join kv8_join(const Kv8AttnArgs& a, const Kv8Seq& s, int64_t at, int h, float M, float sum) {
+  const float NEG_INF = -__builtin_huge_valf();
+  Kv8Join j = {1.0f, 0.0f, s.skip > 0};
+  float top = M;
+  float2 ml = make_float2(NEG_INF, 0.0f);
+  if (j.prior) {
+    ml = *reinterpret_cast<const float2*>(a.prior_ml + 2 * at);
+    top = __builtin_fmaxf(M, ml.x);
+  }
+  const float ref = top == NEG_INF ? 0.0f : top;
+  if (j.prior) {
+    j.own = __builtin_amdgcn_exp2f(M - ref);
+    j.before = __builtin_amdgcn_exp2f(ml.x - ref);
+    sum = sum * j.own + ml.y * j.before;
+  }
+  if (a.sink) sum += __builtin_amdgcn_exp2f(a.sink[h] * kLog2e - ref);
+  const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  j.own *= inv;
+  j.before *= inv;
+  return j;
+}
+// four of the row's sums
+__device__ __forceinline__ float4 kv8_joined(const Kv8AttnArgs& a, const Kv8Join& j, int64_t at, int d, float4 y) {
+  y = make_float4(y.x * j.own, y.y * j.own, y.z * j.own, y.w * j.own);
+  if (j.prior) {
+    const float4 p = *reinterpret_cast<const float4*>(a.prior_acc + at * a.D + d);
+    y = make_float4(y.x + p.x * j.before, y.y + p.y * j.before, y.z + p.z * j.before, y.w + p.w * j.before);
+  }
+  return y;
+}
+
 // Item x of the batch (row tiles in order, the heads of each together) as one segment.
 template <int RT, int TT>
 __device__ __forceinline__ bool kv8_item(const Kv8AttnArgs& a, int64_t x, int* head, Kv8Segment& g) {
@@ -316,11 +373,16 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k, 64);
-  if (a.sink) l += __builtin_amdgcn_exp2f(a.sink[h] * kLog2e - ref);
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  if (d < a.D)
-    *reinterpret_cast<uint2*>(a.o + ((int64_t)(s.row0 + t) * (a.Hkv * a.G) + h) * a.D + d) =
-        make_uint2(kv8_out2<QT>(acc[0] * inv, acc[1] * inv), kv8_out2<QT>(acc[2] * inv, acc[3] * inv));
+  if (d >= a.D) return;
+  const int64_t out = (int64_t)(s.row0 + t) * (a.Hkv * a.G) + h;
+  float4 y = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  if (a.raw) {
+    *reinterpret_cast<float4*>(a.prior_acc + out * a.D + d) = y;
+    if (lane == 0) *reinterpret_cast<float2*>(a.prior_ml + 2 * out) = make_float2(M, l);
+    return;
+  }
+  y = kv8_joined(a, kv8_join(a, s, out, h, M, l), out, d, y);
+  *reinterpret_cast<uint2*>(a.o + out * a.D + d) = make_uint2(kv8_out2<QT>(y.x, y.y), kv8_out2<QT>(y.z, y.w));
 }
 
 // kv8_prefill.hip: row tiles of kv8_chunk_rows(D).

@@ -353,6 +353,13 @@ SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G,
   const int64_t rt = kv8_few_tile(rows, D), items = kv8_attn_items(T, B, Hkv, G, rt);
   return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, 0x7FFFFFFF};
 }
+// What stands for the block table's width where first tokens are seen beside a window: the keys
+// that a row tile's queries can see between them.
+SGL_RULE int64_t kv8_attn_reach(int64_t T, int64_t B, int64_t capacity, int64_t window, int64_t first) {
+  if (window <= 0 || first <= 0 || B <= 0) return capacity;
+  const int64_t reach = window + first + (T + B - 1) / B + 128;
+  return reach < capacity ? reach : capacity;
+}
 // The second launch of a batch of chunks: its sequences of few rows.
 SGL_RULE Kv8AttnPlan kv8_attn_rest(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
                                    int64_t cus) {

@@ -140,6 +140,18 @@ SIGNATURES = {
         [P, I64, I64, c_int, I64, I64, c_int, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P, P, P,
          P, c_float, c_int, I64, P, P, P, c_size_t, P],
     ),
+    "sgl_kv8_attn_first": (
+        c_int,
+        [P, I64, I64, c_int, I64, I64, c_int, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P, P, P,
+         P, c_float, c_int, I64, I64, P, P, P, c_size_t, P],
+    ),
+    "sgl_kv8_attn_first_workspace_size": (c_size_t, [I64, I64, c_int, c_int, c_int, I64, I64, I64]),
+    "sgl_kv8_attn_shared": (
+        c_int,
+        [P, I64, I64, c_int, I64, I64, c_int, c_int, c_int, P, P, P, I64, c_int, c_int, I64, P, P, P,
+         P, c_float, c_int, P, I64, P, P, P, P, c_size_t, P],
+    ),
+    "sgl_kv8_attn_shared_workspace_size": (c_size_t, [I64, I64, c_int, c_int, c_int, I64, I64]),
     "sgl_kv8_attn_workspace_size": (c_size_t, [I64, I64, c_int, c_int, c_int, I64]),
     "sgl_host_f32_to_e4m3": (c_int, [P, P, I64]),
     "sgl_host_e4m3_to_f32": (c_int, [P, P, I64]),

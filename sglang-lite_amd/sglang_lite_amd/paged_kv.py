@@ -108,10 +108,10 @@ def _rows16(x: torch.Tensor, n: int):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace(device: int, *sizes: int) -> int:
+def _workspace(device: int, name: str, *sizes: int) -> int:
     """Bytes for the attention of these sizes: a function of them and of the device's CUs."""
     with torch.cuda.device(device):
-        return _lib.size_of("sgl_kv8_attn_workspace_size", *sizes)
+        return _lib.size_of(name, *sizes)
 
 
 def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -184,18 +184,27 @@ def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: tor
 
 def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens: torch.Tensor, *,
                cu_tokens: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
-               causal: bool = True, window: int = 0, sink: Optional[torch.Tensor] = None,
-               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               causal: bool = True, window: int = 0, first: int = 0,
+               sink: Optional[torch.Tensor] = None, cu_groups: Optional[torch.Tensor] = None,
+               shared: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of ``q`` ``[T, Hq, D]`` (bf16 or f16) over the cache: ``[T, Hq, D]``.
 
     Sequence ``b`` has ``lens[b]`` keys (int32 ``[B]``), its ``n`` queries being
     the last ``n`` of them; query head ``h`` reads kv head ``h // (Hq / Hkv)``.
     ``causal``: a query sees the keys up to its own position, the last ``window``
-    of them if that is not 0; otherwise all.  ``sink`` (float32 ``[Hq]``): a
+    of them if that is not 0 and beside those the sequence's ``first`` tokens; otherwise all.  ``sink`` (float32 ``[Hq]``): a
     logit of each head that takes part in the softmax and has no value.
     ``softmax_scale``: ``D ** -0.5`` by default.  The weights that meet the values
     are rounded by at most 2^-11 of themselves, or 2^-35 of the row's largest (each
-    times its value's scale).  A row that sees no key is zero;
+    times its value's scale).
+
+    ``cu_groups`` (int32 ``[groups + 1]``, never falling) and ``shared`` (int32 ``[groups]``), without
+    a window: sequences ``cu_groups[g]`` to ``cu_groups[g + 1]`` begin alike, the full pages
+    among their first ``shared[g]`` tokens being the same in each one's row of the block table.  Those
+    pages are read once for all of the group's queries, and the result is the same but for the order
+    of its sums.  Sequences may stand outside of all groups.
+
+    A row that sees no key is zero;
     rows behind the last sequence are not written (of a new tensor: they hold
     anything).  ``out`` may be ``q`` itself, or share no memory with its rows."""
     pages, heads, page, dim, block = _check_cache(cache, "paged_attn")
@@ -214,8 +223,20 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
                          f"{tuple(sink.shape)}")
     if window < 0 or (window and not causal):
         raise ValueError(f"paged_attn: window ({window}) must not be negative and is for causal attention")
+    if first < 0 or (first and not window):
+        raise ValueError(f"paged_attn: first ({first}) must not be negative and is for a window")
+    groups = 0
+    if cu_groups is not None or shared is not None:
+        if cu_groups is None or shared is None or window:
+            raise ValueError("paged_attn: cu_groups and shared go together, without a window")
+        groups = shared.shape[0] if shared.dim() == 1 else 0
+        if groups < 1 or shared.dtype is not torch.int32 or cu_groups.dtype is not torch.int32 or \
+                cu_groups.shape != (groups + 1,) or not (shared.is_contiguous() and cu_groups.is_contiguous()):
+            raise ValueError(f"paged_attn: cu_groups and shared must be contiguous int32 [groups + 1] and "
+                             f"[groups], got {cu_groups.dtype} {tuple(cu_groups.shape)} and {shared.dtype} "
+                             f"{tuple(shared.shape)}")
     kc, vc, ks, vs = cache
-    d = _lib.device_of("paged_attn", q, block_table, lens, cu_tokens, sink, out, kc, vc, ks, vs)
+    d = _lib.device_of("paged_attn", q, block_table, lens, cu_tokens, sink, cu_groups, shared, out, kc, vc, ks, vs)
     given = out is not None
     if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -227,13 +248,19 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     q, sq = _rows16(q, 8)
     if given and out is not q:
         check_apart(q, out, "paged_attn")
-    nws = _workspace(d, T, B, heads, hq // heads, dim, columns * page)
+    name, size, more = "sgl_kv8_attn", (T, B, heads, hq // heads, dim, columns * page), (window,)
+    if groups:
+        name, size, more = "sgl_kv8_attn_shared", (*size, groups), ()
+    elif first:
+        name, size, more = "sgl_kv8_attn_first", (*size, window, first), (window, first)
+    nws = _workspace(d, name + "_workspace_size", *size)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    _lib.call_on(d, "sgl_kv8_attn", q.data_ptr(), sq[0], sq[1], dt, T, B, heads, hq // heads, dim,
+    shares = (groups, cu_groups.data_ptr(), shared.data_ptr()) if groups else ()
+    _lib.call_on(d, name, q.data_ptr(), sq[0], sq[1], dt, T, B, heads, hq // heads, dim,
                  _lib.ptr(cu_tokens), lens.data_ptr(), block_table.data_ptr(), columns, page, block,
                  pages, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-                 dim ** -0.5 if softmax_scale is None else softmax_scale, causal, window,
-                 _lib.ptr(sink), out.data_ptr(), _lib.ptr(ws), nws)
+                 dim ** -0.5 if softmax_scale is None else softmax_scale, causal, *more,
+                 _lib.ptr(sink), *shares, out.data_ptr(), _lib.ptr(ws), nws)
     return out
 
 
