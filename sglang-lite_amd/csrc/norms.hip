@@ -32,19 +32,28 @@ struct NormArgs {
   bool e8m0;
 };
 
-// 8 elements from `at` on as they lie; `n` of them are there (the others zero).  Rows may begin
+// 8 elements from `at` on as they lie; `n` of them are there (the others zero; without TAIL all are).  Rows may begin
 // at any element, so the loads ask for no alignment beyond it (gfx950 takes them whole).
 template <int DT>
 struct Raw {
   uint32_t w[DT == SGL_F32 ? 8 : 4];
 };
-template <int DT>
+// ONCE: with the nontemporal policy, for lines that one load takes whole (16-bit elements).
+template <int DT, bool TAIL, bool ONCE = false>
 __device__ __forceinline__ Raw<DT> fetch(const void* base, int64_t at, int n) {
   typedef std::conditional_t<DT == SGL_F32, uint32_t, uint16_t> E;
   const E* p = (const E*)base + at;
   Raw<DT> r;
-  if (__builtin_expect(n == 8, 1)) {
-    __builtin_memcpy(r.w, p, sizeof(r.w));
+  if (!TAIL || __builtin_expect(n == 8, 1)) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef u4 u4h __attribute__((aligned(2)));
+    typedef u4 u4w __attribute__((aligned(4)));
+    typedef std::conditional_t<DT == SGL_F32, u4w, u4h> u4v;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(r.w) / 16; ++i) {
+      const u4 v = ONCE ? __builtin_nontemporal_load((const u4v*)p + i) : ((const u4v*)p)[i];
+      __builtin_memcpy(r.w + 4 * i, &v, 16);
+    }
   } else {
     E e[8];
 #pragma unroll
@@ -59,15 +68,16 @@ __device__ __forceinline__ void widen(const Raw<DT>& r, float* f) {
   __builtin_memcpy(raw, r.w, sizeof(r.w));
   widen8<DT>(raw, f);
 }
+template <bool TAIL>
 __device__ __forceinline__ void fetch_any(int type, const void* base, int64_t at, int n, float* f) {
   if (type == SGL_F32)
-    widen<SGL_F32>(fetch<SGL_F32>(base, at, n), f);
+    widen<SGL_F32>(fetch<SGL_F32, TAIL>(base, at, n), f);
   else if (type == SGL_BF16)
-    widen<SGL_BF16>(fetch<SGL_BF16>(base, at, n), f);
+    widen<SGL_BF16>(fetch<SGL_BF16, TAIL>(base, at, n), f);
   else
-    widen<SGL_F16>(fetch<SGL_F16>(base, at, n), f);
+    widen<SGL_F16>(fetch<SGL_F16, TAIL>(base, at, n), f);
 }
-template <int DT>
+template <int DT, bool TAIL>
 __device__ __forceinline__ void put(void* base, int64_t at, int n, const float* f) {
   typedef std::conditional_t<DT == SGL_F32, uint32_t, uint16_t> E;
   E* p = (E*)base + at;
@@ -77,9 +87,9 @@ __device__ __forceinline__ void put(void* base, int64_t at, int n, const float* 
     for (int i = 0; i < 8; ++i) r.w[i] = f32_bits(f[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.w[i] = pack2<DT>(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) r.w[i] = DT == SGL_BF16 ? pk2_bf16(f[2 * i], f[2 * i + 1]) : pack2<DT>(f[2 * i], f[2 * i + 1]);
   }
-  if (__builtin_expect(n == 8, 1)) {
+  if (!TAIL || __builtin_expect(n == 8, 1)) {
     __builtin_memcpy(p, r.w, sizeof(r.w));
   } else {
     E e[8];
@@ -90,120 +100,139 @@ __device__ __forceinline__ void put(void* base, int64_t at, int n, const float* 
   }
 }
 
-// Sum over a wavefront by DPP moves, the same in every lane.
+// Sums by DPP moves: of 16 lanes in the last of them, then of a wavefront, the same in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float x) {
+  return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), lane));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  v += moved<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  return v;
+}
 __device__ __forceinline__ float wave_sum(float v) {
-  auto move = [](float x, auto ctrl, auto rows) {
-    return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), decltype(ctrl)::value,
-                                                          decltype(rows)::value, 0xF, false));
-  };
-  typedef std::integral_constant<int, 0xF> all;
-  v += move(v, std::integral_constant<int, 0x111>{}, all{});  // row_shr 1, 2, 4, 8
-  v += move(v, std::integral_constant<int, 0x112>{}, all{});
-  v += move(v, std::integral_constant<int, 0x114>{}, all{});
-  v += move(v, std::integral_constant<int, 0x118>{}, all{});
-  v += move(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast 15
-  v += move(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast 31
-  return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), 63));
+  v = row_sum(v);
+  v += moved<0x142, 0xA>(v);  // row_bcast 15
+  v += moved<0x143, 0xC>(v);  // row_bcast 31
+  return lane_of(v, 63);
 }
 
-// DT: type of x and y; RT: of the residual stream; IT: units of a thread.  KEEP: the weights and
-// the next row in registers, which 1024 threads (rows above 8192 elements) leave no room for.
-template <int DT, int RT, int IT, bool KEEP, bool QUANT>
-__global__ __launch_bounds__(KEEP ? 256 * IT : 1024) void norm_kernel(const NormArgs a) {
+// DT: type of x and y; RT: of the residual stream; IT: units of a thread.  KEEP: the weights in
+// registers and the next row's loads in flight, which two units leave no room for.  ONCE: the rows do
+// not fit the last-level cache, and pass it by.  TAIL: H is no multiple of 8.  Without it no load
+// stands under a branch, or the waits for one would be waits for the next row's loads too:
+// threads behind the row's end load its first unit, and a last row again.
+template <int DT, int RT, int IT, bool ONCE, bool TAIL, bool QUANT>
+__global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
+  constexpr bool KEEP = IT == 1;
   __shared__ float part[4][16];
   const int waves = (int)(blockDim.x >> 6), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int at[IT], n[IT];
-  float before[KEEP ? IT : 1][8], after[KEEP ? IT : 1][8], gate[KEEP ? IT : 1][8];
+  float before[KEEP ? IT : 1][8], factor[KEEP ? IT : 1][8];  // factor: after * gate, a row's gate apart
+  // What u is multiplied by, but for a gate of each element.
+  auto load_factor = [&](int k, float* w) __attribute__((always_inline)) {
+    if (a.after) fetch_any<TAIL>(a.after_type, a.after, at[k], n[k], w);
+    if (a.gate_type >= 0 && !a.gate_rows) {
+      float g[8];
+      fetch_any<TAIL>(a.gate_type, a.gate, at[k], n[k], g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = a.after ? w[i] * g[i] : g[i];
+    }
+  };
+  const bool scaled = a.after || (a.gate_type >= 0 && !a.gate_rows);
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
     const int u = k * (int)blockDim.x + (int)threadIdx.x;
-    at[k] = 8 * u;
     const int left = a.H - 8 * u;
     n[k] = u >= a.units ? 0 : left < 8 ? left : 8;
-    if (!KEEP || n[k] == 0) continue;
-    if (a.before) fetch_any(a.before_type, a.before, at[k], n[k], before[KEEP ? k : 0]);
-    if (a.after) fetch_any(a.after_type, a.after, at[k], n[k], after[KEEP ? k : 0]);
-    if (a.gate_type >= 0 && !a.gate_rows) fetch_any(a.gate_type, a.gate, at[k], n[k], gate[KEEP ? k : 0]);
+    at[k] = n[k] ? 8 * u : 0;
+    if (!KEEP) continue;
+    if (a.before) fetch_any<TAIL>(a.before_type, a.before, at[k], n[k], before[k]);
+    load_factor(k, factor[k]);
   }
-  auto sum_over_row = [&](float v, int slot) {
+  int slot = 0;
+  auto sum_over_row = [&](float v) {
     v = wave_sum(v);
     if (waves == 1) return v;
     if ((threadIdx.x & 63) == 0) part[slot][wave] = v;
-    __syncthreads();  // (four slots in turn: nobody writes one that another still reads)
-    float s = 0.0f;
-    for (int i = 0; i < waves; ++i) s += part[slot][i];
-    return s;
+    // (no wait for memory; four slots in turn: nobody writes one that another still reads)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int i = (int)(threadIdx.x & 15);
+    const float s = part[slot][i];
+    slot = (slot + 1) & 3;
+    return lane_of(row_sum(i < waves ? s : 0.0f), 15);
   };
   Raw<DT> x[IT];
   Raw<RT> r[IT];
   auto load = [&](int64_t t) __attribute__((always_inline)) {
+    t = t < a.T ? t : a.T - 1;
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      if (n[k] == 0) continue;
-      x[k] = fetch<DT>(a.x, t * a.xs + at[k], n[k]);
-      r[k] = fetch<RT>(a.res, t * a.rs + at[k], n[k]);
+      x[k] = fetch<DT, TAIL, ONCE>(a.x, t * a.xs + at[k], n[k]);
+      r[k] = fetch<RT, TAIL, ONCE>(a.res, t * a.rs + at[k], n[k]);
     }
   };
-  int slot = 0;
-  if (KEEP && (int64_t)blockIdx.x < a.T) load(blockIdx.x);
+  if (KEEP) load(blockIdx.x);
   for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
     float u[IT][8], h[IT][8];
     if (!KEEP) load(t);
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      if (n[k] == 0) continue;
       widen<DT>(x[k], u[k]);
       widen<RT>(r[k], h[k]);
-      if (KEEP && a.gate_rows) fetch_any(a.gate_type, a.gate, t * a.gs + at[k], n[k], gate[k]);
     }
-    if (KEEP && t + gridDim.x < a.T) load(t + gridDim.x);
+    if (KEEP) load(t + gridDim.x);
+    float f = a.alpha;
     if (a.after) {
       float s = 0.0f;
 #pragma unroll
-      for (int k = 0; k < IT; ++k)
-        if (n[k])
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s = __builtin_fmaf(u[k][i], u[k][i], s);
-      const float f = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum_over_row(s, slot), a.inv_h, a.eps));
-      slot = (slot + 1) & 3;
-#pragma unroll
       for (int k = 0; k < IT; ++k) {
-        if (n[k] == 0) continue;
-        float* w = after[KEEP ? k : 0];
-        if (!KEEP) fetch_any(a.after_type, a.after, at[k], n[k], w);
+        float q = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[k][i] = u[k][i] * f * w[i];
+        for (int i = 0; i < 8; ++i) q = __builtin_fmaf(u[k][i], u[k][i], q);
+        s += n[k] ? q : 0.0f;
       }
+      f *= 1.0f / __builtin_sqrtf(__builtin_fmaf(sum_over_row(s), a.inv_h, a.eps));
     }
     float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      if (n[k] == 0) continue;
-      float* w = gate[KEEP ? k : 0];
-      if (!KEEP && a.gate_type >= 0) fetch_any(a.gate_type, a.gate, (a.gate_rows ? t * a.gs : 0) + at[k], n[k], w);
+      if (a.gate_rows) {
+        float g[8];
+        fetch_any<TAIL>(a.gate_type, a.gate, t * a.gs + at[k], n[k], g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (a.gate_type >= 0) u[k][i] *= w[i];
-        h[k][i] = __builtin_fmaf(a.alpha, u[k][i], h[k][i]);
+        for (int i = 0; i < 8; ++i) u[k][i] *= g[i];
       }
-      put<RT>(a.h, t * a.hs + at[k], n[k], h[k]);
+      if (scaled) {
+        float* w = factor[KEEP ? k : 0];
+        if (!KEEP) load_factor(k, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n[k]) s = __builtin_fmaf(h[k][i], h[k][i], s);
+        for (int i = 0; i < 8; ++i) u[k][i] *= w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[k][i] = __builtin_fmaf(f, u[k][i], h[k][i]);
+      if (n[k]) put<RT, TAIL>(a.h, t * a.hs + at[k], n[k], h[k]);
+      float q = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q = !TAIL || i < n[k] ? __builtin_fmaf(h[k][i], h[k][i], q) : q;
+      s += n[k] ? q : 0.0f;
     }
     if (!a.before) continue;
-    const float f = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum_over_row(s, slot), a.inv_h, a.eps));
-    slot = (slot + 1) & 3;
+    f = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum_over_row(s), a.inv_h, a.eps));
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      if (n[k] == 0) continue;
-      float y[8];
       float* w = before[KEEP ? k : 0];
-      if (!KEEP) fetch_any(a.before_type, a.before, at[k], n[k], w);
+      if (!KEEP) fetch_any<TAIL>(a.before_type, a.before, at[k], n[k], w);
+      float y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = h[k][i] * f * w[i];
       if constexpr (!QUANT) {
-        put<DT>(a.y, t * a.H + at[k], n[k], y);
+        if (n[k]) put<DT, TAIL>(a.y, t * a.H + at[k], n[k], y);
       } else {
         // a group is 4, 8 or 16 neighbouring lanes, all of them on the row or none
         float most = 0.0f;
@@ -214,7 +243,12 @@ __global__ __launch_bounds__(KEEP ? 256 * IT : 1024) void norm_kernel(const Norm
         uint2 q;
         auto code = [&](auto mode) __attribute__((always_inline)) {
           sf = group_scale(decltype(mode)::value, most);
-          q = quant8_e4m3(decltype(mode)::value, y, sf);
+          float v[8];
+          quant_scale<8>(decltype(mode)::value, y, sf, v);
+          if (__builtin_expect(most < __builtin_huge_valf(), 1))  // (a NaN's sign is the conversion's own)
+            q = make_uint2(pk4_e4m3(v[0], v[1], v[2], v[3]), pk4_e4m3(v[4], v[5], v[6], v[7]));
+          else
+            q = make_uint2(pk4_e4m3_exact(v[0], v[1], v[2], v[3]), pk4_e4m3_exact(v[4], v[5], v[6], v[7]));
         };
         if (a.mode == SCALE_TORCH_FP32)
           code(std::integral_constant<int, SCALE_TORCH_FP32>{});
@@ -224,36 +258,46 @@ __global__ __launch_bounds__(KEEP ? 256 * IT : 1024) void norm_kernel(const Norm
           code(std::integral_constant<int, SCALE_TILELANG_FP32>{});
         else
           code(std::integral_constant<int, SCALE_TILELANG_UE8M0>{});
-        *reinterpret_cast<uint2*>((uint8_t*)a.y + t * a.H + at[k]) = q;
-        if (at[k] % a.group == 0) {
-          const int64_t g = t * (a.H / a.group) + at[k] / a.group;
-          if (a.e8m0)
-            ((uint8_t*)a.scales)[g] = pow2_to_e8m0(sf);
-          else
-            ((float*)a.scales)[g] = sf;
+        if (n[k]) {
+          *reinterpret_cast<uint2*>((uint8_t*)a.y + t * a.H + at[k]) = q;
+          if (at[k] % a.group == 0) {
+            const int64_t g = t * (a.H / a.group) + at[k] / a.group;
+            if (a.e8m0)
+              ((uint8_t*)a.scales)[g] = pow2_to_e8m0(sf);
+            else
+              ((float*)a.scales)[g] = sf;
+          }
         }
       }
     }
   }
 }
 
-template <int DT, int RT, int IT, bool KEEP>
+template <int DT, int RT, int IT, bool ONCE>
 void launch_norm(const NormArgs& a, const NormPlan& p, bool quant, hipStream_t st) {
-  if (quant)
-    norm_kernel<DT, RT, IT, KEEP, true><<<(unsigned)p.grid, (unsigned)p.threads, 0, st>>>(a);
+  const dim3 grid((unsigned)p.grid), threads((unsigned)p.threads);
+  if (quant)  // (groups of 32 at least: no tail)
+    norm_kernel<DT, RT, IT, ONCE, false, true><<<grid, threads, 0, st>>>(a);
+  else if (a.H % 8 == 0)
+    norm_kernel<DT, RT, IT, ONCE, false, false><<<grid, threads, 0, st>>>(a);
   else
-    norm_kernel<DT, RT, IT, KEEP, false><<<(unsigned)p.grid, (unsigned)p.threads, 0, st>>>(a);
+    norm_kernel<DT, RT, IT, ONCE, true, false><<<grid, threads, 0, st>>>(a);
 }
 
 template <int DT, int RT>
 void launch_norm_as(const NormArgs& a, bool quant, hipStream_t st) {
   const NormPlan p = norm_plan(a.T, a.units, device_cu_count());
-  if (p.units == 1)
-    launch_norm<DT, RT, 1, true>(a, p, quant, st);
-  else if (p.threads <= 512)
-    launch_norm<DT, RT, 2, true>(a, p, quant, st);
-  else
+  if (p.units == 1) {
+    if constexpr (RT != SGL_F32) {
+      if (norm_once(a.T, a.H)) {
+        launch_norm<DT, RT, 1, true>(a, p, quant, st);
+        return;
+      }
+    }
+    launch_norm<DT, RT, 1, false>(a, p, quant, st);
+  } else {
     launch_norm<DT, RT, 2, false>(a, p, quant, st);
+  }
 }
 
 }  // namespace

@@ -250,16 +250,20 @@ SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cu
 
 // ---- norms between blocks: threads of a row's workgroup, units of 8 elements a
 // thread, and workgroups.
+#ifndef NORM_ONCE
+#define NORM_ONCE 128
+#endif
 constexpr int64_t kNormMost = 16384;  // elements of a row: 1024 threads of two units
 struct NormPlan {
   int64_t threads, units, grid;
 };
 SGL_RULE NormPlan norm_plan(int64_t T, int64_t row_units, int64_t cus) {
-  const int64_t units = row_units <= 256 ? 1 : 2;
+  const int64_t units = row_units <= 1024 ? 1 : 2;
   const int64_t threads = ((row_units + units - 1) / units + 63) / 64 * 64;
-  const int64_t most = cus * (1024 / threads < 1 ? 1 : 1024 / threads);
+  const int64_t most = cus * (1536 / threads);
   return {threads, units, T < most ? T : most};
 }
+SGL_RULE bool norm_once(int64_t T, int64_t H) { return 4 * T * H > ((int64_t)NORM_ONCE << 20); }
 
 // ---- append to the 8-bit cache: the most blocks that T tokens of B sequences
 // touch.  n tokens touch at most (n - 2) / block + 2, and no more than n.

@@ -23,9 +23,7 @@ from .rotary import DTYPES
 MAX_DIM = 16384
 
 
-def _weight(w: Optional[torch.Tensor], H: int, name: str) -> Optional[int]:
-    if w is None:
-        return 0
+def _weight(w: torch.Tensor, H: int, name: str) -> int:
     dt = DTYPES.get(w.dtype)
     if dt is None:
         raise TypeError(f"residual_norm: {name} must be bfloat16, float16 or float32, got {w.dtype}")
@@ -34,10 +32,16 @@ def _weight(w: Optional[torch.Tensor], H: int, name: str) -> Optional[int]:
     return dt
 
 
-def _rows(t: torch.Tensor, H: int) -> torch.Tensor:
-    """``t`` as rows of ``H`` elements, each dense (a copy where its strides do not allow it)."""
-    t = t if t.dim() == 2 else t.reshape(-1, H)
-    return t if t.stride(1) == 1 or H == 1 else t.contiguous()
+def _rows(t: torch.Tensor, H: int):
+    """``t`` as rows of ``H`` elements, each dense (a copy where its strides do not allow it), and
+    the elements between them."""
+    if t.dim() != 2:
+        t = t.reshape(-1, H)
+    s = t.stride()
+    if s[1] != 1 and H > 1:
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[0]
 
 
 def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torch.Tensor] = None, *,
@@ -74,25 +78,27 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torc
     rdt = DTYPES.get(residual.dtype)
     if rdt is None or (rdt != dt and rdt != _lib.SGL_F32):
         raise TypeError(f"residual_norm: residual must be {x.dtype} or float32, got {residual.dtype}")
-    bdt, adt = _weight(before, H, "before"), _weight(after, H, "after")
-    gdt = gs = 0
-    gate_rows = False
+    bdt = adt = gdt = gs = mode = 0
+    if before is not None:
+        bdt = _weight(before, H, "before")
+    if after is not None:
+        adt = _weight(after, H, "after")
     if gate is not None:
         gdt = DTYPES.get(gate.dtype)
         if gdt is None:
             raise TypeError(f"residual_norm: gate must be bfloat16, float16 or float32, got {gate.dtype}")
-    mode = 0
     if quant:
         if before is None:
             raise ValueError("residual_norm: codes are of the norm before the next block, which is missing")
         if block_size not in (32, 64, 128) or H % block_size:
             raise ValueError(f"residual_norm: block_size must be 32, 64 or 128 and divide {H}, got {block_size}")
-        if scale_dtype not in (torch.float32, E8M0):
+        if scale_dtype is not torch.float32 and scale_dtype is not E8M0:
             raise TypeError(f"residual_norm: scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
         mode = scale_mode_for(scale_fmt)
         if scale_dtype is E8M0 and scale_fmt is None:
             raise ValueError("residual_norm: float8_e8m0fnu scales need a scale_fmt (powers of two)")
     d = _lib.device_of("residual_norm", x, residual, before, after, gate)
+    gate_rows = False
     if gate is not None:
         if gate.shape == (H,):
             gate = gate if gate.is_contiguous() else gate.contiguous()
@@ -104,36 +110,36 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torc
                     raise ValueError(f"residual_norm: a gate {tuple(gate.shape)} does not broadcast to "
                                      f"{tuple(shape)}") from e
             gate_rows = True
-            gate = _rows(gate, H)
-            gs = gate.stride(0)
-    xr = _rows(x, H)
+            gate, gs = _rows(gate, H)
+    xr, xs = _rows(x, H)
     T = xr.shape[0]
     if inplace:
         try:
             rr = h = residual.view(-1, H)
         except RuntimeError as e:
             raise ValueError("residual_norm: inplace needs a residual whose rows lie at one stride") from e
-        if (H > 1 and rr.stride(1) != 1) or (T > 1 and rr.stride(0) < H):
+        rs = hs = rr.stride(0)
+        if (H > 1 and rr.stride(1) != 1) or (T > 1 and rs < H):
             raise ValueError("residual_norm: inplace needs dense rows that do not overlap")
         _check_apart(xr, rr, "x")
         if gate_rows:
             _check_apart(gate, rr, "the gate")
         out = residual
     else:
-        rr = _rows(residual, H)
-        out = torch.empty(shape, dtype=residual.dtype, device=x.device)
-        h = out
+        rr, rs = _rows(residual, H)
+        out = h = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        hs = H
     y = scales = None
     if quant:
-        y = torch.empty(shape, dtype=FP8, device=x.device)
-        scales = torch.empty((*shape[:-1], H // block_size), dtype=scale_dtype, device=x.device)
+        y = torch.empty_like(x, dtype=FP8, memory_format=torch.contiguous_format)
+        scales = x.new_empty((*shape[:-1], H // block_size), dtype=scale_dtype)
     elif before is not None:
-        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if T:
-        _lib.call_on(d, "sgl_residual_norm", xr.data_ptr(), dt, T, H, xr.stride(0), rr.data_ptr(), rdt, rr.stride(0),
+        _lib.call_on(d, "sgl_residual_norm", xr.data_ptr(), dt, T, H, xs, rr.data_ptr(), rdt, rs,
                      _lib.ptr(after), adt, _lib.ptr(gate), gdt, gate_rows, gs, scale, _lib.ptr(before), bdt, eps,
-                     h.data_ptr(), rr.stride(0) if inplace else H, _lib.ptr(y), quant, _lib.ptr(scales), block_size,
-                     mode, quant and scale_dtype is E8M0)
+                     h.data_ptr(), hs, _lib.ptr(y), quant, _lib.ptr(scales), block_size, mode,
+                     quant and scale_dtype is E8M0)
     return out, (y, scales) if quant else y
 
 

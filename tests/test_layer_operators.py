@@ -122,5 +122,5 @@ def test_norm_plan(tmp_path):
             lib.plan(T, units, 256, o)
             threads, per, grid = o
             assert threads % 64 == 0 and 64 <= threads <= 1024 and threads * per >= units
-            assert threads <= 256 * per or (per == 2 and threads <= 1024)
+            assert per == (1 if units <= 1024 else 2)
             assert 1 <= grid <= T
