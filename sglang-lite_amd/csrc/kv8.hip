@@ -110,6 +110,80 @@ __device__ __forceinline__ uint32_t codes4(uint32_t ab, uint32_t cd, float s) {
   return __builtin_bit_cast(uint32_t, o);
 }
 
+// cos and sin of a thread's 8 pairs from `pair` on, of several axes.  Where one axis holds
+// all 8 they lie side by side.  Where it does not, they are up to 8 pieces of 8 bytes in as many
+// rows, and the wavefront takes them in the order of the pairs instead: the threads leave their
+// entries' places in LDS, load what stands at 64 neighbouring ones at a time and leave that there.
+// (8000 tokens of 8 heads of 128, the axes in turn: 25 us by themselves.)
+template <int NT>
+__device__ __forceinline__ void turns_of(const AppendArgs& a, const AxisPositions& at, const uint8_t* axis, int pair,
+                                         float* cos, float* sin) {
+  __shared__ __align__(16) float2 sTurn[NT / 64][512];
+  const int lane = threadIdx.x & 63, n = (int)a.n_positions, pairs = a.rot >> 1;
+  bool same = true;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) same = same & (axis[i] == axis[0]);
+  auto place = [&](int x) { return x == 0 ? at.p[0] : x == 1 ? at.p[1] : x == 2 ? at.p[2] : x == 3 ? at.p[3] : n; };
+  if (__ballot(at.turn && !same) == 0) {
+    if (at.turn) load_turn<8>(a.table, n, pairs, place(axis[0]), pair, false, cos, sin);
+    return;
+  }
+  float2* turns = sTurn[threadIdx.x >> 6];
+  int* entries = reinterpret_cast<int*>(turns);
+  auto fence = [] {  // (a wavefront's LDS accesses go in order: nothing to wait for but the compiler)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  int e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int p = place(axis[i]);
+    e[i] = at.turn && p < n ? p * pairs + pair + i : -1;
+  }
+  fence();
+  *reinterpret_cast<int4*>(entries + 8 * lane) = make_int4(e[0], e[1], e[2], e[3]);
+  *reinterpret_cast<int4*>(entries + 8 * lane + 4) = make_int4(e[4], e[5], e[6], e[7]);
+  fence();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = entries[64 * i + lane];
+  float2 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const float2*>(a.table)[e[i] < 0 ? 0 : e[i]];
+  fence();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) turns[64 * i + lane] = e[i] < 0 ? make_float2(__builtin_nanf(""), __builtin_nanf("")) : w[i];
+  fence();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 q = *reinterpret_cast<const float4*>(turns + 8 * lane + 2 * i);
+    cos[2 * i] = q.x;
+    sin[2 * i] = q.y;
+    cos[2 * i + 1] = q.z;
+    sin[2 * i + 1] = q.w;
+  }
+}
+
+// The two chunks of 8 elements of unit u of a row: those of 8 pairs, or two of the others.
+__device__ __forceinline__ void unit_chunks(const AppendArgs& a, int rot, int u, int* p0, int* p1) {
+  if (u < rot >> 4) {
+    *p0 = a.offset + (a.interleaved ? 16 : 8) * u;
+    *p1 = *p0 + (a.interleaved ? 8 : rot >> 1);
+  } else {
+    const int c = 16 * (u - (rot >> 4)), off = rot ? a.offset : 0;
+    *p0 = c < off ? c : c + rot;
+    *p1 = c + 8 < off ? c + 8 : c + 8 + rot;
+  }
+}
+template <int DT>
+__device__ __forceinline__ void load_rows(const AppendArgs& a, const Unit& w, const void* src, int64_t st, int64_t sh,
+                                          int head, int rot, int t, int u, uint4* raw) {
+  int p0, p1;
+  unit_chunks(a, rot, u, &p0, &p1);
+  const int64_t at = (int64_t)(w.row0 + t) * st + (int64_t)head * sh;
+  load_raw8<DT>(src, at + p0, raw);
+  load_raw8<DT>(src, at + p1, raw + (DT == SGL_F32 ? 2 : 1));
+}
+
 // NT threads, IT units of 16 elements a thread
 template <int DT, int NT, int IT, bool AXES>
 __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
@@ -136,21 +210,33 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
     const int i = it * NT + (int)threadIdx.x;
     tok[it] = -1;
     odd[it] = false;
-    if (i < count) {
-      const int t = i * a.per_magic >> 16, u = i - t * per;
-      int p0, p1;  // two chunks of 8 elements: those of 8 pairs, or two of the others
-      if (u < rot_units) {
-        p0 = a.offset + (a.interleaved ? 16 : 8) * u;
-        p1 = p0 + (a.interleaved ? 8 : rot >> 1);
-      } else {
-        const int c = 16 * (u - rot_units), off = rot ? a.offset : 0;
-        p0 = c < off ? c : c + rot;
-        p1 = c + 8 < off ? c + 8 : c + 8 + rot;
+    const int t = i * a.per_magic >> 16, u = i - t * per;
+    uint4 raw[2 * RW];
+    float cs[8], sn[8];
+    AxisPositions place;
+    if constexpr (AXES) {
+      // before the rows: loads return in order, and the table's wait for these
+      const bool mine = i < count && u < rot_units;
+      uint8_t axis[8];
+      place.turn = false;
+      if (rot_units > 0) {
+        __builtin_memcpy(axis, a.axes + (mine ? 8 * u : 0), 8);
+        place = load_axis_positions<false>(a.positions, a.n_axes, a.T, w.row0 + (mine ? t : 0), (int)a.n_positions);
+        place.turn = place.turn && mine;
       }
-      const int64_t at = (int64_t)(w.row0 + t) * st + (int64_t)head * sh;
-      uint4 raw[2 * RW];
-      load_raw8<DT>(src, at + p0, raw);
-      load_raw8<DT>(src, at + p1, raw + RW);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i < count) load_rows<DT>(a, w, src, st, sh, head, rot, t, u, raw);
+      // (all threads of the wavefront, those without a row too)
+      if (rot_units > 0) turns_of<NT>(a, place, axis, mine ? 8 * u : 0, cs, sn);
+    }
+    if (i < count) {
+      int p0, p1;
+      unit_chunks(a, rot, u, &p0, &p1);
+      if constexpr (!AXES) {
+        const int64_t at = (int64_t)(w.row0 + t) * st + (int64_t)head * sh;
+        load_raw8<DT>(src, at + p0, raw);
+        load_raw8<DT>(src, at + p1, raw + RW);
+      }
       tok[it] = t;
       e0[it] = p0;
       e1[it] = p1;
@@ -172,15 +258,9 @@ __global__ __launch_bounds__(NT) void append_kernel(const AppendArgs a) {
       } else {
         widen8<DT>(raw, x);
         widen8<DT>(raw + RW, x + 8);
-        float cs[8], sn[8];
         bool turn = u < rot_units;
         if constexpr (AXES) {
-          if (turn) {
-            const AxisPositions at =
-                load_axis_positions<false>(a.positions, a.n_axes, a.T, w.row0 + t, (int)a.n_positions);
-            turn = at.turn;
-            if (turn) load_turn_axes<8>(a.table, (int)a.n_positions, a.rot >> 1, at, a.axes, 8 * u, false, cs, sn);
-          }
+          turn = place.turn;
         } else {
           const int64_t pos = !turn ? -1 : a.positions ? a.positions[w.row0 + t] : w.at + t;
           turn = pos >= 0;
@@ -349,7 +429,8 @@ int append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const v
   }
   if (AXES) {
     SGL_REQUIRE(n_axes >= 1 && n_axes <= kMaxAxes, "kv8_append: n_axes=%d must be 1 to %d", n_axes, kMaxAxes);
-    SGL_REQUIRE(n_positions <= 0x7FFFFFFF, "kv8_append: n_positions=%lld out of range", (long long)n_positions);
+    SGL_REQUIRE(n_positions <= 0x7FFFFFFF && n_positions * (rot_dim / 2) <= 0x7FFFFFFF,
+                "kv8_append: a table of %lld positions is too large", (long long)n_positions);
   }
   if (T == 0 || B == 0) return SGL_OK;
   SGL_REQUIRE(k && v && start && block_table && k_codes && v_codes && k_scale && v_scale,

@@ -43,12 +43,21 @@ struct RotaryArgs {
 
 constexpr int kHeads = 4;  // heads of a thread in flight
 
-template <int DT, int VEC, bool AXES>
+// STAGE (several axes, 16-byte accesses): the rotations of the wavefront's tokens go through LDS.
+// A pair's table entry lies in its axis' row, so a thread's 8 are up to 8 pieces of 8 bytes, and
+// all threads of a token load the same ones: by themselves 16384 tokens of 32 heads of 128
+// take 71 us.
+// AXES: 0, or several with positions of 32 or 64 bits.
+template <int DT, int VEC, int AXES>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
+  constexpr bool STAGE = AXES != 0 && VEC == 8, POS64 = AXES == 64;
+  extern __shared__ __align__(16) float2 sAll[];  // of each wavefront [tokens][pairs]
   const uint32_t per = (uint32_t)(a.units * a.hsplit);
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t t = i / per;
-  if (t >= a.T) return;
+  const int64_t first = i - (threadIdx.x & 63), t0 = STAGE ? first / per : 0;  // of the wavefront
+  if (STAGE ? t0 >= a.T : t >= a.T) return;
+  const bool there = t < a.T;
   const uint32_t j = (uint32_t)(i - t * per);
   const int hs = (int)(j / (uint32_t)a.units), u = (int)(j - (uint32_t)hs * a.units);
   const int rot_units = a.rot / (2 * VEC);
@@ -62,19 +71,6 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     e0 = c < a.offset ? c : c + a.rot;
     e1 = c + VEC < a.offset ? c + VEC : c + VEC + a.rot;
     two = c + VEC < rest;
-  }
-  float cs[VEC], sn[VEC];
-  bool turn = false;
-  if (AXES && u < rot_units) {
-    const AxisPositions at = a.pos64 ? load_axis_positions<true>(a.positions, a.n_axes, a.T, t, (int)a.n_positions)
-                                     : load_axis_positions<false>(a.positions, a.n_axes, a.T, t, (int)a.n_positions);
-    turn = at.turn;
-    if (turn)
-      load_turn_axes<VEC>(a.table, (int)a.n_positions, a.rot / 2, at, a.axes, VEC * u, a.inverse, cs, sn);
-  } else if (u < rot_units) {
-    const int64_t p = a.pos64 ? ((const int64_t*)a.positions)[t] : ((const int32_t*)a.positions)[t];
-    turn = p >= 0;
-    if (turn) load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, VEC * u, a.inverse, cs, sn);
   }
   auto load = [&](int64_t at, float* f) {
     if constexpr (VEC == 8) {
@@ -95,14 +91,86 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
       ((uint16_t*)a.out)[at] = (uint16_t)pack2<DT>(f[0], 0.0f);
     }
   };
-  for (int h0 = hs; h0 < a.H; h0 += kHeads * a.hsplit) {
-    float x[kHeads][2][VEC];
+  constexpr int RW = DT == SGL_F32 ? 2 : 1;
+  uint4 raw[STAGE ? kHeads : 1][2][RW];  // as they lie, so that nothing waits for them yet
+  auto load_heads = [&](int h0) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < kHeads; ++k) {
       const int h = h0 + k * a.hsplit;
       if (h < a.H) {
-        load(t * a.xt + h * a.xh + e0, x[k][0]);
-        if (two) load(t * a.xt + h * a.xh + e1, x[k][1]);
+        load_raw8<DT>(a.x, t * a.xt + h * a.xh + e0, raw[k][0]);
+        if (two) load_raw8<DT>(a.x, t * a.xt + h * a.xh + e1, raw[k][1]);
+      }
+    }
+  };
+  float cs[VEC], sn[VEC];
+  bool turn = false;
+  if constexpr (STAGE) {
+    const int pairs = a.rot / 2;
+    float2* sTurn = sAll + (threadIdx.x >> 6) * (64 / per + 2) * pairs;
+    int64_t t1 = (first + 63) / per + 1;
+    t1 = t1 < a.T ? t1 : a.T;
+    const int count = (int)(t1 - t0) * pairs;
+    auto fetch = [&](int e) __attribute__((always_inline)) {
+      const int tok = e / pairs, pair = e - tok * pairs, axis = a.axes[pair];
+      const AxisPositions at = load_axis_positions<POS64>(a.positions, a.n_axes, a.T, t0 + tok, (int)a.n_positions);
+      const int p = axis == 0 ? at.p[0] : axis == 1 ? at.p[1] : axis == 2 ? at.p[2] : axis == 3 ? at.p[3] : (int)a.n_positions;
+      const bool in = p >= 0 && p < a.n_positions;  // (a token with a negative one is not turned)
+      const float2 w = reinterpret_cast<const float2*>(a.table)[(int64_t)(in ? p : 0) * pairs + pair];
+      return make_float2(in ? w.x : __builtin_nanf(""), in ? (a.inverse ? -w.y : w.y) : __builtin_nanf(""));
+    };
+    // Loads return in order: first the chain to the table, then the rows, and only then is anything
+    // waited for.
+    const int e0s = (int)(threadIdx.x & 63);
+    const AxisPositions mine = load_axis_positions<POS64>(a.positions, a.n_axes, a.T, there ? t : 0, (int)a.n_positions);
+    const float2 w = fetch(e0s < count ? e0s : 0);
+    if (there) load_heads(hs);
+    __builtin_amdgcn_sched_barrier(0);
+    turn = u < rot_units && mine.turn;
+    if (e0s < count) sTurn[e0s] = w;
+    for (int e = e0s + 64; e < count; e += 64) sTurn[e] = fetch(e);
+    // (a wavefront's LDS accesses go in order: nothing to wait for but the compiler)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (!there) return;
+    if (turn) {
+      const float4* row = reinterpret_cast<const float4*>(sTurn + (t - t0) * pairs + VEC * u);
+#pragma unroll
+      for (int v = 0; v < VEC / 2; ++v) {
+        const float4 w = row[v];
+        cs[2 * v] = w.x;
+        sn[2 * v] = w.y;
+        cs[2 * v + 1] = w.z;
+        sn[2 * v + 1] = w.w;
+      }
+    }
+  } else if (AXES != 0 && u < rot_units) {
+    const AxisPositions at = load_axis_positions<POS64>(a.positions, a.n_axes, a.T, t, (int)a.n_positions);
+    turn = at.turn;
+    uint8_t axis[VEC];
+    __builtin_memcpy(axis, a.axes + VEC * u, VEC);
+    if (turn) load_turn_axes<VEC>(a.table, (int)a.n_positions, a.rot / 2, at, axis, VEC * u, a.inverse, cs, sn);
+  } else if (u < rot_units) {
+    const int64_t p = a.pos64 ? ((const int64_t*)a.positions)[t] : ((const int32_t*)a.positions)[t];
+    turn = p >= 0;
+    if (turn) load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, VEC * u, a.inverse, cs, sn);
+  }
+  for (int h0 = hs; h0 < a.H; h0 += kHeads * a.hsplit) {
+    float x[kHeads][2][VEC];
+    if constexpr (STAGE) {
+      if (h0 > hs) load_heads(h0);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+      const int h = h0 + k * a.hsplit;
+      if (h < a.H) {
+        if constexpr (STAGE) {
+          widen8<DT>(raw[k][0], x[k][0]);
+          if (two) widen8<DT>(raw[k][1], x[k][1]);
+        } else {
+          load(t * a.xt + h * a.xh + e0, x[k][0]);
+          if (two) load(t * a.xt + h * a.xh + e1, x[k][1]);
+        }
       }
     }
 #pragma unroll
@@ -134,14 +202,26 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   }
 }
 
-template <int DT, bool AXES>
+template <int DT, int AXES>
 void launch_rotary(const RotaryArgs& a, bool vec, hipStream_t st) {
   const int64_t threads = (int64_t)a.T * a.units * a.hsplit;
   const dim3 grid((unsigned)ceil_div(threads, 256));
+  // (a token has a thread at least for each 16 rotated elements: 4 (4096 + 8 rot) bytes at most)
+  const size_t lds = AXES ? 4 * (size_t)(64 / ((int64_t)a.units * a.hsplit) + 2) * (a.rot / 2) * sizeof(float2) : 0;
   if (vec)
-    rotary_kernel<DT, 8, AXES><<<grid, 256, 0, st>>>(a);
+    rotary_kernel<DT, 8, AXES><<<grid, 256, lds, st>>>(a);
   else
     rotary_kernel<DT, 1, AXES><<<grid, 256, 0, st>>>(a);
+}
+
+template <int DT, bool AXES>
+void launch_axes(const RotaryArgs& a, bool vec, hipStream_t st) {
+  if constexpr (!AXES)
+    launch_rotary<DT, 0>(a, vec, st);
+  else if (a.pos64)
+    launch_rotary<DT, 64>(a, vec, st);
+  else
+    launch_rotary<DT, 32>(a, vec, st);
 }
 
 template <bool AXES>
@@ -170,7 +250,7 @@ int rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_token_st
   const bool vec = rot_dim % 16 == 0 && offset % 8 == 0 && D % 8 == 0 && aligned(x, 16) &&
                    aligned(out, 16) && aligned(table, 16) && x_token_stride * size % 16 == 0 &&
                    x_head_stride * size % 16 == 0 && out_token_stride * size % 16 == 0 &&
-                   out_head_stride * size % 16 == 0;
+                   out_head_stride * size % 16 == 0 && (!AXES || rot_dim <= 1024);  // (its rotations fit LDS)
   RotaryArgs a;
   a.x = x;
   a.out = out;
@@ -196,11 +276,11 @@ int rotary(const void* x, int dtype, int64_t T, int H, int D, int64_t x_token_st
   a.hsplit = rotary_head_threads(T, H, a.units, device_cu_count());
   SGL_REQUIRE((int64_t)a.T * a.units * a.hsplit <= 256ll * 0x7FFFFFFF, "rotary: too large");
   if (dtype == SGL_BF16)
-    launch_rotary<SGL_BF16, AXES>(a, vec, (hipStream_t)stream);
+    launch_axes<SGL_BF16, AXES>(a, vec, (hipStream_t)stream);
   else if (dtype == SGL_F16)
-    launch_rotary<SGL_F16, AXES>(a, vec, (hipStream_t)stream);
+    launch_axes<SGL_F16, AXES>(a, vec, (hipStream_t)stream);
   else
-    launch_rotary<SGL_F32, AXES>(a, vec, (hipStream_t)stream);
+    launch_axes<SGL_F32, AXES>(a, vec, (hipStream_t)stream);
   return check_launch("rotary");
 }
 

@@ -132,33 +132,37 @@ __device__ __forceinline__ void load_turn(const float* table, int64_t n_position
 
 // A token's positions on up to four axes, and cos and sin of N pairs that turn by one of
 // them each (`axes`: a byte for each pair).  The positions are loaded beside the pairs' axes and
-// chosen in registers, so that the chain to the table is no longer than with one position.
-// Behind the table, and for an axis that there is none of: NaN, as above.  `turn` is false, and
-// nothing is loaded, where any of them is negative.
+// chosen in registers, so that the chain to the table is no longer than with one position; and
+// without branches, so that no load waits for another (an axis too many loads the first again).
+// Behind the table, and for an axis that there is none of: NaN, as above.  `turn` is false
+// where any of them is negative.
 constexpr int kMaxAxes = 4;
 struct AxisPositions {
   int p[kMaxAxes];  // at most n_positions, which is behind the table
   bool turn;
 };
 template <bool POS64>
+__device__ __forceinline__ int64_t load_position(const void* positions, int64_t at) {
+  return POS64 ? ((const int64_t*)positions)[at] : ((const int32_t*)positions)[at];
+}
+template <bool POS64>
 __device__ __forceinline__ AxisPositions load_axis_positions(const void* positions, int n_axes, int64_t T, int64_t t,
                                                              int n_positions) {
   AxisPositions o;
+  int64_t p[kMaxAxes];
+#pragma unroll
+  for (int a = 0; a < kMaxAxes; ++a) p[a] = load_position<POS64>(positions, (a < n_axes ? a : 0) * T + t);
   o.turn = true;
 #pragma unroll
   for (int a = 0; a < kMaxAxes; ++a) {
-    int64_t p = n_positions;
-    if (a < n_axes) p = POS64 ? ((const int64_t*)positions)[a * T + t] : ((const int32_t*)positions)[a * T + t];
-    o.turn = o.turn && p >= 0;
-    o.p[a] = p < n_positions ? (int)p : n_positions;
+    o.turn = o.turn & (p[a] >= 0);
+    o.p[a] = a < n_axes && p[a] < n_positions ? (int)p[a] : n_positions;
   }
   return o;
 }
 template <int N>
 __device__ __forceinline__ void load_turn_axes(const float* table, int n_positions, int pairs, const AxisPositions& at,
-                                               const uint8_t* axes, int pair, bool inverse, float* cos, float* sin) {
-  uint8_t axis[N];
-  __builtin_memcpy(axis, axes + pair, N);
+                                               const uint8_t* axis, int pair, bool inverse, float* cos, float* sin) {
   bool same = true;
 #pragma unroll
   for (int i = 1; i < N; ++i) same = same && axis[i] == axis[0];

@@ -155,6 +155,8 @@ def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, block_table: tor
             if positions is None:
                 raise ValueError("append_kv: axes without positions")
             n_axes = check_axes(axes, rot, positions, T, "append_kv")
+            if n_positions * rot >= 1 << 32:
+                raise ValueError(f"append_kv: a table of {n_positions} positions is too large for axes")
             if positions.dtype is not torch.int32 or not positions.is_contiguous():
                 raise ValueError(f"append_kv: positions must be contiguous int32, got {positions.dtype}")
         elif positions is not None and (positions.dtype is not torch.int32 or positions.shape != (T,)
