@@ -86,8 +86,7 @@ struct Codes {
 
 // DP: head dim rounded up to 64, 128 or 256; NC: 16-row column tiles
 // SPLIT: workgroups share the lines, else a workgroup takes a whole item
-// FIRST: the sequence's first tokens are seen beside the window
-template <int DP, int NC, int QT, bool SPLIT, bool FIRST>
+template <int DP, int NC, int QT, bool SPLIT, int MODE>
 __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
   constexpr int RT = 16 * NC, KI = DP / 64, C = DP / 16, W = C / 4;
   __shared__ __align__(16) float sAcc[kWaves][16][DP + 4];
@@ -97,13 +96,13 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
   const float NEG_INF = -__builtin_huge_valf();
 
   int head, part = 0;
-  Kv8Walk<RT, kTile> walk;
+  Kv8Walk<RT, kTile, MODE> walk;
   Kv8Segment seg;
   if constexpr (SPLIT) {
     kv8_wg_at(a, (int)blockIdx.x, &head, &part);
     if (!walk.start(a, part)) return;
   } else {
-    if (!kv8_item<RT, kTile>(a, (int64_t)blockIdx.x, &head, seg)) return;
+    if (!kv8_item<RT, kTile, MODE>(a, (int64_t)blockIdx.x, &head, seg)) return;
   }
   for (bool more = SPLIT ? walk.next(a, seg) : true; more; more = SPLIT ? walk.next(a, seg) : false) {
     const Kv8Seq& s = seg.s;
@@ -152,10 +151,10 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       for (int j = 0; j < C; ++j) acc[c][j] = v4f{0, 0, 0, 0};
     }
 
-    const int32_t* table = a.pages + (int64_t)(a.table_row ? a.table_row[b] : b) * a.row_pages;
+    const int32_t* table = a.pages + (int64_t)(MODE == kShared && a.table_row ? a.table_row[b] : b) * a.row_pages;
     const int pmask = (1 << a.page_shift) - 1;
     // the wavefront's first token in step i; only the last tile's may lie behind the end
-    auto token = [&](int i) __attribute__((always_inline)) { return s.template tile<FIRST>(t0 + i) * kTile + 32 * wave; };
+    auto token = [&](int i) __attribute__((always_inline)) { return s.template tile<MODE>(t0 + i) * kTile + 32 * wave; };
     const int steps = t1 - t0 - (token(t1 - t0 - 1) < s.len ? 0 : 1);
 
     // Pages and scales of 32 steps at a time: lane l has granule l & 1 of step l >> 1.
@@ -263,7 +262,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
           }
         }
       }
-      const bool plain = tok + 32 <= all_hi && (tok >= all_lo || (FIRST && tok + 32 <= a.first)) && ok == 3;
+      const bool plain = tok + 32 <= all_hi && (tok >= all_lo || (MODE == kFirst && tok + 32 <= a.first)) && ok == 3;
       const uint32_t here = plain ? 3u : (uint32_t)(__ballot(evs != kNoToken) >> l0) & 3u;
       uint32_t seen[NC];  // bit 4 u + i: the row sees token 16 u + 4 g + i
 #pragma unroll
@@ -274,7 +273,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = tok + 16 * (i >> 2) + 4 * g + (i & 3);
-            const bool in = FIRST ? (uint32_t)(key - a.first) >= (uint32_t)(lo[c] > a.first ? lo[c] - a.first : 0) : key >= lo[c];
+            const bool in = MODE == kFirst ? (uint32_t)(key - a.first) >= (uint32_t)(lo[c] > a.first ? lo[c] - a.first : 0) : key >= lo[c];
             if (key < hi[c] && in && key < s.len && ((here >> (i >> 2)) & 1u)) seen[c] |= 1u << i;
           }
         }
@@ -440,15 +439,15 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
           const int row = rt * RT + r, t = row / a.G, h = head * a.G + (row - t * a.G);
           const int64_t at = (int64_t)(s.row0 + t) * (a.Hkv * a.G) + h;
           float4 y0 = make_float4(y[0], y[1], y[2], y[3]), y1 = make_float4(y[4], y[5], y[6], y[7]);
-          if (a.raw) {
+          if (MODE == kShared && a.raw) {
             float4* out = reinterpret_cast<float4*>(a.prior_acc + at * a.D + d);
             out[0] = y0;
             out[1] = y1;
             if (d == 0) *reinterpret_cast<float2*>(a.prior_ml + 2 * at) = make_float2(M, sum);
           } else {
-            const Kv8Join join = kv8_join(a, s, at, h, M, sum);
-            y0 = kv8_joined(a, join, at, d, y0);
-            y1 = kv8_joined(a, join, at, d + 4, y1);
+            const Kv8Join join = kv8_join<MODE>(a, s, at, h, M, sum);
+            y0 = kv8_joined<MODE>(a, join, at, d, y0);
+            y1 = kv8_joined<MODE>(a, join, at, d + 4, y1);
             *reinterpret_cast<uint4*>(a.o + at * a.D + d) =
                 make_uint4(kv8_out2<QT>(y0.x, y0.y), kv8_out2<QT>(y0.z, y0.w), kv8_out2<QT>(y1.x, y1.y),
                            kv8_out2<QT>(y1.z, y1.w));
@@ -464,22 +463,24 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
   }
 }
 
-template <int DP, int NC, int QT, bool FIRST>
+template <int DP, int NC, int QT, int MODE>
 void launch_few_as(const Kv8AttnArgs& a, int64_t items, hipStream_t st) {
   if (a.parts == 0) {
-    kv8_attn_few_kernel<DP, NC, QT, false, FIRST><<<(unsigned)items, 64 * kWaves, 0, st>>>(a);
+    kv8_attn_few_kernel<DP, NC, QT, false, MODE><<<(unsigned)items, 64 * kWaves, 0, st>>>(a);
     return;
   }
-  kv8_attn_few_kernel<DP, NC, QT, true, FIRST><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
-  kv8_merge_kernel<16 * NC, kTile, QT><<<(unsigned)(items * 4 * NC), 256, 0, st>>>(a);
+  kv8_attn_few_kernel<DP, NC, QT, true, MODE><<<a.parts * a.Hkv, 64 * kWaves, 0, st>>>(a);
+  kv8_merge_kernel<16 * NC, kTile, QT, MODE><<<(unsigned)(items * 4 * NC), 256, 0, st>>>(a);
 }
 
 template <int DP, int NC, int QT>
 void launch_few(const Kv8AttnArgs& a, int64_t items, hipStream_t st) {
-  if (a.first > 0)
-    launch_few_as<DP, NC, QT, true>(a, items, st);
+  if (kv8_mode(a) == kPlain)
+    launch_few_as<DP, NC, QT, kPlain>(a, items, st);
+  else if (kv8_mode(a) == kFirst)
+    launch_few_as<DP, NC, QT, kFirst>(a, items, st);
   else
-    launch_few_as<DP, NC, QT, false>(a, items, st);
+    launch_few_as<DP, NC, QT, kShared>(a, items, st);
 }
 
 template <int QT>

@@ -73,10 +73,10 @@ __device__ __forceinline__ uint32_t swt(int t) {
   return DP >= 128 ? (uint32_t)(((t & 3) << 2) | ((t >> 2) & 3)) : (uint32_t)(((t & 2) << 1) | ((t >> 2) & 3));
 }
 
-// DP: head dim rounded up to 64, 128 or 256; NW wavefronts; FIRST: the sequence's first
-// tokens are seen beside the window
-template <int DP, int QT, int NW, bool SPLIT, bool FIRST>
+// DP: head dim rounded up to 64, 128 or 256; NW wavefronts
+template <int DP, int QT, int NW, bool SPLIT, int MODE>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel(const Kv8AttnArgs a, int64_t items) {
+  constexpr bool FIRST = MODE == kFirst;
   constexpr int kKeys = chunk_keys(DP), NG = kKeys / 16, NH = kKeys / 32;  // granules, halves of 32 tokens
   constexpr int RT = 32 * NW, NT = 64 * NW, ROW = 2 * DP, KS = DP / 16, DT = DP / 32;
   constexpr int NS = KS * NH;   // products of each kind in a tile
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 
   if (threadIdx.x < 2) sNan[threadIdx.x] = 0;
   int head, part = 0;
-  Kv8Walk<RT, kKeys> walk;
+  Kv8Walk<RT, kKeys, MODE> walk;
   Kv8Segment seg;
   if constexpr (SPLIT) {
     kv8_wg_at(a, (int)blockIdx.x, &head, &part);
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
   } else {
     // the last row tiles, which see the most keys, first; the heads go round
     // fastest, so that a head's workgroups meet on one XCD and its L2
-    if (!kv8_item<RT, kKeys>(a, items - 1 - (int64_t)blockIdx.x, &head, seg)) return;
+    if (!kv8_item<RT, kKeys, MODE>(a, items - 1 - (int64_t)blockIdx.x, &head, seg)) return;
   }
   for (bool more = SPLIT ? walk.next(a, seg) : true; more; more = SPLIT ? walk.next(a, seg) : false) {
     const Kv8Seq& s = seg.s;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
         else
           return q[k];
       };
-      const int32_t* table = a.pages + (int64_t)(a.table_row ? a.table_row[b] : b) * a.row_pages;
+      const int32_t* table = a.pages + (int64_t)(MODE == kShared && a.table_row ? a.table_row[b] : b) * a.row_pages;
       const int pmask = (1 << a.page_shift) - 1;
 
       // ---- pages and scales of TB tiles at a time: lane l has granule l % NG of tile
@@ -552,8 +552,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     l_run += __shfl_xor(l_run, 32, 64);
     if (live) {
       const int64_t at = (int64_t)(s.row0 + tq) * (a.Hkv * a.G) + hq;
-      if (whole && !a.raw) {
-        Kv8Join join = kv8_join(a, s, at, hq, m_run, l_run);
+      if (whole && !(MODE == kShared && a.raw)) {
+        Kv8Join join = kv8_join<MODE>(a, s, at, hq, m_run, l_run);
         join.own *= kUnlift;
         uint16_t* o = a.o + at * a.D + 4 * g2;
 #pragma unroll
@@ -561,12 +561,12 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if (32 * d + 8 * k < a.D) {
-              const float4 y = kv8_joined(a, join, at, 32 * d + 8 * k + 4 * g2,
+              const float4 y = kv8_joined<MODE>(a, join, at, 32 * d + 8 * k + 4 * g2,
                                           make_float4(acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]));
               *reinterpret_cast<uint2*>(o + 32 * d + 8 * k) = make_uint2(kv8_out2<QT>(y.x, y.y), kv8_out2<QT>(y.z, y.w));
             }
       } else {
-        float* o = (whole ? a.prior_acc + at * a.D : a.ws_acc + (slot * RT + r) * a.D) + 4 * g2;
+        float* o = (MODE == kShared && whole ? a.prior_acc + at * a.D : a.ws_acc + (slot * RT + r) * a.D) + 4 * g2;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -576,42 +576,52 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
                   make_float4(acc[d][4 * k] * kUnlift, acc[d][4 * k + 1] * kUnlift, acc[d][4 * k + 2] * kUnlift,
                               acc[d][4 * k + 3] * kUnlift);
         if (g2 == 0)
-          *reinterpret_cast<float2*>(whole ? a.prior_ml + 2 * at : a.ws_ml + (slot * RT + r) * 2) = make_float2(m_run, l_run);
+          *reinterpret_cast<float2*>(MODE == kShared && whole ? a.prior_ml + 2 * at : a.ws_ml + (slot * RT + r) * 2) = make_float2(m_run, l_run);
       }
     }
   }
 }
 
-template <int DP, int QT, bool FIRST>
+template <int DP, int QT, int MODE>
 void launch_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
   constexpr int NW = DP == 128 ? 8 : 4, RT = 32 * NW;
   static_assert(RT == kv8_chunk_rows(DP), "the plan's row tile");
   const int64_t items = p.items;
   if (p.parts == 0) {
-    kv8_prefill_kernel<DP, QT, NW, false, FIRST><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
+    kv8_prefill_kernel<DP, QT, NW, false, MODE><<<(unsigned)items, 64 * NW, 0, st>>>(a, items);
   } else {
-    kv8_prefill_kernel<DP, QT, NW, true, FIRST><<<a.parts * a.Hkv, 64 * NW, 0, st>>>(a, items);
-    kv8_merge_kernel<RT, chunk_keys(DP), QT><<<(unsigned)(items * (RT / 4)), 256, 0, st>>>(a);
+    kv8_prefill_kernel<DP, QT, NW, true, MODE><<<a.parts * a.Hkv, 64 * NW, 0, st>>>(a, items);
+    kv8_merge_kernel<RT, chunk_keys(DP), QT, MODE><<<(unsigned)(items * (RT / 4)), 256, 0, st>>>(a);
   }
 }
 
-template <int QT, bool FIRST>
+template <int QT, int MODE>
 void launch_prefill_as(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
   if (a.D <= 64)
-    launch_prefill<64, QT, FIRST>(a, p, st);
+    launch_prefill<64, QT, MODE>(a, p, st);
   else if (a.D <= 128)
-    launch_prefill<128, QT, FIRST>(a, p, st);
+    launch_prefill<128, QT, MODE>(a, p, st);
   else
-    launch_prefill<256, QT, FIRST>(a, p, st);
+    launch_prefill<256, QT, MODE>(a, p, st);
+}
+
+template <int QT>
+void launch_mode(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st) {
+  if (kv8_mode(a) == kPlain)
+    launch_prefill_as<QT, kPlain>(a, p, st);
+  else if (kv8_mode(a) == kFirst)
+    launch_prefill_as<QT, kFirst>(a, p, st);
+  else
+    launch_prefill_as<QT, kShared>(a, p, st);
 }
 
 }  // namespace
 
 void launch_kv8_prefill(const Kv8AttnArgs& a, const Kv8AttnPlan& p, int dtype, hipStream_t st) {
   if (dtype == SGL_BF16)
-    a.first > 0 ? launch_prefill_as<SGL_BF16, true>(a, p, st) : launch_prefill_as<SGL_BF16, false>(a, p, st);
+    launch_mode<SGL_BF16>(a, p, st);
   else
-    a.first > 0 ? launch_prefill_as<SGL_F16, true>(a, p, st) : launch_prefill_as<SGL_F16, false>(a, p, st);
+    launch_mode<SGL_F16>(a, p, st);
 }
 
 }  // namespace sgl

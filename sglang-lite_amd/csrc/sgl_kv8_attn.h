@@ -80,6 +80,11 @@ __device__ __forceinline__ float kv8_exponent(bool there, bool good, float vs) {
   return !there ? kNoToken : !good ? kBadScale : vs < 0x1p-100f ? kNoValue : __builtin_amdgcn_logf(vs) + kLift;
 }
 
+// What a kernel is made for: plain calls; first tokens beside the window; either pass of a
+// common prefix.  (In one kernel for all three, the last two cost plain calls 1 to 3 %.)
+enum Kv8Mode { kPlain, kFirst, kShared };
+inline Kv8Mode kv8_mode(const Kv8AttnArgs& a) { return a.raw || a.skip ? kShared : a.first > 0 ? kFirst : kPlain; }
+
 // A sequence as the line sees it.
 struct Kv8Seq {
   int row0, n, len;  // first query row, queries, keys
@@ -89,15 +94,15 @@ struct Kv8Seq {
   int skip;
 
   // the key tile that tile i of the item is
-  template <bool FIRST>
+  template <int MODE>
   __device__ __forceinline__ int tile(int i) const {
-    return FIRST && i < kept ? i : i + tile0;
+    return MODE == kFirst && i < kept ? i : i + tile0;
   }
 };
 
-template <int RT, int TT>
+template <int RT, int TT, int MODE>
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n, int len, int skip) {
-  int lo = skip;
+  int lo = MODE == kShared ? skip : 0;
   if (a.causal && a.window > 0) {
     const int64_t first = (int64_t)len - n - a.window + 1;
     lo = first > 0 ? (int)first : 0;
@@ -107,8 +112,8 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n,
   s.n = n;
   s.len = len;
   s.skip = skip;
-  s.kept = (a.first + TT - 1) / TT;
-  s.tile0 = lo / TT > s.kept ? lo / TT - s.kept : 0;
+  s.kept = MODE == kFirst ? (a.first + TT - 1) / TT : 0;
+  s.tile0 = MODE != kFirst || lo / TT > s.kept ? lo / TT - s.kept : 0;
   const int tiles = (len + TT - 1) / TT - s.tile0;
   s.tiles = tiles > 0 ? tiles : 1;
   s.row_tiles = (n * a.G + RT - 1) / RT;
@@ -122,7 +127,7 @@ struct Kv8Chunk {
   int rts;          // row tiles of the sequences up to and with it
 };
 
-template <int RT, int TT>
+template <int RT, int TT, int MODE>
 __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
   const int b = b0 + (int)(threadIdx.x & 63);
   Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0, 0};
@@ -133,10 +138,10 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
     c.row0 = r.first;
     c.n = r.n;
     c.len = len < 0 ? 0 : len > cap ? cap : len;
-    if (a.skip) c.skip = a.skip[b];
-    const Kv8Seq s = kv8_seq<RT, TT>(a, c.row0, c.n, c.len, c.skip);
+    if (MODE == kShared && a.skip) c.skip = a.skip[b];
+    const Kv8Seq s = kv8_seq<RT, TT, MODE>(a, c.row0, c.n, c.len, c.skip);
     const int rows = r.n * a.G;
-    rts = rows > a.above && rows <= a.upto && !(a.raw && c.len == 0) ? s.row_tiles : 0;
+    rts = rows > a.above && rows <= a.upto && !(MODE == kShared && a.raw && c.len == 0) ? s.row_tiles : 0;
     c.room = rts * (s.tiles + kItemCost);
   }
   c.rooms = wave_incl_scan(c.room);
@@ -144,17 +149,18 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
   return c;
 }
 
-template <int RT, int TT>
+template <int RT, int TT, int MODE>
 __device__ __forceinline__ Kv8Seq kv8_lane(const Kv8AttnArgs& a, const Kv8Chunk& c, int l) {
-  return kv8_seq<RT, TT>(a, __builtin_amdgcn_readlane(c.row0, l), __builtin_amdgcn_readlane(c.n, l),
-                         __builtin_amdgcn_readlane(c.len, l), __builtin_amdgcn_readlane(c.skip, l));
+  return kv8_seq<RT, TT, MODE>(a, __builtin_amdgcn_readlane(c.row0, l), __builtin_amdgcn_readlane(c.n, l),
+                         __builtin_amdgcn_readlane(c.len, l),
+                         MODE == kShared ? __builtin_amdgcn_readlane(c.skip, l) : 0);
 }
 
 // Length of a kv head's line; c: the batch's first 64 sequences.
-template <int RT, int TT>
+template <int RT, int TT, int MODE>
 __device__ __forceinline__ int64_t kv8_total(const Kv8AttnArgs& a, const Kv8Chunk& c) {
   int64_t total = __builtin_amdgcn_readlane(c.rooms, 63);
-  for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(kv8_chunk<RT, TT>(a, b0).rooms, 63);
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(kv8_chunk<RT, TT, MODE>(a, b0).rooms, 63);
   return total;
 }
 
@@ -165,7 +171,7 @@ struct Kv8Place {
   int64_t room;  // places before
   int64_t rts;   // row tiles before
 };
-template <int RT, int TT, bool BY_TILE>
+template <int RT, int TT, int MODE, bool BY_TILE>
 __device__ __forceinline__ Kv8Place kv8_find(const Kv8AttnArgs& a, Kv8Chunk& c, int64_t x) {
   Kv8Place at = {-1, 0, 0};
   for (;;) {
@@ -181,7 +187,7 @@ __device__ __forceinline__ Kv8Place kv8_find(const Kv8AttnArgs& a, Kv8Chunk& c, 
     at.room += __builtin_amdgcn_readlane(c.rooms, 63);
     at.rts += __builtin_amdgcn_readlane(c.rts, 63);
     if (c.b0 + 64 >= a.B) return at;
-    c = kv8_chunk<RT, TT>(a, c.b0 + 64);
+    c = kv8_chunk<RT, TT, MODE>(a, c.b0 + 64);
   }
 }
 
@@ -204,19 +210,19 @@ struct Kv8Segment {
 };
 
 // Walks over the segments of the places [x, end) of a line.
-template <int RT, int TT>
+template <int RT, int TT, int MODE>
 struct Kv8Walk {
   Kv8Chunk c;
   int64_t x, end, base;
   int l;
 
   __device__ __forceinline__ bool start(const Kv8AttnArgs& a, int part) {
-    c = kv8_chunk<RT, TT>(a, 0);
-    const int64_t total = kv8_total<RT, TT>(a, c), per = (total + a.parts - 1) / a.parts;
+    c = kv8_chunk<RT, TT, MODE>(a, 0);
+    const int64_t total = kv8_total<RT, TT, MODE>(a, c), per = (total + a.parts - 1) / a.parts;
     x = (int64_t)part * per;
     end = x + per < total ? x + per : total;
     if (x >= end) return false;
-    const Kv8Place at = kv8_find<RT, TT, false>(a, c, x);
+    const Kv8Place at = kv8_find<RT, TT, MODE, false>(a, c, x);
     base = at.room;
     l = at.l;
     return true;
@@ -229,12 +235,12 @@ struct Kv8Walk {
         base += room;
         if (++l == 64) {
           if (c.b0 + 64 >= a.B) return false;
-          c = kv8_chunk<RT, TT>(a, c.b0 + 64);
+          c = kv8_chunk<RT, TT, MODE>(a, c.b0 + 64);
           l = 0;
         }
         continue;
       }
-      g.s = kv8_lane<RT, TT>(a, c, l);
+      g.s = kv8_lane<RT, TT, MODE>(a, c, l);
       g.b = c.b0 + l;
       const int size = g.s.tiles + kItemCost, off = (int)(x - base);
       g.rt = off / size;
@@ -262,9 +268,10 @@ struct Kv8Join {
   float own, before;
   bool prior;
 };
+template <int MODE>
 __device__ __forceinline__ Kv8Join kv8_join(const Kv8AttnArgs& a, const Kv8Seq& s, int64_t at, int h, float M, float sum) {
   const float NEG_INF = -__builtin_huge_valf();
-  Kv8Join j = {1.0f, 0.0f, s.skip > 0};
+  Kv8Join j = {1.0f, 0.0f, MODE == kShared && s.skip > 0};
   float top = M;
   float2 ml = make_float2(NEG_INF, 0.0f);
   if (j.prior) {
@@ -284,9 +291,10 @@ __device__ __forceinline__ Kv8Join kv8_join(const Kv8AttnArgs& a, const Kv8Seq& 
   return j;
 }
 // four of the row's sums
+template <int MODE>
 __device__ __forceinline__ float4 kv8_joined(const Kv8AttnArgs& a, const Kv8Join& j, int64_t at, int d, float4 y) {
   y = make_float4(y.x * j.own, y.y * j.own, y.z * j.own, y.w * j.own);
-  if (j.prior) {
+  if (MODE == kShared && j.prior) {
     const float4 p = *reinterpret_cast<const float4*>(a.prior_acc + at * a.D + d);
     y = make_float4(y.x + p.x * j.before, y.y + p.y * j.before, y.z + p.z * j.before, y.w + p.w * j.before);
   }
@@ -294,14 +302,14 @@ __device__ __forceinline__ float4 kv8_joined(const Kv8AttnArgs& a, const Kv8Join
 }
 
 // Item x of the batch (row tiles in order, the heads of each together) as one segment.
-template <int RT, int TT>
+template <int RT, int TT, int MODE>
 __device__ __forceinline__ bool kv8_item(const Kv8AttnArgs& a, int64_t x, int* head, Kv8Segment& g) {
   const int64_t tile = x / a.Hkv;
   *head = (int)(x - tile * a.Hkv);
-  Kv8Chunk c = kv8_chunk<RT, TT>(a, 0);
-  const Kv8Place at = kv8_find<RT, TT, true>(a, c, tile);
+  Kv8Chunk c = kv8_chunk<RT, TT, MODE>(a, 0);
+  const Kv8Place at = kv8_find<RT, TT, MODE, true>(a, c, tile);
   if (at.l < 0) return false;
-  g.s = kv8_lane<RT, TT>(a, c, at.l);
+  g.s = kv8_lane<RT, TT, MODE>(a, c, at.l);
   g.b = c.b0 + at.l;
   g.rt = (int)(tile - at.rts);
   g.t0 = 0;
@@ -312,16 +320,16 @@ __device__ __forceinline__ bool kv8_item(const Kv8AttnArgs& a, int64_t x, int* h
 // The items that several workgroups share.  One wavefront a row (four a workgroup,
 // RT / 4 workgroups an item): lane p has part p's reference and weight, and all lanes
 // go over the parts' sums.
-template <int RT, int TT, int QT>
+template <int RT, int TT, int QT, int MODE>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
-  Kv8Chunk c = kv8_chunk<RT, TT>(a, 0);
-  const int64_t total = kv8_total<RT, TT>(a, c), per = (total + a.parts - 1) / a.parts;
+  Kv8Chunk c = kv8_chunk<RT, TT, MODE>(a, 0);
+  const int64_t total = kv8_total<RT, TT, MODE>(a, c), per = (total + a.parts - 1) / a.parts;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t item = blockIdx.x / (RT / 4);
   const int head = (int)(item % a.Hkv);
-  const Kv8Place at = kv8_find<RT, TT, true>(a, c, item / a.Hkv);
+  const Kv8Place at = kv8_find<RT, TT, MODE, true>(a, c, item / a.Hkv);
   if (at.l < 0) return;
-  const Kv8Seq s = kv8_lane<RT, TT>(a, c, at.l);
+  const Kv8Seq s = kv8_lane<RT, TT, MODE>(a, c, at.l);
   const int rt = (int)(item / a.Hkv - at.rts);
   const int64_t xs = at.room + (int64_t)rt * (s.tiles + kItemCost) + kItemCost;
   const int pa = (int)(xs / per), pb = (int)((xs + s.tiles - 1) / per);
@@ -376,12 +384,12 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
   if (d >= a.D) return;
   const int64_t out = (int64_t)(s.row0 + t) * (a.Hkv * a.G) + h;
   float4 y = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  if (a.raw) {
+  if (MODE == kShared && a.raw) {
     *reinterpret_cast<float4*>(a.prior_acc + out * a.D + d) = y;
     if (lane == 0) *reinterpret_cast<float2*>(a.prior_ml + 2 * out) = make_float2(M, l);
     return;
   }
-  y = kv8_joined(a, kv8_join(a, s, out, h, M, l), out, d, y);
+  y = kv8_joined<MODE>(a, kv8_join<MODE>(a, s, out, h, M, l), out, d, y);
   *reinterpret_cast<uint2*>(a.o + out * a.D + d) = make_uint2(kv8_out2<QT>(y.x, y.y), kv8_out2<QT>(y.z, y.w));
 }
 
