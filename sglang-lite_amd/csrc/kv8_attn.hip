@@ -84,30 +84,37 @@ struct Codes {
   uint32_t v[8][DP / 64];  // tokens as above, C = DP / 16 bytes each
 };
 
-// DP: head dim rounded up to 64, 128 or 256; NC: 16-row column tiles
-// SPLIT: workgroups share the lines, else a workgroup takes a whole item
-template <int DP, int NC, int QT, bool SPLIT, int MODE>
-__global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
+// Codes that one workgroup reads, or several (which the nontemporal policy would have all
+// read from memory).
+template <class V, bool ONCE>
+__device__ __forceinline__ V ld_codes(const uint8_t* p) {
+  if constexpr (!ONCE)
+    return *reinterpret_cast<const V*>(p);
+  else if constexpr (sizeof(V) == 16)
+    return ld16_stream(p);
+  else
+    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+
+// What the wavefronts of a workgroup join their sums through, a column tile at a time.
+template <int DP>
+struct Joint {
+  __align__(16) float acc[kWaves][16][DP + 4];
+  float m[kWaves][16], l[kWaves][16];
+};
+
+// One segment.  DP: head dim rounded up to 64, 128 or 256; NC: 16-row column tiles
+template <int DP, int NC, int QT, int MODE, bool ONCE = true>
+__device__ __forceinline__ void few_segment(const Kv8AttnArgs& a, const Kv8Segment& seg, int head, Joint<DP>& lds) {
   constexpr int RT = 16 * NC, KI = DP / 64, C = DP / 16, W = C / 4;
-  __shared__ __align__(16) float sAcc[kWaves][16][DP + 4];
-  __shared__ float sM[kWaves][16], sL[kWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
   const float NEG_INF = -__builtin_huge_valf();
-
-  int head, part = 0;
-  Kv8Walk<RT, kTile, MODE> walk;
-  Kv8Segment seg;
-  if constexpr (SPLIT) {
-    kv8_wg_at(a, (int)blockIdx.x, &head, &part);
-    if (!walk.start(a, part)) return;
-  } else {
-    if (!kv8_item<RT, kTile, MODE>(a, (int64_t)blockIdx.x, &head, seg)) return;
-  }
-  for (bool more = SPLIT ? walk.next(a, seg) : true; more; more = SPLIT ? walk.next(a, seg) : false) {
+  {
     const Kv8Seq& s = seg.s;
     const int b = seg.b, rt = seg.rt, t0 = seg.t0, t1 = seg.t1;
     const int rows = s.n * a.G - rt * RT;  // valid rows of the tile (may be more than RT)
+    const bool causal = a.causal && !(MODE == kJoint && s.group == kIsGroup);
 
     // the rows: their queries and what they see
     typename Op<QT>::V q[NC][2 * KI];
@@ -119,8 +126,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       const bool live = r < rows;
       const int row = rt * RT + (live ? r : 0), t = row / a.G, h = head * a.G + (row - t * a.G);
       const int pos = s.len - s.n + t;
-      hi[c] = !live ? 0 : a.causal ? pos + 1 : s.len;
-      lo[c] = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
+      hi[c] = !live ? 0 : causal ? pos + 1 : s.len;
+      lo[c] = causal && a.window > 0 ? pos - a.window + 1 : 0;
       const uint16_t* src = a.q + (int64_t)(s.row0 + t) * a.qt + (int64_t)h * a.qh;
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
@@ -134,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         q[c][2 * i + 1] = __builtin_bit_cast(typename Op<QT>::V, w);
       }
     }
-    if (a.causal) {
+    if (causal) {
       const int last = rows < RT ? rows - 1 : RT - 1;
       const int p0 = s.len - s.n + (rt * RT) / a.G, p1 = s.len - s.n + (rt * RT + last) / a.G;
       all_hi = p0 + 1 < all_hi ? p0 + 1 : all_hi;
@@ -151,7 +158,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       for (int j = 0; j < C; ++j) acc[c][j] = v4f{0, 0, 0, 0};
     }
 
-    const int32_t* table = a.pages + (int64_t)(MODE == kShared && a.table_row ? a.table_row[b] : b) * a.row_pages;
+    const int32_t* table = a.pages + (int64_t)(MODE == kJoint ? s.table_row : MODE == kShared && a.table_row ? a.table_row[b] : b) * a.row_pages;
     const int pmask = (1 << a.page_shift) - 1;
     // the wavefront's first token in step i; only the last tile's may lie behind the end
     auto token = [&](int i) __attribute__((always_inline)) { return s.template tile<MODE>(t0 + i) * kTile + 32 * wave; };
@@ -195,18 +202,18 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         const uint8_t* kp = a.kc + row;
         const uint8_t* vp = a.vc + row;
 #pragma unroll
-        for (int k = 0; k < KI; ++k) r.k[u][k] = ld16_stream(kp + (uint32_t)kd[k]);
+        for (int k = 0; k < KI; ++k) r.k[u][k] = ld_codes<uint4, ONCE>(kp + (uint32_t)kd[k]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint8_t* at = vp + j * a.D + (uint32_t)vd;
           if constexpr (W == 1) {
-            r.v[4 * u + j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(at));
+            r.v[4 * u + j][0] = ld_codes<uint32_t, ONCE>(at);
           } else if constexpr (W == 2) {
-            const u2v y = __builtin_nontemporal_load(reinterpret_cast<const u2v*>(at));
+            const u2v y = ld_codes<u2v, ONCE>(at);
             r.v[4 * u + j][0] = y.x;
             r.v[4 * u + j][1] = y.y;
           } else {
-            const uint4 y = ld16_stream(at);
+            const uint4 y = ld_codes<uint4, ONCE>(at);
             r.v[4 * u + j][0] = y.x;
             r.v[4 * u + j][1] = y.y;
             r.v[4 * u + j][2] = y.z;
@@ -409,14 +416,14 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
       l += __shfl_xor(l, 32, 64);
       __syncthreads();
       if (g == 0) {
-        sM[wave][m] = m_run[c];
-        sL[wave][m] = l;
+        lds.m[wave][m] = m_run[c];
+        lds.l[wave][m] = l;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < C; j += 4)
-          *reinterpret_cast<float4*>(&sAcc[wave][m][C * (4 * g + i) + j]) =
+          *reinterpret_cast<float4*>(&lds.acc[wave][m][C * (4 * g + i) + j]) =
               make_float4(acc[c][j][i], acc[c][j + 1][i], acc[c][j + 2][i], acc[c][j + 3][i]);
       __syncthreads();
       const int chunks = a.D >> 3;
@@ -425,25 +432,26 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
         if (r >= rows) break;
         float M = NEG_INF;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = __builtin_fmaxf(M, sM[w][n]);
+        for (int w = 0; w < kWaves; ++w) M = __builtin_fmaxf(M, lds.m[w][n]);
         const float ref = M == NEG_INF ? 0.0f : M;
         float sum = 0.0f, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const float f = __builtin_amdgcn_exp2f(sM[w][n] - ref);
-          sum += sL[w][n] * f;
+          const float f = __builtin_amdgcn_exp2f(lds.m[w][n] - ref);
+          sum += lds.l[w][n] * f;
 #pragma unroll
-          for (int v = 0; v < 8; ++v) y[v] += sAcc[w][n][d + v] * (f * kUnlift);
+          for (int v = 0; v < 8; ++v) y[v] += lds.acc[w][n][d + v] * (f * kUnlift);
         }
         if (whole) {
           const int row = rt * RT + r, t = row / a.G, h = head * a.G + (row - t * a.G);
           const int64_t at = (int64_t)(s.row0 + t) * (a.Hkv * a.G) + h;
           float4 y0 = make_float4(y[0], y[1], y[2], y[3]), y1 = make_float4(y[4], y[5], y[6], y[7]);
-          if (MODE == kShared && a.raw) {
-            float4* out = reinterpret_cast<float4*>(a.prior_acc + at * a.D + d);
+          if (MODE == kJoint || (MODE == kShared && a.raw)) {
+            const bool prior = MODE == kShared || s.group == kIsGroup;
+            float4* out = reinterpret_cast<float4*>((prior ? a.prior_acc : a.own_acc) + at * a.D + d);
             out[0] = y0;
             out[1] = y1;
-            if (d == 0) *reinterpret_cast<float2*>(a.prior_ml + 2 * at) = make_float2(M, sum);
+            if (d == 0) *reinterpret_cast<float2*>((prior ? a.prior_ml : a.own_ml) + 2 * at) = make_float2(M, sum);
           } else {
             const Kv8Join join = kv8_join<MODE>(a, s, at, h, M, sum);
             y0 = kv8_joined<MODE>(a, join, at, d, y0);
@@ -453,13 +461,48 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_ke
                            kv8_out2<QT>(y1.z, y1.w));
           }
         } else {
-          float4* out = reinterpret_cast<float4*>(a.ws_acc + (slot * RT + r) * a.D + d);
+          float4* out = reinterpret_cast<float4*>(a.ws_acc + (slot * (MODE == kJoint ? a.slot_rows : RT) + r) * a.D + d);
           out[0] = make_float4(y[0], y[1], y[2], y[3]);
           out[1] = make_float4(y[4], y[5], y[6], y[7]);
-          if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (slot * RT + r) * 2) = make_float2(M, sum);
+          if (d == 0) *reinterpret_cast<float2*>(a.ws_ml + (slot * (MODE == kJoint ? a.slot_rows : RT) + r) * 2) = make_float2(M, sum);
         }
       }
     }
+  }
+}
+
+// SPLIT: workgroups share the lines, else a workgroup takes a whole item
+template <int DP, int NC, int QT, bool SPLIT, int MODE>
+__global__ __launch_bounds__(64 * kWaves, DP == 64 ? 2 : 1) void kv8_attn_few_kernel(const Kv8AttnArgs a) {
+  __shared__ Joint<DP> lds;
+  constexpr int RT = 16 * NC;
+  int head, part = 0;
+  Kv8Segment seg;
+  if constexpr (SPLIT) {
+    Kv8Walk<RT, kTile, MODE> walk;
+    kv8_wg_at(a, (int)blockIdx.x, &head, &part);
+    if (!walk.start(a, part)) return;
+    while (walk.next(a, seg)) few_segment<DP, NC, QT, MODE>(a, seg, head, lds);
+  } else {
+    if (kv8_item<RT, kTile, MODE>(a, (int64_t)blockIdx.x, &head, seg)) few_segment<DP, NC, QT, MODE>(a, seg, head, lds);
+  }
+}
+
+// Sequences and groups on one line, in tiles of NC and NCG column tiles.
+// WGS workgroups a CU.
+template <int DP, int NCG, int NC, int QT, int WGS>
+__global__ __launch_bounds__(64 * kWaves, WGS) void kv8_joint_kernel(const Kv8AttnArgs a) {
+  __shared__ Joint<DP> lds;
+  int head, part = 0;
+  Kv8Segment seg;
+  Kv8Walk<16 * NC, kTile, kJoint> walk;
+  kv8_wg_at(a, (int)blockIdx.x, &head, &part);
+  if (!walk.start(a, part)) return;
+  while (walk.next(a, seg)) {
+    if (seg.s.group == kIsGroup)
+      few_segment<DP, NCG, QT, kJoint, false>(a, seg, head, lds);
+    else
+      few_segment<DP, NC, QT, kJoint>(a, seg, head, lds);
   }
 }
 
@@ -497,6 +540,39 @@ void launch_attn(Kv8AttnArgs a, const Kv8AttnPlan& p, hipStream_t st) {
     p.row_tile == 16 ? launch_few<128, 1, QT>(a, p.items, st) : launch_few<128, 2, QT>(a, p.items, st);
   else
     launch_few<256, 1, QT>(a, p.items, st);
+}
+
+template <int DP, int NCG, int NC, int QT>
+void launch_joint_as(const Kv8AttnArgs& a, const Kv8JointPlan& p, hipStream_t st) {
+  const dim3 grid(a.parts * a.Hkv), threads(64 * kWaves);
+  if constexpr (DP <= 128) {
+    if (p.per_cu == 2)
+      kv8_joint_kernel<DP, NCG, NC, QT, 2><<<grid, threads, 0, st>>>(a);
+    else
+      kv8_joint_kernel<DP, NCG, NC, QT, 1><<<grid, threads, 0, st>>>(a);
+  } else {
+    kv8_joint_kernel<DP, NCG, NC, QT, 1><<<grid, threads, 0, st>>>(a);
+  }
+  const int64_t rows = (int64_t)a.T * a.Hkv * a.G;
+  kv8_joint_merge_kernel<16 * NC, kTile, QT><<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(a);
+}
+template <int DP, int QT>
+void launch_joint_dim(const Kv8AttnArgs& a, const Kv8JointPlan& p, hipStream_t st) {
+  if (p.group_rows == 16)
+    launch_joint_as<DP, 1, 1, QT>(a, p, st);
+  else if (p.row_tile == 16)
+    launch_joint_as<DP, 2, 1, QT>(a, p, st);
+  else if constexpr (DP <= 128)
+    launch_joint_as<DP, 2, 2, QT>(a, p, st);
+}
+template <int QT>
+void launch_joint(const Kv8AttnArgs& a, const Kv8JointPlan& p, hipStream_t st) {
+  if (a.D <= 64)
+    launch_joint_dim<64, QT>(a, p, st);
+  else if (a.D <= 128)
+    launch_joint_dim<128, QT>(a, p, st);
+  else
+    launch_joint_dim<256, QT>(a, p, st);
 }
 
 struct AttnPlans {
@@ -620,6 +696,7 @@ constexpr int kPrefixTile = 128;
 struct PrefixPlan {
   int32_t *cu, *lens, *row;  // of the groups: first token rows [n + 1], covered tokens, a row of the block table
   int32_t* skip;             // of the sequences: covered tokens
+  Kv8Entry* entries;         // in their place, for one pass: of the sequences and behind them the groups
 };
 // Workgroup g takes group g; the last one the sequences of no group.
 __global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, const int32_t* cu_groups,
@@ -634,14 +711,24 @@ __global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, co
     const SeqRows last = seq_rows(a.cu, a.B - 1, a.T);
     return last.first + last.n;
   };
+  const int cap = a.row_pages << a.page_shift;
+  auto cover = [&](int b, int tokens, int group) {
+    if (!o.entries) {
+      o.skip[b] = tokens;
+      return;
+    }
+    const SeqRows r = seq_rows(a.cu, b, a.T);
+    const int len = a.lens[b];
+    o.entries[b] = Kv8Entry{r.first, r.n, len < 0 ? 0 : len > cap ? cap : len, r.n ? tokens : 0, b, group, 0, 0};
+  };
   if (g == n) {
     const int lo = edge(0), hi = edge(n);
     for (int b = (int)threadIdx.x; b < a.B; b += 256)
-      if (b < lo || b >= hi) o.skip[b] = 0;
-    if (threadIdx.x == 0) o.cu[n] = row_of(hi);
+      if (b < lo || b >= hi) cover(b, 0, -1);
+    if (threadIdx.x == 0 && !o.entries) o.cu[n] = row_of(hi);
     return;
   }
-  const int b0 = edge(g), b1 = edge(g + 1), cap = a.row_pages << a.page_shift;
+  const int b0 = edge(g), b1 = edge(g + 1);
   int most = shared[g], with = 0;
   for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) {
     const SeqRows r = seq_rows(a.cu, b, a.T);
@@ -670,28 +757,42 @@ __global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, co
   }
   const int unit = kPrefixTile > (1 << a.page_shift) ? kPrefixTile : 1 << a.page_shift;
   const int covered = with < 2 || most < unit ? 0 : most & ~(unit - 1);
-  for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) o.skip[b] = covered;
-  if (threadIdx.x == 0) {
+  for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) cover(b, covered, g);
+  if (threadIdx.x == 0 && o.entries) {
+    const int row0 = row_of(b0), end = b1 > b0 ? row_of(b1) : row0;
+    o.entries[a.B + g] = Kv8Entry{row0, end > row0 ? end - row0 : 0, covered, 0, b0 < a.B ? b0 : 0, kIsGroup, 0, 0};
+  } else if (threadIdx.x == 0) {
     o.cu[g] = row_of(b0);
     o.lens[g] = covered;
     o.row[g] = b0 < a.B ? b0 : 0;
   }
 }
 
-// The workspace: the plan's numbers, the first pass' sums, then what either pass needs for itself.
+// The workspace: the plan's numbers, the first pass' sums (in one pass: the whole items of groups,
+// then those of sequences), then the parts.
 struct PrefixSpace {
-  size_t plan, acc, ml, rest, total;
+  Kv8JointPlan joint;
+  AttnPlans first, second;  // where it does not serve
+  size_t acc, ml, own_acc, own_ml, rest, total;
 };
 PrefixSpace prefix_space(int64_t T, int64_t B, int Hkv, int G, int D, int64_t tokens, int64_t n) {
   auto round = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t first = attn_workspace(attn_plans(T, n, Hkv, G, D, tokens), Hkv, D);
-  const size_t second = attn_workspace(attn_plans(T, B, Hkv, G, D, tokens), Hkv, D);
   PrefixSpace s;
-  s.plan = 0;
-  s.acc = round((size_t)(3 * n + 1 + B) * 4);
-  s.ml = s.acc + round((size_t)T * Hkv * G * D * 4);
-  s.rest = s.ml + round((size_t)T * Hkv * G * 8);
-  s.total = s.rest + (first > second ? first : second);
+  s.joint = kv8_joint_plan(T, B, n, Hkv, G, D, tokens, device_cu_count());
+  const size_t sums = round((size_t)T * Hkv * G * D * 4), weights = round((size_t)T * Hkv * G * 8);
+  s.acc = s.joint.items ? round((size_t)(B + n) * sizeof(Kv8Entry)) : round((size_t)(3 * n + 1 + B) * 4);
+  s.ml = s.acc + sums;
+  s.own_acc = s.ml + weights;
+  s.own_ml = s.own_acc + (s.joint.items ? sums : 0);
+  s.rest = s.own_ml + (s.joint.items ? weights : 0);
+  if (s.joint.items) {
+    s.total = s.rest + (size_t)(2 * s.joint.parts * Hkv * s.joint.slot_rows * (D + 2)) * sizeof(float);
+  } else {
+    s.first = attn_plans(T, n, Hkv, G, D, tokens);
+    s.second = attn_plans(T, B, Hkv, G, D, tokens);
+    const size_t x = attn_workspace(s.first, Hkv, D), y = attn_workspace(s.second, Hkv, D);
+    s.total = s.rest + (x > y ? x : y);
+  }
   return s;
 }
 
@@ -770,24 +871,51 @@ int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_st
   if (rc != SGL_OK || nothing) return rc;
   SGL_REQUIRE(cu_groups && shared, "kv8_attn: null pointer");
   const int64_t tokens = row_pages * page_size, n = n_groups;
-  const sgl::AttnPlans first = sgl::attn_plans(T, n, Hkv, G, D, tokens);
-  const sgl::AttnPlans second = sgl::attn_plans(T, B, Hkv, G, D, tokens);
   const sgl::PrefixSpace space = sgl::prefix_space(T, B, Hkv, G, D, tokens, n);
+  const bool joint = space.joint.items != 0;
   rc = sgl::check_workspace(workspace, workspace_bytes, space.total);
-  if (rc == SGL_OK) rc = sgl::check_plans(first, tokens);
-  if (rc == SGL_OK) rc = sgl::check_plans(second, tokens);
+  if (rc == SGL_OK && !joint) rc = sgl::check_plans(space.first, tokens);
+  if (rc == SGL_OK && !joint) rc = sgl::check_plans(space.second, tokens);
   if (rc != SGL_OK) return rc;
+  const int64_t items = space.joint.items + space.joint.group_items;
+  SGL_REQUIRE_SUPPORTED(!joint || (items * ((tokens + 31) / 32 + sgl::kItemCost) < (1ll << 31) &&
+                                   T * Hkv * G < (1ll << 31)),
+                        "kv8_attn: %lld row tiles over %lld tokens are too many for one call", (long long)items,
+                        (long long)tokens);
   char* base = (char*)workspace;
-  sgl::PrefixPlan plan;
-  plan.cu = (int32_t*)(base + space.plan);
-  plan.lens = plan.cu + n + 1;
-  plan.row = plan.lens + n;
-  plan.skip = plan.row + n;
+  sgl::PrefixPlan plan = {};
+  if (joint) {
+    plan.entries = (sgl::Kv8Entry*)base;
+  } else {
+    plan.cu = (int32_t*)base;
+    plan.lens = plan.cu + n + 1;
+    plan.row = plan.lens + n;
+    plan.skip = plan.row + n;
+  }
   a.ws_acc = (float*)(base + space.rest);
   a.prior_acc = (float*)(base + space.acc);
   a.prior_ml = (float*)(base + space.ml);
   const hipStream_t st = (hipStream_t)stream;
   sgl::kv8_prefix_kernel<<<(unsigned)(n + 1), 256, 0, st>>>(a, cu_groups, shared, (int)n, plan);
+  if (joint) {
+    const sgl::Kv8JointPlan& p = space.joint;
+    a.B = (int)(B + n);
+    a.groups = (int)n;
+    a.group_rows = (int)p.group_rows;
+    a.slot_rows = (int)p.slot_rows;
+    a.parts = (int)p.parts;
+    a.above = 0;
+    a.upto = 0x7FFFFFFF;
+    a.entries = plan.entries;
+    a.own_acc = (float*)(base + space.own_acc);
+    a.own_ml = (float*)(base + space.own_ml);
+    a.ws_ml = a.ws_acc + 2 * p.parts * Hkv * p.slot_rows * D;
+    if (dtype == SGL_BF16)
+      sgl::launch_joint<SGL_BF16>(a, p, st);
+    else
+      sgl::launch_joint<SGL_F16>(a, p, st);
+    return sgl::check_launch("kv8_attn");
+  }
   sgl::Kv8AttnArgs g = a;
   g.B = (int)n;
   g.cu = plan.cu;
@@ -796,9 +924,9 @@ int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_st
   g.causal = false;
   g.sink = nullptr;
   g.raw = true;
-  sgl::launch_plans(g, dtype, first, st);
+  sgl::launch_plans(g, dtype, space.first, st);
   a.skip = plan.skip;
-  sgl::launch_plans(a, dtype, second, st);
+  sgl::launch_plans(a, dtype, space.second, st);
   return sgl::check_launch("kv8_attn");
 }
 

@@ -56,14 +56,27 @@ struct Kv8AttnArgs {
   int above, upto;  // takes the sequences of more than `above` rows a kv head, and up to `upto`
   float* ws_acc;  // [2 parts Hkv][row tile][D]
   float* ws_ml;   // [2 parts Hkv][row tile][2]: reference point (log2 units), sum
-  // A common prefix: its groups are the sequences of a first pass, whose unnormalised sums go
-  // to `prior` (`raw`); the second pass begins behind what they cover, and joins the two.
+  // A common prefix in two passes: its groups are the sequences of the first, whose unnormalised
+  // sums go to `prior` (`raw`); the second begins behind what they cover, and joins the two.
   const int32_t* table_row;  // first pass: the row of the block table of each group; null: its own
   const int32_t* skip;       // second pass: tokens that the first has covered; null: none
   float* prior_acc;          // [T Hkv G][D]
   float* prior_ml;           // [T Hkv G][2]
   bool raw;
+  // In one: the sequences and behind them the groups on one line, `entries` of them B; whole
+  // items go to `prior` (groups) and `own` (sequences).
+  const struct Kv8Entry* entries;
+  int groups, group_rows, slot_rows;  // of them; rows of a group's tile; of a part
+  float *own_acc, *own_ml;
 };
+
+// A sequence or a group: its query rows, keys, the tokens in front that its group has covered, the
+// row of the block table, its group (-1: none; kIsGroup: it is one).
+struct __attribute__((aligned(16))) Kv8Entry {
+  int row0, n, len, skip;
+  int table_row, group, pad0, pad1;
+};
+constexpr int kIsGroup = -2;
 
 // Key tiles.  1 / 2 / 3 / 5, us: 32 sequences of 4 queries up to 6000 keys 49.3 / 48.2 / 46.1 /
 // 47.2, 16 single ones up to 4000 25.6 / 24.8 / 23.3 / 23.5, 512 queries on 2000 57.0 / 55.2 / 51.8 / 53.8.
@@ -80,9 +93,9 @@ __device__ __forceinline__ float kv8_exponent(bool there, bool good, float vs) {
   return !there ? kNoToken : !good ? kBadScale : vs < 0x1p-100f ? kNoValue : __builtin_amdgcn_logf(vs) + kLift;
 }
 
-// What a kernel is made for: plain calls; first tokens beside the window; either pass of a
-// common prefix.  (In one kernel for all three, the last two cost plain calls 1 to 3 %.)
-enum Kv8Mode { kPlain, kFirst, kShared };
+// What a kernel is made for: plain calls; first tokens beside the window; either of two passes of a
+// common prefix; its only one.  (In one kernel for all, the others cost plain calls 1 to 3 %.)
+enum Kv8Mode { kPlain, kFirst, kShared, kJoint };
 inline Kv8Mode kv8_mode(const Kv8AttnArgs& a) { return a.raw || a.skip ? kShared : a.first > 0 ? kFirst : kPlain; }
 
 // A sequence as the line sees it.
@@ -92,6 +105,7 @@ struct Kv8Seq {
   int kept;          // tiles of the first tokens, which lie before the hidden ones
   int row_tiles;
   int skip;
+  int table_row, group;
 
   // the key tile that tile i of the item is
   template <int MODE>
@@ -101,8 +115,8 @@ struct Kv8Seq {
 };
 
 template <int RT, int TT, int MODE>
-__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n, int len, int skip) {
-  int lo = MODE == kShared ? skip : 0;
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n, int len, int skip, int group) {
+  int lo = MODE == kShared || MODE == kJoint ? skip : 0;
   if (a.causal && a.window > 0) {
     const int64_t first = (int64_t)len - n - a.window + 1;
     lo = first > 0 ? (int)first : 0;
@@ -116,13 +130,17 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8AttnArgs& a, int row0, int n,
   s.tile0 = MODE != kFirst || lo / TT > s.kept ? lo / TT - s.kept : 0;
   const int tiles = (len + TT - 1) / TT - s.tile0;
   s.tiles = tiles > 0 ? tiles : 1;
-  s.row_tiles = (n * a.G + RT - 1) / RT;
+  s.group = group;
+  if (MODE == kJoint && group == kIsGroup)
+    s.row_tiles = (n * a.G + a.group_rows - 1) / a.group_rows;
+  else
+    s.row_tiles = (n * a.G + RT - 1) / RT;
   return s;
 }
 
 // 64 sequences from b0 on, one a lane.
 struct Kv8Chunk {
-  int b0, row0, n, len, skip;
+  int b0, row0, n, len, skip, table_row, group;
   int room, rooms;  // places on the line: of this sequence, of those up to and with it
   int rts;          // row tiles of the sequences up to and with it
 };
@@ -130,18 +148,30 @@ struct Kv8Chunk {
 template <int RT, int TT, int MODE>
 __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
   const int b = b0 + (int)(threadIdx.x & 63);
-  Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0, 0};
+  Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   int rts = 0;
   if (b < a.B) {
-    const int len = a.lens[b], cap = a.row_pages << a.page_shift;
-    const SeqRows r = seq_rows(a.cu, b, a.T);
-    c.row0 = r.first;
-    c.n = r.n;
-    c.len = len < 0 ? 0 : len > cap ? cap : len;
-    if (MODE == kShared && a.skip) c.skip = a.skip[b];
-    const Kv8Seq s = kv8_seq<RT, TT, MODE>(a, c.row0, c.n, c.len, c.skip);
-    const int rows = r.n * a.G;
-    rts = rows > a.above && rows <= a.upto && !(MODE == kShared && a.raw && c.len == 0) ? s.row_tiles : 0;
+    if constexpr (MODE == kJoint) {
+      const Kv8Entry e = a.entries[b];
+      c.row0 = e.row0;
+      c.n = e.n;
+      c.len = e.len;
+      c.skip = e.skip;
+      c.table_row = e.table_row;
+      c.group = e.group;
+    } else {
+      const int len = a.lens[b], cap = a.row_pages << a.page_shift;
+      const SeqRows r = seq_rows(a.cu, b, a.T);
+      c.row0 = r.first;
+      c.n = r.n;
+      c.len = len < 0 ? 0 : len > cap ? cap : len;
+      if (MODE == kShared && a.skip) c.skip = a.skip[b];
+    }
+    const Kv8Seq s = kv8_seq<RT, TT, MODE>(a, c.row0, c.n, c.len, c.skip, c.group);
+    const int rows = c.n * a.G;
+    // (a group that shares nothing has no part in the work)
+    const bool none = c.len == 0 && ((MODE == kShared && a.raw) || (MODE == kJoint && c.group == kIsGroup));
+    rts = rows > a.above && rows <= a.upto && !none ? s.row_tiles : 0;
     c.room = rts * (s.tiles + kItemCost);
   }
   c.rooms = wave_incl_scan(c.room);
@@ -151,9 +181,12 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
 
 template <int RT, int TT, int MODE>
 __device__ __forceinline__ Kv8Seq kv8_lane(const Kv8AttnArgs& a, const Kv8Chunk& c, int l) {
-  return kv8_seq<RT, TT, MODE>(a, __builtin_amdgcn_readlane(c.row0, l), __builtin_amdgcn_readlane(c.n, l),
-                         __builtin_amdgcn_readlane(c.len, l),
-                         MODE == kShared ? __builtin_amdgcn_readlane(c.skip, l) : 0);
+  Kv8Seq s = kv8_seq<RT, TT, MODE>(a, __builtin_amdgcn_readlane(c.row0, l), __builtin_amdgcn_readlane(c.n, l),
+                                   __builtin_amdgcn_readlane(c.len, l),
+                                   MODE == kShared || MODE == kJoint ? __builtin_amdgcn_readlane(c.skip, l) : 0,
+                                   MODE == kJoint ? __builtin_amdgcn_readlane(c.group, l) : 0);
+  if (MODE == kJoint) s.table_row = __builtin_amdgcn_readlane(c.table_row, l);
+  return s;
 }
 
 // Length of a kv head's line; c: the batch's first 64 sequences.
@@ -391,6 +424,125 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(const Kv8AttnArgs a) {
   }
   y = kv8_joined<MODE>(a, kv8_join<MODE>(a, s, out, h, M, l), out, d, y);
   *reinterpret_cast<uint2*>(a.o + out * a.D + d) = make_uint2(kv8_out2<QT>(y.x, y.y), kv8_out2<QT>(y.z, y.w));
+}
+
+// The rows of a batch whose sequences and groups were on one line: a row's own parts and its
+// group's, one wavefront a row (a token's head).
+template <int RT, int TT, int QT>
+__global__ __launch_bounds__(256) void kv8_joint_merge_kernel(const Kv8AttnArgs a) {
+  const int lane = threadIdx.x & 63, sequences = a.B - a.groups;
+  const uint32_t heads = (uint32_t)(a.Hkv * a.G);
+  const uint32_t out = 4 * blockIdx.x + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tok = (int)(out / heads), h = (int)(out - (uint32_t)tok * heads);
+  if (tok >= a.T) return;
+  const int head = h / a.G;
+  // one walk over the line: the row's sequence, behind all of them its group, and the length
+  // (fewer than 2^31 places: the call is checked for it)
+  Kv8Seq s, gs;
+  int entry = -1, total = 0, room = 0, before = 0;
+  bool found = false;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const Kv8Chunk c = kv8_chunk<RT, TT, kJoint>(a, b0);
+    const uint64_t mine = __ballot(b0 + lane < sequences && tok >= c.row0 && tok < c.row0 + c.n);
+    auto rooms_before = [&](int l) { return total + (l > 0 ? __builtin_amdgcn_readlane(c.rooms, l - 1) : 0); };
+    if (!found && mine) {
+      const int l = __builtin_ctzll(mine);
+      found = true;
+      s = kv8_lane<RT, TT, kJoint>(a, c, l);
+      room = rooms_before(l);
+      if (s.skip > 0 && s.group >= 0) entry = sequences + s.group;
+    }
+    if (entry >= b0 && entry < b0 + 64) {
+      gs = kv8_lane<RT, TT, kJoint>(a, c, entry - b0);
+      before = rooms_before(entry - b0);
+    }
+    total += __builtin_amdgcn_readlane(c.rooms, 63);
+  }
+  if (!found) return;
+  const uint32_t per = ((uint32_t)total + a.parts - 1) / a.parts;
+  const int row = (tok - s.row0) * a.G + h - head * a.G;
+
+  // the row's sums: parts [pa, pb] of its item, or (one workgroup took it whole) by its place in the output
+  struct Source {
+    const float *acc, *ml;  // whole
+    int pa, n, r;
+  };
+  auto source = [&](int first, const Kv8Seq& q, uint32_t tile, int r, const float* acc, const float* ml) {
+    const uint32_t x = (uint32_t)first + tile * (uint32_t)(q.tiles + kItemCost) + kItemCost;
+    Source o = {acc + (int64_t)out * a.D, ml + 2 * (int64_t)out, (int)(x / per), 0, r};
+    o.n = (int)((x + q.tiles - 1) / per) - o.pa + 1;
+    return o;
+  };
+  const Source own = source(room, s, (uint32_t)row / RT, row % RT, a.own_acc, a.own_ml);
+  Source shared = own;
+  shared.n = 0;
+  if (entry >= 0) {
+    const int gr = (tok - gs.row0) * a.G + h - head * a.G;
+    const uint32_t tile = (uint32_t)gr / (uint32_t)a.group_rows;
+    if (gr >= 0 && gr < gs.n * a.G)
+      shared = source(before, gs, tile, gr - (int)tile * a.group_rows, a.prior_acc, a.prior_ml);
+  }
+  const int n = own.n + shared.n;
+  auto slot = [&](const Source& o, int i) {
+    return (2 * (int64_t)kv8_wg(a, head, o.pa + i) + (i == 0 ? 1 : 0)) * a.slot_rows + o.r;
+  };
+  auto acc_at = [&](int i) {
+    const bool mine = i < own.n;
+    const Source& o = mine ? own : shared;
+    return o.n == 1 ? o.acc : a.ws_acc + slot(o, mine ? i : i - own.n) * a.D;
+  };
+  auto ml_at = [&](int i) {
+    const bool mine = i < own.n;
+    const Source& o = mine ? own : shared;
+    return *reinterpret_cast<const float2*>(o.n == 1 ? o.ml : a.ws_ml + slot(o, mine ? i : i - own.n) * 2);
+  };
+
+  const float NEG_INF = -__builtin_huge_valf();
+  const int d = 4 * lane, dl = d < a.D ? d : 0;
+  auto fetch = [&](int i, float4* x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const float4*>(acc_at(i + k < n ? i + k : n - 1) + dl);
+  };
+  float4 x[8];
+  fetch(0, x);
+  float M = NEG_INF;
+  for (int i = lane; i < n; i += 64) M = __builtin_fmaxf(M, ml_at(i).x);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, k, 64));
+  const float ref = M == NEG_INF ? 0.0f : M;
+  float l = 0.0f, acc[4] = {0, 0, 0, 0};
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    float f = 0.0f;
+    if (i0 + lane < n) {
+      const float2 ml = ml_at(i0 + lane);
+      f = __builtin_amdgcn_exp2f(ml.x - ref);
+      l += ml.y * f;
+    }
+    const int m = n - i0 < 64 ? n - i0 : 64;
+    for (int i = 0; i < m; i += 8) {
+      float4 y[8];
+      if (i0 + i + 8 < n) fetch(i0 + i + 8, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (i + k < m) {
+          const float w = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(f), i + k));
+          acc[0] += x[k].x * w;
+          acc[1] += x[k].y * w;
+          acc[2] += x[k].z * w;
+          acc[3] += x[k].w * w;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = y[k];
+    }
+  }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k, 64);
+  if (a.sink) l += __builtin_amdgcn_exp2f(a.sink[h] * kLog2e - ref);
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  if (d < a.D)
+    *reinterpret_cast<uint2*>(a.o + (int64_t)out * a.D + d) =
+        make_uint2(kv8_out2<QT>(acc[0] * inv, acc[1] * inv), kv8_out2<QT>(acc[2] * inv, acc[3] * inv));
 }
 
 // kv8_prefill.hip: row tiles of kv8_chunk_rows(D).

@@ -357,6 +357,12 @@ SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G,
   const int64_t rt = kv8_few_tile(rows, D), items = kv8_attn_items(T, B, Hkv, G, rt);
   return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, 0x7FFFFFFF};
 }
+#ifndef FIRST_A
+#define FIRST_A 1024
+#endif
+#ifndef FIRST_B
+#define FIRST_B 2048
+#endif
 // What stands for the block table's width where first tokens are seen beside a window: the keys
 // that a row tile's queries can see between them.
 SGL_RULE int64_t kv8_attn_reach(int64_t T, int64_t B, int64_t capacity, int64_t window, int64_t first) {
@@ -371,6 +377,33 @@ SGL_RULE Kv8AttnPlan kv8_attn_rest(int64_t T, int64_t B, int64_t Hkv, int64_t G,
   const int64_t rt = kv8_few_tile(G, D), upto = kv8_few_rows(D);
   const int64_t items = B * ((upto + rt - 1) / rt) * Hkv;
   return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, upto};
+}
+
+// ---- attention of sequences that share a prefix: in one pass, the few rows' kernel over the
+// sequences and over tiles of 16 or 32 rows of their groups on one line; or (items 0) the groups by
+// chunks' kernel first, whose tiles of 256 rows read the prefix once, and the sequences behind it.
+// One pass / two, us, by 4 T heads D capacity (the capacity standing for the prefix) in 1e9; rows of
+// a group, heads of 128:
+//   8.4: 128 rows 37 / 58; 13: 192 rows 47 / 67; 15: 800 rows 62 / 81; 17: 256 rows 56 / 75; 19: 480
+//   rows 72 / 87; 20: 160 rows 76 / 82; 21: 1024 rows 97 / 115; 33: 256 rows 106 / 97, 512 rows 93 / 87; 36: 512 rows 98 / 96; 150: 1024 rows 285 / 196
+//   of 64: 18: 512 rows 79 / 86; 65: 1024 rows 189 / 147; of 256: 16: 128 rows 65 / 80; 18: 512 rows 60 / 81
+// One workgroup a CU / two (heads of 128): 16 rows 20 / 20, 64 rows 25 / 27, 128 rows 37 / 38, 192 47 /
+// 47, 256 59 / 56, 480 79 / 72, 800 67 / 62.
+struct Kv8JointPlan {
+  int64_t row_tile, group_rows, slot_rows;  // of a sequence's tile, of a group's, of a part
+  int64_t per_cu, parts;
+  int64_t items, group_items;  // at most
+};
+SGL_RULE Kv8JointPlan kv8_joint_plan(int64_t T, int64_t B, int64_t groups, int64_t Hkv, int64_t G, int64_t D,
+                                     int64_t capacity, int64_t cus) {
+  const int64_t rows = B > 0 ? T * G / B : 0, group_rows = groups > 0 ? T * G / groups : 0;
+  if (rows > kv8_few_rows(D) ||
+      (group_rows > kv8_few_rows(D) && (double)(T * Hkv * G * D) * (double)capacity > 7e9))
+    return {0, 0, 0, 0, 0, 0, 0};
+  const int64_t rt = kv8_few_tile(rows, D), rg = rt > 16 || group_rows > 16 ? 32 : 16;
+  const int64_t per_cu = D <= 64 || (D <= 128 && group_rows > 160) ? 2 : 1;
+  return {rt, rg, rg, per_cu, kv8_attn_parts(per_cu * cus, Hkv), kv8_attn_items(T, B, Hkv, G, rt),
+          kv8_attn_items(T, groups, Hkv, G, rg)};
 }
 
 }  // namespace sgl

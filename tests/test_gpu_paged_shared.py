@@ -40,7 +40,7 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("tokens", [0, 16384])
+@pytest.mark.parametrize("tokens", [0, 16384, 1 << 18])  # (wide tables: many rows in two passes)
 @pytest.mark.parametrize("new,lens,cu_groups,shared,Hq,Hkv,D,page,block,dtype,causal,sink", CASES)
 def test_shared_prefix(gpu, tokens, new, lens, cu_groups, shared, Hq, Hkv, D, page, block, dtype, causal, sink):
     print(f"shared new={new} lens={lens} groups={cu_groups} {shared} Hq={Hq} Hkv={Hkv} D={D} page={page}", flush=True)
@@ -58,18 +58,15 @@ def test_shared_prefix(gpu, tokens, new, lens, cu_groups, shared, Hq, Hkv, D, pa
 
 def test_what_is_claimed_may_be_more_or_less_than_what_is_there(gpu):
     """More tokens than any sequence has, none, a negative number; groups that reach past the batch or
-    begin before it: as without."""
+    begin before it.  (The sums' order is the call's own even where nothing is shared.)"""
     lens = [500, 420, 700, 300]
     c = _filled(gpu, lens, 2, 64, 16, 16, seed=3)
     join_tables(c, [0, 4], [299])
     c.table[1:, :300 // 16] = c.table[0, :300 // 16]
     c.bt = torch.from_numpy(c.table).to(gpu)
     q = _queries(gpu, 4, 8, 64, torch.float16, 4)
-    plain = c.P.paged_attn(q, c.kv, c.bt, ints(lens, gpu))
     for groups, shared in (([0, 4], [0]), ([0, 4], [-5]), ([0, 4], [127]), ([4, 4], [256]), ([0, 0], [256]),
-                           ([2, 3], [256]), ([-3, 1], [256]), ([3, 9], [256])):
-        assert torch.equal(_call(c, q, lens, None, groups, shared), plain), (groups, shared)
-    for groups, shared in (([0, 4], [2 ** 31 - 1]), ([0, 4], [299]), ([-1, 7], [299]), ([0, 3], [256]), ([1, 4], [300])):
+                           ([2, 3], [256]), ([-3, 1], [256]), ([3, 9], [256]), ([0, 4], [2 ** 31 - 1]), ([0, 4], [299]), ([-1, 7], [299]), ([0, 3], [256]), ([1, 4], [300])):
         o = _call(c, q, lens, None, groups, shared)
         check(c, o, q, lens, None, parts=2)
 
@@ -99,13 +96,13 @@ def test_parts_whose_references_lie_far_apart(gpu, new, lead):
         check(c, _call(c, q, [L] * B, cu, [0, B], [640]), q, [L] * B, cu, parts=2)
 
 
-@pytest.mark.parametrize("new,B", [(1, 3), (1, 40), (50, 3)])
-def test_every_key_counts_once(gpu, new, B):
+@pytest.mark.parametrize("new,B,tokens", [(1, 3, 16384), (1, 40, 16384), (2, 40, 1 << 18), (50, 3, 16384)])
+def test_every_key_counts_once(gpu, new, B, tokens):
     """Values of zero but for one key in each dim of a kv head: the output is that key's weight."""
     L, H, D = 1100, 8, 64
     c = Cache(gpu, B, L, H, D, 16, 16, seed=4)
     join_tables(c, [0, B], [770])
-    _widen(c, 16384)
+    _widen(c, tokens)
     g = torch.Generator(device=gpu).manual_seed(L)
     k = 0.5 * torch.randn(L, H, D, generator=g, device=gpu)
     q = _queries(gpu, B * new, 2 * H, D, torch.float16, 11)
@@ -122,12 +119,14 @@ def test_every_key_counts_once(gpu, new, B):
         check(c, _call(c, q, [L] * B, cu, [0, B], [770]), q, [L] * B, cu, rms=False, parts=2)
 
 
-@pytest.mark.parametrize("new,D", [(1, 128), (6, 64), (40, 256), (60, 128)])
-def test_nan_reaches_only_the_rows_that_see_it(gpu, new, D):
+@pytest.mark.parametrize("new,D,tokens", [(1, 128, 0), (6, 64, 0), (20, 128, 0), (20, 128, 1 << 18), (40, 256, 0),
+                                          (60, 128, 0)])
+def test_nan_reaches_only_the_rows_that_see_it(gpu, new, D, tokens):
     """In a common page: every sequence of the group; behind it: its own."""
     lens = [700, 650, 800]
     c = _filled(gpu, lens, 2, D, 64, 16, seed=11)
     join_tables(c, [0, 2], [600])
+    _widen(c, tokens)
     spots = [(0, 5, 0, 3), (0, 639, 1, 9), (1, 640 - 64, 0, 4), (2, 100, 0, 11)]  # sequence, token, head, dim
     for b, t, h, d in spots:
         p, spot = int(c.table[b, t // 64]), t % 64
@@ -172,7 +171,7 @@ def test_many_groups_of_many_sizes(gpu, D, Hq, Hkv):
     join_tables(c, edge, shared)
     cu = [0] + np.cumsum(new).tolist()
     q = _queries(gpu, cu[-1] + 3, Hq, D, torch.float16, 6)
-    for tokens in (0, 8192):
+    for tokens in (0, 8192, 1 << 18):
         _widen(c, tokens)
         out = torch.full_like(q, 7.0)
         o = _call(c, q, lens, cu, edge, shared, out=out)
