@@ -578,9 +578,9 @@ void launch_joint(const Kv8AttnArgs& a, const Kv8JointPlan& p, hipStream_t st) {
 struct AttnPlans {
   Kv8AttnPlan p[2];  // one launch, or (chunks and few rows in one batch) two, one after the other on the same workspace
 };
-AttnPlans attn_plans(int64_t T, int64_t B, int Hkv, int G, int D, int64_t tokens) {
+AttnPlans attn_plans(int64_t T, int64_t B, int Hkv, int G, int D, int64_t tokens, bool window = false) {
   const int cus = device_cu_count();
-  return {{kv8_attn_plan(T, B, Hkv, G, D, tokens, cus), kv8_attn_rest(T, B, Hkv, G, D, tokens, cus)}};
+  return {{kv8_attn_plan(T, B, Hkv, G, D, tokens, cus, window), kv8_attn_rest(T, B, Hkv, G, D, tokens, cus, window)}};
 }
 size_t attn_workspace(const AttnPlans& plans, int Hkv, int D) {
   const size_t x = kv8_attn_workspace(plans.p[0], Hkv, D), y = kv8_attn_workspace(plans.p[1], Hkv, D);
@@ -821,7 +821,7 @@ size_t sgl_kv8_attn_first_workspace_size(int64_t T, int64_t B, int Hkv, int G, i
                                          int64_t window, int64_t first) {
   if (!sgl::attn_sizes_ok(T, B, Hkv, G, D, max_tokens) || window < 0 || first < 0) return 0;
   return sgl::attn_workspace(
-      sgl::attn_plans(T, B, Hkv, G, D, sgl::kv8_attn_reach(T, B, max_tokens, window, first)), Hkv, D);
+      sgl::attn_plans(T, B, Hkv, G, D, sgl::kv8_attn_reach(T, B, max_tokens, window, first), first > 0), Hkv, D);
 }
 
 int sgl_kv8_attn_first(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T, int64_t B,
@@ -840,7 +840,7 @@ int sgl_kv8_attn_first(const void* q, int64_t q_token_stride, int64_t q_head_str
   if (rc != SGL_OK || nothing) return rc;
   const int64_t tokens = row_pages * page_size, reach = sgl::kv8_attn_reach(T, B, tokens, window, first);
   a.first = a.window == 0 ? 0 : (int)(first < tokens ? first : tokens);
-  const sgl::AttnPlans plans = sgl::attn_plans(T, B, Hkv, G, D, reach);
+  const sgl::AttnPlans plans = sgl::attn_plans(T, B, Hkv, G, D, reach, first > 0);
   rc = sgl::check_workspace(workspace, workspace_bytes, sgl::attn_workspace(plans, Hkv, D));
   if (rc == SGL_OK) rc = sgl::check_plans(plans, tokens);
   if (rc != SGL_OK) return rc;

@@ -313,6 +313,16 @@ SGL_RULE int64_t kv8_attn_items(int64_t T, int64_t B, int64_t Hkv, int64_t G, in
 SGL_RULE bool kv8_attn_whole(int64_t capacity, int64_t items, int64_t cus) {
   return capacity <= 1024 || (capacity <= 2048 && items >= 2 * cus);
 }
+// The same beside first tokens, where the window and they bound an item (reach): the items
+// of long sequences are alike, and shared lines even out nothing but what is left of the last round of
+// CUs, at the cost of a merge and starts, some 13 key tiles' time.  Items whole / shared, us, 8 kv heads of 128, first tokens and a window of:
+//   1 sequence 500 11 / 16, 1024 14 / 16, 1500 17 / 15.5; 16: 1024 18 / 22, 2000 25 / 26, 3000 33 / 29;
+//   32: 3000 38 / 47, 4096 48 / 56; 40: 4096 80 / 67; 64: 2000 50 / 64, 4096 89 / 97, 8000 160 / 160, 16000
+//   293 / 252 (of sequences up to 30000: the short ones end early); 128: 4096 178 / 183, 8000 326 / 309
+SGL_RULE bool kv8_window_whole(int64_t reach, int64_t items, int64_t cus) {
+  const int64_t tiles = (reach + 127) / 128 + 3;
+  return reach <= 6000 && (items + cus - 1) / cus * tiles * cus <= items * tiles + 13 * cus;
+}
 constexpr int64_t kv8_chunk_rows(int64_t D) { return D > 64 && D <= 128 ? 256 : 128; }
 // Few rows or a chunk, by a sequence's rows on a kv head (few / chunk, us, 4 query heads
 // to each of 8 kv heads; 1 sequence of 16000 tokens and 8 of 4000).  Heads of 128: 64 rows
@@ -345,8 +355,9 @@ SGL_RULE bool kv8_chunk_whole(int64_t capacity, int64_t items, int64_t fit) {
 // rows 21 / 22 and 32 / 30, 48 rows 27 / 25 and 43 / 35, 64 rows 28 / 25 and 54 / 39; 32
 // sequences of 16 rows up to 6000 49 / 57.  Heads above 128 have no room for 32.
 SGL_RULE int64_t kv8_few_tile(int64_t rows, int64_t D) { return D <= 128 && rows > 16 ? 32 : 16; }
+// window: the capacity is what a window and first tokens reach.
 SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
-                                   int64_t cus) {
+                                   int64_t cus, bool window = false) {
   const int64_t rows = B > 0 ? T * G / B : 0;  // of a sequence and kv head, on average
   if (rows > kv8_few_rows(D)) {
     const int64_t rt = kv8_chunk_rows(D), items = kv8_attn_items(T, B, Hkv, G, rt);
@@ -355,14 +366,10 @@ SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G,
             kv8_attn_mixed(T, B, G, D) ? kv8_few_rows(D) : 0, 0x7FFFFFFF};
   }
   const int64_t rt = kv8_few_tile(rows, D), items = kv8_attn_items(T, B, Hkv, G, rt);
-  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, 0x7FFFFFFF};
+  const bool whole = window ? kv8_window_whole(capacity, Hkv * B * ((rows + rt - 1) / rt), cus)
+                            : kv8_attn_whole(capacity, items, cus);
+  return {rt, whole ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, 0x7FFFFFFF};
 }
-#ifndef FIRST_A
-#define FIRST_A 1024
-#endif
-#ifndef FIRST_B
-#define FIRST_B 2048
-#endif
 // What stands for the block table's width where first tokens are seen beside a window: the keys
 // that a row tile's queries can see between them.
 SGL_RULE int64_t kv8_attn_reach(int64_t T, int64_t B, int64_t capacity, int64_t window, int64_t first) {
@@ -372,11 +379,14 @@ SGL_RULE int64_t kv8_attn_reach(int64_t T, int64_t B, int64_t capacity, int64_t 
 }
 // The second launch of a batch of chunks: its sequences of few rows.
 SGL_RULE Kv8AttnPlan kv8_attn_rest(int64_t T, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t capacity,
-                                   int64_t cus) {
+                                   int64_t cus, bool window = false) {
   if (!kv8_attn_mixed(T, B, G, D)) return {16, 0, 0, 0, 0};
   const int64_t rt = kv8_few_tile(G, D), upto = kv8_few_rows(D);
   const int64_t items = B * ((upto + rt - 1) / rt) * Hkv;
-  return {rt, kv8_attn_whole(capacity, items, cus) ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, upto};
+  // (single tokens, for the most part)
+  const bool whole = window ? kv8_window_whole(capacity, Hkv * B * ((G + rt - 1) / rt), cus)
+                            : kv8_attn_whole(capacity, items, cus);
+  return {rt, whole ? 0 : kv8_few_parts(D, Hkv, cus), items, 0, upto};
 }
 
 // ---- attention of sequences that share a prefix: in one pass, the few rows' kernel over the
