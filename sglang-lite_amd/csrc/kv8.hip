@@ -123,9 +123,8 @@ __device__ __forceinline__ void turns_of(const AppendArgs& a, const AxisPosition
   bool same = true;
 #pragma unroll
   for (int i = 1; i < 8; ++i) same = same & (axis[i] == axis[0]);
-  auto place = [&](int x) { return x == 0 ? at.p[0] : x == 1 ? at.p[1] : x == 2 ? at.p[2] : x == 3 ? at.p[3] : n; };
   if (__ballot(at.turn && !same) == 0) {
-    if (at.turn) load_turn<8>(a.table, n, pairs, place(axis[0]), pair, false, cos, sin);
+    if (at.turn) load_turn<8>(a.table, n, pairs, at.of(axis[0], n), pair, false, cos, sin);
     return;
   }
   float2* turns = sTurn[threadIdx.x >> 6];
@@ -137,7 +136,7 @@ __device__ __forceinline__ void turns_of(const AppendArgs& a, const AxisPosition
   int e[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int p = place(axis[i]);
+    const int p = at.of(axis[i], n);
     e[i] = at.turn && p < n ? p * pairs + pair + i : -1;
   }
   fence();

@@ -46,7 +46,8 @@ constexpr int kHeads = 4;  // heads of a thread in flight
 // STAGE (several axes, 16-byte accesses): the rotations of the wavefront's tokens go through LDS.
 // A pair's table entry lies in its axis' row, so a thread's 8 are up to 8 pieces of 8 bytes, and
 // all threads of a token load the same ones: by themselves 16384 tokens of 32 heads of 128
-// take 71 us.
+// take 71 us, so 51 (5.4 TB/s, as with one position).  16 tokens: 3.9 us, the chain position ->
+// table -> rows, which a launch's own time on the host passes.
 // AXES: 0, or several with positions of 32 or 64 bits.
 template <int DT, int VEC, int AXES>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     auto fetch = [&](int e) __attribute__((always_inline)) {
       const int tok = e / pairs, pair = e - tok * pairs, axis = a.axes[pair];
       const AxisPositions at = load_axis_positions<POS64>(a.positions, a.n_axes, a.T, t0 + tok, (int)a.n_positions);
-      const int p = axis == 0 ? at.p[0] : axis == 1 ? at.p[1] : axis == 2 ? at.p[2] : axis == 3 ? at.p[3] : (int)a.n_positions;
+      const int p = at.of(axis, (int)a.n_positions);
       const bool in = p >= 0 && p < a.n_positions;  // (a token with a negative one is not turned)
       const float2 w = reinterpret_cast<const float2*>(a.table)[(int64_t)(in ? p : 0) * pairs + pair];
       return make_float2(in ? w.x : __builtin_nanf(""), in ? (a.inverse ? -w.y : w.y) : __builtin_nanf(""));
@@ -147,9 +148,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   } else if (AXES != 0 && u < rot_units) {
     const AxisPositions at = load_axis_positions<POS64>(a.positions, a.n_axes, a.T, t, (int)a.n_positions);
     turn = at.turn;
-    uint8_t axis[VEC];
-    __builtin_memcpy(axis, a.axes + VEC * u, VEC);
-    if (turn) load_turn_axes<VEC>(a.table, (int)a.n_positions, a.rot / 2, at, axis, VEC * u, a.inverse, cs, sn);
+    const int p = at.of(a.axes[u], (int)a.n_positions);  // (a pair a thread)
+    if (turn) load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, u, a.inverse, cs, sn);
   } else if (u < rot_units) {
     const int64_t p = a.pos64 ? ((const int64_t*)a.positions)[t] : ((const int32_t*)a.positions)[t];
     turn = p >= 0;

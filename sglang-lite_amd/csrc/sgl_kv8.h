@@ -130,16 +130,18 @@ __device__ __forceinline__ void load_turn(const float* table, int64_t n_position
   }
 }
 
-// A token's positions on up to four axes, and cos and sin of N pairs that turn by one of
-// them each (`axes`: a byte for each pair).  The positions are loaded beside the pairs' axes and
-// chosen in registers, so that the chain to the table is no longer than with one position; and
-// without branches, so that no load waits for another (an axis too many loads the first again).
-// Behind the table, and for an axis that there is none of: NaN, as above.  `turn` is false
-// where any of them is negative.
+// A token's positions on up to four axes, each pair turning by one of them.  All are loaded beside
+// the pairs' axes and chosen in registers, so that the chain to the table is no longer than with
+// one position; and without branches, so that no load waits for another (an axis too many loads
+// the first again).  Behind the table, and for an axis that there is none of: NaN, as above.
+// `turn` is false where any of them is negative.
 constexpr int kMaxAxes = 4;
 struct AxisPositions {
   int p[kMaxAxes];  // at most n_positions, which is behind the table
   bool turn;
+  __device__ __forceinline__ int of(int axis, int n_positions) const {
+    return axis == 0 ? p[0] : axis == 1 ? p[1] : axis == 2 ? p[2] : axis == 3 ? p[3] : n_positions;
+  }
 };
 template <bool POS64>
 __device__ __forceinline__ int64_t load_position(const void* positions, int64_t at) {
@@ -160,23 +162,6 @@ __device__ __forceinline__ AxisPositions load_axis_positions(const void* positio
   }
   return o;
 }
-template <int N>
-__device__ __forceinline__ void load_turn_axes(const float* table, int n_positions, int pairs, const AxisPositions& at,
-                                               const uint8_t* axis, int pair, bool inverse, float* cos, float* sin) {
-  bool same = true;
-#pragma unroll
-  for (int i = 1; i < N; ++i) same = same && axis[i] == axis[0];
-  auto place = [&](int a) {
-    return a == 0 ? at.p[0] : a == 1 ? at.p[1] : a == 2 ? at.p[2] : a == 3 ? at.p[3] : n_positions;
-  };
-  if (same) {  // sections of whole chunks: consecutive entries of one row, in 16-byte loads
-    load_turn<N>(table, n_positions, pairs, place(axis[0]), pair, inverse, cos, sin);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) load_turn<1>(table, n_positions, pairs, place(axis[i]), pair + i, inverse, cos + i, sin + i);
-}
-
 // Sum over the lanes up to and with this one, by DPP moves: within rows of 16,
 // then each row's last lane to the row behind it, then lane 31 to the upper half.
 __device__ __forceinline__ int wave_incl_scan(int v) {

@@ -249,10 +249,10 @@ SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cu
 }
 
 // ---- norms between blocks: threads of a row's workgroup, units of 8 elements a
-// thread, and workgroups.
-#ifndef NORM_ONCE
-#define NORM_ONCE 128
-#endif
+// thread, and workgroups.  One unit a thread as far as a workgroup's 1024 threads reach: its
+// weights and the next row's loads fit the registers then.  One unit / two, us: 16384 x 4096
+// 102 / 143.  Workgroups that together have 1536 threads a CU, 16384 x 4096, us: 94.8, with 1024
+// 97, with 2048 105.
 constexpr int64_t kNormMost = 16384;  // elements of a row: 1024 threads of two units
 struct NormPlan {
   int64_t threads, units, grid;
@@ -263,7 +263,11 @@ SGL_RULE NormPlan norm_plan(int64_t T, int64_t row_units, int64_t cus) {
   const int64_t most = cus * (1536 / threads);
   return {threads, units, T < most ? T : most};
 }
-SGL_RULE bool norm_once(int64_t T, int64_t H) { return 4 * T * H > ((int64_t)NORM_ONCE << 20); }
+// Rows that pass the last-level cache by: where the two inputs, of 16 bits, hold more than 128 MiB.
+// By / through, us: 16384 x 4096 with both norms 78.8 / 93, with one 81 / 104, 6000 x 7168 60.7 /
+// 65.6, 8192 x 4096 (at the bound) 43 / 43; below it what the block before left in the cache is
+// read from there.
+SGL_RULE bool norm_once(int64_t T, int64_t H) { return 4 * T * H > 128ll << 20; }
 
 // ---- append to the 8-bit cache: the most blocks that T tokens of B sequences
 // touch.  n tokens touch at most (n - 2) / block + 2, and no more than n.

@@ -124,6 +124,10 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torc
         _check_apart(xr, rr, "x")
         if gate_rows:
             _check_apart(gate, rr, "the gate")
+        elif gate is not None:
+            _check_weight(gate, rr, "the gate")
+        _check_weight(before, rr, "before")
+        _check_weight(after, rr, "after")
         out = residual
     else:
         rr, rs = _rows(residual, H)
@@ -157,6 +161,15 @@ def _check_apart(x: torch.Tensor, h: torch.Tensor, name: str) -> None:
     if a == b and x.dtype is h.dtype and x.stride(0) == h.stride(0):
         return
     raise ValueError(f"residual_norm: the residual written in place overlaps {name} without being it")
+
+
+def _check_weight(w: Optional[torch.Tensor], h: torch.Tensor, name: str) -> None:
+    """Refuse a weight that lies among the rows of an in-place residual: other rows still read it."""
+    if w is None or h.shape[0] == 0:
+        return
+    a, b = w.data_ptr(), h.data_ptr()
+    if b < a + w.numel() * w.element_size() and a < b + ((h.shape[0] - 1) * h.stride(0) + h.shape[1]) * h.element_size():
+        raise ValueError(f"residual_norm: the residual written in place overlaps {name}")
 
 
 __all__ = ["residual_norm"]

@@ -165,6 +165,11 @@ def test_in_place(gpu):
         residual_norm(buf[:T], buf[1:], w, inplace=True)
     with pytest.raises(ValueError, match="overlaps the gate"):
         residual_norm(x, buf[1:], w, gate=buf[:T], inplace=True)
+    both = torch.randn(T + 1, H, device=gpu)
+    for name, given in (("the gate", {"gate": both[0]}), ("before", {"before": both[0]}), ("after", {"after": both[T]})):
+        with pytest.raises(ValueError, match=f"overlaps {name}"):
+            residual_norm(x, both[:T] if name != "after" else both[1:], **given, inplace=True)
+    residual_norm(x, both[1:], both[0], inplace=True)
     with pytest.raises(ValueError, match="inplace"):
         residual_norm(x[:1].expand(T, H), buf[:1].expand(T, H), w, inplace=True)
 
