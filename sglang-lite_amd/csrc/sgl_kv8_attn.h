@@ -479,7 +479,8 @@ __global__ __launch_bounds__(256) void kv8_joint_merge_kernel(const Kv8AttnArgs 
   if (entry >= 0) {
     const int gr = (tok - gs.row0) * a.G + h - head * a.G;
     const uint32_t tile = (uint32_t)gr / (uint32_t)a.group_rows;
-    if (gr >= 0 && gr < gs.n * a.G)
+    // (a group without keys has no place on the line: falling cu_groups could name one)
+    if (gr >= 0 && gr < gs.n * a.G && gs.len > 0)
       shared = source(before, gs, tile, gr - (int)tile * a.group_rows, a.prior_acc, a.prior_ml);
   }
   const int n = own.n + shared.n;
