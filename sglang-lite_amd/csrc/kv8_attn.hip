@@ -687,12 +687,7 @@ void launch_plans(const Kv8AttnArgs& a, int dtype, const AttnPlans& plans, hipSt
   }
 }
 
-// ---- a common prefix.  A group's queries all see the keys [0, covered), so that pass takes
-// the group as one sequence, whose rows meet the keys' tiles together; the second pass
-// takes every sequence from there on.  `covered` is what the caller says, cut to whole
-// pages and key tiles (of every kernel: 128 tokens), and to what lies before the first query of
-// each sequence of the group that has any; 0 for a group of fewer than two such.
-constexpr int kPrefixTile = 128;
+// ---- a common prefix: what its groups cover.
 struct PrefixPlan {
   int32_t *cu, *lens, *row;  // of the groups: first token rows [n + 1], covered tokens, a row of the block table
   int32_t* skip;             // of the sequences: covered tokens
@@ -755,8 +750,7 @@ __global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, co
     most = part[i][0] < most ? part[i][0] : most;
     with += part[i][1];
   }
-  const int unit = kPrefixTile > (1 << a.page_shift) ? kPrefixTile : 1 << a.page_shift;
-  const int covered = with < 2 || most < unit ? 0 : most & ~(unit - 1);
+  const int covered = kv8_covered(a, most, with);
   for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) cover(b, covered, g);
   if (threadIdx.x == 0 && o.entries) {
     const int row0 = row_of(b0), end = b1 > b0 ? row_of(b1) : row0;
@@ -896,7 +890,8 @@ int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_st
   a.prior_acc = (float*)(base + space.acc);
   a.prior_ml = (float*)(base + space.ml);
   const hipStream_t st = (hipStream_t)stream;
-  sgl::kv8_prefix_kernel<<<(unsigned)(n + 1), 256, 0, st>>>(a, cu_groups, shared, (int)n, plan);
+  const bool planned = !joint || !sgl::kv8_joint_alone(B, n);
+  if (planned) sgl::kv8_prefix_kernel<<<(unsigned)(n + 1), 256, 0, st>>>(a, cu_groups, shared, (int)n, plan);
   if (joint) {
     const sgl::Kv8JointPlan& p = space.joint;
     a.B = (int)(B + n);
@@ -906,7 +901,9 @@ int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_st
     a.parts = (int)p.parts;
     a.above = 0;
     a.upto = 0x7FFFFFFF;
-    a.entries = plan.entries;
+    a.entries = planned ? plan.entries : nullptr;
+    a.cu_groups = cu_groups;
+    a.shared = shared;
     a.own_acc = (float*)(base + space.own_acc);
     a.own_ml = (float*)(base + space.own_ml);
     a.ws_ml = a.ws_acc + 2 * p.parts * Hkv * p.slot_rows * D;

@@ -65,7 +65,8 @@ struct Kv8AttnArgs {
   bool raw;
   // In one: the sequences and behind them the groups on one line, `entries` of them B; whole
   // items go to `prior` (groups) and `own` (sequences).
-  const struct Kv8Entry* entries;
+  const struct Kv8Entry* entries;  // null: 64 at most, and each workgroup finds them by itself
+  const int32_t *cu_groups, *shared;  // of the caller
   int groups, group_rows, slot_rows;  // of them; rows of a group's tile; of a part
   float *own_acc, *own_ml;
 };
@@ -145,11 +146,26 @@ struct Kv8Chunk {
   int rts;          // row tiles of the sequences up to and with it
 };
 
+// The chunk's places, once its sequences are there.
+template <int RT, int TT, int MODE>
+__device__ __forceinline__ void kv8_places(const Kv8AttnArgs& a, Kv8Chunk& c) {
+  int rts = 0;
+  if (c.b0 + (int)(threadIdx.x & 63) < a.B) {
+    const Kv8Seq s = kv8_seq<RT, TT, MODE>(a, c.row0, c.n, c.len, c.skip, c.group);
+    const int rows = c.n * a.G;
+    // (a group that shares nothing has no part in the work)
+    const bool none = c.len == 0 && ((MODE == kShared && a.raw) || (MODE == kJoint && c.group == kIsGroup));
+    rts = rows > a.above && rows <= a.upto && !none ? s.row_tiles : 0;
+    c.room = rts * (s.tiles + kItemCost);
+  }
+  c.rooms = wave_incl_scan(c.room);
+  c.rts = wave_incl_scan(rts);
+}
+
 template <int RT, int TT, int MODE>
 __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
   const int b = b0 + (int)(threadIdx.x & 63);
   Kv8Chunk c = {b0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  int rts = 0;
   if (b < a.B) {
     if constexpr (MODE == kJoint) {
       const Kv8Entry e = a.entries[b];
@@ -167,16 +183,87 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
       c.len = len < 0 ? 0 : len > cap ? cap : len;
       if (MODE == kShared && a.skip) c.skip = a.skip[b];
     }
-    const Kv8Seq s = kv8_seq<RT, TT, MODE>(a, c.row0, c.n, c.len, c.skip, c.group);
-    const int rows = c.n * a.G;
-    // (a group that shares nothing has no part in the work)
-    const bool none = c.len == 0 && ((MODE == kShared && a.raw) || (MODE == kJoint && c.group == kIsGroup));
-    rts = rows > a.above && rows <= a.upto && !none ? s.row_tiles : 0;
-    c.room = rts * (s.tiles + kItemCost);
   }
-  c.rooms = wave_incl_scan(c.room);
-  c.rts = wave_incl_scan(rts);
+  kv8_places<RT, TT, MODE>(a, c);
   return c;
+}
+
+// ---- a common prefix.  A group's queries all see the keys [0, covered), so the group is taken
+// as one sequence of these keys, whose rows meet the keys' tiles together, and each of its sequences
+// from there on.  `covered` is what the caller says, cut to whole pages and key tiles (of every
+// kernel: 128 tokens), and to what lies before the first query (`most`) of each of the group's
+// sequences that has any (`with` of them); 0 for a group of fewer than two such.
+constexpr int kPrefixTile = 128;
+__device__ __forceinline__ int kv8_covered(const Kv8AttnArgs& a, int most, int with) {
+  const int unit = kPrefixTile > (1 << a.page_shift) ? kPrefixTile : 1 << a.page_shift;
+  return with < 2 || most < unit ? 0 : most & ~(unit - 1);
+}
+
+// Least of a wavefront by DPP moves, the same in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int least_moved(int v) {
+  const int o = __builtin_amdgcn_update_dpp(0x7FFFFFFF, v, CTRL, ROWS, 0xF, false);
+  return o < v ? o : v;
+}
+__device__ __forceinline__ int wave_min(int v) {
+  v = least_moved<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = least_moved<0x112, 0xF>(v);
+  v = least_moved<0x114, 0xF>(v);
+  v = least_moved<0x118, 0xF>(v);
+  v = least_moved<0x142, 0xA>(v);  // row_bcast 15
+  v = least_moved<0x143, 0xC>(v);  // row_bcast 31
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// All of a line of up to 64 sequences and groups, without a launch before that plans it: a sequence
+// or group a lane, each group's covered tokens from its lanes.
+template <int RT, int TT>
+__device__ __forceinline__ Kv8Chunk kv8_joint_chunk(const Kv8AttnArgs& a) {
+  const int lane = (int)(threadIdx.x & 63), sequences = a.B - a.groups;
+  Kv8Chunk c = {0, 0, 0, 0, 0, lane, -1, 0, 0, 0};
+  int e0 = 0, e1 = 0, most = 0;  // of a group: its sequences, what the caller says
+  if (lane < sequences) {
+    const int len = a.lens[lane], cap = a.row_pages << a.page_shift;
+    const SeqRows r = seq_rows(a.cu, lane, a.T);
+    c.row0 = r.first;
+    c.n = r.n;
+    c.len = len < 0 ? 0 : len > cap ? cap : len;
+  } else if (lane < a.B) {
+    auto edge = [&](int b) { return b < 0 ? 0 : b > sequences ? sequences : b; };
+    e0 = edge(a.cu_groups[lane - sequences]);
+    e1 = edge(a.cu_groups[lane - sequences + 1]);
+    most = a.shared[lane - sequences];
+  }
+  const int behind = __builtin_amdgcn_readlane(c.row0 + c.n, sequences - 1);  // the last one's rows
+  for (int l = sequences; l < a.B; ++l) {
+    const int b0 = __builtin_amdgcn_readlane(e0, l), b1 = __builtin_amdgcn_readlane(e1, l);
+    const bool in = lane >= b0 && lane < b1, counts = in && c.n > 0;
+    const int least = wave_min(counts ? c.len - c.n : 0x7FFFFFFF), said = __builtin_amdgcn_readlane(most, l);
+    const int covered = kv8_covered(a, least < said ? least : said, __builtin_popcountll(__ballot(counts)));
+    if (in) {
+      c.skip = c.n ? covered : 0;
+      c.group = l - sequences;
+    }
+    const int first = b0 < sequences ? __builtin_amdgcn_readlane(c.row0, b0) : behind;
+    const int end = b1 < sequences ? __builtin_amdgcn_readlane(c.row0, b1) : behind;
+    if (lane == l) {
+      c.row0 = first;
+      c.n = b1 > b0 && end > first ? end - first : 0;
+      c.len = covered;
+      c.table_row = b0 < sequences ? b0 : 0;
+      c.group = kIsGroup;
+    }
+  }
+  kv8_places<RT, TT, kJoint>(a, c);
+  return c;
+}
+// the line's first chunk
+template <int RT, int TT, int MODE>
+__device__ __forceinline__ Kv8Chunk kv8_first_chunk(const Kv8AttnArgs& a) {
+  if constexpr (MODE == kJoint) {
+    if (!a.entries) return kv8_joint_chunk<RT, TT>(a);
+  }
+  return kv8_chunk<RT, TT, MODE>(a, 0);
 }
 
 template <int RT, int TT, int MODE>
@@ -250,7 +337,7 @@ struct Kv8Walk {
   int l;
 
   __device__ __forceinline__ bool start(const Kv8AttnArgs& a, int part) {
-    c = kv8_chunk<RT, TT, MODE>(a, 0);
+    c = kv8_first_chunk<RT, TT, MODE>(a);
     const int64_t total = kv8_total<RT, TT, MODE>(a, c), per = (total + a.parts - 1) / a.parts;
     x = (int64_t)part * per;
     end = x + per < total ? x + per : total;
@@ -442,7 +529,7 @@ __global__ __launch_bounds__(256) void kv8_joint_merge_kernel(const Kv8AttnArgs 
   int entry = -1, total = 0, room = 0, before = 0;
   bool found = false;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const Kv8Chunk c = kv8_chunk<RT, TT, kJoint>(a, b0);
+    const Kv8Chunk c = b0 == 0 ? kv8_first_chunk<RT, TT, kJoint>(a) : kv8_chunk<RT, TT, kJoint>(a, b0);
     const uint64_t mine = __ballot(b0 + lane < sequences && tok >= c.row0 && tok < c.row0 + c.n);
     auto rooms_before = [&](int l) { return total + (l > 0 ? __builtin_amdgcn_readlane(c.rooms, l - 1) : 0); };
     if (!found && mine) {

@@ -419,5 +419,11 @@ SGL_RULE Kv8JointPlan kv8_joint_plan(int64_t T, int64_t B, int64_t groups, int64
   return {rt, rg, rg, per_cu, kv8_attn_parts(per_cu * cus, Hkv), kv8_attn_items(T, B, Hkv, G, rt),
           kv8_attn_items(T, groups, Hkv, G, rg)};
 }
+// Up to 64 sequences and groups, a lane of a wavefront for each: every workgroup of the one pass finds
+// for itself what the groups cover, one group after the other, and no launch before it does.  By
+// themselves / planned, us, 8 kv heads of 128: 1 group of 4 sequences on 1500 16.6 / 19.7, of 16 on 4096
+// 22.4 / 24.5, of 60 x 2 on 8192 69.6 / 72; 3 groups of 16 sequences 22.8 / 24.1, of 60 36.0 / 37.2; 16
+// groups of 32 39 / 35, 32 51.6 / 40.8.
+SGL_RULE bool kv8_joint_alone(int64_t B, int64_t groups) { return groups <= 4 && B + groups <= 64; }
 
 }  // namespace sgl

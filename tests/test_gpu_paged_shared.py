@@ -71,6 +71,30 @@ def test_what_is_claimed_may_be_more_or_less_than_what_is_there(gpu):
         check(c, o, q, lens, None, parts=2)
 
 
+@pytest.mark.parametrize("B,cu_groups,shared", [(59, [0, 20, 20, 41, 59], [500, 300, 700, 640]),
+                                                (62, [1, 60, 62], [500, 700]), (2, [0, 2], [1 << 30]),
+                                                (9, [-3, 4, 70], [600, 600]), (5, [2, 5, 5], [-4, 512])])
+@pytest.mark.parametrize("each", [1, 2])
+def test_groups_found_by_each_workgroup_are_the_planned_ones(gpu, B, cu_groups, shared, each):
+    """Few sequences and groups need no plan in front: the same line, so the same bits, as beside empty groups."""
+    rng = np.random.default_rng(B)
+    new = [int(n) for n in rng.integers(0, each + 1, B)]
+    new[-1] = each
+    lens = [int(n) for n in rng.integers(700, 1000, B)]
+    if B > 50:
+        lens[B // 2] = new[B // 2]
+    Hq = 16 if B > 50 else 2  # (groups' tiles of 32 rows, or of 16, on both sides)
+    c = _filled(gpu, lens, 2, 64, 64, 16, seed=B)
+    edges = [min(max(b, 0), B) for b in cu_groups]
+    join_tables(c, edges, [max(0, min(n, 700)) for n in shared])
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], Hq, 64, torch.bfloat16, 5)
+    more = 5 if B < 60 else 2  # empty groups behind: too many, or too many sequences, to go without a plan
+    want = _call(c, q, lens, cu, cu_groups + cu_groups[-1:] * more, shared + [700] * more)
+    assert torch.equal(_call(c, q, lens, cu, cu_groups, shared), want)
+    check(c, want, q, lens, cu, parts=2)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("lead", [0.0, 12.0])
 def test_parts_whose_references_lie_far_apart(gpu, new, lead):
