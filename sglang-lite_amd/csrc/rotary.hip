@@ -48,8 +48,11 @@ constexpr int kHeads = 4;  // heads of a thread in flight
 // all threads of a token load the same ones: by themselves 16384 tokens of 32 heads of 128
 // take 71 us, so 51 (5.4 TB/s, as with one position).  16 tokens: 3.9 us, the chain position ->
 // table -> rows, which a launch's own time on the host passes.
-// AXES: 0, or several with positions of 32 or 64 bits.
-template <int DT, int VEC, int AXES>
+// AXES: 0, or several with positions of 32 or 64 bits.  AHEAD: entries of a lane that are on their
+// way before the rows; what a wavefront's tokens have more than 64 AHEAD of is fetched behind them.
+// 1 / 2 entries where there are up to 128, 8192 tokens, us: 16 heads of 256 34.3 / 32.1, of 128 in fp32
+// 33.6 / 32.3, 32 of 80 22.4 / 20.3.
+template <int DT, int VEC, int AXES, int AHEAD>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   constexpr bool STAGE = AXES != 0 && VEC == 8, POS64 = AXES == 64;
   extern __shared__ __align__(16) float2 sAll[];  // of each wavefront [tokens][pairs]
@@ -124,12 +127,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     // waited for.
     const int e0s = (int)(threadIdx.x & 63);
     const AxisPositions mine = load_axis_positions<POS64>(a.positions, a.n_axes, a.T, there ? t : 0, (int)a.n_positions);
-    const float2 w = fetch(e0s < count ? e0s : 0);
+    float2 w[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) w[k] = fetch(e0s + 64 * k < count ? e0s + 64 * k : 0);
     if (there) load_heads(hs);
     __builtin_amdgcn_sched_barrier(0);
     turn = u < rot_units && mine.turn;
-    if (e0s < count) sTurn[e0s] = w;
-    for (int e = e0s + 64; e < count; e += 64) sTurn[e] = fetch(e);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (e0s + 64 * k < count) sTurn[e0s + 64 * k] = w[k];
+    for (int e = e0s + 64 * AHEAD; e < count; e += 64) sTurn[e] = fetch(e);
     // (a wavefront's LDS accesses go in order: nothing to wait for but the compiler)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -208,10 +215,19 @@ void launch_rotary(const RotaryArgs& a, bool vec, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div(threads, 256));
   // (a token has a thread at least for each 16 rotated elements: 4 (4096 + 8 rot) bytes at most)
   const size_t lds = AXES ? 4 * (size_t)(64 / ((int64_t)a.units * a.hsplit) + 2) * (a.rot / 2) * sizeof(float2) : 0;
-  if (vec)
-    rotary_kernel<DT, 8, AXES><<<grid, 256, lds, st>>>(a);
-  else
-    rotary_kernel<DT, 1, AXES><<<grid, 256, 0, st>>>(a);
+  if (!vec) {
+    rotary_kernel<DT, 1, AXES, 1><<<grid, 256, 0, st>>>(a);
+    return;
+  }
+  if constexpr (AXES != 0) {
+    const int64_t per = (int64_t)a.units * a.hsplit;  // a token's threads
+    const int64_t tokens = 64 % per == 0 ? 64 / per : per % 64 == 0 ? 1 : (62 + per) / per + 1;  // of a wavefront
+    if (tokens * (a.rot / 2) > 64) {
+      rotary_kernel<DT, 8, AXES, 2><<<grid, 256, lds, st>>>(a);
+      return;
+    }
+  }
+  rotary_kernel<DT, 8, AXES, 1><<<grid, 256, lds, st>>>(a);
 }
 
 template <int DT, bool AXES>
