@@ -29,14 +29,15 @@ struct AppendArgs {
   const int32_t* cu;     // [B + 1] or null: one token each
   const float* table;    // or null: no rotation
   const int32_t* positions;  // [T], or of several axes [n_axes][T]; null: a token's place
-  const uint8_t* axes;       // the axis of each pair, or null: one position for all
-  int n_axes;
   int64_t n_positions;
   int64_t n_pages;
   int T, B, Hkv, D, row_pages, page_shift, block_shift;
   int per_magic;  // i / (D / 16) = i per_magic >> 16 for i < 4096
   int rot, offset;
   bool interleaved;
+  // (behind the others, so that those are loaded as they were without)
+  int n_axes;
+  const uint8_t* axes;  // the axis of each pair
 };
 
 // A unit of work: the new tokens of one block of one sequence.

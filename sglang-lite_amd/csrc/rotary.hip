@@ -33,12 +33,12 @@ struct RotaryArgs {
   const float* table;
   int64_t n_positions;
   const void* positions;  // [T], or of several axes [n_axes][T]
-  const uint8_t* axes;    // the axis of each pair
-  int n_axes;
   int T, H, D, rot, offset;
   int units;    // a head's units of 2 VEC elements that there is work on
   int hsplit;   // threads that share a unit's heads
   bool pos64, interleaved, inverse;
+  int n_axes;  // (behind the others, so that those are loaded as they were without)
+  const uint8_t* axes;  // the axis of each pair
 };
 
 constexpr int kHeads = 4;  // heads of a thread in flight

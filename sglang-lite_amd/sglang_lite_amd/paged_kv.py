@@ -250,19 +250,29 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     q, sq = _rows16(q, 8)
     if given and out is not q:
         check_apart(q, out, "paged_attn")
-    name, size, more = "sgl_kv8_attn", (T, B, heads, hq // heads, dim, columns * page), (window,)
+    scale = dim ** -0.5 if softmax_scale is None else softmax_scale
+    G, tokens = hq // heads, columns * page
     if groups:
-        name, size, more = "sgl_kv8_attn_shared", (*size, groups), ()
+        nws = _workspace(d, "sgl_kv8_attn_shared_workspace_size", T, B, heads, G, dim, tokens, groups)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+        _lib.call_on(d, "sgl_kv8_attn_shared", q.data_ptr(), sq[0], sq[1], dt, T, B, heads, G, dim,
+                     _lib.ptr(cu_tokens), lens.data_ptr(), block_table.data_ptr(), columns, page, block, pages,
+                     kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), scale, causal, _lib.ptr(sink),
+                     groups, cu_groups.data_ptr(), shared.data_ptr(), out.data_ptr(), ws.data_ptr(), nws)
     elif first:
-        name, size, more = "sgl_kv8_attn_first", (*size, window, first), (window, first)
-    nws = _workspace(d, name + "_workspace_size", *size)
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    shares = (groups, cu_groups.data_ptr(), shared.data_ptr()) if groups else ()
-    _lib.call_on(d, name, q.data_ptr(), sq[0], sq[1], dt, T, B, heads, hq // heads, dim,
-                 _lib.ptr(cu_tokens), lens.data_ptr(), block_table.data_ptr(), columns, page, block,
-                 pages, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-                 dim ** -0.5 if softmax_scale is None else softmax_scale, causal, *more,
-                 _lib.ptr(sink), *shares, out.data_ptr(), _lib.ptr(ws), nws)
+        nws = _workspace(d, "sgl_kv8_attn_first_workspace_size", T, B, heads, G, dim, tokens, window, first)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+        _lib.call_on(d, "sgl_kv8_attn_first", q.data_ptr(), sq[0], sq[1], dt, T, B, heads, G, dim,
+                     _lib.ptr(cu_tokens), lens.data_ptr(), block_table.data_ptr(), columns, page, block, pages,
+                     kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), scale, causal, window, first,
+                     _lib.ptr(sink), out.data_ptr(), _lib.ptr(ws), nws)
+    else:
+        nws = _workspace(d, "sgl_kv8_attn_workspace_size", T, B, heads, G, dim, tokens)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+        _lib.call_on(d, "sgl_kv8_attn", q.data_ptr(), sq[0], sq[1], dt, T, B, heads, G, dim, _lib.ptr(cu_tokens),
+                     lens.data_ptr(), block_table.data_ptr(), columns, page, block, pages, kc.data_ptr(),
+                     vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), scale, causal, window, _lib.ptr(sink),
+                     out.data_ptr(), _lib.ptr(ws), nws)
     return out
 
 
