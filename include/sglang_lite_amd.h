@@ -609,10 +609,11 @@ size_t sgl_kv8_attn_first_workspace_size(int64_t T, int64_t B, int Hkv, int G, i
 /* sgl_kv8_attn without a window, for sequences that begin alike: those of group g
  * are [cu_groups[g], cu_groups[g + 1]) (int32 [n_groups + 1], device, never falling;
  * sequences outside of all groups are allowed), and the full pages among the first shared[g]
- * tokens (int32 [n_groups], device) are the same in each of their block table rows.  Those
+ * tokens (int32 [n_groups], device) are the same in the block table row of each that has queries.  Those
  * keys are read once for all queries of the group; the result is that of sgl_kv8_attn but for the
  * order of its sums.  What is taken together is cut to whole pages, whole 128 tokens and to the
- * tokens before each sequence's first query; the pages are those of the group's first row.
+ * tokens before each sequence's first query; the pages are those in the row of its first
+ * sequence with queries.
  * Its workspace has sgl_kv8_attn_shared_workspace_size bytes. */
 int sgl_kv8_attn_shared(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int64_t T,
                         int64_t B, int Hkv, int G, int D, const int32_t* cu_tokens, const int32_t* lens,

@@ -724,24 +724,27 @@ __global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, co
     return;
   }
   const int b0 = edge(g), b1 = edge(g + 1);
-  int most = shared[g], with = 0;
+  int most = shared[g], with = 0, from = 0x7FFFFFFF;  // from: the first sequence with queries
   for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) {
     const SeqRows r = seq_rows(a.cu, b, a.T);
     if (r.n == 0) continue;
     const int len = a.lens[b] < cap ? a.lens[b] : cap;
     most = len - r.n < most ? len - r.n : most;
+    from = b < from ? b : from;
     ++with;
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) {
-    const int other = __shfl_xor(most, d, 64);
+    const int other = __shfl_xor(most, d, 64), before = __shfl_xor(from, d, 64);
     most = other < most ? other : most;
+    from = before < from ? before : from;
     with += __shfl_xor(with, d, 64);
   }
-  __shared__ int part[4][2];
+  __shared__ int part[4][3];
   if ((threadIdx.x & 63) == 0) {
     part[threadIdx.x >> 6][0] = most;
     part[threadIdx.x >> 6][1] = with;
+    part[threadIdx.x >> 6][2] = from;
   }
   __syncthreads();
   with = 0;
@@ -749,16 +752,18 @@ __global__ __launch_bounds__(256) void kv8_prefix_kernel(const Kv8AttnArgs a, co
   for (int i = 0; i < 4; ++i) {
     most = part[i][0] < most ? part[i][0] : most;
     with += part[i][1];
+    from = part[i][2] < from ? part[i][2] : from;
   }
+  if (with == 0) from = 0;
   const int covered = kv8_covered(a, most, with);
   for (int b = b0 + (int)threadIdx.x; b < b1; b += 256) cover(b, covered, g);
   if (threadIdx.x == 0 && o.entries) {
     const int row0 = row_of(b0), end = b1 > b0 ? row_of(b1) : row0;
-    o.entries[a.B + g] = Kv8Entry{row0, end > row0 ? end - row0 : 0, covered, 0, b0 < a.B ? b0 : 0, kIsGroup, 0, 0};
+    o.entries[a.B + g] = Kv8Entry{row0, end > row0 ? end - row0 : 0, covered, 0, from, kIsGroup, 0, 0};
   } else if (threadIdx.x == 0) {
     o.cu[g] = row_of(b0);
     o.lens[g] = covered;
-    o.row[g] = b0 < a.B ? b0 : 0;
+    o.row[g] = from;
   }
 }
 

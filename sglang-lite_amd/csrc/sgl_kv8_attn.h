@@ -192,7 +192,8 @@ __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttnArgs& a, int b0) {
 // as one sequence of these keys, whose rows meet the keys' tiles together, and each of its sequences
 // from there on.  `covered` is what the caller says, cut to whole pages and key tiles (of every
 // kernel: 128 tokens), and to what lies before the first query (`most`) of each of the group's
-// sequences that has any (`with` of them); 0 for a group of fewer than two such.
+// sequences that has any (`with` of them); 0 for a group of fewer than two such.  The pages are those of the
+// first of these: of a sequence without queries neither its length nor its row of the block table is looked at.
 constexpr int kPrefixTile = 128;
 __device__ __forceinline__ int kv8_covered(const Kv8AttnArgs& a, int most, int with) {
   const int unit = kPrefixTile > (1 << a.page_shift) ? kPrefixTile : 1 << a.page_shift;
@@ -239,7 +240,8 @@ __device__ __forceinline__ Kv8Chunk kv8_joint_chunk(const Kv8AttnArgs& a) {
     const int b0 = __builtin_amdgcn_readlane(e0, l), b1 = __builtin_amdgcn_readlane(e1, l);
     const bool in = lane >= b0 && lane < b1, counts = in && c.n > 0;
     const int least = wave_min(counts ? c.len - c.n : 0x7FFFFFFF), said = __builtin_amdgcn_readlane(most, l);
-    const int covered = kv8_covered(a, least < said ? least : said, __builtin_popcountll(__ballot(counts)));
+    const uint64_t with = __ballot(counts);
+    const int covered = kv8_covered(a, least < said ? least : said, __builtin_popcountll(with));
     if (in) {
       c.skip = c.n ? covered : 0;
       c.group = l - sequences;
@@ -250,7 +252,7 @@ __device__ __forceinline__ Kv8Chunk kv8_joint_chunk(const Kv8AttnArgs& a) {
       c.row0 = first;
       c.n = b1 > b0 && end > first ? end - first : 0;
       c.len = covered;
-      c.table_row = b0 < sequences ? b0 : 0;
+      c.table_row = with ? __builtin_ctzll(with) : 0;
       c.group = kIsGroup;
     }
   }

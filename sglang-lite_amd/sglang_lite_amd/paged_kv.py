@@ -202,7 +202,7 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
 
     ``cu_groups`` (int32 ``[groups + 1]``, never falling) and ``shared`` (int32 ``[groups]``), without
     a window: sequences ``cu_groups[g]`` to ``cu_groups[g + 1]`` begin alike, the full pages
-    among their first ``shared[g]`` tokens being the same in each one's row of the block table.  Those
+    among their first ``shared[g]`` tokens being the same in the block table row of each that has queries.  Those
     pages are read once for all of the group's queries, and the result is the same but for the order
     of its sums.  Sequences may stand outside of all groups.
 

@@ -203,6 +203,37 @@ def test_many_groups_of_many_sizes(gpu, D, Hq, Hkv):
         check(c, o, q, lens, cu, parts=2)
 
 
+@pytest.mark.parametrize("new,D,tokens,more", [
+    ([0, 1, 1, 0, 1], 128, 0, 0),           # found by each workgroup
+    ([0, 0, 2, 1], 64, 16384, 0),
+    ([0, 1, 1, 0, 1], 128, 0, 5),           # planned in front
+    ([0] * 70 + [1] * 30, 64, 0, 0),
+    ([0] * 300 + [1, 2], 256, 0, 0),
+    ([0, 40, 40], 128, 1 << 18, 0),         # in two passes
+    ([0] * 300 + [60, 1, 0, 60], 64, 1 << 18, 0),
+])
+def test_sequences_without_queries_in_front_of_a_group(gpu, new, D, tokens, more):
+    """Their rows of the block table (no pages, or foreign ones) and lengths are not looked at."""
+    B = len(new)
+    live = [b for b in range(B) if new[b]]
+    lens = [900 if n else 0 for n in new]
+    c = _filled(gpu, lens, 2, D, 16, 16, seed=B)
+    for b in live[1:]:
+        c.table[b, :640 // 16] = c.table[live[0], :640 // 16]
+    c.bt = torch.from_numpy(c.table).to(gpu)
+    _widen(c, tokens)
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], 16, D, torch.bfloat16, 7)
+    for fill, old in ((-1, 0), (int(c.table[live[-1], 50]), 0), (1 << 30, 900), (-1, -3)):
+        for b in range(B):
+            if new[b] == 0:
+                c.table[b] = fill
+                lens[b] = old
+        c.bt = torch.from_numpy(c.table).to(gpu)
+        o = _call(c, q, lens, cu, [0, B] + [B] * more, [650] + [0] * more)
+        check(c, o, q, lens, cu, parts=2)
+
+
 def test_captured_with_other_lengths_and_prefixes(gpu):
     lens0 = [900, 700, 1200, 640]
     c = _filled(gpu, lens0, 2, 128, 64, 64, seed=14)
