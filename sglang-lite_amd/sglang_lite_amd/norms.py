@@ -147,28 +147,38 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torc
     return out, (y, scales) if quant else y
 
 
+def _meet(x: torch.Tensor, h: torch.Tensor) -> bool:
+    """Whether rows ``x`` and ``h`` ``[T, H]``, each dense, share memory; also true of ranges that do where the
+    strides differ."""
+    if x.numel() == 0 or h.numel() == 0:
+        return False
+    m, n, size = x.shape[0], h.shape[0], x.element_size()
+    xs, hs = x.stride(0) * size, h.stride(0) * h.element_size()  # (bytes from here on)
+    wx, wh, far = x.shape[1] * size, h.shape[1] * h.element_size(), x.data_ptr() - h.data_ptr()
+    if far + (m - 1) * xs + wx <= 0 or far >= (n - 1) * hs + wh:
+        return False
+    if m == 1 or xs == 0:
+        m, xs = 1, hs
+    if n == 1:
+        hs = xs
+    if xs != hs or xs == 0:
+        return True
+    # row i of x and row j of h meet where -wx < far + (i - j) xs < wh
+    least, most = (-wx - far) // xs + 1, -((far - wh) // xs) - 1
+    return max(least, 1 - n) <= min(most, m - 1)
+
+
 def _check_apart(x: torch.Tensor, h: torch.Tensor, name: str) -> None:
     """Refuse an in-place residual that shares memory with ``x`` and is not its very rows."""
-    if x.numel() == 0:
+    if x.data_ptr() == h.data_ptr() and x.dtype is h.dtype and (x.shape[0] == 1 or x.stride(0) == h.stride(0)):
         return
-    a, b = x.data_ptr(), h.data_ptr()
-
-    def end(t):
-        return ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-
-    if a + end(x) <= b or b + end(h) <= a:
-        return
-    if a == b and x.dtype is h.dtype and x.stride(0) == h.stride(0):
-        return
-    raise ValueError(f"residual_norm: the residual written in place overlaps {name} without being it")
+    if _meet(x, h):
+        raise ValueError(f"residual_norm: the residual written in place overlaps {name} without being it")
 
 
 def _check_weight(w: Optional[torch.Tensor], h: torch.Tensor, name: str) -> None:
-    """Refuse a weight that lies among the rows of an in-place residual: other rows still read it."""
-    if w is None or h.shape[0] == 0:
-        return
-    a, b = w.data_ptr(), h.data_ptr()
-    if b < a + w.numel() * w.element_size() and a < b + ((h.shape[0] - 1) * h.stride(0) + h.shape[1]) * h.element_size():
+    """Refuse a weight that lies in the rows of an in-place residual: other rows still read it."""
+    if w is not None and _meet(w.view(1, -1), h):
         raise ValueError(f"residual_norm: the residual written in place overlaps {name}")
 
 

@@ -174,6 +174,22 @@ def test_in_place(gpu):
         residual_norm(x[:1].expand(T, H), buf[:1].expand(T, H), w, inplace=True)
 
 
+def test_in_place_beside_its_inputs_in_one_buffer(gpu):
+    from sglang_lite_amd.norms import residual_norm
+
+    for T, H in ((600, 4096), (7, 1003), (1, 64)):
+        x, r, w, v, m = _inputs(gpu, T, H, BF16, BF16, True, "rows", BF16, seed=T)
+        want = residual_norm(x, r, w, after=v, gate=m, scale=0.5)
+        wide = torch.zeros(T, 5, H, dtype=BF16, device=gpu)
+        wide[:, 0], wide[:, 2], wide[:, 3], wide[T // 2, 1], wide[0, 4] = x, r, m, w, v
+        before = wide.clone()
+        h, y = residual_norm(wide[:, 0], wide[:, 2], wide[T // 2, 1], after=wide[0, 4], gate=wide[:, 3], scale=0.5,
+                             inplace=True)
+        assert h.data_ptr() == wide[0, 2].data_ptr() and torch.equal(wide[:, 2], want[0]) and torch.equal(y, want[1])
+        before[:, 2] = want[0]
+        assert torch.equal(wide, before)
+
+
 def test_zeros_infinities_and_nan_stay_in_their_rows(gpu):
     from sglang_lite_amd.norms import residual_norm
 

@@ -84,6 +84,48 @@ def test_norm_refusals():
             residual_norm(*args, **kw)
 
 
+def test_rows_that_meet():
+    """What an in-place residual may lie beside: by the bytes of each element."""
+    from sglang_lite_amd import norms as N
+
+    buf = torch.zeros(64, dtype=torch.float32)
+
+    def bytes_of(t):
+        size = t.element_size()
+        return {t.data_ptr() + (i * t.stride(0) + e) * size + k for i in range(t.shape[0]) for e in range(t.shape[1])
+                for k in range(size)}
+
+    def refused(check, *a):
+        try:
+            check(*a, "x")
+        except ValueError:
+            return True
+        return False
+
+    met = 0
+    for T, H, hs, h0 in ((1, 4, 4, 7), (3, 4, 4, 8), (3, 4, 9, 0), (4, 3, 10, 12), (1, 5, 11, 20)):
+        h = buf.as_strided((T, H), (hs, 1), h0)
+        there = bytes_of(h)
+        for dtype in (torch.float32, torch.bfloat16):
+            flat = buf.view(dtype)
+            for xs in (0, 2, 3, hs, 2 * hs):
+                for x0 in range(0, flat.numel() - (T - 1) * xs - H + 1):
+                    x = flat.as_strided((T, H), (xs, 1), x0)
+                    meets = bool(bytes_of(x) & there)
+                    same = dtype is torch.float32 and x0 == h0 and (xs == hs or T == 1)
+                    if xs * x.element_size() == hs * 4 or xs == 0 or T == 1 or meets:
+                        assert refused(N._check_apart, x, h) == (meets and not same), (T, H, hs, h0, dtype, xs, x0)
+                    met += meets
+            for x0 in range(0, flat.numel() - H + 1):
+                w = flat[x0:x0 + H]
+                assert refused(N._check_weight, w, h) == bool(bytes_of(w[None]) & there)
+    assert met > 100
+    wide = torch.zeros(6, 2, 8)
+    N._check_apart(wide[:, 1], wide[:, 0], "x")
+    N._check_weight(None, wide[:, 0], "before")
+    N._check_apart(wide[:0, 0], wide[:0, 0], "x")
+
+
 def test_entry_points_refuse_before_any_launch():
     from sglang_lite_amd import _lib as L
 
