@@ -230,3 +230,51 @@ def test_graph_and_stream(gpu):
         torch.cuda.synchronize()
         h2, (q2, s2) = call()
         assert torch.equal(h, h2) and torch.equal(s, s2) and torch.equal(q.view(torch.uint8), q2.view(torch.uint8))
+
+
+def _same(a, b):
+    return torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,H,quant", [(8200, 4104, False), (8200, 4100, False), (8320, 4096, True)])
+def test_rows_that_pass_the_cache_by(gpu, dtype, T, H, quant):
+    """More than 128 MiB of inputs: each row as among few rows, and sampled rows against float64."""
+    from sglang_lite_amd.norms import residual_norm
+
+    print(f"norm T={T} H={H} {dtype} quant={quant}", flush=True)
+    x, r, w, v, m = _inputs(gpu, T, H, dtype, dtype, True, "vector", F32, seed=T)
+    kw = dict(after=v, scale=0.7, quant=quant)
+    for gate in (m, torch.tanh(x.float()).to(dtype)):
+        h, y = residual_norm(x, r, w, gate=gate, **kw)
+        y, s = y if quant else (y, None)
+        for lo in range(0, T, 1500):
+            part = slice(lo, lo + 1500)
+            h2, y2 = residual_norm(x[part], r[part], w, gate=gate if gate.dim() == 1 else gate[part], **kw)
+            y2, s2 = y2 if quant else (y2, None)
+            assert _same(h[part], h2) and _same(y[part], y2) and (s is None or _same(s[part], s2))
+        rows = [0, 1, 511, 512, 767, T // 2, T - 2, T - 1]
+        g = _host(gate if gate.dim() == 1 else gate[rows])
+        ho, dh, yo, dy = ON.residual_norm(_host(x[rows]), _host(r[rows]), _host(w), _host(v), g,
+                                          float(np.float32(0.7)), float(np.float32(1e-6)))
+        _near(h[rows], ho, dh, dtype)
+        if not quant:
+            _near(y[rows], yo, dy, dtype)
+        inside = r.clone()
+        h2, y2 = residual_norm(x, inside, w, gate=gate, inplace=True, **kw)
+        assert h2 is inside and _same(inside, h) and _same(y2[0] if quant else y2, y)
+
+
+@pytest.mark.parametrize("T,H,block", [(30, 1024, 128), (700, 2560, 64), (5, 8320, 128)])
+def test_codes_of_16_bit_rows_are_those_of_their_values(gpu, T, H, block):
+    """The arithmetic is fp32 for every type of x and of the residual: the same codes, h rounded once."""
+    from sglang_lite_amd import kernel as K
+    from sglang_lite_amd.norms import residual_norm
+
+    for dtype, res in ((BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)):
+        x, r, w, v, m = _inputs(gpu, T, H, dtype, res, True, "rows", dtype, seed=H)
+        for fmt, sdt in ((None, F32), ("ue8m0", K.E8M0)):
+            kw = dict(quant=True, block_size=block, scale_fmt=fmt, scale_dtype=sdt, scale=-0.6)
+            h, (q, s) = residual_norm(x, r, w, after=v, gate=m, **kw)
+            h32, (q32, s32) = residual_norm(x.float(), r.float(), w, after=v, gate=m, **kw)
+            assert _same(h, h32.to(res)) and _same(q, q32) and _same(s, s32)

@@ -276,6 +276,24 @@ def test_calls_on_two_streams_at_once(gpu):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,Hq,new", [
+    (64, 2, [1] * 3), (64, 8, [1] * 6), (64, 8, [6] * 3),       # tiles of 16 rows; groups' of 32; both
+    (128, 2, [1] * 3), (112, 8, [1] * 6), (128, 8, [6] * 3),
+    (128, 8, [2] * 30), (96, 8, [6] * 10),                      # more than 160 rows of a group
+    (256, 2, [1] * 3), (192, 8, [1] * 6), (256, 8, [3] * 20),
+])
+def test_each_tile_of_one_pass(gpu, D, Hq, new, dtype):
+    lens = [500 + 7 * i for i in range(len(new))]
+    c = _filled(gpu, lens, 2, D, 32, 32, seed=D + Hq)
+    join_tables(c, [0, len(new)], [410])
+    cu = [0] + np.cumsum(new).tolist()
+    q = _queries(gpu, cu[-1], Hq, D, dtype, 3)
+    for tokens in (0, 4096):
+        _widen(c, tokens)
+        check(c, _call(c, q, lens, cu, [0, len(new)], [410]), q, lens, cu, parts=2)
+
+
 def test_exact_of_a_short_row():
     """(the helper's own: a row that sees no key is zero)"""
 

@@ -224,3 +224,89 @@ def test_axes_in_a_graph_and_on_another_stream(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, R.rotary(x, table, pos, axes=axes))
+
+
+@pytest.mark.parametrize("T,H,D,sections,spread,offset,interleaved,dtype", [
+    (16400, 7, 128, (16, 24, 24), False, 0, False, torch.bfloat16),  # two threads a unit: four heads, and three
+    (16400, 5, 128, (16, 24, 24), True, 0, False, torch.float32),
+    (16400, 9, 128, (10, 11, 11), True, 64, True, torch.float16),    # three: three heads each
+    (4100, 32, 128, (24, 20, 20), True, 0, False, torch.bfloat16),   # a token a wavefront
+    (4100, 30, 128, (64,), False, 0, True, torch.float32),
+    (11000, 14, 96, (13, 11), False, 0, False, torch.float16),
+])
+def test_many_tokens_of_several_heads_a_thread(gpu, T, H, D, sections, spread, offset, interleaved, dtype):
+    """Each token as among few, whose threads have a head each; into a new tensor and in place."""
+    from sglang_lite_amd import rotary as R
+
+    print(f"axes T={T} H={H} D={D} {sections}", flush=True)
+    g = torch.Generator(device=gpu).manual_seed(T + H)
+    rot, n = 2 * sum(sections), 5000
+    table = R.rotary_table(n, rot, device=gpu)
+    freq, _ = R.frequencies(rot)
+    axes = R.rotary_axes(sections, spread=spread, device=gpu)
+    x = torch.randn(T, H, D, generator=g, device=gpu).to(dtype)
+    at = torch.randint(0, n, (len(sections), T), generator=g, device=gpu)
+    at[0, T // 2] = -1
+    for pos in (at.int(), at):
+        kw = dict(axes=axes, interleaved=interleaved, offset=offset)
+        y = R.rotary(x, table, pos, **kw)
+        for lo in range(0, T, 400):
+            few = R.rotary(x[lo:lo + 400].contiguous(), table, pos[:, lo:lo + 400].contiguous(), **kw)
+            assert torch.equal(y[lo:lo + 400], few)
+        rows = [0, 1, 2, 63, 64, T // 2 - 1, T // 2 + 1, T - 2, T - 1]
+        ref = OP.rotate_axes(_host(x[rows]), at[:, rows].cpu().numpy(), axes.cpu().numpy(), freq.numpy(), 1.0, offset,
+                             interleaved)
+        bound = _bound(_host(x[rows]), rot, offset, interleaved, dtype)
+        err = np.abs(_host(y[rows]).astype(np.float64) - ref)
+        assert np.all(err <= bound + HALF[dtype] * (np.abs(ref) + bound)), float(err.max())
+        assert torch.equal(y[T // 2], x[T // 2])
+        z = x.clone()
+        assert R.rotary(z, table, pos, out=z, **kw) is z and torch.equal(z, y)
+
+
+@pytest.mark.parametrize("block", [64, 128])
+@pytest.mark.parametrize("dtype,sections,spread,interleaved", [
+    (torch.bfloat16, (40, 44, 44), True, False),
+    (torch.float16, (32, 48, 48), False, True),
+    (torch.float32, (43, 43, 42), False, False),
+])
+def test_append_of_blocks_above_512_threads(gpu, block, dtype, sections, spread, interleaved):
+    """Heads of 256: two or four units a thread, whose turns share the wavefront's LDS."""
+    from sglang_lite_amd import paged_kv as P
+    from sglang_lite_amd import rotary as R
+
+    B, H, D, page, n = 3, 2, 256, 128, 700
+    rng = np.random.default_rng(block)
+    table = R.rotary_table(n, D, device=gpu)
+    axes = R.rotary_axes(sections, spread=spread, device=gpu)
+    kv = P.PagedKV.empty(20, H, page, D, block=block, device=gpu)
+    for c in (kv.k, kv.v):
+        c.view(torch.uint8).fill_(0x7F)
+    for s in (kv.k_scale, kv.v_scale):
+        s.fill_(float("nan"))
+    bt = rng.permutation(20)[:B * 5].reshape(B, 5).astype(np.int32)
+    codes = [_bytes(c).copy() for c in (kv.k, kv.v)]
+    scales = [_host(s).copy() for s in (kv.k_scale, kv.v_scale)]
+    have = [0] * B
+    for step, new in enumerate(([300, 1, 130], [60, 127, 128], [1, 64, 33])):
+        cu = [0] + np.cumsum(new).tolist()
+        T = cu[-1]
+        g = torch.Generator(device=gpu).manual_seed(step)
+        x = (torch.randn(T, 2, H, D, generator=g, device=gpu) * 3).to(dtype)
+        pos = torch.randint(0, n, (len(sections), T), generator=g, device=gpu, dtype=torch.int32)
+        pos[0, 1], pos[-1, 2], pos[0, 3] = -1, -7, n
+        P.append_kv(kv, x[:, 0], x[:, 1], torch.from_numpy(bt).to(gpu),
+                    torch.tensor(have, dtype=torch.int32, device=gpu),
+                    cu_tokens=torch.tensor(cu, dtype=torch.int32, device=gpu), table=table, positions=pos, axes=axes,
+                    interleaved=interleaved)
+        at, tab = pos.cpu().numpy(), _host(table)
+        rows = tab[np.clip(at, 0, n - 1)[axes.cpu().numpy()].T, np.arange(D // 2)]
+        rows[at[axes.cpu().numpy()].T >= n] = np.nan
+        rows[(at < 0).any(0)] = (1.0, 0.0)
+        OP.append(codes[0], scales[0], OP.rotate_f32(_host(x[:, 0]), rows, 0, interleaved), bt, have, cu)
+        OP.append(codes[1], scales[1], _host(x[:, 1]), bt, have, cu)
+        have = [h + m for h, m in zip(have, new)]
+        np.testing.assert_array_equal(_host(kv.k_scale), scales[0])
+        np.testing.assert_array_equal(_host(kv.v_scale), scales[1])
+        np.testing.assert_array_equal(_bytes(kv.k), codes[0])
+        np.testing.assert_array_equal(_bytes(kv.v), codes[1])
