@@ -545,7 +545,10 @@ void launch_attn(Kv8AttnArgs a, const Kv8AttnPlan& p, hipStream_t st) {
 template <int DP, int NCG, int NC, int QT>
 void launch_joint_as(const Kv8AttnArgs& a, const Kv8JointPlan& p, hipStream_t st) {
   const dim3 grid(a.parts * a.Hkv), threads(64 * kWaves);
-  if constexpr (DP <= 128) {
+  // (what the plan says of these heads and tiles: always two, either, always one)
+  if constexpr (DP == 64) {
+    kv8_joint_kernel<DP, NCG, NC, QT, 2><<<grid, threads, 0, st>>>(a);
+  } else if constexpr (DP == 128 && NCG == 2) {
     if (p.per_cu == 2)
       kv8_joint_kernel<DP, NCG, NC, QT, 2><<<grid, threads, 0, st>>>(a);
     else

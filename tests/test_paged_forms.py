@@ -86,6 +86,24 @@ def test_joint_plans(rules):
     assert plan(64, 64, 1, 8, 4, 128, 9192)[5] and not plan(128, 128, 2, 4, 16, 128, 35768)[5]
 
 
+def test_joint_plans_have_a_kernel(rules):
+    """Workgroups a CU that the launch takes for granted: two for heads up to 64, one for groups' tiles of 16 rows
+    of wider heads and for heads above 128."""
+    o = (ctypes.c_int64 * 7)()
+    rng = np.random.default_rng(1)
+    seen = set()
+    for i in range(20000):
+        B, Hkv, G = (int(2 ** rng.uniform(0, n)) for n in (9, 4, 5))
+        n, D = int(rng.integers(1, B + 1)), 16 * int(rng.integers(1, 17))
+        T, cap = int(rng.integers(1, B * 40)), 16 << int(rng.integers(0, 16))
+        rules.joint(T, B, n, Hkv, G, D, cap, o)
+        rt, rg, _, per_cu, _, items, _ = o
+        if items:
+            seen.add((64 if D <= 64 else 128 if D <= 128 else 256, rg, rt, per_cu))
+    assert seen == {(64, 16, 16, 2), (64, 32, 16, 2), (64, 32, 32, 2), (128, 16, 16, 1), (128, 32, 16, 1),
+                    (128, 32, 16, 2), (128, 32, 32, 1), (128, 32, 32, 2), (256, 16, 16, 1), (256, 32, 16, 1)}
+
+
 def _args(B=3, heads=2, hq=4, dim=64, page=32):
     from sglang_lite_amd import paged_kv as P
 
