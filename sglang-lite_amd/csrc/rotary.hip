@@ -41,7 +41,7 @@ struct RotaryArgs {
   const uint8_t* axes;  // the axis of each pair
 };
 
-constexpr int kHeads = 4;  // heads of a thread in flight
+constexpr int kHeads = 4;  // heads of a thread, at most (rotary_head_threads)
 
 // STAGE (several axes, 16-byte accesses): the rotations of the wavefront's tokens go through LDS.
 // A pair's table entry lies in its axis' row, so a thread's 8 are up to 8 pieces of 8 bytes, and
@@ -97,10 +97,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
   };
   constexpr int RW = DT == SGL_F32 ? 2 : 1;
   uint4 raw[STAGE ? kHeads : 1][2][RW];  // as they lie, so that nothing waits for them yet
-  auto load_heads = [&](int h0) __attribute__((always_inline)) {
+  auto load_heads = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < kHeads; ++k) {
-      const int h = h0 + k * a.hsplit;
+      const int h = hs + k * a.hsplit;
       if (h < a.H) {
         load_raw8<DT>(a.x, t * a.xt + h * a.xh + e0, raw[k][0]);
         if (two) load_raw8<DT>(a.x, t * a.xt + h * a.xh + e1, raw[k][1]);
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     float2 w[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) w[k] = fetch(e0s + 64 * k < count ? e0s + 64 * k : 0);
-    if (there) load_heads(hs);
+    if (there) load_heads();
     __builtin_amdgcn_sched_barrier(0);
     turn = u < rot_units && mine.turn;
 #pragma unroll
@@ -162,49 +162,44 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
     turn = p >= 0;
     if (turn) load_turn<VEC>(a.table, a.n_positions, a.rot / 2, p, VEC * u, a.inverse, cs, sn);
   }
-  for (int h0 = hs; h0 < a.H; h0 += kHeads * a.hsplit) {
-    float x[kHeads][2][VEC];
-    if constexpr (STAGE) {
-      if (h0 > hs) load_heads(h0);
-    }
+  float x[kHeads][2][VEC];
 #pragma unroll
-    for (int k = 0; k < kHeads; ++k) {
-      const int h = h0 + k * a.hsplit;
-      if (h < a.H) {
-        if constexpr (STAGE) {
-          widen8<DT>(raw[k][0], x[k][0]);
-          if (two) widen8<DT>(raw[k][1], x[k][1]);
-        } else {
-          load(t * a.xt + h * a.xh + e0, x[k][0]);
-          if (two) load(t * a.xt + h * a.xh + e1, x[k][1]);
-        }
+  for (int k = 0; k < kHeads; ++k) {
+    const int h = hs + k * a.hsplit;
+    if (h < a.H) {
+      if constexpr (STAGE) {
+        widen8<DT>(raw[k][0], x[k][0]);
+        if (two) widen8<DT>(raw[k][1], x[k][1]);
+      } else {
+        load(t * a.xt + h * a.xh + e0, x[k][0]);
+        if (two) load(t * a.xt + h * a.xh + e1, x[k][1]);
       }
     }
+  }
 #pragma unroll
-    for (int k = 0; k < kHeads; ++k) {
-      const int h = h0 + k * a.hsplit;
-      if (h < a.H) {
-        if (turn) {
-          if (VEC == 8 && a.interleaved) {
-            float p[VEC], q[VEC];
+  for (int k = 0; k < kHeads; ++k) {
+    const int h = hs + k * a.hsplit;
+    if (h < a.H) {
+      if (turn) {
+        if (VEC == 8 && a.interleaved) {
+          float p[VEC], q[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              p[v] = x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][2 * v % VEC];
-              q[v] = x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][(2 * v + 1) % VEC];
-            }
-            rotate_pairs<VEC>(p, q, cs, sn);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][2 * v % VEC] = p[v];
-              x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][(2 * v + 1) % VEC] = q[v];
-            }
-          } else {
-            rotate_pairs<VEC>(x[k][0], x[k][1], cs, sn);
+          for (int v = 0; v < VEC; ++v) {
+            p[v] = x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][2 * v % VEC];
+            q[v] = x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][(2 * v + 1) % VEC];
           }
+          rotate_pairs<VEC>(p, q, cs, sn);
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][2 * v % VEC] = p[v];
+            x[k][v / (VEC / 2 > 0 ? VEC / 2 : 1)][(2 * v + 1) % VEC] = q[v];
+          }
+        } else {
+          rotate_pairs<VEC>(x[k][0], x[k][1], cs, sn);
         }
-        store(t * a.ot + h * a.oh + e0, x[k][0]);
-        if (two) store(t * a.ot + h * a.oh + e1, x[k][1]);
       }
+      store(t * a.ot + h * a.oh + e0, x[k][0]);
+      if (two) store(t * a.ot + h * a.oh + e1, x[k][1]);
     }
   }
 }

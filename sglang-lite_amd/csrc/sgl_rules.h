@@ -241,7 +241,7 @@ SGL_RULE int permute_rounds(int E, bool table) {
 }
 
 // ---- rotary positions: threads that share the heads of a token's unit, each
-// with four heads in flight at a time.  One head a thread while that leaves CUs
+// with up to four heads in flight.  One head a thread while that leaves CUs
 // without a full round of wavefronts.  One head / four, us, 32 heads of 128: 512 tokens
 // 7.9 / 8.1, 2048 9.0 / 9.3, 4096 14.9 / 13.2, 16384 64 / 53.
 SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cus) {

@@ -166,3 +166,18 @@ def test_norm_plan(tmp_path):
             assert threads % 64 == 0 and 64 <= threads <= 1024 and threads * per >= units
             assert per == (1 if units <= 1024 else 2)
             assert 1 <= grid <= T
+
+
+def test_rotary_threads_have_all_heads(tmp_path):
+    """Four heads a thread at most: the kernel goes over them once."""
+    src, so = tmp_path / "h.cpp", tmp_path / "h.so"
+    src.write_text('#include "sgl_rules.h"\nextern "C" int threads(int64_t T, int64_t H, int64_t u, int64_t cus) {\n'
+                   "  return sgl::rotary_head_threads(T, H, u, cus);\n}\n")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{CSRC}", str(src), "-o",
+                    str(so)], check=True)
+    lib = ctypes.CDLL(str(so))
+    lib.threads.argtypes = [ctypes.c_int64] * 4
+    for H in list(range(1, 300)) + [4095, 4096, 4097, 65535, 65536]:
+        for T in (1, 1000, 100000, 2 ** 31 - 1):
+            n = lib.threads(T, H, 8, 256)
+            assert n <= H <= 4 * n
