@@ -125,13 +125,16 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
     const int pos = s.len - s.n + tq;
     const int hi = !live ? 0 : a.causal && pos + 1 < s.len ? pos + 1 : s.len;
     const int lo = a.causal && a.window > 0 ? pos - a.window + 1 : 0;
-    // (without branches: of an `or` in the masks below the compiler makes wrong code)
+    // (without branches, and the masks below too, which choose an element's value and always store it.  Where
+    // lanes part and come together around the store of one element of a vector, the compiler (ROCm 7.2)
+    // may empty the block that stores: it made that of `key < hi && (key >= lo || key < first)`, and keys that the
+    // window hides were seen.)
     const uint32_t hidden = lo > a.first ? (uint32_t)(lo - a.first) : 0u;  // keys between the first tokens and the window
     auto sees = [&](int key) __attribute__((always_inline)) {
       if constexpr (FIRST)
         return (key < hi) & ((uint32_t)(key - a.first) >= hidden);
       else
-        return key < hi && key >= lo;
+        return (key < hi) & (key >= lo);
     };
     // what all rows of the wavefront see, and what any row of the tile sees
     int all_hi = s.len, all_lo = 0, any_lo = 0, any_hi = s.len;
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
               const uint32_t dims = *reinterpret_cast<const uint32_t*>(&sDims[buf][t][2 * d]) >> (4 * g2);
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                if (seen && ((dims >> (8 * (i >> 2) + (i & 3))) & 1u)) acc[d][i] = __builtin_nanf("");
+                acc[d][i] = (seen & (((dims >> (8 * (i >> 2) + (i & 3))) & 1u) != 0)) ? __builtin_nanf("") : acc[d][i];
             }
           }
         }
@@ -401,7 +404,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
               for (int t = 0; t < NH; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                  if ((bad >> (2 * t + (e >> 3))) & 1) sc[t][e] = __builtin_nanf("");
+                  sc[t][e] = (bad >> (2 * t + (e >> 3))) & 1 ? __builtin_nanf("") : sc[t][e];
               clear_values((uint32_t)(__ballot(mark == kNoValue) >> l0), raw);
             }
           }
@@ -413,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void kv8_prefill_kernel
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 const int key = tok + 32 * t + 8 * (e >> 2) + 4 * g2 + (e & 3);
-                if (!(sees(key) && ((here >> (2 * t + (e >> 3))) & 1))) sc[t][e] = NEG_INF;
+                sc[t][e] = (sees(key) & (((here >> (2 * t + (e >> 3))) & 1) != 0)) ? sc[t][e] : NEG_INF;
               }
           }
           if (fresh) {
