@@ -377,7 +377,7 @@ SGL_RULE Kv8AttnPlan kv8_attn_plan(int64_t T, int64_t B, int64_t Hkv, int64_t G,
 // What stands for the block table's width where first tokens are seen beside a window: the keys
 // that a row tile's queries can see between them.
 SGL_RULE int64_t kv8_attn_reach(int64_t T, int64_t B, int64_t capacity, int64_t window, int64_t first) {
-  if (window <= 0 || first <= 0 || B <= 0) return capacity;
+  if (window <= 0 || first <= 0 || B <= 0 || window >= capacity || first >= capacity) return capacity;
   const int64_t reach = window + first + (T + B - 1) / B + 128;
   return reach < capacity ? reach : capacity;
 }

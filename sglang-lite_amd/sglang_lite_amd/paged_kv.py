@@ -252,6 +252,7 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
         check_apart(q, out, "paged_attn")
     scale = dim ** -0.5 if softmax_scale is None else softmax_scale
     G, tokens = hq // heads, columns * page
+    window, first = min(window, tokens), min(first, tokens)  # (64 bits hold them then)
     if groups:
         nws = _workspace(d, "sgl_kv8_attn_shared_workspace_size", T, B, heads, G, dim, tokens, groups)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)

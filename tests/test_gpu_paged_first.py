@@ -167,6 +167,20 @@ def test_many_sequences_and_rows_behind_the_last(gpu):
             check(c, o, q, lens, cu, window=80, kept=10)
 
 
+@pytest.mark.parametrize("new", [1, 150])
+def test_windows_and_first_tokens_of_any_length(gpu, new):
+    lens = [900, 333]
+    c = _filled(gpu, lens, 2, 128, 64, 64, seed=6)
+    _widen(c, 16384)
+    cu = [0, new, 2 * new]
+    q = _queries(gpu, cu[-1], 8, 128, torch.bfloat16, 3)
+    want = _call(c, q, lens, cu)
+    for far in (2 ** 62, 2 ** 63 - 1, 2 ** 64 + 5):
+        for kw in (dict(window=far), dict(window=far, first=far), dict(window=far, first=3)):
+            assert torch.equal(_call(c, q, lens, cu, **kw), want)
+        check(c, _call(c, q, lens, cu, window=3, first=far), q, lens, cu)
+
+
 def test_captured_with_other_lengths(gpu):
     c = _filled(gpu, [3000, 17, 900], 2, 128, 64, 64, seed=14)
     _widen(c, 8192)

@@ -58,6 +58,13 @@ def test_window_rules(rules):
     assert rules.plan_parts(64, 64, 8, 4, 128, 4240, 0) == 32 and rules.plan_parts(64, 64, 8, 4, 128, 4240, 1) == 0
 
 
+def test_windows_and_first_tokens_of_any_length(rules):
+    """Longer than any table: the table's width, whatever their sum does in 64 bits."""
+    for window, first in ((1 << 62, 1 << 62), (2 ** 63 - 1, 1), (1, 2 ** 63 - 1), (2 ** 63 - 1, 2 ** 63 - 1)):
+        assert rules.reach(1, 1, 20000, window, first) == 20000
+    assert rules.reach(1, 1, 20000, 19000, 900) == 20000 and rules.reach(1, 1, 20000, 9000, 9000) == 18129
+
+
 def test_joint_plans(rules):
     o = (ctypes.c_int64 * 7)()
 
