@@ -181,6 +181,21 @@ def test_windows_and_first_tokens_of_any_length(gpu, new):
         check(c, _call(c, q, lens, cu, window=3, first=far), q, lens, cu)
 
 
+@pytest.mark.parametrize("new,tokens", [([1, 4], 0), ([3, 1], 16384), ([130, 1, 0, 300], 0), ([130, 1, 0, 300], 16384)])
+def test_strided_queries_and_into_the_queries_themselves(gpu, new, tokens):
+    lens = [900 + 7 * i for i in range(len(new))]
+    c = _filled(gpu, lens, 2, 128, 64, 32, seed=22)
+    _widen(c, tokens)
+    cu = [0] + np.cumsum(new).tolist()
+    wide = _queries(gpu, cu[-1], 24, 128, torch.bfloat16, 8)
+    q = wide[:, 8:16]
+    want = _call(c, q, lens, cu, window=200, first=70)
+    check(c, want, q.contiguous(), lens, cu, window=200, kept=70)
+    held = q.contiguous()
+    assert _call(c, held, lens, cu, window=200, first=70, out=held) is held
+    assert torch.equal(held, want)
+
+
 def test_captured_with_other_lengths(gpu):
     c = _filled(gpu, [3000, 17, 900], 2, 128, 64, 64, seed=14)
     _widen(c, 8192)

@@ -294,6 +294,26 @@ def test_each_tile_of_one_pass(gpu, D, Hq, new, dtype):
         check(c, _call(c, q, lens, cu, [0, len(new)], [410]), q, lens, cu, parts=2)
 
 
+@pytest.mark.parametrize("new,tokens,more", [([1] * 5, 0, 0), ([2] * 5, 16384, 5), ([60, 1, 0, 40], 1 << 18, 0),
+                                             ([200, 150], 1 << 18, 0)])
+def test_strided_queries_and_into_the_queries_themselves(gpu, new, tokens, more):
+    """By the workgroups themselves, planned in front, in two passes: as into a new tensor."""
+    B = len(new)
+    lens = [900 + 7 * i for i in range(B)]
+    c = _filled(gpu, lens, 2, 128, 64, 32, seed=21)
+    join_tables(c, [0, B], [640])
+    _widen(c, tokens)
+    cu = [0] + np.cumsum(new).tolist()
+    wide = _queries(gpu, cu[-1], 48, 128, torch.bfloat16, 8)
+    q = wide[:, 16:32]
+    groups, shared = [0, B] + [B] * more, [640] + [0] * more
+    want = _call(c, q, lens, cu, groups, shared)
+    check(c, want, q.contiguous(), lens, cu, parts=2)
+    held = q.contiguous()
+    assert _call(c, held, lens, cu, groups, shared, out=held) is held
+    assert torch.equal(held, want)
+
+
 def test_exact_of_a_short_row():
     """(the helper's own: a row that sees no key is zero)"""
 
