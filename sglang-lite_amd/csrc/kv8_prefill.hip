@@ -2,7 +2,7 @@
 // chunks).  The mathematics, and the kernel for few rows: kv8_attn.hip.
 //
 // Bound by the matrix cores and, beside them, the softmax's VALU work (8192 queries
-// of 32 heads of 128 on 8 kv heads: 560 us, 0.98 PFLOP/s; MFMA 47 %, VALU 45 % busy).
+// of 32 heads of 128 on 8 kv heads: 550 to 564 us, 0.98 to 1.0 PFLOP/s; MFMA 47 %, VALU 45 % busy).
 // Eight wavefronts (heads up to 64 and above 128: four) of 32 rows each share the key
 // tiles of 64 tokens (heads above 128: 32), whose codes are converted once, on the
 // way into LDS (exact in bf16 and f16), and both products are v_mfma_f32_32x32x16:

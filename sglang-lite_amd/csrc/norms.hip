@@ -12,8 +12,9 @@
 // takes a row, 8 elements a thread and unit in registers across both sums, and goes on
 // with the row that lies a grid's length behind, whose loads are on their way during
 // the sums; the weights and a gate of channels stay in registers.  bf16, both norms: 16384 rows of
-// 4096 with codes 79 us, 6.0 TB/s of what it reads and writes; 1900 of 7168, 36 us, 5.3 TB/s; 8 rows
-// 4.8 us, two sums over a workgroup behind one another and the way to memory.
+// 4096 with codes 78 to 81 us on three sets of inputs in turn, 5.8 to 6.0 TB/s of what it reads and writes, 82 to
+// 94 us on inputs just written; 1900 of 7168 with an fp32 residual and a gate of each element 35 and 40 us, 5.4
+// and 4.8 TB/s; 8 rows with one norm 3.9 us, two sums over a workgroup behind one another and the way to memory.
 #include "sgl_kv8.h"
 
 namespace sgl {

@@ -250,9 +250,11 @@ SGL_RULE int rotary_head_threads(int64_t T, int64_t H, int64_t units, int64_t cu
 
 // ---- norms between blocks: threads of a row's workgroup, units of 8 elements a
 // thread, and workgroups.  One unit a thread as far as a workgroup's 1024 threads reach: its
-// weights and the next row's loads fit the registers then.  One unit / two, us: 16384 x 4096
-// 102 / 143.  Workgroups that together have 1536 threads a CU, 16384 x 4096, us: 94.8, with 1024
-// 97, with 2048 105.
+// weights and the next row's loads fit the registers then.  One unit / two, us: 16384 x 4096, through the
+// cache, 102 / 143.  Workgroups that together have 1536 threads a CU / 1024 / 2048, us, both norms, inputs in turn
+// (just written): 16384 x 4096 with codes 81 / 84 / 86 (82 / 84 / 93), without 83 / 82 / 84 (89 / 86 / 88);
+// 6000 x 7168 61 / 61 / 58 (69 / 69 / 68); through the cache 8192 x 4096 43 / 42 / 43 (47 / 49 / 49), 1900 x 7168
+// 21 / 21 / 19 (24 / 24 / 22).
 constexpr int64_t kNormMost = 16384;  // elements of a row: 1024 threads of two units
 struct NormPlan {
   int64_t threads, units, grid;
@@ -264,9 +266,9 @@ SGL_RULE NormPlan norm_plan(int64_t T, int64_t row_units, int64_t cus) {
   return {threads, units, T < most ? T : most};
 }
 // Rows that pass the last-level cache by: where the two inputs, of 16 bits, hold more than 128 MiB.
-// By / through, us: 16384 x 4096 with both norms 78.8 / 93, with one 81 / 104, 6000 x 7168 60.7 /
-// 65.6, 8192 x 4096 (at the bound) 43 / 43; below it what the block before left in the cache is
-// read from there.
+// By / through, us, inputs in turn (just written): 16384 x 4096 with both norms and codes 81 / 93 (82 / 93),
+// without codes 83 / 104 (89 / 101), with one norm 81 / 102 (87 / 99), 6000 x 7168 61 / 65 (69 / 65), 8200 x 4096,
+// just above the bound, 45 / 44 (52 / 48); below it what the block before left in the cache is read from there.
 SGL_RULE bool norm_once(int64_t T, int64_t H) { return 4 * T * H > 128ll << 20; }
 
 // ---- append to the 8-bit cache: the most blocks that T tokens of B sequences

@@ -57,7 +57,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, before: Optional[torc
 
     with ``rms(v) = v / sqrt(mean(v^2) + eps)``.  ``x`` is bf16, f16 or f32,
     ``residual`` of the same type or f32, the weights ``[H]`` and the gate
-    (``[H]``, or a shape of x's that broadcasts) any of the three.  ``h`` has residual's type,
+    (``[H]``, or a shape that broadcasts to x's, which is copied out to it where its rows are not dense or
+    not at one stride) any of the three.  ``h`` has residual's type,
     or is ``residual`` itself with ``inplace``; ``y`` has x's.  Everything is
     computed in fp32 and each output rounded once (``y`` is of the unrounded ``h``);
     squares that pass fp32 make zeros and NaN of their row.

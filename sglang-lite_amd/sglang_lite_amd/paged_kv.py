@@ -204,7 +204,9 @@ def paged_attn(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, lens:
     a window: sequences ``cu_groups[g]`` to ``cu_groups[g + 1]`` begin alike, the full pages
     among their first ``shared[g]`` tokens being the same in the block table row of each that has queries.  Those
     pages are read once for all of the group's queries, and the result is the same but for the order
-    of its sums.  Sequences may stand outside of all groups.
+    of its sums.  Sequences may stand outside of all groups.  It pays where many rows of few queries each
+    share thousands of tokens (60 sequences of two on 8192: 70 us, 176 without), not on short prefixes of
+    few sequences, nor for a few chunks of dozens of queries, whose tiles read the prefix once each anyway.
 
     A row that sees no key is zero;
     rows behind the last sequence are not written (of a new tensor: they hold
